@@ -243,6 +243,17 @@ jsm_status jsm_rope_apply(const void* d_x, void* d_out, jsm_dtype dtype, const f
 jsm_status jsm_rope_apply_qk(const void* d_q, void* d_q_out, int Hq, const void* d_k, void* d_k_out, int Hkv, jsm_dtype dtype,
                              const float* d_table, int d, const int32_t* d_positions, int T, void* stream);
 
+/* Rotary positions on the first rot_dim components of the query and key heads of token rows of any pitch (the pieces of a fused [q | k | v]
+ * row, say), forward or transposed (the gradient of the rotation).  Pair i is (2i, 2i + 1) or (i, i + rot_dim / 2); with (c, s) the
+ * entry of the row's position and pair i in d_table, (x1, x2) -> (x1 c - x2 s, x2 c + x1 s), transposed with -s; components behind rot_dim are copied.
+ * d_table: F32 [table_len, rot_dim / 2, 2] of jsm_rope_half_table / jsm_rope_scaled_table (either layout).  positions: I32 [T] or NULL (= t).
+ * q, k, q_out, k_out: F32 or BF16, row pitches in elements; out may be the input itself (same pitch) but not overlap it otherwise.  Hq or Hkv may
+ * be 0.  A position outside the table leaves its row as it was and is reported by jsm_check_device_errors (JSM_INVALID_ARG). */
+typedef enum jsm_rope_layout { JSM_ROPE_ADJACENT = 0, JSM_ROPE_HALF = 1 } jsm_rope_layout;
+jsm_status jsm_rope_rotate(const void* d_q, int64_t q_row_stride, void* d_q_out, int64_t q_out_row_stride, int Hq, const void* d_k, int64_t k_row_stride,
+                           void* d_k_out, int64_t k_out_row_stride, int Hkv, jsm_dtype dtype, int D, const float* d_table, int table_len, int rot_dim,
+                           int layout, int transposed, const int32_t* d_positions, int T, void* stream);
+
 /* ---- attention (mat_head_gen_t::forward, mat_mha_t.hpp:45-74) -----------
  * q:[T_q, Hq*D], k,v:[T_k, Hkv*D] token-major, per sequence b of `batch`
  * equally long sequences; out:[T_q, Hq*D].  scores = q.k / sqrt(D) (scale passed
@@ -315,6 +326,38 @@ jsm_status jsm_attn_decode_static_scratch(const void* d_q, int64_t q_row_stride,
                                           const int32_t* d_context_lens, int n_seqs, int Hq, int Hkv, int D,
                                           float scale, const float* d_rope_table, int max_context, void* d_out,
                                           void* stream);
+
+/* ---- new tokens of many sequences over a paged cache, bf16 or 8-bit (not in the reference) -------------------------------
+ * Sequence s brings the rows d_starts[s] <= t < d_starts[s + 1] (I32 [n_seqs + 1], ascending; none, one, or many) of the T rows of the call; its context
+ * d_context_lens[s] counts them, so row t is position d_context_lens[s] - (d_starts[s + 1] - t).  Rows of no sequence (behind the last
+ * one, say) are neither read nor written.  A sequence whose lengths do not fit (more rows than context, a context beyond its table's
+ * max_pages * 64, beyond max_new / max_context where a call has them) is left out, a page outside 0 .. n_pages-1 is not accessed (what would come from it is
+ * meaningless); both are reported by jsm_check_device_errors (JSM_INVALID_ARG).  No two positions of a call may share a place in the pool.
+ * Make the first call on a device outside a stream capture.
+ *
+ * 8-bit cache: pool int8 [n_pages][2 (K,V)][Hkv][64][D] and scales bf16 [n_pages][2][Hkv][64]; it stands for bf16(number * scale).
+ * jsm_kv_append_q8 quantises the new keys - rotated first in fp32 where a table is given, see jsm_rope_rotate - and values (bf16 rows, head h at
+ * column h * D): scale = max |x| / 127 rounded up to bf16, number = rint(x / scale).  A row below 2^-100 becomes zero; a row with a NaN, an
+ * infinity or a magnitude above 2^127 gets the scale NaN and reads back as NaN.  D: a multiple of 16, up to 256.
+ * jsm_kv_read reads the call's positions back (token-major, head h at column h * D, BF16 or F32); d_scales NULL: a bf16 pool (jsm_kv_append).
+ *
+ * jsm_attn_chunk: attention of the new tokens over everything their sequence has in the cache, the tokens themselves included (append first).  The
+ * query at position p sees the keys max(0, p - window + 1) .. p (window 0: all before it); query head h reads kv head h / (Hq / Hkv).  The sum
+ * runs over the keys that are seen only: what the others hold, infinities and NaN too, has no influence, and pages that no query of the call
+ * sees are not read.  q, out: BF16 rows (16-byte aligned, pitch a multiple of 8); D 64 or 128; scale > 0; Hq / Hkv up to 128.
+ * max_new, max_context: bounds of the new tokens and of the context of one sequence.  d_scratch: jsm_attn_chunk_scratch_bytes(...) bytes for these arguments
+ * (contents do not matter, before or after; not monotone in the arguments); calls that may run at the same time need scratch of their own. */
+jsm_status jsm_kv_append_q8(void* d_pool, void* d_scales, int n_pages, const int32_t* d_block_table, int max_pages, const void* d_k, const void* d_v,
+                            int64_t kv_row_stride, const int32_t* d_starts, const int32_t* d_context_lens, int n_seqs, int T, int Hkv, int D,
+                            const float* d_rope_table, int table_len, int rot_dim, int layout, void* stream);
+jsm_status jsm_kv_read(const void* d_pool, const void* d_scales, int n_pages, const int32_t* d_block_table, int max_pages, const int32_t* d_starts,
+                       const int32_t* d_context_lens, int n_seqs, int T, int Hkv, int D, void* d_k_out, void* d_v_out, int64_t out_row_stride,
+                       jsm_dtype out_dtype, void* stream);
+size_t jsm_attn_chunk_scratch_bytes(int n_seqs, int T, int max_new, int max_context, int Hq, int Hkv, int D);
+jsm_status jsm_attn_chunk(const void* d_q, int64_t q_row_stride, const void* d_pool, const void* d_scales, int n_pages, const int32_t* d_block_table,
+                          int max_pages, const int32_t* d_starts, const int32_t* d_context_lens, int n_seqs, int T, int max_new, int max_context, int Hq,
+                          int Hkv, int D, int window, float scale, void* d_scratch, size_t scratch_bytes, void* d_out, int64_t out_row_stride,
+                          void* stream);
 
 /* ---- token-level helpers (not in the reference) ------------------------- */
 /* Sampling from F32 logits [n_rows, vocab] (row pitch row_stride elements): temperature, top-k (0 = 1024, the most the

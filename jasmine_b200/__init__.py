@@ -30,6 +30,8 @@ F32, BF16, I32 = 0, 1, 2
 # jsm_rows_kind
 ROWS_SUM, ROWS_MAX, ROWS_MEAN, ROWS_ARGMAX, ROWS_SOFTMAX, ROWS_LAYERNORM, ROWS_RMSNORM = range(7)
 PAGE_SIZE = 64
+# jsm_rope_layout
+ROPE_ADJACENT, ROPE_HALF = 0, 1
 
 
 class JsmError(RuntimeError):
@@ -118,6 +120,11 @@ SYMBOLS = {
     "jsm_rope_scaled_table": (_i, [_vp, _i, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, _i]),
     "jsm_rope_apply": (_i, [_vp, _vp, _i, _vp, _i, _i, _vp, _i, _vp]),
     "jsm_rope_apply_qk": (_i, [_vp, _vp, _i, _vp, _vp, _i, _i, _vp, _i, _vp, _i, _vp]),
+    "jsm_rope_rotate": (_i, [_vp, _i64, _vp, _i64, _i, _vp, _i64, _vp, _i64, _i, _i, _i, _vp, _i, _i, _i, _i, _vp, _i, _vp]),
+    "jsm_kv_append_q8": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _i64, _vp, _vp, _i, _i, _i, _i, _vp, _i, _i, _i, _vp]),
+    "jsm_kv_read": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _i64, _i, _vp]),
+    "jsm_attn_chunk_scratch_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
+    "jsm_attn_chunk": (_i, [_vp, _i64, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _sz, _vp, _i64, _vp]),
     "jsm_attn_prefill": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _i, _vp]),
     "jsm_kv_append": (_i, [_vp, _vp, _i, _vp, _vp, _i64, _vp, _vp, _i, _i, _i, _vp, _vp]),
     "jsm_attn_decode_scratch_bytes": (_sz, [_i, _i, _i, _i]),
@@ -500,6 +507,108 @@ def attn_decode_static_scratch(q, pool, block_table, context_lens, Hq, Hkv, D, m
                                                block_table.shape[1], context_lens.data_ptr(), n, Hq, Hkv, D, scale,
                                                rope.data_ptr() if rope is not None else None, max_context,
                                                out.data_ptr(), stream_ptr()))
+    return out
+
+
+def _need(ok, what):
+    if not ok:
+        raise JsmError(INVALID_ARG, what)
+
+
+def _rows(t, columns, what):
+    _need(t.dim() == 2 and t.shape[1] == columns and (columns <= 1 or t.stride(1) == 1), f"{what}: rows of {columns} adjacent elements are wanted")
+
+
+def _pitch(t):
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])  # (a single row's pitch means nothing)
+
+
+def _ints(t, shape, what):
+    _need(tuple(t.shape) == shape and t.dtype == _torch().int32 and t.is_contiguous(), f"{what}: a contiguous int32 tensor of shape {shape} is wanted")
+
+
+def rope_rotate(q, k, table, Hq, Hkv, D, rot_dim, positions=None, layout=ROPE_HALF, inverse=False, q_out=None, k_out=None):
+    """Query and key rows [T, Hq * D] and [T, Hkv * D] of any pitch, rotated on the first rot_dim components of every head (jsm_rope_rotate); inverse: the transposed
+    rotation (the gradient).  Either may be None with no heads.  table: F32 [positions, rot_dim / 2, 2]."""
+    torch = _torch()
+    x = q if q is not None else k
+    _need(x is not None, "rope_rotate: no rows")
+    T = x.shape[0]
+    _need((q is None) == (Hq == 0) and (k is None) == (Hkv == 0), "rope_rotate: rows without heads, or heads without rows")
+    _need(table.dtype == torch.float32 and table.is_contiguous() and table.dim() == 3 and tuple(table.shape[1:]) == (rot_dim // 2, 2), "rope_rotate: a contiguous "
+          "fp32 table [positions, rot_dim / 2, 2] is wanted")
+    q_out = torch.empty(T, Hq * D, dtype=q.dtype, device=q.device) if q is not None and q_out is None else q_out
+    k_out = torch.empty(T, Hkv * D, dtype=k.dtype, device=k.device) if k is not None and k_out is None else k_out
+    for t, n, what in ((q, Hq, "q"), (q_out, Hq, "q_out"), (k, Hkv, "k"), (k_out, Hkv, "k_out")):
+        if n:
+            _need(t.shape[0] == T and t.dtype == x.dtype, f"rope_rotate: {what} has other rows or another type")
+            _rows(t, n * D, "rope_rotate: " + what)
+    if positions is not None:
+        _ints(positions, (T,), "rope_rotate: positions")
+    p = lambda t, n: (t.data_ptr(), _pitch(t)) if n else (None, 0)  # noqa: E731
+    check(lib().jsm_rope_rotate(*p(q, Hq), *p(q_out, Hq), Hq, *p(k, Hkv), *p(k_out, Hkv), Hkv, dtype_of(x), D, table.data_ptr(), table.shape[0], rot_dim, layout,
+                                int(inverse), positions.data_ptr() if positions is not None else None, T, stream_ptr()))
+    return q_out, k_out
+
+
+def _cache(what, pool, scales, block_table, starts, context_lens, Hkv, D):
+    """Checks of a pool, its table and its sequences; (pool, scales, pages, table, pages of a sequence, starts, context lengths, sequences) for the C calls."""
+    torch = _torch()
+    n = context_lens.shape[0]
+    _need(pool.is_contiguous() and tuple(pool.shape[1:]) == (2, Hkv, PAGE_SIZE, D), f"{what}: a contiguous pool [pages, 2, {Hkv}, {PAGE_SIZE}, {D}] is wanted")
+    _need(pool.dtype == (torch.int8 if scales is not None else torch.bfloat16), f"{what}: an int8 pool has scales, a bf16 pool has none")
+    if scales is not None:
+        _need(scales.dtype == torch.bfloat16 and scales.is_contiguous() and scales.shape == pool.shape[:4], f"{what}: contiguous bf16 scales [pages, 2, {Hkv}, {PAGE_SIZE}]")
+    _need(block_table.dim() == 2, f"{what}: a block table [sequences, pages] is wanted")
+    _ints(block_table, (n, block_table.shape[1]), f"{what}: block table")
+    _ints(starts, (n + 1,), f"{what}: starts")
+    _ints(context_lens, (n,), f"{what}: context_lens")
+    return (pool.data_ptr(), scales.data_ptr() if scales is not None else None, pool.shape[0], block_table.data_ptr(), block_table.shape[1]), (
+        starts.data_ptr(), context_lens.data_ptr(), n)
+
+
+def kv_append_q8(pool, scales, block_table, k, v, starts, context_lens, Hkv, D, rope=None, rot_dim=0, layout=ROPE_HALF):
+    """New keys (rotated with the table `rope` [positions, rot_dim / 2, 2]) and values [T, Hkv * D] into an 8-bit cache (jsm_kv_append_q8)."""
+    torch = _torch()
+    at, seqs = _cache("kv_append_q8", pool, scales, block_table, starts, context_lens, Hkv, D)
+    for t, what in ((k, "k"), (v, "v")):
+        _rows(t, Hkv * D, "kv_append_q8: " + what)
+        _need(t.dtype == torch.bfloat16, f"kv_append_q8: {what} in bf16")
+    _need(k.shape == v.shape and _pitch(k) == _pitch(v), "kv_append_q8: k and v of one pitch")
+    if rope is not None:
+        _need(rope.dtype == torch.float32 and rope.is_contiguous() and rope.dim() == 3 and tuple(rope.shape[1:]) == (rot_dim // 2, 2),
+              "kv_append_q8: a contiguous fp32 table [positions, rot_dim / 2, 2] is wanted")
+    check(lib().jsm_kv_append_q8(*at, k.data_ptr(), v.data_ptr(), _pitch(k), *seqs, k.shape[0], Hkv, D, rope.data_ptr() if rope is not None else None,
+                                 rope.shape[0] if rope is not None else 0, rot_dim, layout, stream_ptr()))
+
+
+def kv_read(pool, block_table, starts, context_lens, T, Hkv, D, scales=None, dtype=None, k_out=None, v_out=None):
+    """Keys and values [T, Hkv * D] (bf16, or dtype) of the new tokens' positions as the cache holds them (jsm_kv_read); rows of no sequence are left as they are."""
+    torch = _torch()
+    at, seqs = _cache("kv_read", pool, scales, block_table, starts, context_lens, Hkv, D)
+    k_out = torch.empty(T, Hkv * D, dtype=dtype or torch.bfloat16, device=pool.device) if k_out is None else k_out
+    v_out = torch.empty_like(k_out) if v_out is None else v_out
+    for t in (k_out, v_out):
+        _rows(t, Hkv * D, "kv_read: out")
+    _need(k_out.shape == v_out.shape and k_out.shape[0] == T and k_out.dtype == v_out.dtype and _pitch(k_out) == _pitch(v_out), "kv_read: outputs of one shape, type and pitch")
+    check(lib().jsm_kv_read(*at, *seqs, T, Hkv, D, k_out.data_ptr(), v_out.data_ptr(), _pitch(k_out), dtype_of(k_out), stream_ptr()))
+    return k_out, v_out
+
+
+def attn_chunk(q, pool, block_table, starts, context_lens, Hq, Hkv, D, max_new, max_context, scales=None, window=0, scale=None, scratch=None, out=None):
+    """Attention of the new tokens q [T, Hq * D] of every sequence over its paged cache, bf16 or (with scales) 8-bit (jsm_attn_chunk)."""
+    torch = _torch()
+    at, seqs = _cache("attn_chunk", pool, scales, block_table, starts, context_lens, Hkv, D)
+    T = q.shape[0]
+    out = torch.empty(T, Hq * D, dtype=q.dtype, device=q.device) if out is None else out
+    for t, what in ((q, "q"), (out, "out")):
+        _rows(t, Hq * D, "attn_chunk: " + what)
+        _need(t.dtype == torch.bfloat16 and t.shape[0] == T, f"attn_chunk: {what} of {T} rows in bf16")
+    if scratch is None:
+        scratch = torch.empty(lib().jsm_attn_chunk_scratch_bytes(seqs[2], T, max_new, max_context, Hq, Hkv, D), dtype=torch.uint8, device=q.device)
+    scale = float(D) ** -0.5 if scale is None else scale
+    check(lib().jsm_attn_chunk(q.data_ptr(), _pitch(q), *at, *seqs, T, max_new, max_context, Hq, Hkv, D, window, scale, scratch.data_ptr(),
+                               scratch.numel() * scratch.element_size(), out.data_ptr(), _pitch(out), stream_ptr()))
     return out
 
 

@@ -1,0 +1,75 @@
+// What the operators over sequences of a paged cache share: which sequence a row of new tokens belongs to, where a position lies in the pool, and
+// how a sequence's lengths are checked on the device.
+//
+// Row t of the new tokens belongs to the sequence s with starts[s] <= t < starts[s + 1]; context_lens[s] counts the new tokens, so row t is
+// position context_lens[s] - (starts[s + 1] - t).  Pool: [page][keys, values][kv head][64 positions][D], bf16 or int8; an int8 pool has a bf16
+// scale per position, [page][keys, values][kv head][64], and stands for bf16(number * scale).
+#pragma once
+#include "common.cuh"
+
+namespace jsm {
+
+// codes of the device error word (jsm_check_device_errors)
+enum CacheError : int { CACHE_BAD_POSITION = 33, CACHE_BAD_PAGE = 34, CACHE_BAD_LENGTH = 35 };
+
+struct CacheView {
+    void* pool;
+    uint16_t* scales;            // null: a bf16 pool
+    int n_pages;
+    const int32_t* table;        // [n_seqs][max_pages]
+    int max_pages;
+    const int32_t* starts;       // [n_seqs + 1]
+    const int32_t* context_lens; // [n_seqs]
+    int n_seqs, Hkv, D;
+    int* err;
+};
+
+#ifdef __CUDACC__
+__device__ __forceinline__ void cache_error(int* err, int code) {
+    if (err) atomicCAS(err, 0, code);
+}
+
+// new tokens and context of sequence s; false (and an error) where they do not fit the table or one another
+__device__ __forceinline__ bool cache_lengths(const CacheView& c, int s, int T, int& first_row, int& n_new, int& ctx) {
+    first_row = c.starts[s];
+    const int end = c.starts[s + 1];
+    n_new = end - first_row;
+    ctx = c.context_lens[s];
+    if (n_new <= 0) return false;
+    if (first_row < 0 || end > T || ctx < n_new || (ctx - 1) / JSM_PAGE_SIZE >= c.max_pages) {
+        cache_error(c.err, CACHE_BAD_LENGTH);
+        return false;
+    }
+    return true;
+}
+
+// The sequence of row t, for a whole block: every thread looks at one sequence, one round of loads for as many sequences as the block has threads.  -1: none.
+__device__ __forceinline__ int find_sequence(const CacheView& c, int t, int* found) {
+    if (threadIdx.x == 0) *found = -1;
+    __syncthreads();
+    for (int s = threadIdx.x; s < c.n_seqs; s += blockDim.x)
+        if (c.starts[s] <= t && t < c.starts[s + 1]) *found = s;
+    __syncthreads();
+    return *found;
+}
+
+// page of a position of sequence s (within its table row); -1 and an error for an entry outside the pool
+__device__ __forceinline__ int cache_page(const CacheView& c, int s, int pos) {
+    const int page = c.table[(long long)s * c.max_pages + pos / JSM_PAGE_SIZE];
+    if (page >= 0 && page < c.n_pages) return page;
+    cache_error(c.err, CACHE_BAD_PAGE);
+    return -1;
+}
+// row of a position (elements / D of the pool, and the index of its scale); value: 0 keys, 1 values
+__device__ __forceinline__ long long cache_row(const CacheView& c, int page, int value, int head, int pos) {
+    return (((long long)page * 2 + value) * c.Hkv + head) * JSM_PAGE_SIZE + pos % JSM_PAGE_SIZE;
+}
+
+// rotation of a pair, every product rounded on its own
+__device__ __forceinline__ void rotate_pair(float x1, float x2, float c, float s, float& y1, float& y2) {
+    y1 = __fsub_rn(__fmul_rn(x1, c), __fmul_rn(x2, s));
+    y2 = __fadd_rn(__fmul_rn(x2, c), __fmul_rn(x1, s));
+}
+#endif
+
+}  // namespace jsm

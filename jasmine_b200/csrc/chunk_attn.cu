@@ -1,0 +1,65 @@
+// Attention of new tokens over a paged cache, bf16 or 8-bit: entry points and kernels.
+#include "chunk_attn.cuh"
+#include <math.h>
+
+namespace jsm {
+
+jsm_status cache_view_check(const char* who, CacheView& c, void* pool, void* scales, int n_pages, const int32_t* table, int max_pages, const int32_t* starts,
+                            const int32_t* context_lens, int n_seqs, int T, int Hkv, int D);
+
+// a warp per (row, query head)
+template <int D, bool Q8>
+__global__ void __launch_bounds__(128) chunk_rows_kernel(ChunkArgs a) {
+    __shared__ int found;
+    chain_trigger();
+    chain_wait();
+    const int t = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5);
+    const int s = find_sequence(a.c, t, &found);
+    if (s < 0 || head >= a.Hq) return;
+    int first, n_new, ctx;
+    if (!chunk_lengths(a, s, first, n_new, ctx)) return;
+    attend_row<D, Q8>(a, s, t, head, ctx - n_new + t - first);
+}
+
+template <int D, bool Q8>
+static jsm_status chunk_rows_launch(const ChunkArgs& a, cudaStream_t st) {
+    JSM_CUDA_CHECK(launch_chained(chunk_rows_kernel<D, Q8>, dim3(a.T, (a.Hq + 3) / 4), dim3(128), 0, st, a));
+    JSM_LAUNCH_CHECK();
+    return JSM_OK;
+}
+
+}  // namespace jsm
+
+using namespace jsm;
+
+extern "C" size_t jsm_attn_chunk_scratch_bytes(int n_seqs, int T, int max_new, int max_context, int Hq, int Hkv, int D) { return 0; }
+
+extern "C" jsm_status jsm_attn_chunk(const void* d_q, int64_t q_row_stride, const void* d_pool, const void* d_scales, int n_pages, const int32_t* d_block_table,
+                                     int max_pages, const int32_t* d_starts, const int32_t* d_context_lens, int n_seqs, int T, int max_new, int max_context, int Hq,
+                                     int Hkv, int D, int window, float scale, void* d_scratch, size_t scratch_bytes, void* d_out, int64_t out_row_stride,
+                                     void* stream) {
+    ChunkArgs a{};
+    const jsm_status s = cache_view_check("jsm_attn_chunk", a.c, const_cast<void*>(d_pool), const_cast<void*>(d_scales), n_pages, d_block_table, max_pages, d_starts,
+                                          d_context_lens, n_seqs, T, Hkv, D);
+    if (s != JSM_OK) return s;
+    if (D != 64 && D != 128) JSM_FAIL(JSM_UNSUPPORTED, "jsm_attn_chunk: head_dim %d (64 or 128)", D);
+    if (Hq <= 0 || Hq % Hkv) JSM_FAIL(JSM_SHAPE, "d_model must be divisible by num_heads (Hq %d, Hkv %d)", Hq, Hkv);
+    if (Hq / Hkv > 128) JSM_FAIL(JSM_UNSUPPORTED, "jsm_attn_chunk: %d query heads per kv head (up to 128)", Hq / Hkv);
+    if (window < 0) JSM_FAIL(JSM_INVALID_ARG, "jsm_attn_chunk: window %d", window);
+    if (!(scale > 0.0f) || scale > 1e30f) JSM_FAIL(JSM_UNSUPPORTED, "jsm_attn_chunk: the softmax scale (%g) must be positive", (double)scale);
+    if (T == 0 || n_seqs == 0) return JSM_OK;
+    if (max_new <= 0 || max_context < max_new) JSM_FAIL(JSM_INVALID_ARG, "jsm_attn_chunk: up to %d new tokens of contexts up to %d", max_new, max_context);
+    if (!d_q || !d_out) JSM_FAIL(JSM_INVALID_ARG, "jsm_attn_chunk: null pointer");
+    if (q_row_stride < (int64_t)Hq * D || out_row_stride < (int64_t)Hq * D || q_row_stride % 8 || out_row_stride % 8)
+        JSM_FAIL(JSM_INVALID_ARG, "jsm_attn_chunk: rows of %lld and %lld elements for %d heads of %d (multiples of 8)", (long long)q_row_stride, (long long)out_row_stride, Hq, D);
+    if ((reinterpret_cast<uintptr_t>(d_q) & 15) || (reinterpret_cast<uintptr_t>(d_out) & 15)) JSM_FAIL(JSM_INVALID_ARG, "jsm_attn_chunk: q and out must be 16-byte aligned");
+    a.q = static_cast<const __nv_bfloat16*>(d_q);
+    a.out = static_cast<__nv_bfloat16*>(d_out);
+    a.q_rs = q_row_stride; a.out_rs = out_row_stride;
+    a.T = T; a.max_new = max_new; a.max_context = max_context;
+    a.Hq = Hq; a.G = Hq / Hkv; a.window = window;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    const cudaStream_t st = as_stream(stream);
+    if (D == 64) return d_scales ? chunk_rows_launch<64, true>(a, st) : chunk_rows_launch<64, false>(a, st);
+    return d_scales ? chunk_rows_launch<128, true>(a, st) : chunk_rows_launch<128, false>(a, st);
+}

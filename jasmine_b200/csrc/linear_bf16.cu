@@ -395,6 +395,9 @@ jsm_status linear_bf16_launch(const LinearArgs& a, cudaStream_t st) {
 
 jsm_status tc_error_status(int code, const char* who) {
     if (code == 32) JSM_FAIL(JSM_SHAPE, "%s: context overflow: a decode step met a sequence that already holds max_context tokens", who);
+    if (code == 33) JSM_FAIL(JSM_INVALID_ARG, "%s: a position lies outside the rotation table (its row was left as it was)", who);
+    if (code == 34) JSM_FAIL(JSM_INVALID_ARG, "%s: a block table names a page outside the pool", who);
+    if (code == 35) JSM_FAIL(JSM_INVALID_ARG, "%s: the lengths of a sequence do not fit its context, its table or the call's bounds (its rows were left as they were)", who);
     JSM_FAIL(JSM_TIMEOUT, "%s: a bounded device-side wait ran out (code %d)", who, code);
 }
 jsm_status tc_check_error(cudaStream_t st, const char* who) {

@@ -1,0 +1,92 @@
+// Rotary positions on the query and key heads of token rows of any pitch: adjacent pairs or halves, on the first rot_dim components of a head, from
+// the (cos, sin) tables of jsm_rope_half_table / jsm_rope_scaled_table; transposed, it is the gradient of the rotation.
+//   pair (x1, x2) -> (x1 c - x2 s, x2 c + x1 s),  transposed: s -> -s
+// Bound by memory: every row is read and written once.  The table (8 bytes per pair, twice the bytes of a bf16 pair) would cost more than one head, so a thread keeps
+// the entries of its eight (fp32: four) pairs and walks the heads with them.
+#include "cache_view.cuh"
+
+namespace jsm {
+
+int* tc_error_word();
+
+struct RotateArgs {
+    const void *q, *k;
+    void *q_out, *k_out;
+    long long q_rs, k_rs, qo_rs, ko_rs;  // row pitches, elements
+    int Hq, Hk, D, rot, adjacent;
+    float sign;                          // -1: transposed
+    const float2* table;
+    int table_len;
+    const int32_t* positions;
+    int T;
+    int* err;
+};
+
+template <typename T>
+__device__ __forceinline__ float rot_load(const T* p);
+template <>
+__device__ __forceinline__ float rot_load<float>(const float* p) { return *p; }
+template <>
+__device__ __forceinline__ float rot_load<__nv_bfloat16>(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void rot_store(float* p, float v) { *p = v; }
+__device__ __forceinline__ void rot_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// any sizes, pitches and alignments: a thread per pair or unrotated component
+template <typename T>
+__global__ void __launch_bounds__(256) rope_rotate_scalar_kernel(RotateArgs a) {
+    chain_trigger();
+    chain_wait();
+    const int half = a.rot / 2, units = a.D - half, heads = a.Hq + a.Hk;
+    for (int t = blockIdx.x; t < a.T; t += gridDim.x) {
+        const int pos = a.positions ? a.positions[t] : t;
+        if (pos < 0 || pos >= a.table_len) {
+            if (threadIdx.x == 0) cache_error(a.err, CACHE_BAD_POSITION);
+            continue;
+        }
+        for (int i = threadIdx.x; i < heads * units; i += blockDim.x) {
+            const int h = i / units, u = i % units;
+            const bool is_q = h < a.Hq;
+            const T* src = is_q ? static_cast<const T*>(a.q) + t * a.q_rs + (long long)h * a.D : static_cast<const T*>(a.k) + t * a.k_rs + (long long)(h - a.Hq) * a.D;
+            T* dst = is_q ? static_cast<T*>(a.q_out) + t * a.qo_rs + (long long)h * a.D : static_cast<T*>(a.k_out) + t * a.ko_rs + (long long)(h - a.Hq) * a.D;
+            if (u < half) {
+                const float2 e = a.table[(long long)pos * half + u];
+                const int i1 = a.adjacent ? 2 * u : u, i2 = a.adjacent ? 2 * u + 1 : u + half;
+                float y1, y2;
+                rotate_pair(rot_load(src + i1), rot_load(src + i2), e.x, a.sign * e.y, y1, y2);
+                rot_store(dst + i1, y1);
+                rot_store(dst + i2, y2);
+            } else {
+                dst[u + half] = src[u + half];
+            }
+        }
+    }
+}
+
+}  // namespace jsm
+
+using namespace jsm;
+
+extern "C" jsm_status jsm_rope_rotate(const void* d_q, int64_t q_row_stride, void* d_q_out, int64_t q_out_row_stride, int Hq, const void* d_k, int64_t k_row_stride,
+                                      void* d_k_out, int64_t k_out_row_stride, int Hkv, jsm_dtype dtype, int D, const float* d_table, int table_len, int rot_dim,
+                                      int layout, int transposed, const int32_t* d_positions, int T, void* stream) {
+    if (T < 0 || Hq < 0 || Hkv < 0 || Hq + (int64_t)Hkv > INT32_MAX / 4) JSM_FAIL(JSM_INVALID_ARG, "jsm_rope_rotate: T %d, heads %d and %d", T, Hq, Hkv);
+    if (D <= 0 || D > 4096 || rot_dim <= 0 || rot_dim % 2 || rot_dim > D) JSM_FAIL(JSM_SHAPE, "jsm_rope_rotate: rotation of %d components of a head of %d", rot_dim, D);
+    if ((Hq + (int64_t)Hkv) * D > INT32_MAX) JSM_FAIL(JSM_SHAPE, "jsm_rope_rotate: heads %d and %d of %d", Hq, Hkv, D);
+    if (layout != JSM_ROPE_ADJACENT && layout != JSM_ROPE_HALF) JSM_FAIL(JSM_INVALID_ARG, "jsm_rope_rotate: layout %d", layout);
+    if (dtype != JSM_F32 && dtype != JSM_BF16) JSM_FAIL(JSM_UNSUPPORTED, "jsm_rope_rotate: dtype %d", (int)dtype);
+    if (table_len <= 0) JSM_FAIL(JSM_INVALID_ARG, "jsm_rope_rotate: a table of %d positions", table_len);
+    if (T == 0 || Hq + Hkv == 0) return JSM_OK;
+    if (!d_table || (Hq > 0 && (!d_q || !d_q_out)) || (Hkv > 0 && (!d_k || !d_k_out))) JSM_FAIL(JSM_INVALID_ARG, "jsm_rope_rotate: null pointer");
+    if (Hq > 0 && (q_row_stride < (int64_t)Hq * D || q_out_row_stride < (int64_t)Hq * D)) JSM_FAIL(JSM_INVALID_ARG, "jsm_rope_rotate: query rows overlap");
+    if (Hkv > 0 && (k_row_stride < (int64_t)Hkv * D || k_out_row_stride < (int64_t)Hkv * D)) JSM_FAIL(JSM_INVALID_ARG, "jsm_rope_rotate: key rows overlap");
+    if (reinterpret_cast<uintptr_t>(d_table) & 7) JSM_FAIL(JSM_INVALID_ARG, "jsm_rope_rotate: the table is not 8-byte aligned");
+    const uintptr_t odd = reinterpret_cast<uintptr_t>(d_q) | reinterpret_cast<uintptr_t>(d_q_out) | reinterpret_cast<uintptr_t>(d_k) | reinterpret_cast<uintptr_t>(d_k_out);
+    if (odd & (dtype == JSM_F32 ? 3 : 1)) JSM_FAIL(JSM_INVALID_ARG, "jsm_rope_rotate: rows that are not aligned to their elements");
+    RotateArgs a{d_q, d_k, d_q_out, d_k_out, q_row_stride, k_row_stride, q_out_row_stride, k_out_row_stride, Hq, Hkv, D, rot_dim, layout == JSM_ROPE_ADJACENT ? 1 : 0,
+                 transposed ? -1.0f : 1.0f, reinterpret_cast<const float2*>(d_table), table_len, d_positions, T, tc_error_word()};
+    const dim3 grid(T < sm_count() * 8 ? T : sm_count() * 8);
+    if (dtype == JSM_F32) JSM_CUDA_CHECK(launch_chained(rope_rotate_scalar_kernel<float>, grid, dim3(256), 0, as_stream(stream), a));
+    else JSM_CUDA_CHECK(launch_chained(rope_rotate_scalar_kernel<__nv_bfloat16>, grid, dim3(256), 0, as_stream(stream), a));
+    JSM_LAUNCH_CHECK();
+    return JSM_OK;
+}

@@ -1,0 +1,169 @@
+"""Attention of new tokens over a paged cache (jsm_attn_chunk), bf16 and 8-bit, against 64 bits."""
+import pytest
+import torch
+
+import jasmine_b200 as jb
+from cache_util import PAGE, Cache, check_attention
+
+pytestmark = pytest.mark.gpu
+BITS = (16, 8)
+
+#  new tokens, contexts, Hq, Hkv, D, window
+CASES = [
+    ([1], [1], 1, 1, 64, 0),
+    ([1], [1], 8, 2, 128, 0),
+    ([1], [64], 4, 4, 128, 0),
+    ([1], [65], 8, 1, 128, 0),
+    ([1, 1, 1], [63, 64, 700], 32, 8, 128, 0),
+    ([1, 1], [2500, 130], 16, 2, 64, 0),
+    ([1] * 9, [1, 2, 5, 64, 65, 127, 128, 129, 500], 6, 2, 128, 0),
+    ([1, 1, 1], [300, 20, 129], 12, 4, 128, 100),
+    ([2, 0, 3], [2, 0, 40], 4, 2, 128, 0),
+    ([4], [260], 8, 2, 128, 0),
+    ([5, 1, 3], [200, 77, 3], 10, 2, 64, 0),
+    ([9], [9], 16, 1, 128, 0),
+    ([17], [300], 4, 4, 128, 0),
+    ([64], [64], 8, 2, 128, 0),
+    ([128], [128], 2, 2, 128, 0),
+    ([129], [1000], 4, 1, 128, 0),
+    ([200, 1, 33], [200, 400, 290], 8, 2, 128, 0),
+    ([300], [300], 7, 1, 64, 0),
+    ([257], [700], 3, 3, 64, 0),
+    ([150], [900], 12, 4, 128, 64),
+    ([90, 2], [400, 600], 10, 2, 128, 33),
+    ([70], [200], 4, 4, 64, 1),
+    ([513], [2048], 4, 4, 128, 0),
+    ([40, 700], [1500, 700], 16, 2, 64, 200),
+    ([3, 500], [4000, 500], 40, 8, 128, 0),
+    ([2], [3], 100, 1, 128, 0),
+    ([6], [100], 128, 1, 64, 0),
+    ([50], [80], 65, 1, 128, 0),
+]
+
+
+@pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("new,ctx,Hq,Hkv,D,window", CASES)
+def test_against_64_bits(new, ctx, Hq, Hkv, D, window, bits):
+    c = Cache(new, ctx, Hkv, D, bits, seed=len(new) + sum(ctx)).to_device()
+    q = c.queries(Hq)
+    got = c.attend(q.cuda(), window)
+    jb.check_device_errors()
+    check_attention(got, *c.reference(q, window))
+
+
+@pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("new,ctx,Hq", [([1, 1], [900, 40], 8), ([70, 3], [300, 500], 8), ([200], [1400], 4)])
+def test_sharp_scores(new, ctx, Hq, bits):
+    """Large scores: the running maximum moves, weights underflow."""
+    c = Cache(new, ctx, 2, 128, bits, seed=5).to_device()
+    q = c.queries(Hq, 6.0)
+    got = c.attend(q.cuda(), 0, 0.3)
+    want, mag = c.reference(q, 0, 0.3)
+    # scores of up to 0.3 * 6 * 128 * 3 in fp32: 128 products of 2^-24 each give errors of up to 1e-4 in an exponent
+    check_attention(got, want, mag * 1.1)
+
+
+@pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("new,ctx,window", [([1, 3], [200, 260], 0), ([100], [300], 0), ([100, 1], [300, 200], 70), ([4], [150], 20)])
+@pytest.mark.parametrize("bad", (float("nan"), float("inf"), -float("inf")))
+def test_unseen_keys_have_no_part(new, ctx, window, bits, bad):
+    """Keys and values that are not numbers, at places that some queries see and others do not."""
+    c = Cache(new, ctx, 2, 128, bits, seed=9)
+    for b, (n, x) in enumerate(zip(new, ctx)):
+        c.values[b][1, 0, x - 1 - n // 2] = bad      # a value among the new tokens: later queries see it
+        c.values[b][0, 1, x - 1, 5] = bad            # a key that the last query sees alone
+        c.values[b][1, 1, max(0, x - n - 30), 3] = bad  # in the window of some
+        c.write(b)
+    c.to_device()
+    q = c.queries(8)
+    got = c.attend(q.cuda(), window).double().cpu()
+    want, mag = c.reference(q, window)
+    # an infinite value under a weight gives an infinity or a NaN: neither a number
+    assert torch.equal(got.isfinite(), want.isfinite())
+    fine = want.isfinite()
+    check_attention(torch.where(fine, got, 0.0), torch.where(fine, want, 0.0), torch.where(fine, mag, 0.0))
+
+
+def test_rows_of_no_sequence_and_pitches():
+    c = Cache([3, 0, 40, 1], [70, 9, 300, 130], 2, 128, 8, rows=7).to_device()
+    q = c.queries(6)
+    wide = torch.full((c.T, 6 * 128 + 24), float("nan"), dtype=torch.bfloat16, device="cuda")
+    wide[:, 8:8 + 768] = q.cuda()
+    out = torch.full((c.T, 6 * 128 + 40), 3.0, dtype=torch.bfloat16, device="cuda")
+    c.attend(wide[:, 8:8 + 768], out=out[:, 16:16 + 768])
+    jb.check_device_errors()
+    check_attention(out[:, 16:16 + 768], *c.reference(q))
+    assert bool((out[44:] == 3).all()) and bool((out[:, :16] == 3).all()) and bool((out[:, 784:] == 3).all())
+
+
+@pytest.mark.parametrize("bits", BITS)
+def test_pages_behind_the_window_are_not_read(bits):
+    c = Cache([1, 70, 2], [900, 800, 640], 2, 64, bits, seed=3)
+    q = c.queries(4)
+    want = c.reference(q, 100)
+    for b, (n, x) in enumerate(zip(c.new, c.ctx)):
+        c.table[b, :max(0, x - n - 99) // PAGE] = -7
+    c.to_device()
+    got = c.attend(q.cuda(), 100)
+    jb.check_device_errors()
+    check_attention(got, *want)
+
+
+@pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("new,ctx", [([1] * 5, [3000, 40, 900, 64, 1]), ([150, 20], [2000, 90])])
+def test_the_same_bits_again_from_a_graph_and_on_another_stream(new, ctx, bits):
+    c = Cache(new, ctx, 2, 128, bits, seed=4).to_device()
+    q = c.queries(8).cuda()
+    first = c.attend(q)
+    out = torch.empty_like(first)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c.attend(q, out=out)
+    side.synchronize()
+    assert torch.equal(first, out)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.attend(q, out=out)
+    out.zero_()
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(first, out)
+    jb.check_device_errors()
+
+
+def test_lengths_and_pages_that_do_not_fit_are_reported():
+    def fresh():
+        c = Cache([2, 5], [100, 200], 2, 128, 8, seed=1).to_device()
+        q = c.queries(4)
+        return c, q, c.reference(q), torch.full((c.T, 512), 9.0, dtype=torch.bfloat16, device="cuda")
+
+    for change in ("context", "max_new", "max_context", "table"):
+        c, q, (want, mag), out = fresh()
+        kw = dict(max_new=5, max_context=200)
+        if change == "context":
+            c.lens[0] = 1
+        elif change == "max_new":
+            kw["max_new"] = 4
+        elif change == "max_context":
+            kw["max_context"] = 150
+        else:
+            c.table = c.table[:, :2].contiguous()
+        left = slice(0, 2) if change == "context" else slice(2, 7)
+        jb.attn_chunk(q.cuda(), c.pool, c.table, c.starts, c.lens, 4, 2, 128, scales=c.scales, out=out, **kw)
+        with pytest.raises(jb.JsmError, match="lengths of a sequence") as e:
+            jb.check_device_errors()
+        assert e.value.status == jb.INVALID_ARG
+        assert bool((out[left] == 9).all())
+        want[left] = float("nan")
+        check_attention(out, want, mag)
+    for page in (-1, 1 << 20):
+        c, q, (want, mag), out = fresh()
+        c.table[1, 1] = page
+        c.attend(q.cuda(), out=out)
+        with pytest.raises(jb.JsmError, match="page outside the pool"):
+            jb.check_device_errors()
+        want[2:] = float("nan")
+        check_attention(out, want, mag)
+    jb.check_device_errors()
