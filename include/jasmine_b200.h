@@ -353,7 +353,7 @@ jsm_status jsm_kv_append_q8(void* d_pool, void* d_scales, int n_pages, const int
 jsm_status jsm_kv_read(const void* d_pool, const void* d_scales, int n_pages, const int32_t* d_block_table, int max_pages, const int32_t* d_starts,
                        const int32_t* d_context_lens, int n_seqs, int T, int Hkv, int D, void* d_k_out, void* d_v_out, int64_t out_row_stride,
                        jsm_dtype out_dtype, void* stream);
-size_t jsm_attn_chunk_scratch_bytes(int n_seqs, int T, int max_new, int max_context, int Hq, int Hkv, int D);
+size_t jsm_attn_chunk_scratch_bytes(int n_seqs, int T, int max_new, int max_context, int Hq, int Hkv, int D, int window);
 jsm_status jsm_attn_chunk(const void* d_q, int64_t q_row_stride, const void* d_pool, const void* d_scales, int n_pages, const int32_t* d_block_table,
                           int max_pages, const int32_t* d_starts, const int32_t* d_context_lens, int n_seqs, int T, int max_new, int max_context, int Hq,
                           int Hkv, int D, int window, float scale, void* d_scratch, size_t scratch_bytes, void* d_out, int64_t out_row_stride,

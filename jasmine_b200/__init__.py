@@ -123,7 +123,7 @@ SYMBOLS = {
     "jsm_rope_rotate": (_i, [_vp, _i64, _vp, _i64, _i, _vp, _i64, _vp, _i64, _i, _i, _i, _vp, _i, _i, _i, _i, _vp, _i, _vp]),
     "jsm_kv_append_q8": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _i64, _vp, _vp, _i, _i, _i, _i, _vp, _i, _i, _i, _vp]),
     "jsm_kv_read": (_i, [_vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _i64, _i, _vp]),
-    "jsm_attn_chunk_scratch_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
+    "jsm_attn_chunk_scratch_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
     "jsm_attn_chunk": (_i, [_vp, _i64, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _sz, _vp, _i64, _vp]),
     "jsm_attn_prefill": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _i, _vp]),
     "jsm_kv_append": (_i, [_vp, _vp, _i, _vp, _vp, _i64, _vp, _vp, _i, _i, _i, _vp, _vp]),
@@ -605,7 +605,7 @@ def attn_chunk(q, pool, block_table, starts, context_lens, Hq, Hkv, D, max_new, 
         _rows(t, Hq * D, "attn_chunk: " + what)
         _need(t.dtype == torch.bfloat16 and t.shape[0] == T, f"attn_chunk: {what} of {T} rows in bf16")
     if scratch is None:
-        scratch = torch.empty(lib().jsm_attn_chunk_scratch_bytes(seqs[2], T, max_new, max_context, Hq, Hkv, D), dtype=torch.uint8, device=q.device)
+        scratch = torch.empty(lib().jsm_attn_chunk_scratch_bytes(seqs[2], T, max_new, max_context, Hq, Hkv, D, window), dtype=torch.uint8, device=q.device)
     scale = float(D) ** -0.5 if scale is None else scale
     check(lib().jsm_attn_chunk(q.data_ptr(), _pitch(q), *at, *seqs, T, max_new, max_context, Hq, Hkv, D, window, scale, scratch.data_ptr(),
                                scratch.numel() * scratch.element_size(), out.data_ptr(), _pitch(out), stream_ptr()))

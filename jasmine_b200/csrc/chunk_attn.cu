@@ -9,7 +9,7 @@ jsm_status cache_view_check(const char* who, CacheView& c, void* pool, void* sca
 
 // a warp per (row, query head)
 template <int D, bool Q8>
-__global__ void __launch_bounds__(128) chunk_rows_kernel(ChunkArgs a) {
+__global__ void __launch_bounds__(128) chunk_rows_kernel(const __grid_constant__ ChunkArgs a, int few_rows) {
     __shared__ int found;
     chain_trigger();
     chain_wait();
@@ -17,22 +17,46 @@ __global__ void __launch_bounds__(128) chunk_rows_kernel(ChunkArgs a) {
     const int s = find_sequence(a.c, t, &found);
     if (s < 0 || head >= a.Hq) return;
     int first, n_new, ctx;
-    if (!chunk_lengths(a, s, first, n_new, ctx)) return;
+    if (!chunk_lengths(a, s, first, n_new, ctx) || n_new * a.G <= few_rows) return;
     attend_row<D, Q8>(a, s, t, head, ctx - n_new + t - first);
 }
 
 template <int D, bool Q8>
-static jsm_status chunk_rows_launch(const ChunkArgs& a, cudaStream_t st) {
-    JSM_CUDA_CHECK(launch_chained(chunk_rows_kernel<D, Q8>, dim3(a.T, (a.Hq + 3) / 4), dim3(128), 0, st, a));
+static jsm_status chunk_rows_launch(const ChunkArgs& a, int few_rows, cudaStream_t st) {
+    JSM_CUDA_CHECK(launch_chained(chunk_rows_kernel<D, Q8>, dim3(a.T, (a.Hq + 3) / 4), dim3(128), 0, st, a, few_rows));
     JSM_LAUNCH_CHECK();
     return JSM_OK;
 }
+
+namespace {
+// What runs for a call: sequences of up to few_rows rows of queries per kv head take chunk_few.cu, the others (if there can be any) the other kernel.
+struct Plan {
+    int few_rows;
+    bool many;
+    FewPlan few;
+    size_t bytes;
+};
+Plan plan_of(int n_seqs, int T, int max_new, int max_context, int Hkv, int G, int D, int window) {
+    Plan p;
+    const long long most = (long long)max_new * G;
+    p.few_rows = most <= 8 ? 8 : most <= 16 ? 16 : G <= 8 ? 8 : 16;
+    p.many = most > 16;
+    // (with one sequence of more rows there is nothing for the kernel of few)
+    if (p.many && n_seqs == 1 && T == max_new) p.few_rows = 0;
+    p.few = p.few_rows ? chunk_few_plan(n_seqs, max_new, max_context, Hkv, window, p.few_rows, D) : FewPlan{0, 0, 0};
+    p.bytes = p.few.bytes;
+    return p;
+}
+}  // namespace
 
 }  // namespace jsm
 
 using namespace jsm;
 
-extern "C" size_t jsm_attn_chunk_scratch_bytes(int n_seqs, int T, int max_new, int max_context, int Hq, int Hkv, int D) { return 0; }
+extern "C" size_t jsm_attn_chunk_scratch_bytes(int n_seqs, int T, int max_new, int max_context, int Hq, int Hkv, int D, int window) {
+    if (n_seqs <= 0 || T <= 0 || max_new <= 0 || max_context < max_new || Hkv <= 0 || Hq <= 0 || Hq % Hkv || (D != 64 && D != 128) || window < 0) return 0;
+    return plan_of(n_seqs, T, max_new, max_context, Hkv, Hq / Hkv, D, window).bytes;
+}
 
 extern "C" jsm_status jsm_attn_chunk(const void* d_q, int64_t q_row_stride, const void* d_pool, const void* d_scales, int n_pages, const int32_t* d_block_table,
                                      int max_pages, const int32_t* d_starts, const int32_t* d_context_lens, int n_seqs, int T, int max_new, int max_context, int Hq,
@@ -44,6 +68,7 @@ extern "C" jsm_status jsm_attn_chunk(const void* d_q, int64_t q_row_stride, cons
     if (s != JSM_OK) return s;
     if (D != 64 && D != 128) JSM_FAIL(JSM_UNSUPPORTED, "jsm_attn_chunk: head_dim %d (64 or 128)", D);
     if (Hq <= 0 || Hq % Hkv) JSM_FAIL(JSM_SHAPE, "d_model must be divisible by num_heads (Hq %d, Hkv %d)", Hq, Hkv);
+    if (Hq > 65535) JSM_FAIL(JSM_UNSUPPORTED, "jsm_attn_chunk: %d query heads", Hq);
     if (Hq / Hkv > 128) JSM_FAIL(JSM_UNSUPPORTED, "jsm_attn_chunk: %d query heads per kv head (up to 128)", Hq / Hkv);
     if (window < 0) JSM_FAIL(JSM_INVALID_ARG, "jsm_attn_chunk: window %d", window);
     if (!(scale > 0.0f) || scale > 1e30f) JSM_FAIL(JSM_UNSUPPORTED, "jsm_attn_chunk: the softmax scale (%g) must be positive", (double)scale);
@@ -60,6 +85,13 @@ extern "C" jsm_status jsm_attn_chunk(const void* d_q, int64_t q_row_stride, cons
     a.Hq = Hq; a.G = Hq / Hkv; a.window = window;
     a.scale_log2 = scale * 1.4426950408889634f;
     const cudaStream_t st = as_stream(stream);
-    if (D == 64) return d_scales ? chunk_rows_launch<64, true>(a, st) : chunk_rows_launch<64, false>(a, st);
-    return d_scales ? chunk_rows_launch<128, true>(a, st) : chunk_rows_launch<128, false>(a, st);
+    const Plan p = plan_of(n_seqs, T, max_new, max_context, Hkv, a.G, D, window);
+    if (p.bytes && (!d_scratch || scratch_bytes < p.bytes || (reinterpret_cast<uintptr_t>(d_scratch) & 15)))
+        JSM_FAIL(JSM_INVALID_ARG, "jsm_attn_chunk: %zu bytes of scratch (16-byte aligned), %zu are needed", d_scratch ? scratch_bytes : 0, p.bytes);
+    if (p.many) {
+        const jsm_status m = D == 64 ? (d_scales ? chunk_rows_launch<64, true>(a, p.few_rows, st) : chunk_rows_launch<64, false>(a, p.few_rows, st))
+                                     : (d_scales ? chunk_rows_launch<128, true>(a, p.few_rows, st) : chunk_rows_launch<128, false>(a, p.few_rows, st));
+        if (m != JSM_OK) return m;
+    }
+    return p.few_rows ? chunk_few_launch(a, p.few, p.few_rows, d_scratch, st) : JSM_OK;
 }

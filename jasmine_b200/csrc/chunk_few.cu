@@ -1,0 +1,475 @@
+// Attention of a few new tokens of each sequence over a paged cache (bf16 or 8-bit): single tokens, drafts being verified.  Up to 16 rows of queries
+// (tokens x query heads of a kv head) share every cached byte, so the kernel is bound by the bytes of the cache.
+//
+// A CTA has a run of pages of one (sequence, kv head): a producer thread keeps a ring of pages in flight (TMA boxes in the 128-byte swizzle, the scales of an
+// 8-bit page by bulk copies), four warps have 16 keys of each page:
+//   scores, transposed:   S^T[16 keys x 8 rows] = K[16 x D] . Q^T,  keys as the 16-row operand of mma.m16n8k16, so that no row of it is padding
+//   softmax over the keys: running maximum and sum per warp, base 2
+//   O^T[D x 8 rows]     += V^T[D x 16 keys] . P^T
+// bf16 pages come into the operands by ldmatrix.  Numbers of an 8-bit page are taken from shared memory in 16-byte pieces and become bf16 in registers: which
+// component an element of an operand stands for is free as long as both operands agree, so the pieces of a thread are the components that its operand
+// registers need, and the transposition of V costs no instruction beyond the byte permutation that spreads the numbers anyway.
+//   n (a byte) -> bf16: 0x4300 | low seven bits is 128 + them, 0x4300 | sign bit is 128 or 256; their difference is n, exactly.  Times the scale, one rounding.
+// Partial results of the runs meet in chunk_merge_kernel, in the order of the runs.
+// A row whose result is not a number is worked out again over exactly its own keys (attend_row): a weight of zero times what a hidden key holds is no zero then.
+#include "chunk_attn.cuh"
+#include "tc_utils.cuh"
+#include "mma_utils.cuh"
+#include <math.h>
+#include <algorithm>
+
+namespace jsm {
+
+using namespace tc;
+
+constexpr int CF_WARPS = 4;
+constexpr int CF_THREADS = (CF_WARPS + 1) * 32;
+constexpr int CF_ERR_FULL = 43, CF_ERR_EMPTY = 44;
+
+__device__ __forceinline__ uint32_t cf_trans(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+// two numbers, in the low bytes of the halves of p, as bf16
+__device__ __forceinline__ uint32_t q8_pair(uint32_t p) {
+    const uint32_t lo = (p & 0x007F007Fu) | 0x43004300u, hi = (p & 0x00800080u) | 0x43004300u;
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&hi));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+template <int D, bool Q8>
+struct FewSizes {
+    static constexpr int TILE = JSM_PAGE_SIZE * D * (Q8 ? 1 : 2);     // keys, or values, of a page
+    static constexpr int STAGE = 2 * TILE + (Q8 ? 1024 : 0);          // keys | values | scales of both (1024-byte steps: the swizzle counts from there)
+    static constexpr int STAGES = 3;
+    static constexpr int SMEM = STAGES * STAGE + 1024;
+};
+
+template <int D, int NT, bool Q8>
+__global__ void __launch_bounds__(CF_THREADS) chunk_few_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ ChunkArgs a, int few_rows, int n_runs, int run_pages,
+                                                               float* __restrict__ part) {
+    using Z = FewSizes<D, Q8>;
+    constexpr int KS = D / 16;  // steps of 16 components; tiles of 16 components of O^T
+    extern __shared__ uint8_t cf_dyn[];
+    uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(cf_dyn) + 1023) & ~uintptr_t(1023));
+    __shared__ uint64_t full_bar[Z::STAGES], empty_bar[Z::STAGES];
+    __shared__ int abort_flag;
+    __shared__ float sm_m[CF_WARPS][NT * 8], sm_l[CF_WARPS][NT * 8];
+    chain_trigger();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < Z::STAGES; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&empty_bar[s], CF_WARPS);
+        }
+        abort_flag = 0;
+        mbar_fence_init();
+    }
+    __syncthreads();
+    chain_wait();
+    const int run = blockIdx.x % n_runs, seq = blockIdx.x / n_runs, hk = blockIdx.y;
+    int row0, n_new, ctx;
+    if (!chunk_lengths(a, seq, row0, n_new, ctx) || n_new * a.G > few_rows) return;
+    const int rows = n_new * a.G;
+    const int lo = first_key(a.window, ctx - n_new);  // no row sees a key before it
+    const int page0 = lo / JSM_PAGE_SIZE, n_pages = (ctx - 1) / JSM_PAGE_SIZE + 1 - page0;
+    const int p_begin = run * run_pages, p_end = min(n_pages, p_begin + run_pages);
+    if (p_begin >= p_end) return;
+    const bool whole = n_pages <= run_pages;  // the only run: its result is final
+
+    float m[NT][2], l[NT][2];  // rows (lane % 4) * 2 and + 1 of each tile
+    float o[NT][KS][4];        // O^T
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < KS; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.0f;
+    }
+
+    if (warp == CF_WARPS) {
+        if (lane == 0) {
+            tma_prefetch_desc(&tmap);
+            int issued = 0;
+            for (int p = p_begin; p < p_end; ++p) {
+                const int it = p - p_begin, s = it % Z::STAGES;
+                if (it >= Z::STAGES && !mbar_wait(&empty_bar[s], ((it / Z::STAGES) - 1) & 1, &abort_flag, a.c.err, CF_ERR_EMPTY)) break;
+                const int page = cache_page(a.c, seq, (page0 + p) * JSM_PAGE_SIZE);
+                uint8_t* dst = stages + s * Z::STAGE;
+                // (a page outside the pool: rows before the first one, which read as zeros)
+                const int rk = page < 0 ? -JSM_PAGE_SIZE : (int)cache_row(a.c, page, 0, hk, 0), rv = page < 0 ? -JSM_PAGE_SIZE : (int)cache_row(a.c, page, 1, hk, 0);
+                if constexpr (Q8) {
+                    mbar_expect_tx(&full_bar[s], 2 * Z::TILE + (page < 0 ? 0 : 256));
+                    tma_load_2d(dst, &tmap, 0, D == 64 ? rk / 2 : rk, &full_bar[s]);  // (heads of 64: a line of 128 bytes has two positions)
+                    tma_load_2d(dst + Z::TILE, &tmap, 0, D == 64 ? rv / 2 : rv, &full_bar[s]);
+                    if (page >= 0) {
+                        bulk_load(dst + 2 * Z::TILE, a.c.scales + rk, 128, &full_bar[s]);
+                        bulk_load(dst + 2 * Z::TILE + 128, a.c.scales + rv, 128, &full_bar[s]);
+                    }
+                } else {
+                    mbar_expect_tx(&full_bar[s], 2 * Z::TILE);
+#pragma unroll
+                    for (int c = 0; c < D / 64; ++c) {
+                        tma_load_2d(dst + c * 8192, &tmap, c * 64, rk, &full_bar[s]);
+                        tma_load_2d(dst + Z::TILE + c * 8192, &tmap, c * 64, rv, &full_bar[s]);
+                    }
+                }
+                issued = it + 1;
+            }
+            if (abort_flag) {  // let the copies in flight land before the CTA exits (bounded)
+                const long long t0 = clock64();
+                for (int it = max(0, issued - Z::STAGES); it < issued; ++it)
+                    while (!mbar_try_wait(&full_bar[it % Z::STAGES], (it / Z::STAGES) & 1) && clock64() - t0 < WAIT_LIMIT_CYCLES) {}
+            }
+        }
+    } else {
+        const int g = lane >> 2, t4 = lane & 3;
+        // B operand of the scores: row n * 8 + g, components of thread t4 in each step
+        uint32_t qb[NT][KS][2];
+        int last[NT][2], first[NT][2];  // keys that the thread's two columns of each tile see
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = n * 8 + g;
+            const __nv_bfloat16* qp = a.q + (row0 + r / a.G) * a.q_rs + (long long)(hk * a.G + r % a.G) * D;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if constexpr (Q8) {
+                    const uint2 w = r < rows ? *reinterpret_cast<const uint2*>(qp + (D / 4) * t4 + 4 * ks) : make_uint2(0, 0);
+                    qb[n][ks][0] = w.x;
+                    qb[n][ks][1] = w.y;
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) qb[n][ks][h] = r < rows ? *reinterpret_cast<const uint32_t*>(qp + ks * 16 + h * 8 + t4 * 2) : 0u;
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int pos = ctx - n_new + min(n * 8 + t4 * 2 + h, rows - 1) / a.G;
+                last[n][h] = pos;
+                first[n][h] = first_key(a.window, pos);
+            }
+        }
+        const int all_from = first_key(a.window, ctx - 1), all_to = ctx - n_new;  // keys that every row sees
+        const int mi = lane >> 3, mr = lane & 7;
+        const int krow = warp * 16 + (mi & 1) * 8 + mr, kchunk = mi >> 1;   // ldmatrix, keys
+        const int vrow = warp * 16 + (mi >> 1) * 8 + mr, vchunk = mi & 1;   // ldmatrix, values transposed
+        for (int p = p_begin; p < p_end; ++p) {
+            const int it = p - p_begin, s = it % Z::STAGES;
+            if (!mbar_wait(&full_bar[s], (it / Z::STAGES) & 1, &abort_flag, a.c.err, CF_ERR_FULL)) break;
+            uint8_t* stage = stages + s * Z::STAGE;
+            const int key0 = (page0 + p) * JSM_PAGE_SIZE + warp * 16;
+            if (key0 < ctx && key0 + 16 > lo) {
+                const bool edge = key0 < lo || key0 + 16 > ctx;
+                if (!Q8 && edge) {  // values that no row sees: a weight of zero meets a number
+                    uint8_t* vb = stage + Z::TILE;
+                    for (int i = lane; i < 16 * (D / 8); i += 32) {
+                        const int row = warp * 16 + i / (D / 8), c = i % (D / 8), key = key0 + i / (D / 8);
+                        if (key < lo || key >= ctx) *reinterpret_cast<uint4*>(vb + (c >> 3) * 8192 + row * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();  // the stage is overwritten by a bulk copy later
+                    __syncwarp();
+                }
+                float sc[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
+                if constexpr (Q8) {
+                    const uint16_t* scales = reinterpret_cast<const uint16_t*>(stage + 2 * Z::TILE);
+                    uint32_t kw[2][D / 16];  // D / 4 numbers of keys g and g + 8
+                    uint32_t ks2[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int key = warp * 16 + g + h * 8;
+                        ks2[h] = scales[key] * 0x00010001u;
+#pragma unroll
+                        for (int c = 0; c < D / 64; ++c) {
+                            const int byte = key * D + (D / 4) * t4 + c * 16, line = byte >> 7;
+                            const uint4 w = *reinterpret_cast<const uint4*>(stage + line * 128 + ((((byte >> 4) & 7) ^ (line & 7)) << 4));
+                            kw[h][c * 4] = w.x; kw[h][c * 4 + 1] = w.y; kw[h][c * 4 + 2] = w.z; kw[h][c * 4 + 3] = w.w;
+                        }
+                    }
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        uint32_t f[4];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            f[h] = mul_bf16x2(q8_pair(__byte_perm(kw[h][ks], 0, 0x1100)), ks2[h]);
+                            f[h + 2] = mul_bf16x2(q8_pair(__byte_perm(kw[h][ks], 0, 0x3322)), ks2[h]);
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma_16816(sc[n], f, qb[n][ks][0], qb[n][ks][1]);
+                    }
+                } else {
+                    const uint32_t kbase = smem_u32(stage);
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        const int c = ks * 2 + kchunk;
+                        uint32_t f[4];
+                        ldsm_x4(kbase + (c >> 3) * 8192 + krow * 128 + (((c & 7) ^ (krow & 7)) << 4), f);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma_16816(sc[n], f, qb[n][ks][0], qb[n][ks][1]);
+                    }
+                }
+                // sc[n][0], [1]: key g, the thread's two rows; [2], [3]: key g + 8
+                const bool plain = key0 >= all_from && key0 + 15 <= all_to;
+                uint32_t pb[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float x[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x[i] = sc[n][i] * a.scale_log2;
+                        const int key = key0 + g + (i >> 1) * 8;
+                        if (!plain && (key < first[n][i & 1] || key > last[n][i & 1])) x[i] = -INFINITY;
+                    }
+                    float corr[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float mx = fmaxf(x[h], x[h + 2]);
+#pragma unroll
+                        for (int sh = 4; sh < 32; sh <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
+                        const float mn = fmaxf(m[n][h], mx), ref = mn == -INFINITY ? 0.0f : mn;  // (nothing seen so far: weights of 0)
+                        corr[h] = exp2f(m[n][h] - ref);
+                        m[n][h] = mn;
+                        x[h] = exp2f(x[h] - ref);
+                        x[h + 2] = exp2f(x[h + 2] - ref);
+                        l[n][h] = fmaf(l[n][h], corr[h], x[h] + x[h + 2]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < KS; ++j) {
+                        o[n][j][0] *= corr[0];
+                        o[n][j][1] *= corr[1];
+                        o[n][j][2] *= corr[0];
+                        o[n][j][3] *= corr[1];
+                    }
+                    pb[n][0] = cf_trans(pack_bf16x2(x[0], x[1]));
+                    pb[n][1] = cf_trans(pack_bf16x2(x[2], x[3]));
+                }
+                if constexpr (Q8) {
+                    const uint16_t* scales = reinterpret_cast<const uint16_t*>(stage + 2 * Z::TILE + 128);
+                    uint32_t vw[4][D / 32], vs[2];  // D / 8 numbers of keys 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9: components (D / 8) g and up
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int k2 = warp * 16 + t4 * 2 + h * 8, key = key0 + t4 * 2 + h * 8;
+                        vs[h] = *reinterpret_cast<const uint32_t*>(scales + k2);
+                        if (edge) {
+                            if (key < lo || key >= ctx) vs[h] &= 0xFFFF0000u;
+                            if (key + 1 < lo || key + 1 >= ctx) vs[h] &= 0x0000FFFFu;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int byte = (k2 + i) * D + (D / 8) * g, line = byte >> 7;
+                            const uint8_t* at = stage + Z::TILE + line * 128 + ((((byte >> 4) & 7) ^ (line & 7)) << 4);
+                            if constexpr (D == 128) {
+                                const uint4 w = *reinterpret_cast<const uint4*>(at);
+                                vw[h * 2 + i][0] = w.x; vw[h * 2 + i][1] = w.y; vw[h * 2 + i][2] = w.z; vw[h * 2 + i][3] = w.w;
+                            } else {
+                                const uint2 w = *reinterpret_cast<const uint2*>(at + (byte & 8));
+                                vw[h * 2 + i][0] = w.x; vw[h * 2 + i][1] = w.y;
+                            }
+                        }
+                    }
+                    // tile j: components (D / 8) g + 2 j (the tile's row g) and + 1 (its row g + 8)
+#pragma unroll
+                    for (int j = 0; j < KS; ++j) {
+                        uint32_t f[4];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t w0 = vw[h * 2][j >> 1], w1 = vw[h * 2 + 1][j >> 1];
+                            f[h * 2] = mul_bf16x2(q8_pair(__byte_perm(w0, w1, j & 1 ? 0x6622 : 0x4400)), vs[h]);
+                            f[h * 2 + 1] = mul_bf16x2(q8_pair(__byte_perm(w0, w1, j & 1 ? 0x7733 : 0x5511)), vs[h]);
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma_16816(o[n][j], f, pb[n][0], pb[n][1]);
+                    }
+                } else {
+                    const uint32_t vbase = smem_u32(stage + Z::TILE);
+#pragma unroll
+                    for (int j = 0; j < KS; ++j) {
+                        const int c = j * 2 + vchunk;
+                        uint32_t f[4];
+                        ldsm_x4_trans(vbase + (c >> 3) * 8192 + vrow * 128 + (((c & 7) ^ (vrow & 7)) << 4), f);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma_16816(o[n][j], f, pb[n][0], pb[n][1]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty_bar[s]);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int sh = 4; sh < 32; sh <<= 1) l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], sh);
+    }
+    __syncthreads();
+    if (abort_flag) return;  // (the error is recorded)
+    // every stage has been consumed: the ring becomes [warp][row][component]
+    float* sm_o = reinterpret_cast<float*>(stages);
+    if (warp < CF_WARPS) {
+        const int g = lane >> 2, t4 = lane & 3;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = n * 8 + t4 * 2 + h;
+                float* dst = sm_o + (warp * NT * 8 + r) * D;
+#pragma unroll
+                for (int j = 0; j < KS; ++j) {
+                    dst[Q8 ? (D / 8) * g + 2 * j : j * 16 + g] = o[n][j][h];
+                    dst[Q8 ? (D / 8) * g + 2 * j + 1 : j * 16 + g + 8] = o[n][j][h + 2];
+                }
+                if (g == 0) {
+                    sm_m[warp][r] = m[n][h];
+                    sm_l[warp][r] = l[n][h];
+                }
+            }
+    }
+    __syncthreads();
+    // a warp per row: the four warps' sums under their largest maximum
+    constexpr int N = D / 32;
+    for (int r = warp; r < rows; r += CF_WARPS + 1) {
+        float M = -INFINITY, L = 0.0f, acc[N];
+#pragma unroll
+        for (int w = 0; w < CF_WARPS; ++w) M = fmaxf(M, sm_m[w][r]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < CF_WARPS; ++w) {
+            // a warp that saw no key has sums of zero, or (NaN scores leave no maximum) what is to be handed on
+            const float f = sm_m[w][r] == -INFINITY ? 1.0f : exp2f(sm_m[w][r] - M);
+            L += f * sm_l[w][r];
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] += f * sm_o[(w * NT * 8 + r) * D + lane * N + i];
+        }
+        const int row = row0 + r / a.G, head = hk * a.G + r % a.G;
+        if (whole) {
+            bool fine = true;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                acc[i] /= L;
+                fine = fine && fabsf(acc[i]) <= 3.402823466e38f;
+            }
+            if (__all_sync(0xffffffffu, fine)) {
+                __nv_bfloat16* dst = a.out + row * a.out_rs + (long long)head * D + lane * N;
+#pragma unroll
+                for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16x2(acc[i], acc[i + 1]);
+            } else {
+                attend_row<D, Q8>(a, seq, row, head, ctx - n_new + r / a.G);
+            }
+        } else {
+            float* dst = part + (((long long)seq * a.c.Hkv + hk) * n_runs + run) * (few_rows * (D + 2)) + r * (D + 2);
+#pragma unroll
+            for (int i = 0; i < N; i += 2) *reinterpret_cast<float2*>(dst + lane * N + i) = make_float2(acc[i], acc[i + 1]);
+            if (lane == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(M, L);
+        }
+    }
+}
+
+// The runs of a (row, head) under their largest maximum, in the order of the runs; a warp each.
+template <int D, bool Q8>
+__global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant__ ChunkArgs a, int few_rows, int n_runs, int run_pages, const float* __restrict__ part) {
+    constexpr int N = D / 32;
+    __shared__ int found;
+    chain_trigger();
+    chain_wait();
+    const int t = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int s = find_sequence(a.c, t, &found);
+    if (s < 0 || head >= a.Hq) return;
+    int row0, n_new, ctx;
+    if (!chunk_lengths(a, s, row0, n_new, ctx) || n_new * a.G > few_rows) return;
+    const int n_pages = (ctx - 1) / JSM_PAGE_SIZE + 1 - first_key(a.window, ctx - n_new) / JSM_PAGE_SIZE, n = (n_pages + run_pages - 1) / run_pages;
+    if (n == 1) return;
+    const int hk = head / a.G, r = (t - row0) * a.G + head % a.G;
+    const float* src = part + ((long long)s * a.c.Hkv + hk) * n_runs * (few_rows * (D + 2)) + r * (D + 2);
+    const int step = few_rows * (D + 2);
+    float M = -INFINITY, L = 0.0f, acc[N];
+    for (int c = lane; c < n; c += 32) M = fmaxf(M, src[(long long)c * step + D]);
+    M = warp_max(M);
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+    for (int c0 = 0; c0 < n; c0 += 32) {
+        float f = 0.0f, lc = 0.0f;
+        if (c0 + lane < n) {
+            const float2 ml = *reinterpret_cast<const float2*>(src + (long long)(c0 + lane) * step + D);
+            f = ml.x == -INFINITY ? 1.0f : exp2f(ml.x - M);
+            lc = f * ml.y;
+        }
+        L += warp_sum(lc);
+        const int k = min(32, n - c0);
+#pragma unroll 8
+        for (int c = 0; c < k; ++c) {
+            const float w = __shfl_sync(0xffffffffu, f, c);
+            const float* x = src + (long long)(c0 + c) * step + lane * N;
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
+                const float2 v = *reinterpret_cast<const float2*>(x + i);
+                acc[i] = fmaf(w, v.x, acc[i]);
+                acc[i + 1] = fmaf(w, v.y, acc[i + 1]);
+            }
+        }
+    }
+    bool fine = true;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        acc[i] /= L;
+        fine = fine && fabsf(acc[i]) <= 3.402823466e38f;
+    }
+    if (!__all_sync(0xffffffffu, fine)) {
+        attend_row<D, Q8>(a, s, t, head, ctx - n_new + t - row0);
+        return;
+    }
+    __nv_bfloat16* dst = a.out + t * a.out_rs + (long long)head * D + lane * N;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16x2(acc[i], acc[i + 1]);
+}
+
+// Pages of a run: enough CTAs to fill the chip's slots (four per SM), runs of up to eight pages so that long contexts even out.
+FewPlan chunk_few_plan(int n_seqs, int max_new, int max_context, int Hkv, int window, int few_rows, int D) {
+    long long pages = (max_context + JSM_PAGE_SIZE - 1) / JSM_PAGE_SIZE;
+    if (window > 0) pages = std::min(pages, ((long long)window + max_new + JSM_PAGE_SIZE - 3) / JSM_PAGE_SIZE + 1);
+    FewPlan f;
+    const long long slots = 4ll * sm_count(), all = pages * n_seqs * Hkv;
+    f.run_pages = (int)std::min(8ll, std::max(1ll, (all + slots - 1) / slots));
+    f.n_runs = (int)((pages + f.run_pages - 1) / f.run_pages);
+    f.bytes = f.n_runs > 1 ? (size_t)n_seqs * Hkv * f.n_runs * few_rows * (D + 2) * sizeof(float) : 0;
+    return f;
+}
+
+template <int D, int NT, bool Q8>
+static jsm_status few_go(const ChunkArgs& a, const FewPlan& f, float* part, cudaStream_t st) {
+    using Z = FewSizes<D, Q8>;
+    CUtensorMap map;
+    const uint64_t rows = (uint64_t)a.c.n_pages * 2 * a.c.Hkv * JSM_PAGE_SIZE;
+    const jsm_status s = Q8 ? make_tmap_u8_lines(&map, a.c.pool, rows * D / 128, JSM_PAGE_SIZE * D / 128)
+                            : make_tmap_bf16_2d(&map, a.c.pool, rows, D, D, JSM_PAGE_SIZE, 64);
+    if (s != JSM_OK) return s;
+    static DeviceOnce once;
+    JSM_CUDA_CHECK(allow_shared(once, chunk_few_kernel<D, NT, Q8>, Z::SMEM));
+    JSM_CUDA_CHECK(launch_chained(chunk_few_kernel<D, NT, Q8>, dim3((unsigned)f.n_runs * a.c.n_seqs, a.c.Hkv), dim3(CF_THREADS), (size_t)Z::SMEM, st, map, a, NT * 8, f.n_runs,
+                                  f.run_pages, part));
+    JSM_LAUNCH_CHECK();
+    if (f.n_runs > 1) {
+        JSM_CUDA_CHECK(launch_chained(chunk_merge_kernel<D, Q8>, dim3(a.T, (a.Hq + 3) / 4), dim3(128), 0, st, a, NT * 8, f.n_runs, f.run_pages, (const float*)part));
+        JSM_LAUNCH_CHECK();
+    }
+    return JSM_OK;
+}
+
+jsm_status chunk_few_launch(const ChunkArgs& a, const FewPlan& f, int few_rows, void* scratch, cudaStream_t st) {
+    float* part = static_cast<float*>(scratch);
+    if (a.c.D == 64) {
+        if (a.c.scales) return few_rows == 8 ? few_go<64, 1, true>(a, f, part, st) : few_go<64, 2, true>(a, f, part, st);
+        return few_rows == 8 ? few_go<64, 1, false>(a, f, part, st) : few_go<64, 2, false>(a, f, part, st);
+    }
+    if (a.c.scales) return few_rows == 8 ? few_go<128, 1, true>(a, f, part, st) : few_go<128, 2, true>(a, f, part, st);
+    return few_rows == 8 ? few_go<128, 1, false>(a, f, part, st) : few_go<128, 2, false>(a, f, part, st);
+}
+
+}  // namespace jsm

@@ -72,6 +72,20 @@ jsm_status make_tmap_bf16_3d(CUtensorMap* map, const void* base, uint64_t d0, ui
     return JSM_OK;
 }
 
+jsm_status make_tmap_u8_lines(CUtensorMap* map, const void* base, uint64_t lines, uint32_t box_lines) {
+    encode_tiled_fn enc = get_encode();
+    if (!enc) JSM_FAIL(JSM_CUDA, "cuTensorMapEncodeTiled is not available (no CUDA driver)");
+    if (reinterpret_cast<uintptr_t>(base) & 15) JSM_FAIL(JSM_INVALID_ARG, "TMA operand must be 16-byte aligned");
+    cuuint64_t dims[2] = {128, lines};
+    cuuint64_t strides[1] = {128};
+    cuuint32_t box[2] = {128, box_lines};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) JSM_FAIL(JSM_CUDA, "cuTensorMapEncodeTiled failed with %d (%llu lines)", (int)r, (unsigned long long)lines);
+    return JSM_OK;
+}
+
 int* tc_error_word() {
     static int* words[64] = {nullptr};
     int dev = 0;

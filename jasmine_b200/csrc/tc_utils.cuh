@@ -224,6 +224,8 @@ jsm_status make_tmap_bf16_2d(CUtensorMap* map, const void* base, uint64_t rows, 
 // bf16 [d2, d1, d0] tensor with element strides (s2, s1, 1)
 jsm_status make_tmap_bf16_3d(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t s1_elems,
                              uint64_t s2_elems, uint32_t b0, uint32_t b1, uint32_t b2);
+// int8 memory as lines of 128 bytes, box = box_lines lines, 128-byte swizzle
+jsm_status make_tmap_u8_lines(CUtensorMap* map, const void* base, uint64_t lines, uint32_t box_lines);
 // device error word shared by the tensor-core kernels (one per device)
 int* tc_error_word();
 

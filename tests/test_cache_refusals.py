@@ -126,4 +126,5 @@ def test_scratch_of_arguments_that_cannot_be_right():
     f.restype = C.c_size_t
     for a in ((0, 3, 1, 64, 4, 2, 128), (2, 0, 1, 64, 4, 2, 128), (2, 3, 1, 64, 5, 2, 128), (2, 3, 0, 64, 4, 2, 128), (2, 3, 1, 0, 4, 2, 128), (2, 3, 1, 64, 4, 0, 128),
               (2, 3, 1, 64, 4, 2, 96)):
-        assert f(*a) == 0
+        assert f(*a, 0) == 0
+    assert f(2, 3, 1, 64, 4, 2, 128, -1) == 0
