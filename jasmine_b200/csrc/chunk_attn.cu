@@ -1,4 +1,4 @@
-// Attention of new tokens over a paged cache, bf16 or 8-bit: entry points and kernels.
+// Attention of new tokens over a paged cache, bf16 or 8-bit: entry points, and which kernel takes which sequence.
 #include "chunk_attn.cuh"
 #include <math.h>
 
@@ -6,27 +6,6 @@ namespace jsm {
 
 jsm_status cache_view_check(const char* who, CacheView& c, void* pool, void* scales, int n_pages, const int32_t* table, int max_pages, const int32_t* starts,
                             const int32_t* context_lens, int n_seqs, int T, int Hkv, int D);
-
-// a warp per (row, query head)
-template <int D, bool Q8>
-__global__ void __launch_bounds__(128) chunk_rows_kernel(const __grid_constant__ ChunkArgs a, int few_rows) {
-    __shared__ int found;
-    chain_trigger();
-    chain_wait();
-    const int t = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5);
-    const int s = find_sequence(a.c, t, &found);
-    if (s < 0 || head >= a.Hq) return;
-    int first, n_new, ctx;
-    if (!chunk_lengths(a, s, first, n_new, ctx) || n_new * a.G <= few_rows) return;
-    attend_row<D, Q8>(a, s, t, head, ctx - n_new + t - first);
-}
-
-template <int D, bool Q8>
-static jsm_status chunk_rows_launch(const ChunkArgs& a, int few_rows, cudaStream_t st) {
-    JSM_CUDA_CHECK(launch_chained(chunk_rows_kernel<D, Q8>, dim3(a.T, (a.Hq + 3) / 4), dim3(128), 0, st, a, few_rows));
-    JSM_LAUNCH_CHECK();
-    return JSM_OK;
-}
 
 namespace {
 // What runs for a call: sequences of up to few_rows rows of queries per kv head take chunk_few.cu, the others (if there can be any) the other kernel.
@@ -89,8 +68,7 @@ extern "C" jsm_status jsm_attn_chunk(const void* d_q, int64_t q_row_stride, cons
     if (p.bytes && (!d_scratch || scratch_bytes < p.bytes || (reinterpret_cast<uintptr_t>(d_scratch) & 15)))
         JSM_FAIL(JSM_INVALID_ARG, "jsm_attn_chunk: %zu bytes of scratch (16-byte aligned), %zu are needed", d_scratch ? scratch_bytes : 0, p.bytes);
     if (p.many) {
-        const jsm_status m = D == 64 ? (d_scales ? chunk_rows_launch<64, true>(a, p.few_rows, st) : chunk_rows_launch<64, false>(a, p.few_rows, st))
-                                     : (d_scales ? chunk_rows_launch<128, true>(a, p.few_rows, st) : chunk_rows_launch<128, false>(a, p.few_rows, st));
+        const jsm_status m = chunk_flash_launch(a, p.few_rows, st);
         if (m != JSM_OK) return m;
     }
     return p.few_rows ? chunk_few_launch(a, p.few, p.few_rows, d_scratch, st) : JSM_OK;

@@ -24,6 +24,9 @@ FewPlan chunk_few_plan(int n_seqs, int max_new, int max_context, int Hkv, int wi
 // sequences of up to few_rows (8 or 16) rows of queries per kv head; the others are left to another kernel
 jsm_status chunk_few_launch(const ChunkArgs& a, const FewPlan& f, int few_rows, void* scratch, cudaStream_t st);
 
+// sequences of more than few_rows rows
+jsm_status chunk_flash_launch(const ChunkArgs& a, int few_rows, cudaStream_t st);
+
 #ifdef __CUDACC__
 // lengths of a sequence that the kernels may rely on; false: no new tokens, or lengths that do not fit (an error)
 __device__ __forceinline__ bool chunk_lengths(const ChunkArgs& a, int s, int& first_row, int& n_new, int& ctx) {

@@ -1,0 +1,714 @@
+// Attention of many new tokens of a sequence over its paged cache, bf16 or 8-bit, on the 5th-generation tensor cores (tcgen05 + TMEM).
+//
+// The query rows of a kv head's group are one matrix, token after token, head after head within a token (row = token * G + head): a short portion of grouped
+// queries fills the 128 rows of a tensor-core tile, and a key tile is fetched once for the whole group.  A CTA owns two such tiles of one (sequence, kv head)
+// and walks the keys of its pages in tiles of 128 (two pages), as flash_attn.cu does: scores one key tile ahead of the products with V, the softmax of one
+// query tile beside the tensor work of the other, the accumulator rescaled only where the maximum grew by 2^8, a quarter of the exponentials on the FMA pipe.
+//   warp 0        copies: Q once (a box of tokens x heads x 64 components), key and value pages through rings
+//   warp 1        issues the products: S_t = Q_t K^T, O_t += P_t V (P_t in TMEM over the first half of S_t)
+//   warps 4-11    softmax, one thread per query row; register shares moved here from warps 0-3 (setmaxnreg)
+//   warps 12-15   8-bit caches: numbers of a raw page -> bf16(n * scale) in the swizzled tiles that the tensor cores read.  Every number is exact in bf16 and every product
+//                 rounded once, so scores and sums are those of a bf16 cache of these values; the conversion is spread over the whole group's rows
+// Few tiles and long contexts: the CTAs of a cluster share the key tiles of one pair of query tiles and meet in shared memory (each then joins its share of the rows, in
+// the order of the ranks), so that nothing goes through global memory and no second launch is needed.
+// Values that no row of the CTA sees (behind the context, before the window) become zeros before they are multiplied; a row whose result is not a number is worked out
+// again over exactly its own keys (attend_row).  Every wait is bounded.
+#include "chunk_attn.cuh"
+#include "tc_utils.cuh"
+#include "softmax_rows.cuh"
+#include "mma_utils.cuh"
+#include <math.h>
+#include <algorithm>
+#include <mutex>
+
+namespace jsm {
+
+using namespace tc;
+
+constexpr int CK_BM = 128, CK_BN = 128;
+constexpr int CK_SOFTMAX = 4, CK_CONVERT = 12;  // first warp of a role
+constexpr float CK_RESCALE = 8.0f;
+constexpr float CK_NONE = -1.0e30f;             // the maximum of a row that has seen nothing
+
+template <int D, bool Q8>
+struct FlashSizes {
+    static constexpr int THREADS = Q8 ? 512 : 384;
+    static constexpr uint32_t SLAB = CK_BM * 64 * 2;                          // 64 columns of a tile
+    static constexpr uint32_t TILE = D / 64 * SLAB;                           // 128 rows of Q, K or V
+    static constexpr int ST = 2;
+    static constexpr uint32_t RAW = Q8 ? JSM_PAGE_SIZE * D : 0;               // an 8-bit page of keys or values
+    static constexpr uint32_t SMEM = (2 + 2 * ST) * TILE + 4 * RAW + 1024;    // Q | K ring | V ring | raw pages: keys 0, keys 1, values 0, values 1
+};
+
+struct FlashArgs {
+    ChunkArgs a;
+    int few_rows;      // sequences of so many rows are another kernel's
+    int tile_tokens;   // tokens of a query tile
+    int slots;         // pairs of query tiles, at most
+    int share;         // CTAs (a cluster) of one pair of query tiles and kv head
+};
+
+__device__ __forceinline__ void ck_cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void ck_cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ uint32_t ck_peer(uint32_t local, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float2 ck_load2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ck_load4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// The slot-th pair of query tiles: its sequence and its number there; a whole warp.  False: there are fewer.
+__device__ __forceinline__ bool find_tile(const FlashArgs& f, int slot, int& seq, int& tile, int& n_tiles) {
+    const ChunkArgs& a = f.a;
+    const int lane = threadIdx.x & 31, tokens = 2 * f.tile_tokens;
+    for (int s0 = 0; s0 < a.c.n_seqs; s0 += 32) {
+        const int s = s0 + lane;
+        int n = 0;
+        if (s < a.c.n_seqs) {
+            const int from = a.c.starts[s], n_new = a.c.starts[s + 1] - from;
+            if (n_new > a.max_new || from < 0 || from + (long long)n_new > a.T) cache_error(a.c.err, CACHE_BAD_LENGTH);
+            else if (n_new > 0 && n_new * a.G > f.few_rows) n = (n_new + tokens - 1) / tokens;
+        }
+        int sum = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        const unsigned here = __ballot_sync(0xffffffffu, sum > slot);
+        if (here) {
+            const int w = __ffs(here) - 1;
+            n_tiles = __shfl_sync(0xffffffffu, n, w);
+            tile = slot - (__shfl_sync(0xffffffffu, sum, w) - n_tiles);
+            seq = s0 + w;
+            return true;
+        }
+        slot -= __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return false;
+}
+
+__device__ __forceinline__ uint32_t ck_q8_pair(uint32_t p, uint32_t scale2) {
+    const uint32_t lo = (p & 0x007F007Fu) | 0x43004300u, hi = (p & 0x00800080u) | 0x43004300u;
+    const __nv_bfloat162 n = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&hi));
+    const __nv_bfloat162 r = __hmul2(n, *reinterpret_cast<const __nv_bfloat162*>(&scale2));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+template <int D, bool Q8>
+__global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
+    chunk_flash_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_kv, const __grid_constant__ FlashArgs f) {
+    using Z = FlashSizes<D, Q8>;
+    constexpr int ST = Z::ST, POLY = 1;
+    const ChunkArgs& a = f.a;
+    extern __shared__ uint8_t ck_smem[];
+    uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ck_smem) + 1023) & ~uintptr_t(1023));
+    uint8_t* q_smem = tiles;
+    uint8_t* k_smem = tiles + 2 * Z::TILE;
+    uint8_t* v_smem = k_smem + ST * Z::TILE;
+    uint8_t* raw_smem = v_smem + ST * Z::TILE;
+    // a cluster's meeting, in place of tiles and rings: [256 rows][D] sums, then maximum and sum of the weights of each row
+    float2* sm_ml = reinterpret_cast<float2*>(tiles + 2 * CK_BM * D * 4);
+    __shared__ __align__(8) uint64_t q_full, o_done;
+    __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], raw_full[4], raw_empty[4];
+    __shared__ __align__(8) uint64_t s_full[2], p_ready[2];
+    __shared__ __align__(16) uint16_t raw_scales[4][JSM_PAGE_SIZE];
+    __shared__ uint32_t tmem_base_smem;
+    __shared__ int abort_flag, sh_seq, sh_tile;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    chain_trigger();
+    if (warp == 2 && elect_one()) {
+        abort_flag = 0;
+        mbar_init(&q_full, 1);
+        mbar_init(&o_done, 1);
+        for (int s = 0; s < ST; ++s) {
+            mbar_init(&k_full[s], Q8 ? 4 : 1);
+            mbar_init(&v_full[s], Q8 ? 4 : 1);
+            mbar_init(&k_empty[s], 1);
+            mbar_init(&v_empty[s], 1);
+        }
+        for (int s = 0; s < 4; ++s) { mbar_init(&raw_full[s], 1); mbar_init(&raw_empty[s], 4); }
+        for (int t = 0; t < 2; ++t) { mbar_init(&s_full[t], 1); mbar_init(&p_ready[t], 4); }
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(&tmem_base_smem, 512);
+        tmem_relinquish();
+    }
+    chain_wait();
+    const int part = blockIdx.x % f.share, hk = blockIdx.x / f.share % a.c.Hkv;
+    if (warp == 0) {
+        int seq = -1, tile = 0, n = 0;
+        if (!find_tile(f, blockIdx.x / f.share / a.c.Hkv, seq, tile, n)) seq = -1;
+        if (lane == 0) {
+            sh_seq = seq;
+            sh_tile = n - 1 - tile;  // the last tokens see the most keys: first
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_base_smem;
+    const uint32_t S_COL[2] = {0, 128}, O_COL[2] = {256, 256 + D};
+    const int seq = sh_seq;
+    int row0 = 0, n_new = 0, ctx = 0;
+    const bool work = seq >= 0 && chunk_lengths(a, seq, row0, n_new, ctx);
+
+    // query tile t: tokens tok[t] and up (none: tile empty); key tiles from the page that holds the first key of the first token
+    const int tok[2] = {sh_tile * 2 * f.tile_tokens, (sh_tile * 2 + 1) * f.tile_tokens};
+    const int past = ctx - n_new;
+    const int lo = work ? first_key(a.window, past + tok[0]) : 0;   // no row of the CTA sees a key before it
+    const int base = lo / JSM_PAGE_SIZE * JSM_PAGE_SIZE;
+    int jb[2] = {0, 0}, je[2] = {0, 0};
+    if (work) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+            if (tok[t] < n_new) {
+                jb[t] = (first_key(a.window, past + tok[t]) - base) / CK_BN;
+                je[t] = (past + min(tok[t] + f.tile_tokens, n_new) - 1 - base) / CK_BN + 1;
+            }
+    }
+    int j_lo = jb[0], n_max = max(je[0], je[1]);
+    if (f.share > 1) {  // this CTA's share of the key tiles
+        const int len = (n_max - j_lo + f.share - 1) / f.share, from = j_lo + part * len, to = min(n_max, from + len);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            jb[t] = max(jb[t], from);
+            je[t] = max(jb[t], min(je[t], to));
+        }
+        j_lo = min(from, to);
+        n_max = to;
+    }
+    const int end = work ? past + min(tok[0] + 2 * f.tile_tokens, n_new) : 0;  // keys behind it: no row of the CTA sees them
+
+    if (warp < CK_SOFTMAX) regs_dec<Q8 ? 40 : 56>();
+    if (warp == 0) {
+        if (work && n_max > j_lo) {
+            if (elect_one()) {
+                const uint32_t box = (uint32_t)(f.tile_tokens * a.G) * 128;
+                const int n_q = tok[1] < n_new ? 2 : 1;
+                mbar_expect_tx(&q_full, n_q * (D / 64) * box);
+                for (int t = 0; t < n_q; ++t)
+#pragma unroll
+                    for (int c = 0; c < D / 64; ++c) tma_load_3d(q_smem + t * Z::TILE + c * Z::SLAB, &tmap_q, c * 64, hk * a.G, row0 + tok[t], &q_full);
+            }
+            __syncwarp();
+            // pages of 16 key tiles at a time: lane i has the i-th; behind the context the last page again (hidden keys)
+            const int page0 = base / JSM_PAGE_SIZE, last_page = (end - 1) / JSM_PAGE_SIZE;
+            int pages = 0, k_issued = 0, v_issued = 0;
+            auto page_row = [&](int i, int half, int value) {  // row of the pool where the page of a key tile's half starts
+                const int page = __shfl_sync(0xffffffffu, pages, (2 * i + half) & 31);
+                return page < 0 ? -JSM_PAGE_SIZE : (int)cache_row(a.c, page, value, hk, 0);  // (outside the pool: rows before the first one, zeros)
+            };
+            for (int j = j_lo; j < n_max; ++j) {
+                const int i = j - j_lo, s = i % ST;
+                if ((i & 15) == 0) {
+                    const int p = page0 + 2 * j + lane;
+                    pages = p <= last_page ? cache_page(a.c, seq, p * JSM_PAGE_SIZE) : 0;
+                }
+                int rows[2][2];
+#pragma unroll
+                for (int value = 0; value < 2; ++value)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) rows[value][half] = page_row(i, page0 + 2 * j + half <= last_page ? half : 0, value);
+                if constexpr (Q8) {
+                    bool ok = true;
+#pragma unroll
+                    for (int value = 0; value < 2; ++value)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const int slot = value * 2 + half, r = rows[value][half];
+                            if (ok && i >= 1 && !mbar_wait_warp(&raw_empty[slot], (i & 1) ^ 1, &abort_flag, a.c.err, TC_TIMEOUT_EMPTY)) ok = false;
+                            if (ok && elect_one()) {
+                                mbar_expect_tx(&raw_full[slot], Z::RAW + (r < 0 ? 0 : 128));
+                                tma_load_2d(raw_smem + slot * Z::RAW, &tmap_kv, 0, D == 64 ? r / 2 : r, &raw_full[slot]);  // (heads of 64: two positions in a line)
+                                if (r >= 0) bulk_load(raw_scales[slot], a.c.scales + r, 128, &raw_full[slot]);
+                            }
+                            __syncwarp();
+                            if (ok) k_issued = i * 4 + slot + 1;
+                        }
+                    if (!ok) break;
+                } else {
+                    if (i >= ST && !mbar_wait_warp(&k_empty[s], ((i / ST) & 1) ^ 1, &abort_flag, a.c.err, TC_TIMEOUT_EMPTY)) break;
+                    if (elect_one()) {
+                        mbar_expect_tx(&k_full[s], Z::TILE);
+#pragma unroll
+                        for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+                            for (int half = 0; half < 2; ++half)
+                                tma_load_2d(k_smem + s * Z::TILE + c * Z::SLAB + half * (Z::SLAB / 2), &tmap_kv, c * 64, rows[0][half], &k_full[s]);
+                    }
+                    __syncwarp();
+                    k_issued = i + 1;
+                    if (i >= ST && !mbar_wait_warp(&v_empty[s], ((i / ST) & 1) ^ 1, &abort_flag, a.c.err, TC_TIMEOUT_EMPTY)) break;
+                    if (elect_one()) {
+                        mbar_expect_tx(&v_full[s], Z::TILE);
+#pragma unroll
+                        for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+                            for (int half = 0; half < 2; ++half)
+                                tma_load_2d(v_smem + s * Z::TILE + c * Z::SLAB + half * (Z::SLAB / 2), &tmap_kv, c * 64, rows[1][half], &v_full[s]);
+                    }
+                    __syncwarp();
+                    v_issued = i + 1;
+                }
+            }
+            if (abort_flag) {  // let the copies in flight land before the CTA exits (bounded)
+                const long long t0 = clock64();
+                if constexpr (Q8) {
+                    for (int i = max(0, k_issued - 4); i < k_issued; ++i)
+                        while (!mbar_try_wait(&raw_full[i & 3], (i >> 2) & 1) && clock64() - t0 < WAIT_LIMIT_CYCLES) {}
+                } else {
+                    for (int i = max(0, k_issued - ST); i < k_issued; ++i)
+                        while (!mbar_try_wait(&k_full[i % ST], (i / ST) & 1) && clock64() - t0 < WAIT_LIMIT_CYCLES) {}
+                    for (int i = max(0, v_issued - ST); i < v_issued; ++i)
+                        while (!mbar_try_wait(&v_full[i % ST], (i / ST) & 1) && clock64() - t0 < WAIT_LIMIT_CYCLES) {}
+                }
+                while (!mbar_try_wait(&q_full, 0) && clock64() - t0 < WAIT_LIMIT_CYCLES) {}
+            }
+        }
+    } else if (warp == 1) {
+        if (work && n_max > j_lo) {
+            constexpr uint32_t idesc_qk = instr_desc_bf16(CK_BM, CK_BN, 0, 0), idesc_pv = instr_desc_bf16(CK_BM, D, 0, 1);
+            bool ok = mbar_wait_warp(&q_full, 0, &abort_flag, a.c.err, TC_TIMEOUT_FULL);
+            // S_t(j) = Q_t . K(j)^T over P_t(j - 1): the tensor pipe runs the products of this thread in order, the product with V has read P by then
+            auto issue_s = [&](int t, uint32_t k_addr) {
+                const uint32_t q_addr = smem_u32(q_smem + t * Z::TILE);
+                if (elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t off = (kk / 4) * Z::SLAB;
+                        mma_ss(tmem_base + S_COL[t], smem_desc_sw128(q_addr + off) + (uint64_t)((kk % 4) * 2), smem_desc_sw128(k_addr + off) + (uint64_t)((kk % 4) * 2),
+                               idesc_qk, kk > 0 ? 1u : 0u);
+                    }
+                    mma_commit(&s_full[t]);
+                }
+                __syncwarp();
+            };
+            auto active = [&](int t, int j) { return j >= jb[t] && j < je[t]; };
+            if (ok) {
+                ok = mbar_wait_warp(&k_full[0], 0, &abort_flag, a.c.err, TC_TIMEOUT_FULL);
+                tc_fence_after();
+                if (ok) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                        if (active(t, j_lo)) issue_s(t, smem_u32(k_smem));
+                    if (elect_one()) mma_commit(&k_empty[0]);
+                    __syncwarp();
+                }
+            }
+            for (int j = j_lo; j < n_max && ok; ++j) {
+                const int i = j - j_lo, vs = i % ST, s1 = (i + 1) % ST;
+                const bool more = j + 1 < n_max;
+                if (!mbar_wait_warp(&v_full[vs], (i / ST) & 1, &abort_flag, a.c.err, TC_TIMEOUT_FULL)) { ok = false; break; }
+                if (!Q8) {  // values that no row sees: a weight of zero meets a number
+                    const int key0 = base + j * CK_BN;
+                    if (key0 < lo || key0 + CK_BN > end) {
+                        uint8_t* vb = v_smem + vs * Z::TILE;
+                        for (int n = lane; n < CK_BN * (D / 8); n += 32) {
+                            const int row = n / (D / 8), c = n % (D / 8);
+                            if (key0 + row < lo || key0 + row >= end)
+                                *reinterpret_cast<uint4*>(vb + (c >> 3) * Z::SLAB + row * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                }
+                tc_fence_after();
+                const uint32_t v_addr = smem_u32(v_smem + vs * Z::TILE), k_addr = smem_u32(k_smem + s1 * Z::TILE);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (active(t, j)) {
+                        if (!mbar_wait_warp(&p_ready[t], (j - jb[t]) & 1, &abort_flag, a.c.err, TC_TIMEOUT_MISC)) { ok = false; break; }
+                        tc_fence_after();
+                        if (elect_one()) {
+#pragma unroll
+                            for (int kk = 0; kk < CK_BN / 16; ++kk)
+                                mma_ts(tmem_base + O_COL[t], tmem_base + S_COL[t] + kk * 8, smem_desc_sw128_mn(v_addr + kk * 2048, Z::SLAB), idesc_pv,
+                                       (j > jb[t] || kk > 0) ? 1u : 0u);
+                        }
+                        __syncwarp();
+                    }
+                    if (t == 0 && more) {
+                        if (!mbar_wait_warp(&k_full[s1], ((i + 1) / ST) & 1, &abort_flag, a.c.err, TC_TIMEOUT_FULL)) { ok = false; break; }
+                        tc_fence_after();
+                    }
+                    if (active(t, j + 1)) issue_s(t, k_addr);
+                }
+                if (!ok) break;
+                if (elect_one()) {
+                    mma_commit(&v_empty[vs]);
+                    if (more) mma_commit(&k_empty[s1]);
+                }
+                __syncwarp();
+            }
+            if (ok && elect_one()) mma_commit(&o_done);
+            __syncwarp();
+        }
+    } else if (warp >= CK_SOFTMAX && warp < CK_CONVERT) {
+        regs_inc<Q8 ? 200 : 224>();
+        const int t = (warp - CK_SOFTMAX) / 4, quad = warp & 3, row = quad * 32 + lane;
+        const int rows = f.tile_tokens * a.G;                       // rows of the tile that are queries
+        const int token = tok[t] + row / a.G, pos = past + token;   // (a row that is none has a position all the same)
+        const bool query = work && row < rows && token < n_new;
+        const uint32_t lane_addr = tmem_base + ((uint32_t)(quad * 32) << 16), s_addr = lane_addr + S_COL[t], o_addr = lane_addr + O_COL[t];
+        const int pos_lo = past + tok[t], pos_hi = past + min(tok[t] + f.tile_tokens, n_new) - 1;  // first and last query of the tile
+        float m_ref = CK_NONE, l = 0.0f;
+        bool ok = true;
+        for (int j = jb[t]; j < je[t] && ok; ++j) {
+            if (!mbar_wait_warp(&s_full[t], (j - jb[t]) & 1, &abort_flag, a.c.err, TC_TIMEOUT_ACC)) { ok = false; break; }
+            tc_fence_after();
+            uint32_t sr[CK_BN];
+#pragma unroll
+            for (int c = 0; c < CK_BN; c += 32) tmem_ld32(s_addr + c, reinterpret_cast<uint32_t(&)[32]>(sr[c]));
+            tmem_ld_wait();
+            float sv[CK_BN];
+#pragma unroll
+            for (int i = 0; i < CK_BN; ++i) sv[i] = __uint_as_float(sr[i]);
+            const int key0 = base + j * CK_BN;
+            const bool masked = key0 + CK_BN - 1 > pos_lo || key0 < first_key(a.window, pos_hi);
+            if (masked) {
+                const int from = first_key(a.window, pos) - key0, to = pos - key0;
+#pragma unroll
+                for (int i = 0; i < CK_BN; ++i)
+                    if (i < from || i > to) sv[i] = -INFINITY;
+            }
+            float mxs[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) mxs[k] = sv[k];
+#pragma unroll
+            for (int i = 8; i + 16 <= CK_BN; i += 16)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) mxs[k] = fmax3(mxs[k], sv[i + k], sv[i + 8 + k]);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) mxs[k] = fmaxf(mxs[k], sv[CK_BN - 8 + k]);
+            float mx = fmaxf(fmax3(mxs[0], mxs[1], mxs[2]), fmaxf(fmax3(mxs[3], mxs[4], mxs[5]), fmaxf(mxs[6], mxs[7])));
+            mx *= a.scale_log2;
+            const bool grow = mx > m_ref + CK_RESCALE;
+            if (__any_sync(0xffffffffu, grow)) {  // (TMEM accesses are the warp's: lanes whose maximum stands use the factor 1)
+                const float alpha = grow ? ex2_approx(m_ref - mx) : 1.0f;
+                if (j > jb[t]) {
+#pragma unroll
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t r[32];
+                        tmem_ld32(o_addr + c, r);
+                        tmem_ld_wait();
+                        uint32_t w[16];
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(r[half * 16 + i]) * alpha);
+                            tmem_st16(o_addr + c + half * 16, w);
+                        }
+                    }
+                }
+                if (grow) {
+                    l *= alpha;
+                    m_ref = mx;
+                }
+            }
+            // p = 2^(s - m_ref) as bf16 pairs over the first 64 columns of S
+            uint64_t ls2[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) ls2[k] = pack2(0.0f, 0.0f);
+            const uint64_t neg_m2 = pack2(-m_ref, -m_ref), sc2 = pack2(a.scale_log2, a.scale_log2);
+#pragma unroll
+            for (int c = 0; c < CK_BN / 2; c += 16) {
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint64_t x2 = ffma2(pack2(sv[2 * (c + i)], sv[2 * (c + i) + 1]), sc2, neg_m2);
+                    float p0, p1;
+                    if ((i & 3) < POLY) {
+                        ex2_poly2(x2, p0, p1);
+                        if (masked) {  // (the polynomial ends at 2^-126: a hidden key's weight is nothing at all)
+                            if (sv[2 * (c + i)] == -INFINITY) p0 = 0.0f;
+                            if (sv[2 * (c + i) + 1] == -INFINITY) p1 = 0.0f;
+                        }
+                    } else {
+                        float x0, x1;
+                        unpack2(x2, x0, x1);
+                        p0 = ex2_approx(x0);
+                        p1 = ex2_approx(x1);
+                    }
+                    ls2[i & 3] = fadd2(ls2[i & 3], pack2(p0, p1));
+                    w[i] = pack_bf16x2(p0, p1);
+                }
+                tmem_st16(s_addr + c, w);
+            }
+            float la, lb;
+            unpack2(fadd2(fadd2(ls2[0], ls2[1]), fadd2(ls2[2], ls2[3])), la, lb);
+            l += la + lb;
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_ready[t]);
+        }
+        if (ok && n_max > j_lo) ok = mbar_wait_warp(&o_done, 0, &abort_flag, a.c.err, TC_TIMEOUT_ACC);
+        tc_fence_after();
+        const bool any = ok && je[t] > jb[t];  // (the whole query tile)
+        if (f.share > 1) {
+            // the row's sums into shared memory, 16-byte pieces swizzled by the row; every product has been taken, so tiles and rings are free
+            const int r = t * CK_BM + row;
+            sm_ml[r] = make_float2(any ? m_ref : CK_NONE, any ? l : 0.0f);
+            if (any) {
+                uint8_t* dst = tiles + (size_t)r * (D * 4);
+#pragma unroll
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(o_addr + c, o);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(dst + ((((c + i) / 4) ^ (r & 7)) * 16)) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                }
+            }
+        } else if (any) {
+            const float inv = 1.0f / l;
+            bool bad = false;
+            // a thread has a row: the warp's 32 rows pass through the queries' place and leave whole, 16 bytes per lane
+            uint8_t* staged = q_smem + t * Z::TILE + quad * (32 * D * 2);
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+                uint32_t r[32];
+                tmem_ld32(o_addr + c, r);
+                tmem_ld_wait();
+                float x[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    x[i] = __uint_as_float(r[i]) * inv;
+                    bad = bad || !(fabsf(x[i]) <= 3.402823466e38f);
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i += 8)
+                    *reinterpret_cast<uint4*>(staged + lane * (D * 2) + ((((c + i) / 8) ^ (lane & 7)) * 16)) =
+                        make_uint4(pack_bf16x2(x[i], x[i + 1]), pack_bf16x2(x[i + 2], x[i + 3]), pack_bf16x2(x[i + 4], x[i + 5]), pack_bf16x2(x[i + 6], x[i + 7]));
+            }
+            __syncwarp();
+            constexpr int PIECES = D / 8, STEP = 32 / PIECES;
+            const int piece = lane % PIECES;
+#pragma unroll 4
+            for (int r = lane / PIECES; r < 32; r += STEP) {
+                const int at = quad * 32 + r, tk = tok[t] + at / a.G;
+                if (at < rows && tk < n_new)
+                    *reinterpret_cast<uint4*>(a.out + (row0 + tk) * a.out_rs + (long long)(hk * a.G + at % a.G) * D + piece * 8) =
+                        *reinterpret_cast<const uint4*>(staged + r * (D * 2) + ((piece ^ (r & 7)) * 16));
+            }
+            __syncwarp();
+            unsigned again = __ballot_sync(0xffffffffu, bad && query);
+            while (again) {
+                const int r = __ffs(again) - 1, at = quad * 32 + r, tk = tok[t] + at / a.G;
+                again &= again - 1;
+                attend_row<D, Q8>(a, seq, row0 + tk, hk * a.G + at % a.G, past + tk);
+            }
+        }
+    } else if (Q8 && warp >= CK_CONVERT) {
+        regs_dec<72>();
+        if constexpr (Q8) {
+            const int cw = warp - CK_CONVERT;
+            // Reads and writes of 16 bytes, eight lanes at a time over all banks: the lanes have four pieces of two rows whose numbers differ in bit 0 (the places of the
+            // bf16 pieces) and, where a row is a whole line, in bit 2 (the places of the raw pieces).
+            const int c4 = lane & 3, second = (lane >> 2) & 1;
+            bool ok = true;
+            for (int j = j_lo; j < n_max && ok; ++j) {
+                const int i = j - j_lo, s = i % ST;
+#pragma unroll
+                for (int value = 0; value < 2 && ok; ++value) {
+                    uint8_t* dst = (value ? v_smem : k_smem) + s * Z::TILE;
+                    if (i >= ST && !mbar_wait_warp(value ? &v_empty[s] : &k_empty[s], ((i / ST) & 1) ^ 1, &abort_flag, a.c.err, TC_TIMEOUT_EMPTY)) { ok = false; break; }
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const int slot = value * 2 + half;
+                        if (!mbar_wait_warp(&raw_full[slot], i & 1, &abort_flag, a.c.err, TC_TIMEOUT_FULL)) { ok = false; break; }
+                        const uint8_t* raw = raw_smem + slot * Z::RAW;
+                        const int key0 = base + j * CK_BN + half * JSM_PAGE_SIZE;
+#pragma unroll
+                        for (int n = 0; n < (D == 128 ? 4 : 2); ++n) {
+                            int r, piece, slab;  // row of the page, piece of 16 numbers in the row, slab of 64 columns
+                            const uint8_t* src;
+                            if constexpr (D == 128) {
+                                slab = (lane >> 3) & 1;
+                                const int pair = (n & 1) * 2 + (lane >> 4);
+                                r = cw * 16 + (n >> 1) * 8 + (second ? pair ^ 5 : pair);
+                                piece = slab * 4 + c4;
+                                src = raw + r * 128 + ((piece ^ (r & 7)) << 4);
+                            } else {
+                                slab = 0;
+                                r = cw * 16 + n * 8 + (lane >> 3) * 2 + second;
+                                piece = c4;
+                                const int line = r >> 1;
+                                src = raw + line * 128 + ((((r & 1) * 4 + piece) ^ (line & 7)) << 4);
+                            }
+                            const uint4 w = *reinterpret_cast<const uint4*>(src);
+                            uint32_t scale = raw_scales[slot][r];
+                            if (value && (key0 + r < lo || key0 + r >= end)) scale = 0;  // (a value that no row sees: a weight of zero meets a number)
+                            scale *= 0x00010001u;
+                            const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+                            uint32_t out[8];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                out[2 * k] = ck_q8_pair(__byte_perm(in[k], 0, 0x1100), scale);
+                                out[2 * k + 1] = ck_q8_pair(__byte_perm(in[k], 0, 0x3322), scale);
+                            }
+                            uint8_t* to = dst + slab * Z::SLAB + (half * JSM_PAGE_SIZE + r) * 128;
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                *reinterpret_cast<uint4*>(to + (((c4 * 2 + e) ^ (r & 7)) << 4)) = make_uint4(out[4 * e], out[4 * e + 1], out[4 * e + 2], out[4 * e + 3]);
+                        }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&raw_empty[slot]);
+                    }
+                    if (!ok) break;
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(value ? &v_full[s] : &k_full[s]);
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+    if (f.share == 1) return;
+    ck_cluster_arrive();
+    ck_cluster_wait();  // every CTA's sums are in its shared memory
+    if (work && !abort_flag && warp >= CK_SOFTMAX && warp < CK_CONVERT) {
+        constexpr int N = D / 32;
+        const int n_rows = f.tile_tokens * a.G;
+        const uint32_t sums = smem_u32(tiles), ml = smem_u32(sm_ml);
+        for (int r = part + f.share * (warp - CK_SOFTMAX); r < 2 * CK_BM; r += f.share * 8) {
+            const int t = r / CK_BM, at = r % CK_BM, tk = tok[t] + at / a.G;
+            if (at >= n_rows || tk >= n_new) continue;
+            float M = CK_NONE, L = 0.0f, acc[N];
+            for (int p = 0; p < f.share; ++p) M = fmaxf(M, ck_load2(ck_peer(ml + r * 8, p)).x);
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+            for (int p = 0; p < f.share; ++p) {
+                const float2 v = ck_load2(ck_peer(ml + r * 8, p));
+                if (v.x == CK_NONE && v.y == 0.0f) continue;  // it had none of the row's keys
+                const float w = ex2_approx(v.x - M);
+                L = fmaf(w, v.y, L);
+                const uint32_t src = ck_peer(sums + r * (D * 4) + (((lane * N / 4) ^ (r & 7)) * 16) + (N == 2 ? (lane & 1) * 8 : 0), p);
+                if constexpr (N == 4) {
+                    const float4 x = ck_load4(src);
+                    acc[0] = fmaf(w, x.x, acc[0]); acc[1] = fmaf(w, x.y, acc[1]); acc[2] = fmaf(w, x.z, acc[2]); acc[3] = fmaf(w, x.w, acc[3]);
+                } else {
+                    const float2 x = ck_load2(src);
+                    acc[0] = fmaf(w, x.x, acc[0]); acc[1] = fmaf(w, x.y, acc[1]);
+                }
+            }
+            bool fine = true;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                acc[i] /= L;
+                fine = fine && fabsf(acc[i]) <= 3.402823466e38f;
+            }
+            if (__all_sync(0xffffffffu, fine)) {
+                __nv_bfloat16* dst = a.out + (row0 + tk) * a.out_rs + (long long)(hk * a.G + at % a.G) * D + lane * N;
+#pragma unroll
+                for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16x2(acc[i], acc[i + 1]);
+            } else {
+                attend_row<D, Q8>(a, seq, row0 + tk, hk * a.G + at % a.G, past + tk);
+            }
+        }
+    }
+    ck_cluster_arrive();
+    ck_cluster_wait();  // no CTA leaves while a peer reads its shared memory
+}
+
+// clusters of S CTAs that the chip holds at once (15 of eight, 33 of four, although it has 148 multiprocessors)
+template <int D, bool Q8>
+static int flash_capacity(int S) {
+    static std::mutex mu;
+    static int known[64][9];  // per device
+    int dev = -1;
+    const int guess = S == 1 ? sm_count() : sm_count() / S * 3 / 4;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return guess;
+    std::lock_guard<std::mutex> lock(mu);
+    if (known[dev][S] == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(S * 256);
+        cfg.blockDim = dim3(FlashSizes<D, Q8>::THREADS);
+        cfg.dynamicSmemBytes = FlashSizes<D, Q8>::SMEM;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = S;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, chunk_flash_kernel<D, Q8>, &cfg) != cudaSuccess || n <= 0) {
+            cudaGetLastError();
+            n = guess;
+        }
+        known[dev][S] = n;
+    }
+    return known[dev][S];
+}
+
+template <int D, bool Q8>
+static jsm_status flash_launch(const ChunkArgs& a, int few_rows, cudaStream_t st) {
+    using Z = FlashSizes<D, Q8>;
+    FlashArgs f{a, few_rows, CK_BM / a.G, 0, 1};
+    const long long tokens = 2ll * f.tile_tokens, per_seq = (a.max_new + tokens - 1) / tokens;
+    f.slots = (int)std::min(per_seq * a.c.n_seqs, a.T / tokens + a.c.n_seqs);
+    static DeviceOnce once;
+    JSM_CUDA_CHECK(allow_shared(once, chunk_flash_kernel<D, Q8>, (int)Z::SMEM));
+    // CTAs of a pair of query tiles: a key tile takes about 1.2 us, what is around the walk 5 us, the meeting of a cluster 3 us; those that do not fit at once wait
+    long long keys = a.max_context;
+    if (a.window > 0) keys = std::min(keys, (long long)a.window + tokens);
+    const long long key_tiles = (keys + CK_BN - 1) / CK_BN, pairs = (long long)f.slots * a.c.Hkv;
+    float best = 0.0f;
+    for (int S = 1; S <= 8; S *= 2) {
+        if (S > 1 && key_tiles < 4 * S) break;
+        const int cap = flash_capacity<D, Q8>(S);
+        const float cost = (float)((pairs + cap - 1) / cap) * (5.0f + (S > 1 ? 3.0f : 0.0f) + 1.2f * (float)((key_tiles + S - 1) / S));
+        if (S == 1 || cost < best) { best = cost; f.share = S; }
+    }
+    if (pairs * f.share > INT32_MAX) JSM_FAIL(JSM_UNSUPPORTED, "jsm_attn_chunk: %lld tiles of queries", pairs);
+    CUtensorMap mq, mkv;
+    jsm_status s = make_tmap_bf16_3d(&mq, a.q, D, a.Hq, a.T, D, a.q_rs, 64, a.G, f.tile_tokens);
+    if (s != JSM_OK) return s;
+    const uint64_t rows = (uint64_t)a.c.n_pages * 2 * a.c.Hkv * JSM_PAGE_SIZE;
+    s = Q8 ? make_tmap_u8_lines(&mkv, a.c.pool, rows * D / 128, JSM_PAGE_SIZE * D / 128) : make_tmap_bf16_2d(&mkv, a.c.pool, rows, D, D, JSM_PAGE_SIZE, 64);
+    if (s != JSM_OK) return s;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(pairs * f.share));
+    cfg.blockDim = dim3(Z::THREADS);
+    cfg.dynamicSmemBytes = Z::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = f.share;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = chained_launch_enabled() ? attr : attr + 1;
+    cfg.numAttrs = (chained_launch_enabled() ? 1 : 0) + (f.share > 1 ? 1 : 0);
+    JSM_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_flash_kernel<D, Q8>, mq, mkv, f));
+    JSM_LAUNCH_CHECK();
+    return JSM_OK;
+}
+
+jsm_status chunk_flash_launch(const ChunkArgs& a, int few_rows, cudaStream_t st) {
+    if (a.c.D == 64) return a.c.scales ? flash_launch<64, true>(a, few_rows, st) : flash_launch<64, false>(a, few_rows, st);
+    return a.c.scales ? flash_launch<128, true>(a, few_rows, st) : flash_launch<128, false>(a, few_rows, st);
+}
+
+}  // namespace jsm
