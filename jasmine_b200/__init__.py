@@ -535,10 +535,13 @@ def rope_rotate(q, k, table, Hq, Hkv, D, rot_dim, positions=None, layout=ROPE_HA
     _need(x is not None, "rope_rotate: no rows")
     T = x.shape[0]
     _need((q is None) == (Hq == 0) and (k is None) == (Hkv == 0), "rope_rotate: rows without heads, or heads without rows")
-    _need(table.dtype == torch.float32 and table.is_contiguous() and table.dim() == 3 and tuple(table.shape[1:]) == (rot_dim // 2, 2), "rope_rotate: a contiguous "
-          "fp32 table [positions, rot_dim / 2, 2] is wanted")
     q_out = torch.empty(T, Hq * D, dtype=q.dtype, device=q.device) if q is not None and q_out is None else q_out
     k_out = torch.empty(T, Hkv * D, dtype=k.dtype, device=k.device) if k is not None and k_out is None else k_out
+    m = _calls_module or _calls()
+    if m and _done(m.rope_rotate(q, k, table, Hq, Hkv, D, rot_dim, positions, layout, inverse, q_out, k_out)):
+        return q_out, k_out
+    _need(table.dtype == torch.float32 and table.is_contiguous() and table.dim() == 3 and tuple(table.shape[1:]) == (rot_dim // 2, 2), "rope_rotate: a contiguous "
+          "fp32 table [positions, rot_dim / 2, 2] is wanted")
     for t, n, what in ((q, Hq, "q"), (q_out, Hq, "q_out"), (k, Hkv, "k"), (k_out, Hkv, "k_out")):
         if n:
             _need(t.shape[0] == T and t.dtype == x.dtype, f"rope_rotate: {what} has other rows or another type")
@@ -569,6 +572,9 @@ def _cache(what, pool, scales, block_table, starts, context_lens, Hkv, D):
 
 def kv_append_q8(pool, scales, block_table, k, v, starts, context_lens, Hkv, D, rope=None, rot_dim=0, layout=ROPE_HALF):
     """New keys (rotated with the table `rope` [positions, rot_dim / 2, 2]) and values [T, Hkv * D] into an 8-bit cache (jsm_kv_append_q8)."""
+    m = _calls_module or _calls()
+    if m and _done(m.kv_append_q8(pool, scales, block_table, k, v, starts, context_lens, Hkv, D, rope, rot_dim, layout)):
+        return
     torch = _torch()
     at, seqs = _cache("kv_append_q8", pool, scales, block_table, starts, context_lens, Hkv, D)
     for t, what in ((k, "k"), (v, "v")):
@@ -585,9 +591,12 @@ def kv_append_q8(pool, scales, block_table, k, v, starts, context_lens, Hkv, D, 
 def kv_read(pool, block_table, starts, context_lens, T, Hkv, D, scales=None, dtype=None, k_out=None, v_out=None):
     """Keys and values [T, Hkv * D] (bf16, or dtype) of the new tokens' positions as the cache holds them (jsm_kv_read); rows of no sequence are left as they are."""
     torch = _torch()
-    at, seqs = _cache("kv_read", pool, scales, block_table, starts, context_lens, Hkv, D)
     k_out = torch.empty(T, Hkv * D, dtype=dtype or torch.bfloat16, device=pool.device) if k_out is None else k_out
     v_out = torch.empty_like(k_out) if v_out is None else v_out
+    m = _calls_module or _calls()
+    if m and _done(m.kv_read(pool, scales, block_table, starts, context_lens, T, Hkv, D, k_out, v_out)):
+        return k_out, v_out
+    at, seqs = _cache("kv_read", pool, scales, block_table, starts, context_lens, Hkv, D)
     for t in (k_out, v_out):
         _rows(t, Hkv * D, "kv_read: out")
     _need(k_out.shape == v_out.shape and k_out.shape[0] == T and k_out.dtype == v_out.dtype and _pitch(k_out) == _pitch(v_out), "kv_read: outputs of one shape, type and pitch")
@@ -598,15 +607,19 @@ def kv_read(pool, block_table, starts, context_lens, T, Hkv, D, scales=None, dty
 def attn_chunk(q, pool, block_table, starts, context_lens, Hq, Hkv, D, max_new, max_context, scales=None, window=0, scale=None, scratch=None, out=None):
     """Attention of the new tokens q [T, Hq * D] of every sequence over its paged cache, bf16 or (with scales) 8-bit (jsm_attn_chunk)."""
     torch = _torch()
-    at, seqs = _cache("attn_chunk", pool, scales, block_table, starts, context_lens, Hkv, D)
     T = q.shape[0]
     out = torch.empty(T, Hq * D, dtype=q.dtype, device=q.device) if out is None else out
+    scale = float(D) ** -0.5 if scale is None else scale
+    m = _calls_module or _calls()
+    if m and _done(m.attn_chunk(q, pool, scales, block_table, starts, context_lens, Hq, Hkv, D, max_new, max_context, window, scale, scratch, out)):
+        return out
+    at, seqs = _cache("attn_chunk", pool, scales, block_table, starts, context_lens, Hkv, D)
     for t, what in ((q, "q"), (out, "out")):
         _rows(t, Hq * D, "attn_chunk: " + what)
         _need(t.dtype == torch.bfloat16 and t.shape[0] == T, f"attn_chunk: {what} of {T} rows in bf16")
     if scratch is None:
         scratch = torch.empty(lib().jsm_attn_chunk_scratch_bytes(seqs[2], T, max_new, max_context, Hq, Hkv, D, window), dtype=torch.uint8, device=q.device)
-    scale = float(D) ** -0.5 if scale is None else scale
+    _need(scratch.is_contiguous(), "attn_chunk: contiguous scratch is wanted")
     check(lib().jsm_attn_chunk(q.data_ptr(), _pitch(q), *at, *seqs, T, max_new, max_context, Hq, Hkv, D, window, scale, scratch.data_ptr(),
                                scratch.numel() * scratch.element_size(), out.data_ptr(), _pitch(out), stream_ptr()))
     return out

@@ -65,6 +65,20 @@ __device__ __forceinline__ long long cache_row(const CacheView& c, int page, int
     return (((long long)page * 2 + value) * c.Hkv + head) * JSM_PAGE_SIZE + pos % JSM_PAGE_SIZE;
 }
 
+// Two numbers of an 8-bit cache, in the low bytes of the halves of p, as bf16: 0x4300 | the low seven bits is 128 + them, 0x4300 | the sign bit is 128 or 256, and the
+// difference is the number, exactly.
+__device__ __forceinline__ uint32_t q8_pair(uint32_t p) {
+    const uint32_t lo = (p & 0x007F007Fu) | 0x43004300u, hi = (p & 0x00800080u) | 0x43004300u;
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&hi));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+// times their scales: the values that the cache stands for, one rounding
+__device__ __forceinline__ uint32_t q8_value2(uint32_t p, uint32_t scale2) {
+    const uint32_t n = q8_pair(p);
+    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&n), *reinterpret_cast<const __nv_bfloat162*>(&scale2));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
 // rotation of a pair, every product rounded on its own
 __device__ __forceinline__ void rotate_pair(float x1, float x2, float c, float s, float& y1, float& y2) {
     y1 = __fsub_rn(__fmul_rn(x1, c), __fmul_rn(x2, s));

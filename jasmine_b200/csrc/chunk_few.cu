@@ -9,7 +9,6 @@
 // bf16 pages come into the operands by ldmatrix.  Numbers of an 8-bit page are taken from shared memory in 16-byte pieces and become bf16 in registers: which
 // component an element of an operand stands for is free as long as both operands agree, so the pieces of a thread are the components that its operand
 // registers need, and the transposition of V costs no instruction beyond the byte permutation that spreads the numbers anyway.
-//   n (a byte) -> bf16: 0x4300 | low seven bits is 128 + them, 0x4300 | sign bit is 128 or 256; their difference is n, exactly.  Times the scale, one rounding.
 // Partial results of the runs meet in chunk_merge_kernel, in the order of the runs.
 // A row whose result is not a number is worked out again over exactly its own keys (attend_row): a weight of zero times what a hidden key holds is no zero then.
 #include "chunk_attn.cuh"
@@ -31,17 +30,6 @@ __device__ __forceinline__ uint32_t cf_trans(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-// two numbers, in the low bytes of the halves of p, as bf16
-__device__ __forceinline__ uint32_t q8_pair(uint32_t p) {
-    const uint32_t lo = (p & 0x007F007Fu) | 0x43004300u, hi = (p & 0x00800080u) | 0x43004300u;
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&hi));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-
 template <int D, bool Q8>
 struct FewSizes {
     static constexpr int TILE = JSM_PAGE_SIZE * D * (Q8 ? 1 : 2);     // keys, or values, of a page
@@ -197,8 +185,8 @@ __global__ void __launch_bounds__(CF_THREADS) chunk_few_kernel(const __grid_cons
                         uint32_t f[4];
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            f[h] = mul_bf16x2(q8_pair(__byte_perm(kw[h][ks], 0, 0x1100)), ks2[h]);
-                            f[h + 2] = mul_bf16x2(q8_pair(__byte_perm(kw[h][ks], 0, 0x3322)), ks2[h]);
+                            f[h] = q8_value2(__byte_perm(kw[h][ks], 0, 0x1100), ks2[h]);
+                            f[h + 2] = q8_value2(__byte_perm(kw[h][ks], 0, 0x3322), ks2[h]);
                         }
 #pragma unroll
                         for (int n = 0; n < NT; ++n) mma_16816(sc[n], f, qb[n][ks][0], qb[n][ks][1]);
@@ -280,8 +268,8 @@ __global__ void __launch_bounds__(CF_THREADS) chunk_few_kernel(const __grid_cons
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const uint32_t w0 = vw[h * 2][j >> 1], w1 = vw[h * 2 + 1][j >> 1];
-                            f[h * 2] = mul_bf16x2(q8_pair(__byte_perm(w0, w1, j & 1 ? 0x6622 : 0x4400)), vs[h]);
-                            f[h * 2 + 1] = mul_bf16x2(q8_pair(__byte_perm(w0, w1, j & 1 ? 0x7733 : 0x5511)), vs[h]);
+                            f[h * 2] = q8_value2(__byte_perm(w0, w1, j & 1 ? 0x6622 : 0x4400), vs[h]);
+                            f[h * 2 + 1] = q8_value2(__byte_perm(w0, w1, j & 1 ? 0x7733 : 0x5511), vs[h]);
                         }
 #pragma unroll
                         for (int n = 0; n < NT; ++n) mma_16816(o[n][j], f, pb[n][0], pb[n][1]);

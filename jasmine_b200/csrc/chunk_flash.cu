@@ -101,13 +101,6 @@ __device__ __forceinline__ bool find_tile(const FlashArgs& f, int slot, int& seq
     return false;
 }
 
-__device__ __forceinline__ uint32_t ck_q8_pair(uint32_t p, uint32_t scale2) {
-    const uint32_t lo = (p & 0x007F007Fu) | 0x43004300u, hi = (p & 0x00800080u) | 0x43004300u;
-    const __nv_bfloat162 n = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&hi));
-    const __nv_bfloat162 r = __hmul2(n, *reinterpret_cast<const __nv_bfloat162*>(&scale2));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-
 template <int D, bool Q8>
 __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
     chunk_flash_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_kv, const __grid_constant__ FlashArgs f) {
@@ -560,8 +553,8 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
                             uint32_t out[8];
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
-                                out[2 * k] = ck_q8_pair(__byte_perm(in[k], 0, 0x1100), scale);
-                                out[2 * k + 1] = ck_q8_pair(__byte_perm(in[k], 0, 0x3322), scale);
+                                out[2 * k] = q8_value2(__byte_perm(in[k], 0, 0x1100), scale);
+                                out[2 * k + 1] = q8_value2(__byte_perm(in[k], 0, 0x3322), scale);
                             }
                             uint8_t* to = dst + slab * Z::SLAB + (half * JSM_PAGE_SIZE + r) * 128;
 #pragma unroll

@@ -32,7 +32,7 @@ __device__ __forceinline__ float q8_scale(float most) {
 }
 __device__ __forceinline__ float q8_inverse(float scale) { return scale == 0.0f ? 0.0f : __fdiv_rn(1.0f, scale); }
 
-// one warp per (token, keys or values, kv head)
+// any pitches, alignments and rotations: one warp per (token, keys or values, kv head)
 __global__ void __launch_bounds__(256) kv_append_q8_kernel(AppendArgs a) {
     __shared__ int found;
     chain_trigger();
@@ -81,6 +81,106 @@ __global__ void __launch_bounds__(256) kv_append_q8_kernel(AppendArgs a) {
     }
 }
 
+// Whole 16-byte pieces: LPR lanes have eight components each of a row (token, keys or values, kv head); a row's first loads do not wait for its page.  The partner of a
+// half is fetched a second time (from L1) rather than passed between lanes: the lanes of a half are four to sixteen apart in four registers.
+// Rounding to a whole number: adding 1.5 * 2^23 leaves it in the low bits of the sum.
+__device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
+    x[0] = bf16lo(w.x); x[1] = bf16hi(w.x); x[2] = bf16lo(w.y); x[3] = bf16hi(w.y);
+    x[4] = bf16lo(w.z); x[5] = bf16hi(w.z); x[6] = bf16lo(w.w); x[7] = bf16hi(w.w);
+}
+template <int LPR>
+__global__ void __launch_bounds__(256) kv_append_q8_vec_kernel(AppendArgs a) {
+    constexpr int ROWS = 256 / LPR, U = 4;
+    __shared__ int found;
+    chain_trigger();
+    chain_wait();
+    const int t = blockIdx.x, D = a.c.D, Hkv = a.c.Hkv, n_rows = 2 * Hkv;
+    const int i0 = threadIdx.x % LPR * 8, group = threadIdx.x / LPR;
+    const bool on = i0 < D, turns = a.table && i0 < a.rot;
+    const int half = a.rot / 2;
+    const bool second = !a.adjacent && i0 >= half;
+    uint4 w[U], w2[U];
+    auto load = [&](int r0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * ROWS;
+            if (r >= n_rows || !on) break;
+            const __nv_bfloat16* src = (r < Hkv ? a.k + t * a.kv_rs + (long long)r * D : a.v + t * a.kv_rs + (long long)(r - Hkv) * D) + i0;
+            w[u] = *reinterpret_cast<const uint4*>(src);
+            if (r < Hkv && turns && !a.adjacent) w2[u] = *reinterpret_cast<const uint4*>(second ? src - half : src + half);
+        }
+    };
+    load(group);
+    const int s = find_sequence(a.c, t, &found);
+    if (s < 0) return;
+    int first, n_new, ctx;
+    if (!cache_lengths(a.c, s, a.T, first, n_new, ctx)) return;
+    const int pos = ctx - n_new + t - first;
+    if (a.table && pos >= a.table_len) {
+        if (threadIdx.x == 0) cache_error(a.c.err, CACHE_BAD_POSITION);
+        return;
+    }
+    const int page = cache_page(a.c, s, pos);
+    if (page < 0) return;
+    float c[8], sn[8];  // adjacent: four pairs; halves: eight
+    if (turns) {
+        const float4* e = reinterpret_cast<const float4*>(a.table + (long long)pos * half + (a.adjacent ? i0 / 2 : second ? i0 - half : i0));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < 2 || !a.adjacent) {
+                const float4 v = e[i];
+                c[2 * i] = v.x; sn[2 * i] = v.y; c[2 * i + 1] = v.z; sn[2 * i + 1] = v.w;
+            }
+    }
+    const int ahead = threadIdx.x % 32 / LPR;  // (a warp's rows take their turns together: lanes meet in shuffles)
+    for (int r0 = group; r0 - ahead < n_rows; r0 += U * ROWS) {
+        if (r0 != group) load(r0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * ROWS;
+            float x[8] = {0, 0, 0, 0, 0, 0, 0, 0}, most = 0.0f, sum = 0.0f;
+            if (r < n_rows && on) {
+                unpack8(w[u], x);
+                if (r < Hkv && turns) {
+                    if (a.adjacent) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) rotate_pair(x[2 * i], x[2 * i + 1], c[i], sn[i], x[2 * i], x[2 * i + 1]);
+                    } else {
+                        float y[8];
+                        unpack8(w2[u], y);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            float y1, y2;
+                            rotate_pair(second ? y[i] : x[i], second ? x[i] : y[i], c[i], sn[i], y1, y2);
+                            x[i] = second ? y2 : y1;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    most = fmaxf(most, fabsf(x[i]));
+                    sum += x[i] * 0.0f;  // a NaN where a component is one, or infinite (fmaxf passes over a NaN)
+                }
+                if (!(sum == 0.0f)) most = INFINITY;
+            }
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            if (r >= n_rows || !on) continue;
+            const float scale = q8_scale(most), inv = q8_inverse(scale);
+            uint32_t n[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) n[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], inv), 12582912.0f));
+            uint2 o;
+            o.x = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
+            o.y = __byte_perm(__byte_perm(n[4], n[5], 0x0040), __byte_perm(n[6], n[7], 0x0040), 0x5410);
+            if (!(scale == scale)) o = make_uint2(0, 0);
+            const long long row = r < Hkv ? cache_row(a.c, page, 0, r, pos) : cache_row(a.c, page, 1, r - Hkv, pos);
+            *reinterpret_cast<uint2*>(static_cast<int8_t*>(a.c.pool) + row * D + i0) = o;
+            if (i0 == 0) a.c.scales[row] = (uint16_t)(__float_as_uint(scale) >> 16);
+        }
+    }
+}
+
 struct ReadArgs {
     CacheView c;
     void *k_out, *v_out;
@@ -111,6 +211,68 @@ __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a) {
             else static_cast<__nv_bfloat16*>(value ? a.v_out : a.k_out)[to + i] = y;
         }
     }
+}
+
+// whole 16-byte pieces of the outputs: eight components per lane, four rows' loads in flight
+template <int LPR, bool Q8, bool F32>
+__global__ void __launch_bounds__(256) kv_read_vec_kernel(ReadArgs a) {
+    constexpr int ROWS = 256 / LPR, U = 4;
+    __shared__ int found;
+    chain_trigger();
+    chain_wait();
+    const int t = blockIdx.x, D = a.c.D, Hkv = a.c.Hkv, n_rows = 2 * Hkv;
+    const int i0 = threadIdx.x % LPR * 8, group = threadIdx.x / LPR;
+    const int s = find_sequence(a.c, t, &found);
+    if (s < 0 || i0 >= D) return;
+    int first, n_new, ctx;
+    if (!cache_lengths(a.c, s, a.T, first, n_new, ctx)) return;
+    const int pos = ctx - n_new + t - first;
+    const int page = cache_page(a.c, s, pos);
+    if (page < 0) return;
+    for (int r0 = group; r0 < n_rows; r0 += U * ROWS) {
+        uint4 w[U];
+        uint32_t scale[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * ROWS;
+            if (r >= n_rows) break;
+            const long long row = r < Hkv ? cache_row(a.c, page, 0, r, pos) : cache_row(a.c, page, 1, r - Hkv, pos);
+            if constexpr (Q8) {
+                const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.c.pool) + row * D + i0);
+                w[u].x = v.x;
+                w[u].z = v.y;
+                scale[u] = a.c.scales[row] * 0x00010001u;
+            } else {
+                w[u] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.c.pool) + row * D + i0);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * ROWS;
+            if (r >= n_rows) break;
+            uint4 o = w[u];
+            if constexpr (Q8) {
+                o.x = q8_value2(__byte_perm(w[u].x, 0, 0x1100), scale[u]);
+                o.y = q8_value2(__byte_perm(w[u].x, 0, 0x3322), scale[u]);
+                o.z = q8_value2(__byte_perm(w[u].z, 0, 0x1100), scale[u]);
+                o.w = q8_value2(__byte_perm(w[u].z, 0, 0x3322), scale[u]);
+            }
+            const long long to = t * a.out_rs + (long long)(r < Hkv ? r : r - Hkv) * D + i0;
+            void* out = r < Hkv ? a.k_out : a.v_out;
+            if constexpr (F32) {
+                float* dst = static_cast<float*>(out) + to;
+                reinterpret_cast<float4*>(dst)[0] = make_float4(bf16lo(o.x), bf16hi(o.x), bf16lo(o.y), bf16hi(o.y));
+                reinterpret_cast<float4*>(dst)[1] = make_float4(bf16lo(o.z), bf16hi(o.z), bf16lo(o.w), bf16hi(o.w));
+            } else {
+                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + to) = o;
+            }
+        }
+    }
+}
+template <int LPR>
+static cudaError_t read_vec_launch(const ReadArgs& a, cudaStream_t st) {
+    if (a.c.scales) return a.f32 ? launch_chained(kv_read_vec_kernel<LPR, true, true>, dim3(a.T), dim3(256), 0, st, a) : launch_chained(kv_read_vec_kernel<LPR, true, false>, dim3(a.T), dim3(256), 0, st, a);
+    return a.f32 ? launch_chained(kv_read_vec_kernel<LPR, false, true>, dim3(a.T), dim3(256), 0, st, a) : launch_chained(kv_read_vec_kernel<LPR, false, false>, dim3(a.T), dim3(256), 0, st, a);
 }
 
 // what the calls over a paged cache check alike
@@ -154,7 +316,12 @@ extern "C" jsm_status jsm_kv_append_q8(void* d_pool, void* d_scales, int n_pages
     a.T = T;
     a.table = reinterpret_cast<const float2*>(d_rope_table);
     a.table_len = table_len; a.rot = rot_dim; a.adjacent = layout == JSM_ROPE_ADJACENT;
-    JSM_CUDA_CHECK(launch_chained(kv_append_q8_kernel, dim3(T), dim3(256), 0, as_stream(stream), a));
+    const uintptr_t at = reinterpret_cast<uintptr_t>(d_k) | reinterpret_cast<uintptr_t>(d_v) | reinterpret_cast<uintptr_t>(d_rope_table);
+    const bool pieces = !(at & 15) && kv_row_stride % 8 == 0 && (!d_rope_table || (layout == JSM_ROPE_ADJACENT ? rot_dim : rot_dim / 2) % 8 == 0);
+    JSM_CUDA_CHECK(!pieces    ? launch_chained(kv_append_q8_kernel, dim3(T), dim3(256), 0, as_stream(stream), a)
+                   : D <= 64  ? launch_chained(kv_append_q8_vec_kernel<8>, dim3(T), dim3(256), 0, as_stream(stream), a)
+                   : D <= 128 ? launch_chained(kv_append_q8_vec_kernel<16>, dim3(T), dim3(256), 0, as_stream(stream), a)
+                              : launch_chained(kv_append_q8_vec_kernel<32>, dim3(T), dim3(256), 0, as_stream(stream), a));
     JSM_LAUNCH_CHECK();
     return JSM_OK;
 }
@@ -173,7 +340,11 @@ extern "C" jsm_status jsm_kv_read(const void* d_pool, const void* d_scales, int 
     if ((reinterpret_cast<uintptr_t>(d_k_out) | reinterpret_cast<uintptr_t>(d_v_out)) & (out_dtype == JSM_F32 ? 3 : 1))
         JSM_FAIL(JSM_INVALID_ARG, "jsm_kv_read: rows that are not aligned to their elements");
     a.k_out = d_k_out; a.v_out = d_v_out; a.out_rs = out_row_stride; a.T = T; a.f32 = out_dtype == JSM_F32;
-    JSM_CUDA_CHECK(launch_chained(kv_read_kernel, dim3(T), dim3(256), 0, as_stream(stream), a));
+    const bool pieces = !((reinterpret_cast<uintptr_t>(d_k_out) | reinterpret_cast<uintptr_t>(d_v_out)) & 15) && out_row_stride % (a.f32 ? 4 : 8) == 0;
+    JSM_CUDA_CHECK(!pieces    ? launch_chained(kv_read_kernel, dim3(T), dim3(256), 0, as_stream(stream), a)
+                   : D <= 64  ? read_vec_launch<8>(a, as_stream(stream))
+                   : D <= 128 ? read_vec_launch<16>(a, as_stream(stream))
+                              : read_vec_launch<32>(a, as_stream(stream)));
     JSM_LAUNCH_CHECK();
     return JSM_OK;
 }

@@ -9,6 +9,9 @@
 #include <Python.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
+#include <algorithm>
+#include <initializer_list>
+#include <ATen/ops/empty.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include "../../include/jasmine_b200.h"
 
@@ -21,6 +24,11 @@ struct Library {
     decltype(&jsm_embedding) embedding;
     decltype(&jsm_attn_prefill) attn_prefill;
     decltype(&jsm_attn_decode) attn_decode;
+    decltype(&jsm_rope_rotate) rope_rotate;
+    decltype(&jsm_kv_append_q8) kv_append_q8;
+    decltype(&jsm_kv_read) kv_read;
+    decltype(&jsm_attn_chunk_scratch_bytes) attn_chunk_scratch_bytes;
+    decltype(&jsm_attn_chunk) attn_chunk;
 } L = {};
 
 // a plain dense CUDA tensor: nothing between it and its memory
@@ -126,7 +134,9 @@ JSM_FAST(bind) {  // address of the shared library's handle
     if (PyErr_Occurred()) return nullptr;
     auto find = [&](auto& f, const char* name) { f = reinterpret_cast<std::remove_reference_t<decltype(f)>>(dlsym(h, name)); return f != nullptr; };
     if (!find(L.eval_elementwise, "jsm_eval_elementwise") || !find(L.eval_rows, "jsm_eval_rows") || !find(L.dot_f32, "jsm_dot_f32") ||
-        !find(L.embedding, "jsm_embedding") || !find(L.attn_prefill, "jsm_attn_prefill") || !find(L.attn_decode, "jsm_attn_decode"))
+        !find(L.embedding, "jsm_embedding") || !find(L.attn_prefill, "jsm_attn_prefill") || !find(L.attn_decode, "jsm_attn_decode") ||
+        !find(L.rope_rotate, "jsm_rope_rotate") || !find(L.kv_append_q8, "jsm_kv_append_q8") || !find(L.kv_read, "jsm_kv_read") ||
+        !find(L.attn_chunk_scratch_bytes, "jsm_attn_chunk_scratch_bytes") || !find(L.attn_chunk, "jsm_attn_chunk"))
         return PyErr_Format(PyExc_ImportError, "libjasmine_b200: a symbol is missing");
     Py_RETURN_NONE;
 }
@@ -201,6 +211,131 @@ JSM_FAST(attn_decode) {  // q, pool, block_table, context_lens, Hq, Hkv, D, max_
     });
 }
 
+// Rows [T, columns] of adjacent elements; a single row's pitch means nothing.
+struct Rows {
+    void* data = nullptr;
+    int64_t T = 0, pitch = 0;
+    int type = -1;
+};
+bool as_rows(PyObject* o, int64_t columns, Rows& r) {
+    const at::Tensor* t = plain(o);
+    if (!t || t->dim() != 2 || t->size(1) != columns || (columns > 1 && t->stride(1) != 1) || t->size(0) > INT32_MAX) return false;
+    r.data = t->mutable_data_ptr();
+    r.T = t->size(0);
+    r.pitch = r.T > 1 ? t->stride(0) : std::max(t->stride(0), columns);
+    r.type = type_of(*t);
+    return true;
+}
+bool as_ints(PyObject* o, std::initializer_list<int64_t> shape, const int32_t*& p) {
+    const at::Tensor* t = plain(o);
+    if (!t || t->scalar_type() != at::kInt || !t->is_contiguous() || t->dim() != (int64_t)shape.size() || !std::equal(shape.begin(), shape.end(), t->sizes().begin())) return false;
+    p = (const int32_t*)t->mutable_data_ptr();
+    return true;
+}
+// a table [positions, rot / 2, 2], or None
+bool as_rotation(PyObject* o, int rot, const float*& p, int& n) {
+    p = nullptr;
+    n = 0;
+    if (o == Py_None) return true;
+    const at::Tensor* t = plain(o);
+    if (!t || t->scalar_type() != at::kFloat || !t->is_contiguous() || t->dim() != 3 || t->size(1) != rot / 2 || t->size(2) != 2 || t->size(0) > INT32_MAX) return false;
+    p = (const float*)t->mutable_data_ptr();
+    n = (int)t->size(0);
+    return true;
+}
+// pool, scales (or None), block table, starts, context lengths
+struct Cache {
+    void *pool, *scales = nullptr;
+    int pages, max_pages, seqs;
+    const int32_t *table, *starts, *lens;
+};
+bool as_cache(PyObject* pool, PyObject* scales, PyObject* table, PyObject* starts, PyObject* lens, int hkv, int d, Cache& c) {
+    const at::Tensor *p = plain(pool), *b = plain(table), *l = plain(lens);
+    if (!p || !b || !l || p->dim() != 5 || !p->is_contiguous() || p->size(1) != 2 || p->size(2) != hkv || p->size(3) != JSM_PAGE_SIZE || p->size(4) != d || p->size(0) > INT32_MAX)
+        return false;
+    if (b->dim() != 2 || l->dim() != 1 || b->size(1) > INT32_MAX || l->size(0) > INT32_MAX) return false;
+    if (scales != Py_None) {
+        const at::Tensor* s = plain(scales);
+        if (!s || s->scalar_type() != at::kBFloat16 || !s->is_contiguous() || s->dim() != 4 || !std::equal(s->sizes().begin(), s->sizes().end(), p->sizes().begin())) return false;
+        c.scales = s->mutable_data_ptr();
+    }
+    if (p->scalar_type() != (scales != Py_None ? at::kChar : at::kBFloat16)) return false;
+    c.pool = p->mutable_data_ptr();
+    c.pages = (int)p->size(0);
+    c.max_pages = (int)b->size(1);
+    c.seqs = (int)l->size(0);
+    return as_ints(table, {c.seqs, c.max_pages}, c.table) && as_ints(starts, {c.seqs + 1ll}, c.starts) && as_ints(lens, {c.seqs}, c.lens);
+}
+
+JSM_FAST(rope_rotate) {  // q, k, table, Hq, Hkv, D, rot, positions, layout, inverse, q_out, k_out
+    int hq, hkv, d, rot, layout, n;
+    const float* table;
+    JSM_NEED(n_args == 12 && as_int(a[3], hq) && as_int(a[4], hkv) && as_int(a[5], d) && as_int(a[6], rot) && as_int(a[8], layout) && a[2] != Py_None &&
+             as_rotation(a[2], rot, table, n) && hq >= 0 && hkv >= 0 && d > 0 && (hq > 0 || hkv > 0));
+    JSM_NEED((hq > 0) == (a[0] != Py_None) && (hkv > 0) == (a[1] != Py_None));
+    Rows q, k, qo, ko;
+    JSM_NEED(!hq || (as_rows(a[0], (int64_t)hq * d, q) && as_rows(a[10], (int64_t)hq * d, qo) && q.T == qo.T && q.type == qo.type));
+    JSM_NEED(!hkv || (as_rows(a[1], (int64_t)hkv * d, k) && as_rows(a[11], (int64_t)hkv * d, ko) && k.T == ko.T && k.type == ko.type));
+    JSM_NEED(!hq || !hkv || (q.T == k.T && q.type == k.type));
+    const int T = (int)(hq ? q.T : k.T), type = hq ? q.type : k.type;
+    const int32_t* at = nullptr;
+    JSM_NEED(type >= 0 && (a[7] == Py_None || as_ints(a[7], {T}, at)) && (a[9] == Py_True || a[9] == Py_False));
+    const int inverse = a[9] == Py_True;
+    return status_of([&](void* st) {
+        return L.rope_rotate(q.data, q.pitch, qo.data, qo.pitch, hq, k.data, k.pitch, ko.data, ko.pitch, hkv, (jsm_dtype)type, d, table, n, rot, layout, inverse, at, T, st);
+    });
+}
+
+JSM_FAST(kv_append_q8) {  // pool, scales, block_table, k, v, starts, context_lens, Hkv, D, rope, rot, layout
+    int hkv, d, rot, layout, n;
+    const float* table;
+    Cache c;
+    Rows k, v;
+    JSM_NEED(n_args == 12 && as_int(a[7], hkv) && as_int(a[8], d) && as_int(a[10], rot) && as_int(a[11], layout) && as_rotation(a[9], rot, table, n) && hkv > 0 && d > 0 &&
+             a[1] != Py_None && as_cache(a[0], a[1], a[2], a[5], a[6], hkv, d, c) && as_rows(a[3], (int64_t)hkv * d, k) && as_rows(a[4], (int64_t)hkv * d, v));
+    JSM_NEED(k.type == JSM_BF16 && v.type == JSM_BF16 && k.T == v.T && k.pitch == v.pitch);
+    return status_of([&](void* st) {
+        return L.kv_append_q8(c.pool, c.scales, c.pages, c.table, c.max_pages, k.data, v.data, k.pitch, c.starts, c.lens, c.seqs, (int)k.T, hkv, d, table, n, rot, layout, st);
+    });
+}
+
+JSM_FAST(kv_read) {  // pool, scales, block_table, starts, context_lens, T, Hkv, D, k_out, v_out
+    int T, hkv, d;
+    Cache c;
+    Rows k, v;
+    JSM_NEED(n_args == 10 && as_int(a[5], T) && as_int(a[6], hkv) && as_int(a[7], d) && hkv > 0 && d > 0 && as_cache(a[0], a[1], a[2], a[3], a[4], hkv, d, c) &&
+             as_rows(a[8], (int64_t)hkv * d, k) && as_rows(a[9], (int64_t)hkv * d, v));
+    JSM_NEED(k.type >= 0 && k.type == v.type && k.T == T && v.T == T && k.pitch == v.pitch);
+    return status_of([&](void* st) {
+        return L.kv_read(c.pool, c.scales, c.pages, c.table, c.max_pages, c.starts, c.lens, c.seqs, T, hkv, d, k.data, v.data, k.pitch, (jsm_dtype)k.type, st);
+    });
+}
+
+JSM_FAST(attn_chunk) {  // q, pool, scales, block_table, starts, context_lens, Hq, Hkv, D, max_new, max_context, window, scale, scratch, out
+    int hq, hkv, d, most_new, most, window;
+    float scale;
+    Cache c;
+    Rows q, out;
+    JSM_NEED(n_args == 15 && as_int(a[6], hq) && as_int(a[7], hkv) && as_int(a[8], d) && as_int(a[9], most_new) && as_int(a[10], most) && as_int(a[11], window) &&
+             as_float(a[12], scale) && hq > 0 && hkv > 0 && d > 0 && as_cache(a[1], a[2], a[3], a[4], a[5], hkv, d, c) && as_rows(a[0], (int64_t)hq * d, q) &&
+             as_rows(a[14], (int64_t)hq * d, out));
+    JSM_NEED(q.type == JSM_BF16 && out.type == JSM_BF16 && q.T == out.T);
+    void* scratch = nullptr;
+    size_t bytes = 0;
+    at::Tensor own;
+    if (a[13] != Py_None) {
+        JSM_NEED(as_pointer(a[13], scratch) && THPVariable_Unpack(a[13]).is_contiguous());
+        bytes = THPVariable_Unpack(a[13]).nbytes();
+    } else if ((bytes = L.attn_chunk_scratch_bytes(c.seqs, (int)q.T, most_new, most, hq, hkv, d, window)) > 0) {
+        own = at::empty({(int64_t)bytes}, THPVariable_Unpack(a[0]).options().dtype(at::kByte));
+        scratch = own.mutable_data_ptr();
+    }
+    return status_of([&](void* st) {
+        return L.attn_chunk(q.data, q.pitch, c.pool, c.scales, c.pages, c.table, c.max_pages, c.starts, c.lens, c.seqs, (int)q.T, most_new, most, hq, hkv, d, window, scale,
+                            scratch, bytes, out.data, out.pitch, st);
+    });
+}
+
 // torch throws for tensors that keep their memory to themselves (sizes or addresses that are not to be read): the Python code meets the same and raises
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
@@ -213,7 +348,7 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 
 #define JSM_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&guarded<name>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {JSM_METHOD(bind), JSM_METHOD(eval_elementwise), JSM_METHOD(eval_rows), JSM_METHOD(dot_f32), JSM_METHOD(embedding),
-                         JSM_METHOD(attn_prefill), JSM_METHOD(attn_decode), {nullptr, nullptr, 0, nullptr}};
+                         JSM_METHOD(attn_prefill), JSM_METHOD(attn_decode), JSM_METHOD(rope_rotate), JSM_METHOD(kv_append_q8), JSM_METHOD(kv_read), JSM_METHOD(attn_chunk), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

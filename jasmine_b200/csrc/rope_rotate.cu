@@ -62,6 +62,107 @@ __global__ void __launch_bounds__(256) rope_rotate_scalar_kernel(RotateArgs a) {
     }
 }
 
+// Whole 16-byte pieces: a thread has one unit of a head - a piece of each half, a piece of adjacent pairs, or a piece that is not rotated - with its table entries in
+// registers, and takes that unit of every HL-th head, four heads' loads in flight.
+template <typename T>
+struct RotPiece {
+    static constexpr int V = 16 / sizeof(T);
+    float x[V];
+    __device__ __forceinline__ void unpack(const uint4& w) {
+        const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 2) {
+                x[2 * i] = bf16lo(in[i]);
+                x[2 * i + 1] = bf16hi(in[i]);
+            } else {
+                x[i] = __uint_as_float(in[i]);
+            }
+        }
+    }
+    __device__ __forceinline__ uint4 pack() const {
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 2) o[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+            else o[i] = __float_as_uint(x[i]);
+        }
+        return make_uint4(o[0], o[1], o[2], o[3]);
+    }
+};
+
+constexpr int RV_THREADS = 128;
+template <typename T, bool ADJACENT>
+__global__ void __launch_bounds__(RV_THREADS) rope_rotate_vec_kernel(RotateArgs a, int units, int head_lanes) {
+    constexpr int V = RotPiece<T>::V, PAIRS = ADJACENT ? V / 2 : V, U = 4;
+    chain_trigger();
+    chain_wait();
+    const int u = threadIdx.x % units, hl = threadIdx.x / units, heads = a.Hq + a.Hk;
+    if (hl >= head_lanes) return;
+    const int rotated = (ADJACENT ? a.rot : a.rot / 2) / V;      // units that are
+    const int first = (ADJACENT || u < rotated ? u : u + rotated) * V;  // component of the unit's (first) piece
+    const int t = blockIdx.x, pos = a.positions ? a.positions[t] : t;
+    if (pos < 0 || pos >= a.table_len) {
+        if (threadIdx.x == 0) cache_error(a.err, CACHE_BAD_POSITION);
+        return;
+    }
+    float c[PAIRS], s[PAIRS];
+    if (u < rotated) {
+        const float4* e = reinterpret_cast<const float4*>(a.table + (long long)pos * (a.rot / 2) + u * PAIRS);
+#pragma unroll
+        for (int i = 0; i < PAIRS / 2; ++i) {
+            const float4 v = e[i];
+            c[2 * i] = v.x; s[2 * i] = a.sign * v.y; c[2 * i + 1] = v.z; s[2 * i + 1] = a.sign * v.w;
+        }
+    }
+    const T *q = static_cast<const T*>(a.q) + t * a.q_rs + first, *k = static_cast<const T*>(a.k) + t * a.k_rs + first;
+    T *qo = static_cast<T*>(a.q_out) + t * a.qo_rs + first, *ko = static_cast<T*>(a.k_out) + t * a.ko_rs + first;
+    const int half = a.rot / 2;
+    for (int h0 = hl; h0 < heads; h0 += U * head_lanes) {
+        uint4 w[U], w2[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int h = h0 + i * head_lanes;
+            if (h >= heads) break;
+            const T* src = h < a.Hq ? q + (long long)h * a.D : k + (long long)(h - a.Hq) * a.D;
+            w[i] = *reinterpret_cast<const uint4*>(src);
+            if (!ADJACENT && u < rotated) w2[i] = *reinterpret_cast<const uint4*>(src + half);
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int h = h0 + i * head_lanes;
+            if (h >= heads) break;
+            T* dst = h < a.Hq ? qo + (long long)h * a.D : ko + (long long)(h - a.Hq) * a.D;
+            if (u < rotated) {
+                RotPiece<T> x, y;
+                x.unpack(w[i]);
+                if constexpr (ADJACENT) {
+#pragma unroll
+                    for (int n = 0; n < PAIRS; ++n) rotate_pair(x.x[2 * n], x.x[2 * n + 1], c[n], s[n], x.x[2 * n], x.x[2 * n + 1]);
+                } else {
+                    y.unpack(w2[i]);
+#pragma unroll
+                    for (int n = 0; n < PAIRS; ++n) rotate_pair(x.x[n], y.x[n], c[n], s[n], x.x[n], y.x[n]);
+                    *reinterpret_cast<uint4*>(dst + half) = y.pack();
+                }
+                w[i] = x.pack();
+            }
+            *reinterpret_cast<uint4*>(dst) = w[i];
+        }
+    }
+}
+
+template <typename T>
+static jsm_status rotate_vec_launch(const RotateArgs& a, cudaStream_t st) {
+    constexpr int V = RotPiece<T>::V;
+    const int units = a.adjacent ? a.D / V : a.D / V - a.rot / 2 / V, heads = a.Hq + a.Hk;
+    const int head_lanes = RV_THREADS / units < heads ? RV_THREADS / units : heads;
+    JSM_CUDA_CHECK(a.adjacent ? launch_chained(rope_rotate_vec_kernel<T, true>, dim3(a.T), dim3(units * head_lanes), 0, st, a, units, head_lanes)
+                              : launch_chained(rope_rotate_vec_kernel<T, false>, dim3(a.T), dim3(units * head_lanes), 0, st, a, units, head_lanes));
+    JSM_LAUNCH_CHECK();
+    return JSM_OK;
+}
+
 }  // namespace jsm
 
 using namespace jsm;
@@ -84,6 +185,10 @@ extern "C" jsm_status jsm_rope_rotate(const void* d_q, int64_t q_row_stride, voi
     if (odd & (dtype == JSM_F32 ? 3 : 1)) JSM_FAIL(JSM_INVALID_ARG, "jsm_rope_rotate: rows that are not aligned to their elements");
     RotateArgs a{d_q, d_k, d_q_out, d_k_out, q_row_stride, k_row_stride, q_out_row_stride, k_out_row_stride, Hq, Hkv, D, rot_dim, layout == JSM_ROPE_ADJACENT ? 1 : 0,
                  transposed ? -1.0f : 1.0f, reinterpret_cast<const float2*>(d_table), table_len, d_positions, T, tc_error_word()};
+    const int V = dtype == JSM_F32 ? 4 : 8;
+    const int64_t pitches = (Hq ? q_row_stride | q_out_row_stride : 0) | (Hkv ? k_row_stride | k_out_row_stride : 0);
+    if (!((odd | reinterpret_cast<uintptr_t>(d_table)) & 15) && pitches % V == 0 && D % V == 0 && (layout == JSM_ROPE_ADJACENT ? rot_dim : rot_dim / 2) % V == 0 && D / V <= RV_THREADS)
+        return dtype == JSM_F32 ? rotate_vec_launch<float>(a, as_stream(stream)) : rotate_vec_launch<__nv_bfloat16>(a, as_stream(stream));
     const dim3 grid(T < sm_count() * 8 ? T : sm_count() * 8);
     if (dtype == JSM_F32) JSM_CUDA_CHECK(launch_chained(rope_rotate_scalar_kernel<float>, grid, dim3(256), 0, as_stream(stream), a));
     else JSM_CUDA_CHECK(launch_chained(rope_rotate_scalar_kernel<__nv_bfloat16>, grid, dim3(256), 0, as_stream(stream), a));
