@@ -21,7 +21,7 @@ Plan plan_of(int n_seqs, int T, int max_new, int max_context, int Hkv, int G, in
     p.few_rows = most <= 8 ? 8 : most <= 16 ? 16 : G <= 8 ? 8 : 16;
     p.many = most > 16;
     // (with one sequence of more rows there is nothing for the kernel of few)
-    if (p.many && n_seqs == 1 && T == max_new) p.few_rows = 0;
+    if (p.many && ((n_seqs == 1 && T == max_new) || G > p.few_rows)) p.few_rows = 0;
     p.few = p.few_rows ? chunk_few_plan(n_seqs, max_new, max_context, Hkv, window, p.few_rows, D) : FewPlan{0, 0, 0};
     p.bytes = p.few.bytes;
     return p;

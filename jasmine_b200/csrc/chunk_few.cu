@@ -23,6 +23,8 @@ using namespace tc;
 
 constexpr int CF_WARPS = 4;
 constexpr int CF_THREADS = (CF_WARPS + 1) * 32;
+constexpr float CF_NONE = -1.0e30f;  // the reference of a row that has seen nothing
+constexpr float CF_RAISE = 8.0f;     // weights go up to 2^8 before the reference follows the maximum
 constexpr int CF_ERR_FULL = 43, CF_ERR_EMPTY = 44;
 
 __device__ __forceinline__ uint32_t cf_trans(uint32_t x) {
@@ -34,13 +36,13 @@ template <int D, bool Q8>
 struct FewSizes {
     static constexpr int TILE = JSM_PAGE_SIZE * D * (Q8 ? 1 : 2);     // keys, or values, of a page
     static constexpr int STAGE = 2 * TILE + (Q8 ? 1024 : 0);          // keys | values | scales of both (1024-byte steps: the swizzle counts from there)
-    static constexpr int STAGES = 3;
-    static constexpr int SMEM = STAGES * STAGE + 1024;
+    static constexpr int STAGES = 3;                                  // at most: a run of fewer pages has as many
+    static constexpr int smem(int stages, int rows) { return std::max(stages * STAGE, CF_WARPS * rows * D * 4) + 1024; }
 };
 
 template <int D, int NT, bool Q8>
-__global__ void __launch_bounds__(CF_THREADS) chunk_few_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ ChunkArgs a, int few_rows, int n_runs, int run_pages,
-                                                               float* __restrict__ part) {
+__global__ void __launch_bounds__(CF_THREADS, NT == 1 ? 4 : 2) chunk_few_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ ChunkArgs a, int few_rows,
+                                                                                int n_runs, int run_pages, int n_stages, float* __restrict__ part) {
     using Z = FewSizes<D, Q8>;
     constexpr int KS = D / 16;  // steps of 16 components; tiles of 16 components of O^T
     extern __shared__ uint8_t cf_dyn[];
@@ -48,10 +50,9 @@ __global__ void __launch_bounds__(CF_THREADS) chunk_few_kernel(const __grid_cons
     __shared__ uint64_t full_bar[Z::STAGES], empty_bar[Z::STAGES];
     __shared__ int abort_flag;
     __shared__ float sm_m[CF_WARPS][NT * 8], sm_l[CF_WARPS][NT * 8];
-    chain_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < Z::STAGES; ++s) {
+        for (int s = 0; s < n_stages; ++s) {
             mbar_init(&full_bar[s], 1);
             mbar_init(&empty_bar[s], CF_WARPS);
         }
@@ -60,6 +61,7 @@ __global__ void __launch_bounds__(CF_THREADS) chunk_few_kernel(const __grid_cons
     }
     __syncthreads();
     chain_wait();
+    chain_trigger();  // (now: what the merge reads before its own wait was there before this kernel)
     const int run = blockIdx.x % n_runs, seq = blockIdx.x / n_runs, hk = blockIdx.y;
     int row0, n_new, ctx;
     if (!chunk_lengths(a, seq, row0, n_new, ctx) || n_new * a.G > few_rows) return;
@@ -74,7 +76,7 @@ __global__ void __launch_bounds__(CF_THREADS) chunk_few_kernel(const __grid_cons
     float o[NT][KS][4];        // O^T
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        m[n][0] = m[n][1] = -INFINITY;
+        m[n][0] = m[n][1] = CF_NONE;
         l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
         for (int j = 0; j < KS; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.0f;
@@ -84,9 +86,8 @@ __global__ void __launch_bounds__(CF_THREADS) chunk_few_kernel(const __grid_cons
         if (lane == 0) {
             tma_prefetch_desc(&tmap);
             int issued = 0;
-            for (int p = p_begin; p < p_end; ++p) {
-                const int it = p - p_begin, s = it % Z::STAGES;
-                if (it >= Z::STAGES && !mbar_wait(&empty_bar[s], ((it / Z::STAGES) - 1) & 1, &abort_flag, a.c.err, CF_ERR_EMPTY)) break;
+            for (int p = p_begin, s = 0, round = 0; p < p_end; ++p, s = s + 1 == n_stages ? (++round, 0) : s + 1) {
+                if (round > 0 && !mbar_wait(&empty_bar[s], (round - 1) & 1, &abort_flag, a.c.err, CF_ERR_EMPTY)) break;
                 const int page = cache_page(a.c, seq, (page0 + p) * JSM_PAGE_SIZE);
                 uint8_t* dst = stages + s * Z::STAGE;
                 // (a page outside the pool: rows before the first one, which read as zeros)
@@ -107,12 +108,12 @@ __global__ void __launch_bounds__(CF_THREADS) chunk_few_kernel(const __grid_cons
                         tma_load_2d(dst + Z::TILE + c * 8192, &tmap, c * 64, rv, &full_bar[s]);
                     }
                 }
-                issued = it + 1;
+                issued = p - p_begin + 1;
             }
             if (abort_flag) {  // let the copies in flight land before the CTA exits (bounded)
                 const long long t0 = clock64();
-                for (int it = max(0, issued - Z::STAGES); it < issued; ++it)
-                    while (!mbar_try_wait(&full_bar[it % Z::STAGES], (it / Z::STAGES) & 1) && clock64() - t0 < WAIT_LIMIT_CYCLES) {}
+                for (int it = max(0, issued - n_stages); it < issued; ++it)
+                    while (!mbar_try_wait(&full_bar[it % n_stages], (it / n_stages) & 1) && clock64() - t0 < WAIT_LIMIT_CYCLES) {}
             }
         }
     } else {
@@ -146,9 +147,8 @@ __global__ void __launch_bounds__(CF_THREADS) chunk_few_kernel(const __grid_cons
         const int mi = lane >> 3, mr = lane & 7;
         const int krow = warp * 16 + (mi & 1) * 8 + mr, kchunk = mi >> 1;   // ldmatrix, keys
         const int vrow = warp * 16 + (mi >> 1) * 8 + mr, vchunk = mi & 1;   // ldmatrix, values transposed
-        for (int p = p_begin; p < p_end; ++p) {
-            const int it = p - p_begin, s = it % Z::STAGES;
-            if (!mbar_wait(&full_bar[s], (it / Z::STAGES) & 1, &abort_flag, a.c.err, CF_ERR_FULL)) break;
+        for (int p = p_begin, s = 0, round = 0; p < p_end; ++p, s = s + 1 == n_stages ? (++round, 0) : s + 1) {
+            if (!mbar_wait_warp(&full_bar[s], round & 1, &abort_flag, a.c.err, CF_ERR_FULL)) break;
             uint8_t* stage = stages + s * Z::STAGE;
             const int key0 = (page0 + p) * JSM_PAGE_SIZE + warp * 16;
             if (key0 < ctx && key0 + 16 > lo) {
@@ -214,25 +214,32 @@ __global__ void __launch_bounds__(CF_THREADS) chunk_few_kernel(const __grid_cons
                         const int key = key0 + g + (i >> 1) * 8;
                         if (!plain && (key < first[n][i & 1] || key > last[n][i & 1])) x[i] = -INFINITY;
                     }
-                    float corr[2];
+                    // The reference follows the maximum only where a weight would pass 2^8: seldom after the first keys, so sums and accumulators are mostly left alone.
+                    if (__any_sync(0xffffffffu, fmaxf(x[0], x[2]) > m[n][0] + CF_RAISE || fmaxf(x[1], x[3]) > m[n][1] + CF_RAISE)) {
+                        float corr[2];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float mx = fmaxf(x[h], x[h + 2]);
+                        for (int h = 0; h < 2; ++h) {
+                            float mx = fmaxf(x[h], x[h + 2]);
 #pragma unroll
-                        for (int sh = 4; sh < 32; sh <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
-                        const float mn = fmaxf(m[n][h], mx), ref = mn == -INFINITY ? 0.0f : mn;  // (nothing seen so far: weights of 0)
-                        corr[h] = exp2f(m[n][h] - ref);
-                        m[n][h] = mn;
-                        x[h] = exp2f(x[h] - ref);
-                        x[h + 2] = exp2f(x[h + 2] - ref);
-                        l[n][h] = fmaf(l[n][h], corr[h], x[h] + x[h + 2]);
+                            for (int sh = 4; sh < 32; sh <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
+                            const float mn = fmaxf(m[n][h], mx);
+                            corr[h] = fast_ex2(m[n][h] - mn);
+                            m[n][h] = mn;
+                            l[n][h] *= corr[h];
+                        }
+#pragma unroll
+                        for (int j = 0; j < KS; ++j) {
+                            o[n][j][0] *= corr[0];
+                            o[n][j][1] *= corr[1];
+                            o[n][j][2] *= corr[0];
+                            o[n][j][3] *= corr[1];
+                        }
                     }
 #pragma unroll
-                    for (int j = 0; j < KS; ++j) {
-                        o[n][j][0] *= corr[0];
-                        o[n][j][1] *= corr[1];
-                        o[n][j][2] *= corr[0];
-                        o[n][j][3] *= corr[1];
+                    for (int h = 0; h < 2; ++h) {
+                        x[h] = fast_ex2(x[h] - m[n][h]);
+                        x[h + 2] = fast_ex2(x[h + 2] - m[n][h]);
+                        l[n][h] += x[h] + x[h + 2];
                     }
                     pb[n][0] = cf_trans(pack_bf16x2(x[0], x[1]));
                     pb[n][1] = cf_trans(pack_bf16x2(x[2], x[3]));
@@ -323,15 +330,14 @@ __global__ void __launch_bounds__(CF_THREADS) chunk_few_kernel(const __grid_cons
     // a warp per row: the four warps' sums under their largest maximum
     constexpr int N = D / 32;
     for (int r = warp; r < rows; r += CF_WARPS + 1) {
-        float M = -INFINITY, L = 0.0f, acc[N];
+        float M = CF_NONE, L = 0.0f, acc[N];
 #pragma unroll
         for (int w = 0; w < CF_WARPS; ++w) M = fmaxf(M, sm_m[w][r]);
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] = 0.0f;
 #pragma unroll
         for (int w = 0; w < CF_WARPS; ++w) {
-            // a warp that saw no key has sums of zero, or (NaN scores leave no maximum) what is to be handed on
-            const float f = sm_m[w][r] == -INFINITY ? 1.0f : exp2f(sm_m[w][r] - M);
+            const float f = fast_ex2(sm_m[w][r] - M);
             L += f * sm_l[w][r];
 #pragma unroll
             for (int i = 0; i < N; ++i) acc[i] += f * sm_o[(w * NT * 8 + r) * D + lane * N + i];
@@ -360,48 +366,68 @@ __global__ void __launch_bounds__(CF_THREADS) chunk_few_kernel(const __grid_cons
     }
 }
 
-// The runs of a (row, head) under their largest maximum, in the order of the runs; a warp each.
+// The runs of a (row, head) under their largest reference, in the order of the runs.  A block per row (of the sequences of few rows) and head: each of four warps takes eight runs of every 32, all their
+// loads in flight, with a reference of its own; the warps meet in shared memory.  What depends on the lengths alone is worked out while the runs are still under way.
+constexpr int CM_RUNS = 8;
 template <int D, bool Q8>
-__global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant__ ChunkArgs a, int few_rows, int n_runs, int run_pages, const float* __restrict__ part) {
+__global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant__ ChunkArgs a, int few_rows, int n_runs, int run_pages, const float* part) {
     constexpr int N = D / 32;
-    __shared__ int found;
-    chain_trigger();
+    __shared__ float sm_m[4], sm_l[4], sm_o[4][D];
+    const int tokens = gridDim.x / a.c.n_seqs, s = blockIdx.x / tokens, i = blockIdx.x % tokens, head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int row0 = 0, n_new = 0, ctx = 0;
+    const bool mine = chunk_lengths(a, s, row0, n_new, ctx) && n_new * a.G <= few_rows && i < n_new;
+    const int n_pages = (ctx - 1) / JSM_PAGE_SIZE + 1 - first_key(a.window, ctx - n_new) / JSM_PAGE_SIZE, n = mine ? (n_pages + run_pages - 1) / run_pages : 0;
+    const int t = row0 + i, hk = head / a.G, r = i * a.G + head % a.G, step = few_rows * (D + 2);
+    const float* src = part + ((long long)s * a.c.Hkv + hk) * n_runs * step + r * (D + 2);
     chain_wait();
-    const int t = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int s = find_sequence(a.c, t, &found);
-    if (s < 0 || head >= a.Hq) return;
-    int row0, n_new, ctx;
-    if (!chunk_lengths(a, s, row0, n_new, ctx) || n_new * a.G > few_rows) return;
-    const int n_pages = (ctx - 1) / JSM_PAGE_SIZE + 1 - first_key(a.window, ctx - n_new) / JSM_PAGE_SIZE, n = (n_pages + run_pages - 1) / run_pages;
-    if (n == 1) return;
-    const int hk = head / a.G, r = (t - row0) * a.G + head % a.G;
-    const float* src = part + ((long long)s * a.c.Hkv + hk) * n_runs * (few_rows * (D + 2)) + r * (D + 2);
-    const int step = few_rows * (D + 2);
-    float M = -INFINITY, L = 0.0f, acc[N];
-    for (int c = lane; c < n; c += 32) M = fmaxf(M, src[(long long)c * step + D]);
-    M = warp_max(M);
+    chain_trigger();
+    if (n <= 1) return;
+    float m = CF_NONE, l = 0.0f, acc[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] = 0.0f;
+    for (int c0 = warp * CM_RUNS; c0 < n; c0 += 4 * CM_RUNS) {
+        float v[CM_RUNS][N];
+        float2 ml = make_float2(CF_NONE, 0.0f);
+        if (lane < CM_RUNS && c0 + lane < n) ml = *reinterpret_cast<const float2*>(src + (long long)(c0 + lane) * step + D);
+#pragma unroll
+        for (int c = 0; c < CM_RUNS; ++c) {
+            const float* x = src + (long long)min(c0 + c, n - 1) * step + lane * N;
+#pragma unroll
+            for (int i = 0; i < N; i += 2) *reinterpret_cast<float2*>(&v[c][i]) = *reinterpret_cast<const float2*>(x + i);
+        }
+        const float mn = fmaxf(m, warp_max(ml.x)), corr = fast_ex2(m - mn);
+        const float f = lane < CM_RUNS && c0 + lane < n ? fast_ex2(ml.x - mn) : 0.0f;
+        m = mn;
+        l = fmaf(l, corr, warp_sum(f * ml.y));
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] *= corr;
+#pragma unroll
+        for (int c = 0; c < CM_RUNS; ++c) {
+            const float w = __shfl_sync(0xffffffffu, f, c);
+            if (c0 + c < n)
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc[i] = fmaf(w, v[c][i], acc[i]);
+        }
+    }
+    if (lane == 0) {
+        sm_m[warp] = m;
+        sm_l[warp] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) sm_o[warp][lane * N + i] = acc[i];
+    __syncthreads();
+    if (warp != 0) return;
+    float M = CF_NONE, L = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_m[w]);
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = 0.0f;
-    for (int c0 = 0; c0 < n; c0 += 32) {
-        float f = 0.0f, lc = 0.0f;
-        if (c0 + lane < n) {
-            const float2 ml = *reinterpret_cast<const float2*>(src + (long long)(c0 + lane) * step + D);
-            f = ml.x == -INFINITY ? 1.0f : exp2f(ml.x - M);
-            lc = f * ml.y;
-        }
-        L += warp_sum(lc);
-        const int k = min(32, n - c0);
-#pragma unroll 8
-        for (int c = 0; c < k; ++c) {
-            const float w = __shfl_sync(0xffffffffu, f, c);
-            const float* x = src + (long long)(c0 + c) * step + lane * N;
 #pragma unroll
-            for (int i = 0; i < N; i += 2) {
-                const float2 v = *reinterpret_cast<const float2*>(x + i);
-                acc[i] = fmaf(w, v.x, acc[i]);
-                acc[i + 1] = fmaf(w, v.y, acc[i + 1]);
-            }
-        }
+    for (int w = 0; w < 4; ++w) {
+        const float f = fast_ex2(sm_m[w] - M);
+        L += f * sm_l[w];
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] += f * sm_o[w][lane * N + i];
     }
     bool fine = true;
 #pragma unroll
@@ -410,7 +436,7 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant_
         fine = fine && fabsf(acc[i]) <= 3.402823466e38f;
     }
     if (!__all_sync(0xffffffffu, fine)) {
-        attend_row<D, Q8>(a, s, t, head, ctx - n_new + t - row0);
+        attend_row<D, Q8>(a, s, t, head, ctx - n_new + i);
         return;
     }
     __nv_bfloat16* dst = a.out + t * a.out_rs + (long long)head * D + lane * N;
@@ -439,12 +465,13 @@ static jsm_status few_go(const ChunkArgs& a, const FewPlan& f, float* part, cuda
                             : make_tmap_bf16_2d(&map, a.c.pool, rows, D, D, JSM_PAGE_SIZE, 64);
     if (s != JSM_OK) return s;
     static DeviceOnce once;
-    JSM_CUDA_CHECK(allow_shared(once, chunk_few_kernel<D, NT, Q8>, Z::SMEM));
-    JSM_CUDA_CHECK(launch_chained(chunk_few_kernel<D, NT, Q8>, dim3((unsigned)f.n_runs * a.c.n_seqs, a.c.Hkv), dim3(CF_THREADS), (size_t)Z::SMEM, st, map, a, NT * 8, f.n_runs,
-                                  f.run_pages, part));
+    JSM_CUDA_CHECK(allow_shared(once, chunk_few_kernel<D, NT, Q8>, Z::smem(Z::STAGES, NT * 8)));
+    const int stages = std::min(f.run_pages, Z::STAGES);
+    JSM_CUDA_CHECK(launch_chained(chunk_few_kernel<D, NT, Q8>, dim3((unsigned)f.n_runs * a.c.n_seqs, a.c.Hkv), dim3(CF_THREADS), (size_t)Z::smem(stages, NT * 8), st, map, a,
+                                  NT * 8, f.n_runs, f.run_pages, stages, part));
     JSM_LAUNCH_CHECK();
     if (f.n_runs > 1) {
-        JSM_CUDA_CHECK(launch_chained(chunk_merge_kernel<D, Q8>, dim3(a.T, (a.Hq + 3) / 4), dim3(128), 0, st, a, NT * 8, f.n_runs, f.run_pages, (const float*)part));
+        JSM_CUDA_CHECK(launch_chained(chunk_merge_kernel<D, Q8>, dim3((unsigned)a.c.n_seqs * std::min(a.max_new, NT * 8 / a.G), a.Hq), dim3(128), 0, st, a, NT * 8, f.n_runs, f.run_pages, (const float*)part));
         JSM_LAUNCH_CHECK();
     }
     return JSM_OK;

@@ -513,61 +513,59 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
         if constexpr (Q8) {
             const int cw = warp - CK_CONVERT;
             // Reads and writes of 16 bytes, eight lanes at a time over all banks: the lanes have four pieces of two rows whose numbers differ in bit 0 (the places of the
-            // bf16 pieces) and, where a row is a whole line, in bit 2 (the places of the raw pieces).
+            // bf16 pieces) and, where a row is a whole line, in bit 2 (the places of the raw pieces).  The loops over keys / values and the two pages stay rolled: unrolled,
+            // the four warps wait for instructions (27 KB of them; 335 us for 1000 of 9000 positions).
+            constexpr int STEPS = D == 128 ? 4 : 2;
             const int c4 = lane & 3, second = (lane >> 2) & 1;
+            int row[STEPS];
+            uint32_t src[STEPS], dst[STEPS];
+#pragma unroll
+            for (int n = 0; n < STEPS; ++n) {
+                if constexpr (D == 128) {
+                    const int slab = (lane >> 3) & 1, pair = (n & 1) * 2 + (lane >> 4), r = cw * 16 + (n >> 1) * 8 + (second ? pair ^ 5 : pair);
+                    row[n] = r;
+                    src[n] = r * 128 + (((slab * 4 + c4) ^ (r & 7)) << 4);
+                    dst[n] = slab * Z::SLAB + r * 128 + (((c4 * 2) ^ (r & 7)) << 4);
+                } else {
+                    const int r = cw * 16 + n * 8 + (lane >> 3) * 2 + second, line = r >> 1;
+                    row[n] = r;
+                    src[n] = line * 128 + ((((r & 1) * 4 + c4) ^ (line & 7)) << 4);
+                    dst[n] = r * 128 + (((c4 * 2) ^ (r & 7)) << 4);
+                }
+            }
             bool ok = true;
             for (int j = j_lo; j < n_max && ok; ++j) {
                 const int i = j - j_lo, s = i % ST;
+#pragma unroll 1
+                for (int slot = 0; slot < 4; ++slot) {
+                    const int value = slot >> 1, half = slot & 1;
+                    if (half == 0 && i >= ST && !mbar_wait_warp(value ? &v_empty[s] : &k_empty[s], ((i / ST) & 1) ^ 1, &abort_flag, a.c.err, TC_TIMEOUT_EMPTY)) { ok = false; break; }
+                    if (!mbar_wait_warp(&raw_full[slot], i & 1, &abort_flag, a.c.err, TC_TIMEOUT_FULL)) { ok = false; break; }
+                    const uint8_t* raw = raw_smem + slot * Z::RAW;
+                    uint8_t* to = (value ? v_smem : k_smem) + s * Z::TILE + half * (JSM_PAGE_SIZE * 128);
+                    // values that no row sees become zeros: a weight of zero meets a number
+                    const int key0 = base + j * CK_BN + half * JSM_PAGE_SIZE, from = value ? lo - key0 : -1, until = value ? end - key0 : JSM_PAGE_SIZE;
+                    uint4 w[STEPS];
+                    uint32_t scale[STEPS];
 #pragma unroll
-                for (int value = 0; value < 2 && ok; ++value) {
-                    uint8_t* dst = (value ? v_smem : k_smem) + s * Z::TILE;
-                    if (i >= ST && !mbar_wait_warp(value ? &v_empty[s] : &k_empty[s], ((i / ST) & 1) ^ 1, &abort_flag, a.c.err, TC_TIMEOUT_EMPTY)) { ok = false; break; }
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const int slot = value * 2 + half;
-                        if (!mbar_wait_warp(&raw_full[slot], i & 1, &abort_flag, a.c.err, TC_TIMEOUT_FULL)) { ok = false; break; }
-                        const uint8_t* raw = raw_smem + slot * Z::RAW;
-                        const int key0 = base + j * CK_BN + half * JSM_PAGE_SIZE;
-#pragma unroll
-                        for (int n = 0; n < (D == 128 ? 4 : 2); ++n) {
-                            int r, piece, slab;  // row of the page, piece of 16 numbers in the row, slab of 64 columns
-                            const uint8_t* src;
-                            if constexpr (D == 128) {
-                                slab = (lane >> 3) & 1;
-                                const int pair = (n & 1) * 2 + (lane >> 4);
-                                r = cw * 16 + (n >> 1) * 8 + (second ? pair ^ 5 : pair);
-                                piece = slab * 4 + c4;
-                                src = raw + r * 128 + ((piece ^ (r & 7)) << 4);
-                            } else {
-                                slab = 0;
-                                r = cw * 16 + n * 8 + (lane >> 3) * 2 + second;
-                                piece = c4;
-                                const int line = r >> 1;
-                                src = raw + line * 128 + ((((r & 1) * 4 + piece) ^ (line & 7)) << 4);
-                            }
-                            const uint4 w = *reinterpret_cast<const uint4*>(src);
-                            uint32_t scale = raw_scales[slot][r];
-                            if (value && (key0 + r < lo || key0 + r >= end)) scale = 0;  // (a value that no row sees: a weight of zero meets a number)
-                            scale *= 0x00010001u;
-                            const uint32_t in[4] = {w.x, w.y, w.z, w.w};
-                            uint32_t out[8];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                out[2 * k] = q8_value2(__byte_perm(in[k], 0, 0x1100), scale);
-                                out[2 * k + 1] = q8_value2(__byte_perm(in[k], 0, 0x3322), scale);
-                            }
-                            uint8_t* to = dst + slab * Z::SLAB + (half * JSM_PAGE_SIZE + r) * 128;
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                                *reinterpret_cast<uint4*>(to + (((c4 * 2 + e) ^ (r & 7)) << 4)) = make_uint4(out[4 * e], out[4 * e + 1], out[4 * e + 2], out[4 * e + 3]);
-                        }
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&raw_empty[slot]);
+                    for (int n = 0; n < STEPS; ++n) {
+                        w[n] = *reinterpret_cast<const uint4*>(raw + src[n]);
+                        scale[n] = raw_scales[slot][row[n]];
                     }
-                    if (!ok) break;
-                    fence_proxy_async_smem();
+#pragma unroll
+                    for (int n = 0; n < STEPS; ++n) {
+                        const uint32_t sc = row[n] < from || row[n] >= until ? 0u : scale[n] * 0x00010001u;
+                        *reinterpret_cast<uint4*>(to + dst[n]) = make_uint4(q8_value2(__byte_perm(w[n].x, 0, 0x1100), sc), q8_value2(__byte_perm(w[n].x, 0, 0x3322), sc),
+                                                                            q8_value2(__byte_perm(w[n].y, 0, 0x1100), sc), q8_value2(__byte_perm(w[n].y, 0, 0x3322), sc));
+                        *reinterpret_cast<uint4*>(to + (dst[n] ^ 16)) = make_uint4(q8_value2(__byte_perm(w[n].z, 0, 0x1100), sc), q8_value2(__byte_perm(w[n].z, 0, 0x3322), sc),
+                                                                                   q8_value2(__byte_perm(w[n].w, 0, 0x1100), sc), q8_value2(__byte_perm(w[n].w, 0, 0x3322), sc));
+                    }
+                    if (half == 1) fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(value ? &v_full[s] : &k_full[s]);
+                    if (lane == 0) {
+                        mbar_arrive(&raw_empty[slot]);
+                        if (half == 1) mbar_arrive(value ? &v_full[s] : &k_full[s]);
+                    }
                 }
             }
         }
@@ -582,42 +580,80 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
     ck_cluster_arrive();
     ck_cluster_wait();  // every CTA's sums are in its shared memory
     if (work && !abort_flag && warp >= CK_SOFTMAX && warp < CK_CONVERT) {
-        constexpr int N = D / 32;
+        constexpr int N = D / 32, R = 4;
         const int n_rows = f.tile_tokens * a.G;
         const uint32_t sums = smem_u32(tiles), ml = smem_u32(sm_ml);
-        for (int r = part + f.share * (warp - CK_SOFTMAX); r < 2 * CK_BM; r += f.share * 8) {
-            const int t = r / CK_BM, at = r % CK_BM, tk = tok[t] + at / a.G;
-            if (at >= n_rows || tk >= n_new) continue;
-            float M = CK_NONE, L = 0.0f, acc[N];
-            for (int p = 0; p < f.share; ++p) M = fmaxf(M, ck_load2(ck_peer(ml + r * 8, p)).x);
+        // Four rows at a time, every CTA's part of them requested before the first is used: lane 8 i + p has maximum and sum of row i in CTA p.
+        for (int k0 = (warp - CK_SOFTMAX) * R; part + f.share * k0 < 2 * CK_BM; k0 += 8 * R) {
+            int row[R], at[R], tk[R];
+            bool on[R];
 #pragma unroll
-            for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+            for (int i = 0; i < R; ++i) {
+                row[i] = part + f.share * (k0 + i);
+                const int t = row[i] / CK_BM;
+                at[i] = row[i] % CK_BM;
+                tk[i] = (t ? tok[1] : tok[0]) + at[i] / a.G;
+                on[i] = row[i] < 2 * CK_BM && at[i] < n_rows && tk[i] < n_new;
+            }
+            if (!on[0] && !on[1] && !on[2] && !on[3]) continue;
+            const int li = lane >> 3, lp = lane & 7, lrow = part + f.share * (k0 + li);
+            float2 mine = make_float2(CK_NONE, 0.0f);
+            if (lp < f.share && lrow < 2 * CK_BM) mine = ck_load2(ck_peer(ml + lrow * 8, lp));
+            float M = mine.x;
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+            const bool none = mine.x == CK_NONE && mine.y == 0.0f;  // that CTA had none of the row's keys
+            const float weight = none ? 0.0f : ex2_approx(mine.x - M);
+            float L = weight * mine.y;
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+            float acc[R][N];
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+#pragma unroll
+                for (int n = 0; n < N; ++n) acc[i][n] = 0.0f;
+            const unsigned nothing = __ballot_sync(0xffffffffu, none);
+#pragma unroll 2
             for (int p = 0; p < f.share; ++p) {
-                const float2 v = ck_load2(ck_peer(ml + r * 8, p));
-                if (v.x == CK_NONE && v.y == 0.0f) continue;  // it had none of the row's keys
-                const float w = ex2_approx(v.x - M);
-                L = fmaf(w, v.y, L);
-                const uint32_t src = ck_peer(sums + r * (D * 4) + (((lane * N / 4) ^ (r & 7)) * 16) + (N == 2 ? (lane & 1) * 8 : 0), p);
-                if constexpr (N == 4) {
-                    const float4 x = ck_load4(src);
-                    acc[0] = fmaf(w, x.x, acc[0]); acc[1] = fmaf(w, x.y, acc[1]); acc[2] = fmaf(w, x.z, acc[2]); acc[3] = fmaf(w, x.w, acc[3]);
-                } else {
-                    const float2 x = ck_load2(src);
-                    acc[0] = fmaf(w, x.x, acc[0]); acc[1] = fmaf(w, x.y, acc[1]);
+                float x[R][N];
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    const int r = min(row[i], 2 * CK_BM - 1);
+                    const uint32_t src = ck_peer(sums + r * (D * 4) + (((lane * N / 4) ^ (r & 7)) * 16) + (N == 2 ? (lane & 1) * 8 : 0), p);
+                    if constexpr (N == 4) {
+                        const float4 v = ck_load4(src);
+                        x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
+                    } else {
+                        const float2 v = ck_load2(src);
+                        x[i][0] = v.x; x[i][1] = v.y;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    const float w = __shfl_sync(0xffffffffu, weight, i * 8 + p);
+                    if (!(nothing >> (i * 8 + p) & 1))
+#pragma unroll
+                        for (int n = 0; n < N; ++n) acc[i][n] = fmaf(w, x[i][n], acc[i][n]);
                 }
             }
-            bool fine = true;
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                acc[i] /= L;
-                fine = fine && fabsf(acc[i]) <= 3.402823466e38f;
-            }
-            if (__all_sync(0xffffffffu, fine)) {
-                __nv_bfloat16* dst = a.out + (row0 + tk) * a.out_rs + (long long)(hk * a.G + at % a.G) * D + lane * N;
+            for (int i = 0; i < R; ++i) {
+                if (!on[i]) continue;
+                const float inv = 1.0f / __shfl_sync(0xffffffffu, L, i * 8);
+                bool fine = true;
 #pragma unroll
-                for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16x2(acc[i], acc[i + 1]);
-            } else {
-                attend_row<D, Q8>(a, seq, row0 + tk, hk * a.G + at % a.G, past + tk);
+                for (int n = 0; n < N; ++n) {
+                    acc[i][n] *= inv;
+                    fine = fine && fabsf(acc[i][n]) <= 3.402823466e38f;
+                }
+                const int head = hk * a.G + at[i] % a.G;
+                if (__all_sync(0xffffffffu, fine)) {
+                    __nv_bfloat16* dst = a.out + (row0 + tk[i]) * a.out_rs + (long long)head * D + lane * N;
+#pragma unroll
+                    for (int n = 0; n < N; n += 2) *reinterpret_cast<uint32_t*>(dst + n) = pack_bf16x2(acc[i][n], acc[i][n + 1]);
+                } else {
+                    attend_row<D, Q8>(a, seq, row0 + tk[i], head, past + tk[i]);
+                }
             }
         }
     }
