@@ -65,18 +65,44 @@ __device__ __forceinline__ long long cache_row(const CacheView& c, int page, int
     return (((long long)page * 2 + value) * c.Hkv + head) * JSM_PAGE_SIZE + pos % JSM_PAGE_SIZE;
 }
 
-// Two numbers of an 8-bit cache, in the low bytes of the halves of p, as bf16: 0x4300 | the low seven bits is 128 + them, 0x4300 | the sign bit is 128 or 256, and the
-// difference is the number, exactly.
-__device__ __forceinline__ uint32_t q8_pair(uint32_t p) {
-    const uint32_t lo = (p & 0x007F007Fu) | 0x43004300u, hi = (p & 0x00800080u) | 0x43004300u;
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&hi));
-    return *reinterpret_cast<const uint32_t*>(&r);
+// shared memory by its 32-bit address: a pointer that has been rounded up is generic to the compiler, with 64-bit arithmetic for every access
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
 }
-// times their scales: the values that the cache stands for, one rounding
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts128(uint32_t a, const uint4& v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// Two numbers of an 8-bit cache, in the low bytes of the halves of p, times their scales: the values that the cache stands for.  0x4300 | the low seven bits is 128 + them
+// as bf16, 0x4300 | the sign bit is 128 or 256; the difference is the number, exactly, and its product with the scale is rounded once.
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t c) {
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(mask), "r"(c));
+    return d;
+}
 __device__ __forceinline__ uint32_t q8_value2(uint32_t p, uint32_t scale2) {
-    const uint32_t n = q8_pair(p);
-    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&n), *reinterpret_cast<const __nv_bfloat162*>(&scale2));
-    return *reinterpret_cast<const uint32_t*>(&r);
+    const uint32_t lo = and_or(p, 0x007F007Fu, 0x43004300u), hi = and_or(p, 0x00800080u, 0x43004300u);
+    uint32_t n, r;
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(n) : "r"(lo), "r"(hi));
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(n), "r"(scale2));
+    return r;
 }
 
 // rotation of a pair, every product rounded on its own

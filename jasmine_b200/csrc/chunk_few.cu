@@ -16,6 +16,7 @@
 #include "mma_utils.cuh"
 #include <math.h>
 #include <algorithm>
+#include <type_traits>
 
 namespace jsm {
 
@@ -35,18 +36,19 @@ __device__ __forceinline__ uint32_t cf_trans(uint32_t x) {
 template <int D, bool Q8>
 struct FewSizes {
     static constexpr int TILE = JSM_PAGE_SIZE * D * (Q8 ? 1 : 2);     // keys, or values, of a page
-    static constexpr int STAGE = 2 * TILE + (Q8 ? 1024 : 0);          // keys | values | scales of both (1024-byte steps: the swizzle counts from there)
+    static constexpr int STAGE = 2 * TILE + (Q8 ? 1024 : 0);          // keys | values | scales of both; bf16: for each 64 columns keys | values (1024-byte steps: the swizzle counts from there)
     static constexpr int STAGES = 3;                                  // at most: a run of fewer pages has as many
     static constexpr int smem(int stages, int rows) { return std::max(stages * STAGE, CF_WARPS * rows * D * 4) + 1024; }
 };
 
 template <int D, int NT, bool Q8>
-__global__ void __launch_bounds__(CF_THREADS, NT == 1 ? 4 : 2) chunk_few_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ ChunkArgs a, int few_rows,
-                                                                                int n_runs, int run_pages, int n_stages, float* __restrict__ part) {
+__global__ void __launch_bounds__(CF_THREADS, NT == 1 ? 4 : 2) chunk_few_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ CUtensorMap tmap_scales,
+                                                                                const __grid_constant__ ChunkArgs a, int few_rows,                                                                                int n_runs, int run_pages, int n_stages, float* __restrict__ part) {
     using Z = FewSizes<D, Q8>;
     constexpr int KS = D / 16;  // steps of 16 components; tiles of 16 components of O^T
     extern __shared__ uint8_t cf_dyn[];
     uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(cf_dyn) + 1023) & ~uintptr_t(1023));
+    const uint32_t stages_u32 = smem_u32(stages);
     __shared__ uint64_t full_bar[Z::STAGES], empty_bar[Z::STAGES];
     __shared__ int abort_flag;
     __shared__ float sm_m[CF_WARPS][NT * 8], sm_l[CF_WARPS][NT * 8];
@@ -85,28 +87,22 @@ __global__ void __launch_bounds__(CF_THREADS, NT == 1 ? 4 : 2) chunk_few_kernel(
     if (warp == CF_WARPS) {
         if (lane == 0) {
             tma_prefetch_desc(&tmap);
+            if (Q8) tma_prefetch_desc(&tmap_scales);
             int issued = 0;
             for (int p = p_begin, s = 0, round = 0; p < p_end; ++p, s = s + 1 == n_stages ? (++round, 0) : s + 1) {
                 if (round > 0 && !mbar_wait(&empty_bar[s], (round - 1) & 1, &abort_flag, a.c.err, CF_ERR_EMPTY)) break;
                 const int page = cache_page(a.c, seq, (page0 + p) * JSM_PAGE_SIZE);
                 uint8_t* dst = stages + s * Z::STAGE;
-                // (a page outside the pool: rows before the first one, which read as zeros)
-                const int rk = page < 0 ? -JSM_PAGE_SIZE : (int)cache_row(a.c, page, 0, hk, 0), rv = page < 0 ? -JSM_PAGE_SIZE : (int)cache_row(a.c, page, 1, hk, 0);
+                // Keys and values of a page come by one request (a slab of 64 columns each, for bf16), the scales of both by another: the rate of a thread's requests would
+                // bound the stream.  A page outside the pool: a place before the first page, which reads as zeros.
+                const int z = page < 0 ? -2 : 2 * page;
+                mbar_expect_tx(&full_bar[s], 2 * Z::TILE + (Q8 ? 256 : 0));
                 if constexpr (Q8) {
-                    mbar_expect_tx(&full_bar[s], 2 * Z::TILE + (page < 0 ? 0 : 256));
-                    tma_load_2d(dst, &tmap, 0, D == 64 ? rk / 2 : rk, &full_bar[s]);  // (heads of 64: a line of 128 bytes has two positions)
-                    tma_load_2d(dst + Z::TILE, &tmap, 0, D == 64 ? rv / 2 : rv, &full_bar[s]);
-                    if (page >= 0) {
-                        bulk_load(dst + 2 * Z::TILE, a.c.scales + rk, 128, &full_bar[s]);
-                        bulk_load(dst + 2 * Z::TILE + 128, a.c.scales + rv, 128, &full_bar[s]);
-                    }
+                    tma_load_3d(dst, &tmap, 0, hk * (JSM_PAGE_SIZE * D / 128), z, &full_bar[s]);
+                    tma_load_3d(dst + 2 * Z::TILE, &tmap_scales, 0, hk, z, &full_bar[s]);
                 } else {
-                    mbar_expect_tx(&full_bar[s], 2 * Z::TILE);
 #pragma unroll
-                    for (int c = 0; c < D / 64; ++c) {
-                        tma_load_2d(dst + c * 8192, &tmap, c * 64, rk, &full_bar[s]);
-                        tma_load_2d(dst + Z::TILE + c * 8192, &tmap, c * 64, rv, &full_bar[s]);
-                    }
+                    for (int c = 0; c < D / 64; ++c) tma_load_3d(dst + c * 16384, &tmap, c * 64, hk * JSM_PAGE_SIZE, z, &full_bar[s]);
                 }
                 issued = p - p_begin + 1;
             }
@@ -147,152 +143,163 @@ __global__ void __launch_bounds__(CF_THREADS, NT == 1 ? 4 : 2) chunk_few_kernel(
         const int mi = lane >> 3, mr = lane & 7;
         const int krow = warp * 16 + (mi & 1) * 8 + mr, kchunk = mi >> 1;   // ldmatrix, keys
         const int vrow = warp * 16 + (mi >> 1) * 8 + mr, vchunk = mi & 1;   // ldmatrix, values transposed
-        for (int p = p_begin, s = 0, round = 0; p < p_end; ++p, s = s + 1 == n_stages ? (++round, 0) : s + 1) {
-            if (!mbar_wait_warp(&full_bar[s], round & 1, &abort_flag, a.c.err, CF_ERR_FULL)) break;
-            uint8_t* stage = stages + s * Z::STAGE;
-            const int key0 = (page0 + p) * JSM_PAGE_SIZE + warp * 16;
-            if (key0 < ctx && key0 + 16 > lo) {
-                const bool edge = key0 < lo || key0 + 16 > ctx;
-                if (!Q8 && edge) {  // values that no row sees: a weight of zero meets a number
-                    uint8_t* vb = stage + Z::TILE;
-                    for (int i = lane; i < 16 * (D / 8); i += 32) {
-                        const int row = warp * 16 + i / (D / 8), c = i % (D / 8), key = key0 + i / (D / 8);
-                        if (key < lo || key >= ctx) *reinterpret_cast<uint4*>(vb + (c >> 3) * 8192 + row * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_proxy_async_smem();  // the stage is overwritten by a bulk copy later
-                    __syncwarp();
-                }
-                float sc[NT][4];
+        // 8-bit pages: places of this lane's pieces in a stage (the keys of a warp are whole swizzle groups apart)
+        uint32_t k_at[2], v_at[2][2];
+        if constexpr (Q8) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
-                if constexpr (Q8) {
-                    const uint16_t* scales = reinterpret_cast<const uint16_t*>(stage + 2 * Z::TILE);
-                    uint32_t kw[2][D / 16];  // D / 4 numbers of keys g and g + 8
-                    uint32_t ks2[2];
+            for (int h = 0; h < 2; ++h) {
+                const int byte = (warp * 16 + g + h * 8) * D + (D / 4) * t4, line = byte >> 7;
+                k_at[h] = line * 128 + ((((byte >> 4) & 7) ^ (line & 7)) << 4);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int key = warp * 16 + g + h * 8;
-                        ks2[h] = scales[key] * 0x00010001u;
-#pragma unroll
-                        for (int c = 0; c < D / 64; ++c) {
-                            const int byte = key * D + (D / 4) * t4 + c * 16, line = byte >> 7;
-                            const uint4 w = *reinterpret_cast<const uint4*>(stage + line * 128 + ((((byte >> 4) & 7) ^ (line & 7)) << 4));
-                            kw[h][c * 4] = w.x; kw[h][c * 4 + 1] = w.y; kw[h][c * 4 + 2] = w.z; kw[h][c * 4 + 3] = w.w;
-                        }
-                    }
-#pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        uint32_t f[4];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            f[h] = q8_value2(__byte_perm(kw[h][ks], 0, 0x1100), ks2[h]);
-                            f[h + 2] = q8_value2(__byte_perm(kw[h][ks], 0, 0x3322), ks2[h]);
-                        }
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) mma_16816(sc[n], f, qb[n][ks][0], qb[n][ks][1]);
-                    }
-                } else {
-                    const uint32_t kbase = smem_u32(stage);
-#pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        const int c = ks * 2 + kchunk;
-                        uint32_t f[4];
-                        ldsm_x4(kbase + (c >> 3) * 8192 + krow * 128 + (((c & 7) ^ (krow & 7)) << 4), f);
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) mma_16816(sc[n], f, qb[n][ks][0], qb[n][ks][1]);
-                    }
-                }
-                // sc[n][0], [1]: key g, the thread's two rows; [2], [3]: key g + 8
-                const bool plain = key0 >= all_from && key0 + 15 <= all_to;
-                uint32_t pb[NT][2];
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float x[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        x[i] = sc[n][i] * a.scale_log2;
-                        const int key = key0 + g + (i >> 1) * 8;
-                        if (!plain && (key < first[n][i & 1] || key > last[n][i & 1])) x[i] = -INFINITY;
-                    }
-                    // The reference follows the maximum only where a weight would pass 2^8: seldom after the first keys, so sums and accumulators are mostly left alone.
-                    if (__any_sync(0xffffffffu, fmaxf(x[0], x[2]) > m[n][0] + CF_RAISE || fmaxf(x[1], x[3]) > m[n][1] + CF_RAISE)) {
-                        float corr[2];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            float mx = fmaxf(x[h], x[h + 2]);
-#pragma unroll
-                            for (int sh = 4; sh < 32; sh <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
-                            const float mn = fmaxf(m[n][h], mx);
-                            corr[h] = fast_ex2(m[n][h] - mn);
-                            m[n][h] = mn;
-                            l[n][h] *= corr[h];
-                        }
-#pragma unroll
-                        for (int j = 0; j < KS; ++j) {
-                            o[n][j][0] *= corr[0];
-                            o[n][j][1] *= corr[1];
-                            o[n][j][2] *= corr[0];
-                            o[n][j][3] *= corr[1];
-                        }
-                    }
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        x[h] = fast_ex2(x[h] - m[n][h]);
-                        x[h + 2] = fast_ex2(x[h + 2] - m[n][h]);
-                        l[n][h] += x[h] + x[h + 2];
-                    }
-                    pb[n][0] = cf_trans(pack_bf16x2(x[0], x[1]));
-                    pb[n][1] = cf_trans(pack_bf16x2(x[2], x[3]));
-                }
-                if constexpr (Q8) {
-                    const uint16_t* scales = reinterpret_cast<const uint16_t*>(stage + 2 * Z::TILE + 128);
-                    uint32_t vw[4][D / 32], vs[2];  // D / 8 numbers of keys 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9: components (D / 8) g and up
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int k2 = warp * 16 + t4 * 2 + h * 8, key = key0 + t4 * 2 + h * 8;
-                        vs[h] = *reinterpret_cast<const uint32_t*>(scales + k2);
-                        if (edge) {
-                            if (key < lo || key >= ctx) vs[h] &= 0xFFFF0000u;
-                            if (key + 1 < lo || key + 1 >= ctx) vs[h] &= 0x0000FFFFu;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const int byte = (k2 + i) * D + (D / 8) * g, line = byte >> 7;
-                            const uint8_t* at = stage + Z::TILE + line * 128 + ((((byte >> 4) & 7) ^ (line & 7)) << 4);
-                            if constexpr (D == 128) {
-                                const uint4 w = *reinterpret_cast<const uint4*>(at);
-                                vw[h * 2 + i][0] = w.x; vw[h * 2 + i][1] = w.y; vw[h * 2 + i][2] = w.z; vw[h * 2 + i][3] = w.w;
-                            } else {
-                                const uint2 w = *reinterpret_cast<const uint2*>(at + (byte & 8));
-                                vw[h * 2 + i][0] = w.x; vw[h * 2 + i][1] = w.y;
-                            }
-                        }
-                    }
-                    // tile j: components (D / 8) g + 2 j (the tile's row g) and + 1 (its row g + 8)
-#pragma unroll
-                    for (int j = 0; j < KS; ++j) {
-                        uint32_t f[4];
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const uint32_t w0 = vw[h * 2][j >> 1], w1 = vw[h * 2 + 1][j >> 1];
-                            f[h * 2] = q8_value2(__byte_perm(w0, w1, j & 1 ? 0x6622 : 0x4400), vs[h]);
-                            f[h * 2 + 1] = q8_value2(__byte_perm(w0, w1, j & 1 ? 0x7733 : 0x5511), vs[h]);
-                        }
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) mma_16816(o[n][j], f, pb[n][0], pb[n][1]);
-                    }
-                } else {
-                    const uint32_t vbase = smem_u32(stage + Z::TILE);
-#pragma unroll
-                    for (int j = 0; j < KS; ++j) {
-                        const int c = j * 2 + vchunk;
-                        uint32_t f[4];
-                        ldsm_x4_trans(vbase + (c >> 3) * 8192 + vrow * 128 + (((c & 7) ^ (vrow & 7)) << 4), f);
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) mma_16816(o[n][j], f, pb[n][0], pb[n][1]);
-                    }
+                for (int i = 0; i < 2; ++i) {
+                    const int vb = (warp * 16 + t4 * 2 + h * 8 + i) * D + (D / 8) * g, vl = vb >> 7;
+                    v_at[h][i] = Z::TILE + vl * 128 + ((((vb >> 4) & 7) ^ (vl & 7)) << 4) + (D == 64 ? vb & 8 : 0);
                 }
             }
+        }
+        // 16 keys of a page; MASKED: some of them are hidden from some row (the pages at both ends of what the sequence sees)
+        auto step = [&](auto masked_tag, const uint32_t at, const int key0) {
+            constexpr bool MASKED = decltype(masked_tag)::value;
+            if (!Q8 && MASKED && (key0 < lo || key0 + 16 > ctx)) {  // values that no row sees: a weight of zero meets a number
+                uint8_t* vb = stages + (at - stages_u32) + 8192;
+                for (int i = lane; i < 16 * (D / 8); i += 32) {
+                    const int row = warp * 16 + i / (D / 8), c = i % (D / 8), key = key0 + i / (D / 8);
+                    if (key < lo || key >= ctx) *reinterpret_cast<uint4*>(vb + (c >> 3) * 16384 + row * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();  // the stage is overwritten by a bulk copy later
+                __syncwarp();
+            }
+            float sc[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
+            if constexpr (Q8) {
+                uint32_t kw[2][D / 16];  // D / 4 numbers of keys g and g + 8
+                uint32_t ks2[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    ks2[h] = lds16(at + 2 * Z::TILE + (warp * 16 + g + h * 8) * 2) * 0x00010001u;
+#pragma unroll
+                    for (int c = 0; c < D / 64; ++c) {  // (the second piece of an even place is the next one, or the one before: bit 4 of the place)
+                        const uint4 w = lds128(at + (k_at[h] ^ (c << 4)));
+                        kw[h][c * 4] = w.x; kw[h][c * 4 + 1] = w.y; kw[h][c * 4 + 2] = w.z; kw[h][c * 4 + 3] = w.w;
+                    }
+                }
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    uint32_t f[4];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        f[h] = q8_value2(__byte_perm(kw[h][ks], 0, 0x1100), ks2[h]);
+                        f[h + 2] = q8_value2(__byte_perm(kw[h][ks], 0, 0x3322), ks2[h]);
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma_16816(sc[n], f, qb[n][ks][0], qb[n][ks][1]);
+                }
+            } else {
+                const uint32_t kbase = at;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const int c = ks * 2 + kchunk;
+                    uint32_t f[4];
+                    ldsm_x4(kbase + (c >> 3) * 16384 + krow * 128 + (((c & 7) ^ (krow & 7)) << 4), f);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma_16816(sc[n], f, qb[n][ks][0], qb[n][ks][1]);
+                }
+            }
+            // sc[n][0], [1]: key g, the thread's two rows; [2], [3]: key g + 8
+            uint32_t pb[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[i] = sc[n][i] * a.scale_log2;
+                    if constexpr (MASKED) {
+                        const int key = key0 + g + (i >> 1) * 8;
+                        if (key < first[n][i & 1] || key > last[n][i & 1]) x[i] = -INFINITY;
+                    }
+                }
+                // The reference follows the maximum only where a weight would pass 2^8: seldom after the first keys, so sums and accumulators are mostly left alone.
+                if (__any_sync(0xffffffffu, fmaxf(x[0], x[2]) > m[n][0] + CF_RAISE || fmaxf(x[1], x[3]) > m[n][1] + CF_RAISE)) {
+                    float corr[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float mx = fmaxf(x[h], x[h + 2]);
+#pragma unroll
+                        for (int sh = 4; sh < 32; sh <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
+                        const float mn = fmaxf(m[n][h], mx);
+                        corr[h] = fast_ex2(m[n][h] - mn);
+                        m[n][h] = mn;
+                        l[n][h] *= corr[h];
+                    }
+#pragma unroll
+                    for (int j = 0; j < KS; ++j) {
+                        o[n][j][0] *= corr[0];
+                        o[n][j][1] *= corr[1];
+                        o[n][j][2] *= corr[0];
+                        o[n][j][3] *= corr[1];
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    x[h] = fast_ex2(x[h] - m[n][h]);
+                    x[h + 2] = fast_ex2(x[h + 2] - m[n][h]);
+                    l[n][h] += x[h] + x[h + 2];
+                }
+                pb[n][0] = cf_trans(pack_bf16x2(x[0], x[1]));
+                pb[n][1] = cf_trans(pack_bf16x2(x[2], x[3]));
+            }
+            if constexpr (Q8) {
+                uint32_t vw[4][D / 32], vs[2];  // D / 8 numbers of keys 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9: components (D / 8) g and up
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    vs[h] = lds32(at + 2 * Z::TILE + 128 + (warp * 16 + t4 * 2 + h * 8) * 2);
+                    if constexpr (MASKED) {
+                        const int key = key0 + t4 * 2 + h * 8;
+                        if (key < lo || key >= ctx) vs[h] &= 0xFFFF0000u;
+                        if (key + 1 < lo || key + 1 >= ctx) vs[h] &= 0x0000FFFFu;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if constexpr (D == 128) {
+                            const uint4 w = lds128(at + v_at[h][i]);
+                            vw[h * 2 + i][0] = w.x; vw[h * 2 + i][1] = w.y; vw[h * 2 + i][2] = w.z; vw[h * 2 + i][3] = w.w;
+                        } else {
+                            const uint2 w = lds64(at + v_at[h][i]);
+                            vw[h * 2 + i][0] = w.x; vw[h * 2 + i][1] = w.y;
+                        }
+                    }
+                }
+                // tile j: components (D / 8) g + 2 j (the tile's row g) and + 1 (its row g + 8)
+#pragma unroll
+                for (int j = 0; j < KS; ++j) {
+                    uint32_t f[4];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t w0 = vw[h * 2][j >> 1], w1 = vw[h * 2 + 1][j >> 1];
+                        f[h * 2] = q8_value2(__byte_perm(w0, w1, j & 1 ? 0x6622 : 0x4400), vs[h]);
+                        f[h * 2 + 1] = q8_value2(__byte_perm(w0, w1, j & 1 ? 0x7733 : 0x5511), vs[h]);
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma_16816(o[n][j], f, pb[n][0], pb[n][1]);
+                }
+            } else {
+                const uint32_t vbase = at + 8192;
+#pragma unroll
+                for (int j = 0; j < KS; ++j) {
+                    const int c = j * 2 + vchunk;
+                    uint32_t f[4];
+                    ldsm_x4_trans(vbase + (c >> 3) * 16384 + vrow * 128 + (((c & 7) ^ (vrow & 7)) << 4), f);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma_16816(o[n][j], f, pb[n][0], pb[n][1]);
+                }
+            }
+        };
+        for (int p = p_begin, s = 0, round = 0; p < p_end; ++p, s = s + 1 == n_stages ? (++round, 0) : s + 1) {
+            if (!mbar_wait_warp(&full_bar[s], round & 1, &abort_flag, a.c.err, CF_ERR_FULL)) break;
+            const int key0 = (page0 + p) * JSM_PAGE_SIZE + warp * 16;
+            if (key0 >= all_from && key0 + 15 <= all_to) step(std::false_type{}, stages_u32 + s * Z::STAGE, key0);
+            else if (key0 < ctx && key0 + 16 > lo) step(std::true_type{}, stages_u32 + s * Z::STAGE, key0);
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty_bar[s]);
         }
@@ -459,15 +466,17 @@ FewPlan chunk_few_plan(int n_seqs, int max_new, int max_context, int Hkv, int wi
 template <int D, int NT, bool Q8>
 static jsm_status few_go(const ChunkArgs& a, const FewPlan& f, float* part, cudaStream_t st) {
     using Z = FewSizes<D, Q8>;
-    CUtensorMap map;
-    const uint64_t rows = (uint64_t)a.c.n_pages * 2 * a.c.Hkv * JSM_PAGE_SIZE;
-    const jsm_status s = Q8 ? make_tmap_u8_lines(&map, a.c.pool, rows * D / 128, JSM_PAGE_SIZE * D / 128)
-                            : make_tmap_bf16_2d(&map, a.c.pool, rows, D, D, JSM_PAGE_SIZE, 64);
+    // pool and scales as [keys or values of a page][kv heads x positions][D]
+    CUtensorMap map, scales;
+    const uint64_t Hkv = a.c.Hkv, halves = (uint64_t)a.c.n_pages * 2, lines = JSM_PAGE_SIZE * D / 128;
+    jsm_status s = Q8 ? make_tmap_u8_3d(&map, a.c.pool, 128, Hkv * lines, halves, 128, Hkv * lines * 128, 128, lines, 2, true)
+                      : make_tmap_bf16_3d(&map, a.c.pool, D, Hkv * JSM_PAGE_SIZE, halves, D, Hkv * JSM_PAGE_SIZE * D, 64, JSM_PAGE_SIZE, 2);
+    if (s == JSM_OK && Q8) s = make_tmap_u8_3d(&scales, a.c.scales, 128, Hkv, halves, 128, Hkv * 128, 128, 1, 2, false);
     if (s != JSM_OK) return s;
     static DeviceOnce once;
     JSM_CUDA_CHECK(allow_shared(once, chunk_few_kernel<D, NT, Q8>, Z::smem(Z::STAGES, NT * 8)));
     const int stages = std::min(f.run_pages, Z::STAGES);
-    JSM_CUDA_CHECK(launch_chained(chunk_few_kernel<D, NT, Q8>, dim3((unsigned)f.n_runs * a.c.n_seqs, a.c.Hkv), dim3(CF_THREADS), (size_t)Z::smem(stages, NT * 8), st, map, a,
+    JSM_CUDA_CHECK(launch_chained(chunk_few_kernel<D, NT, Q8>, dim3((unsigned)f.n_runs * a.c.n_seqs, a.c.Hkv), dim3(CF_THREADS), (size_t)Z::smem(stages, NT * 8), st, map, Q8 ? scales : map, a,
                                   NT * 8, f.n_runs, f.run_pages, stages, part));
     JSM_LAUNCH_CHECK();
     if (f.n_runs > 1) {

@@ -533,6 +533,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
                     dst[n] = r * 128 + (((c4 * 2) ^ (r & 7)) << 4);
                 }
             }
+            const uint32_t k_u32 = smem_u32(k_smem), v_u32 = smem_u32(v_smem), raw_sc = smem_u32(raw_scales);
             bool ok = true;
             for (int j = j_lo; j < n_max && ok; ++j) {
                 const int i = j - j_lo, s = i % ST;
@@ -541,24 +542,24 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
                     const int value = slot >> 1, half = slot & 1;
                     if (half == 0 && i >= ST && !mbar_wait_warp(value ? &v_empty[s] : &k_empty[s], ((i / ST) & 1) ^ 1, &abort_flag, a.c.err, TC_TIMEOUT_EMPTY)) { ok = false; break; }
                     if (!mbar_wait_warp(&raw_full[slot], i & 1, &abort_flag, a.c.err, TC_TIMEOUT_FULL)) { ok = false; break; }
-                    const uint8_t* raw = raw_smem + slot * Z::RAW;
-                    uint8_t* to = (value ? v_smem : k_smem) + s * Z::TILE + half * (JSM_PAGE_SIZE * 128);
+                    const uint32_t raw = smem_u32(raw_smem) + slot * Z::RAW;
+                    const uint32_t to = (value ? v_u32 : k_u32) + s * Z::TILE + half * (JSM_PAGE_SIZE * 128);
                     // values that no row sees become zeros: a weight of zero meets a number
                     const int key0 = base + j * CK_BN + half * JSM_PAGE_SIZE, from = value ? lo - key0 : -1, until = value ? end - key0 : JSM_PAGE_SIZE;
                     uint4 w[STEPS];
                     uint32_t scale[STEPS];
 #pragma unroll
                     for (int n = 0; n < STEPS; ++n) {
-                        w[n] = *reinterpret_cast<const uint4*>(raw + src[n]);
-                        scale[n] = raw_scales[slot][row[n]];
+                        w[n] = lds128(raw + src[n]);
+                        scale[n] = lds16(raw_sc + slot * (JSM_PAGE_SIZE * 2) + row[n] * 2);
                     }
 #pragma unroll
                     for (int n = 0; n < STEPS; ++n) {
                         const uint32_t sc = row[n] < from || row[n] >= until ? 0u : scale[n] * 0x00010001u;
-                        *reinterpret_cast<uint4*>(to + dst[n]) = make_uint4(q8_value2(__byte_perm(w[n].x, 0, 0x1100), sc), q8_value2(__byte_perm(w[n].x, 0, 0x3322), sc),
-                                                                            q8_value2(__byte_perm(w[n].y, 0, 0x1100), sc), q8_value2(__byte_perm(w[n].y, 0, 0x3322), sc));
-                        *reinterpret_cast<uint4*>(to + (dst[n] ^ 16)) = make_uint4(q8_value2(__byte_perm(w[n].z, 0, 0x1100), sc), q8_value2(__byte_perm(w[n].z, 0, 0x3322), sc),
-                                                                                   q8_value2(__byte_perm(w[n].w, 0, 0x1100), sc), q8_value2(__byte_perm(w[n].w, 0, 0x3322), sc));
+                        sts128(to + dst[n], make_uint4(q8_value2(__byte_perm(w[n].x, 0, 0x1100), sc), q8_value2(__byte_perm(w[n].x, 0, 0x3322), sc),
+                                                       q8_value2(__byte_perm(w[n].y, 0, 0x1100), sc), q8_value2(__byte_perm(w[n].y, 0, 0x3322), sc)));
+                        sts128(to + (dst[n] ^ 16), make_uint4(q8_value2(__byte_perm(w[n].z, 0, 0x1100), sc), q8_value2(__byte_perm(w[n].z, 0, 0x3322), sc),
+                                                              q8_value2(__byte_perm(w[n].w, 0, 0x1100), sc), q8_value2(__byte_perm(w[n].w, 0, 0x3322), sc)));
                     }
                     if (half == 1) fence_proxy_async_smem();
                     __syncwarp();
