@@ -1,6 +1,7 @@
 // Attention of new tokens over a paged cache, bf16 or 8-bit: entry points, and which kernel takes which sequence.
 #include "chunk_attn.cuh"
 #include <math.h>
+#include <algorithm>
 
 namespace jsm {
 
@@ -15,14 +16,14 @@ struct Plan {
     FewPlan few;
     size_t bytes;
 };
-Plan plan_of(int n_seqs, int T, int max_new, int max_context, int Hkv, int G, int D, int window) {
+Plan plan_of(int n_seqs, int T, int max_new, int max_context, int Hkv, int G, int D, int window, bool q8) {
     Plan p;
     const long long most = (long long)max_new * G;
     p.few_rows = most <= 8 ? 8 : most <= 16 ? 16 : G <= 8 ? 8 : 16;
     p.many = most > 16;
     // (with one sequence of more rows there is nothing for the kernel of few)
     if (p.many && ((n_seqs == 1 && T == max_new) || G > p.few_rows)) p.few_rows = 0;
-    p.few = p.few_rows ? chunk_few_plan(n_seqs, max_new, max_context, Hkv, window, p.few_rows, D) : FewPlan{0, 0, 0};
+    p.few = p.few_rows ? chunk_few_plan(n_seqs, max_new, max_context, Hkv, window, p.few_rows, D, q8) : FewPlan{0, false, 0};
     p.bytes = p.few.bytes;
     return p;
 }
@@ -34,7 +35,8 @@ using namespace jsm;
 
 extern "C" size_t jsm_attn_chunk_scratch_bytes(int n_seqs, int T, int max_new, int max_context, int Hq, int Hkv, int D, int window) {
     if (n_seqs <= 0 || T <= 0 || max_new <= 0 || max_context < max_new || Hkv <= 0 || Hq <= 0 || Hq % Hkv || (D != 64 && D != 128) || window < 0) return 0;
-    return plan_of(n_seqs, T, max_new, max_context, Hkv, Hq / Hkv, D, window).bytes;
+    // (the larger of both kinds of cache)
+    return std::max(plan_of(n_seqs, T, max_new, max_context, Hkv, Hq / Hkv, D, window, false).bytes, plan_of(n_seqs, T, max_new, max_context, Hkv, Hq / Hkv, D, window, true).bytes);
 }
 
 extern "C" jsm_status jsm_attn_chunk(const void* d_q, int64_t q_row_stride, const void* d_pool, const void* d_scales, int n_pages, const int32_t* d_block_table,
@@ -64,7 +66,7 @@ extern "C" jsm_status jsm_attn_chunk(const void* d_q, int64_t q_row_stride, cons
     a.Hq = Hq; a.G = Hq / Hkv; a.window = window;
     a.scale_log2 = scale * 1.4426950408889634f;
     const cudaStream_t st = as_stream(stream);
-    const Plan p = plan_of(n_seqs, T, max_new, max_context, Hkv, a.G, D, window);
+    const Plan p = plan_of(n_seqs, T, max_new, max_context, Hkv, a.G, D, window, d_scales != nullptr);
     if (p.bytes && (!d_scratch || scratch_bytes < p.bytes || (reinterpret_cast<uintptr_t>(d_scratch) & 15)))
         JSM_FAIL(JSM_INVALID_ARG, "jsm_attn_chunk: %zu bytes of scratch (16-byte aligned), %zu are needed", d_scratch ? scratch_bytes : 0, p.bytes);
     if (p.many) {

@@ -15,12 +15,13 @@ struct ChunkArgs {
     float scale_log2;
 };
 
-// How the pages of a sequence are shared out where it has a few new tokens only (chunk_few.cu): runs of run_pages pages, at most n_runs of them; bytes of partial results.
+// Sequences with a few new tokens only (chunk_few.cu): runs of pages, whether partial results can meet, their bytes.
 struct FewPlan {
-    int run_pages, n_runs;
+    int n_runs;
+    bool merge;
     size_t bytes;
 };
-FewPlan chunk_few_plan(int n_seqs, int max_new, int max_context, int Hkv, int window, int few_rows, int D);
+FewPlan chunk_few_plan(int n_seqs, int max_new, int max_context, int Hkv, int window, int few_rows, int D, bool q8);
 // sequences of up to few_rows (8 or 16) rows of queries per kv head; the others are left to another kernel
 jsm_status chunk_few_launch(const ChunkArgs& a, const FewPlan& f, int few_rows, void* scratch, cudaStream_t st);
 

@@ -1,15 +1,17 @@
 // Attention of a few new tokens of each sequence over a paged cache (bf16 or 8-bit): single tokens, drafts being verified.  Up to 16 rows of queries
 // (tokens x query heads of a kv head) share every cached byte, so the kernel is bound by the bytes of the cache.
 //
-// A CTA has a run of pages of one (sequence, kv head): a producer thread keeps a ring of pages in flight (TMA boxes in the 128-byte swizzle, the scales of an
-// 8-bit page by bulk copies), four warps have 16 keys of each page:
+// All pages that any (sequence, kv head) sees are one row of work, cut into equal runs, one per CTA: as many CTAs as the chip holds, each with the same number of bytes
+// however ragged the contexts are.  A run holds the end of one (sequence, kv head), perhaps whole ones, and the beginning of another: at most two partial results per
+// CTA, so the scratch does not grow with contexts or sequences.  A producer thread keeps a ring of pages in flight across these borders (TMA boxes in the 128-byte
+// swizzle); four warps have 16 keys of each page:
 //   scores, transposed:   S^T[16 keys x 8 rows] = K[16 x D] . Q^T,  keys as the 16-row operand of mma.m16n8k16, so that no row of it is padding
 //   softmax over the keys: running maximum and sum per warp, base 2
 //   O^T[D x 8 rows]     += V^T[D x 16 keys] . P^T
 // bf16 pages come into the operands by ldmatrix.  Numbers of an 8-bit page are taken from shared memory in 16-byte pieces and become bf16 in registers: which
 // component an element of an operand stands for is free as long as both operands agree, so the pieces of a thread are the components that its operand
 // registers need, and the transposition of V costs no instruction beyond the byte permutation that spreads the numbers anyway.
-// Partial results of the runs meet in chunk_merge_kernel, in the order of the runs.
+// Partial results meet in chunk_merge_kernel, in the order of the runs.
 // A row whose result is not a number is worked out again over exactly its own keys (attend_row): a weight of zero times what a hidden key holds is no zero then.
 #include "chunk_attn.cuh"
 #include "tc_utils.cuh"
@@ -28,74 +30,112 @@ constexpr float CF_NONE = -1.0e30f;  // the reference of a row that has seen not
 constexpr float CF_RAISE = 8.0f;     // weights go up to 2^8 before the reference follows the maximum
 constexpr int CF_ERR_FULL = 43, CF_ERR_EMPTY = 44;
 
+__device__ __forceinline__ void cf_meet() { asm volatile("bar.sync 1, 128;" ::: "memory"); }  // the four warps that have keys
 __device__ __forceinline__ uint32_t cf_trans(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-template <int D, bool Q8>
+template <int D, int NT, bool Q8>
 struct FewSizes {
+    static constexpr int ROWS = NT * 8;
     static constexpr int TILE = JSM_PAGE_SIZE * D * (Q8 ? 1 : 2);     // keys, or values, of a page
     static constexpr int STAGE = 2 * TILE + (Q8 ? 1024 : 0);          // keys | values | scales of both; bf16: for each 64 columns keys | values (1024-byte steps: the swizzle counts from there)
-    static constexpr int STAGES = 3;                                  // at most: a run of fewer pages has as many
-    static constexpr int smem(int stages, int rows) { return std::max(stages * STAGE, CF_WARPS * rows * D * 4) + 1024; }
+    static constexpr int STAGES = D == 128 && !Q8 ? 2 : 3;
+    static constexpr int MEET = CF_WARPS * ROWS * D * 4;              // the warps' sums of a (sequence, kv head)
+    static constexpr int SMEM = STAGES * STAGE + MEET + 1024;
+    static constexpr int PER_SM = NT == 1 ? (Q8 ? 3 : 2) : 2;         // CTAs that share a multiprocessor
 };
 
+// Pages that the queries of sequence s see, from page0 on; 0 where it has none, or too many rows for this kernel.
+__device__ __forceinline__ int few_pages(const ChunkArgs& a, int few_rows, int s, int& row0, int& n_new, int& ctx, int& page0) {
+    if (!chunk_lengths(a, s, row0, n_new, ctx) || n_new * a.G > few_rows) return 0;
+    page0 = first_key(a.window, ctx - n_new) / JSM_PAGE_SIZE;
+    return (ctx - 1) / JSM_PAGE_SIZE + 1 - page0;
+}
+// Pages of a run, of the `all` pages of the call
+__device__ __forceinline__ long long run_length(long long all, int n_runs) { return (all + n_runs - 1) / n_runs; }
+
 template <int D, int NT, bool Q8>
-__global__ void __launch_bounds__(CF_THREADS, NT == 1 ? 4 : 2) chunk_few_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ CUtensorMap tmap_scales,
-                                                                                const __grid_constant__ ChunkArgs a, int few_rows,                                                                                int n_runs, int run_pages, int n_stages, float* __restrict__ part) {
-    using Z = FewSizes<D, Q8>;
+__global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk_few_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ CUtensorMap tmap_scales,
+                                                                                            const __grid_constant__ ChunkArgs a, float* __restrict__ part) {
+    using Z = FewSizes<D, NT, Q8>;
     constexpr int KS = D / 16;  // steps of 16 components; tiles of 16 components of O^T
+    constexpr int few_rows = Z::ROWS;
     extern __shared__ uint8_t cf_dyn[];
     uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(cf_dyn) + 1023) & ~uintptr_t(1023));
     const uint32_t stages_u32 = smem_u32(stages);
     __shared__ uint64_t full_bar[Z::STAGES], empty_bar[Z::STAGES];
-    __shared__ int abort_flag;
-    __shared__ float sm_m[CF_WARPS][NT * 8], sm_l[CF_WARPS][NT * 8];
+    __shared__ int abort_flag, sh_seq, sh_head, sh_page, sh_pages;
+    __shared__ float sm_m[CF_WARPS][few_rows], sm_l[CF_WARPS][few_rows];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < n_stages; ++s) {
+    if (threadIdx.x == CF_WARPS * 32) {
+        for (int s = 0; s < Z::STAGES; ++s) {
             mbar_init(&full_bar[s], 1);
             mbar_init(&empty_bar[s], CF_WARPS);
         }
         abort_flag = 0;
         mbar_fence_init();
     }
-    __syncthreads();
     chain_wait();
     chain_trigger();  // (now: what the merge reads before its own wait was there before this kernel)
-    const int run = blockIdx.x % n_runs, seq = blockIdx.x / n_runs, hk = blockIdx.y;
-    int row0, n_new, ctx;
-    if (!chunk_lengths(a, seq, row0, n_new, ctx) || n_new * a.G > few_rows) return;
-    const int rows = n_new * a.G;
-    const int lo = first_key(a.window, ctx - n_new);  // no row sees a key before it
-    const int page0 = lo / JSM_PAGE_SIZE, n_pages = (ctx - 1) / JSM_PAGE_SIZE + 1 - page0;
-    const int p_begin = run * run_pages, p_end = min(n_pages, p_begin + run_pages);
-    if (p_begin >= p_end) return;
-    const bool whole = n_pages <= run_pages;  // the only run: its result is final
-
-    float m[NT][2], l[NT][2];  // rows (lane % 4) * 2 and + 1 of each tile
-    float o[NT][KS][4];        // O^T
+    if (warp == 0) {  // where this CTA's run begins
+        int row0, n_new, ctx, page0;
+        long long all = 0;
+        for (int s0 = 0; s0 < a.c.n_seqs; s0 += 32) all += s0 + lane < a.c.n_seqs ? few_pages(a, few_rows, s0 + lane, row0, n_new, ctx, page0) : 0;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        m[n][0] = m[n][1] = CF_NONE;
-        l[n][0] = l[n][1] = 0.0f;
+        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        all *= a.c.Hkv;
+        const long long len = run_length(all, gridDim.x), begin = blockIdx.x * len;
+        if (lane == 0) sh_pages = (int)max(0ll, min(len, all - begin));
+        long long before = 0;
+        for (int s0 = 0; s0 < a.c.n_seqs && begin < all; s0 += 32) {
+            const int n = s0 + lane < a.c.n_seqs ? few_pages(a, few_rows, s0 + lane, row0, n_new, ctx, page0) : 0;
+            long long sum = (long long)n * a.c.Hkv;
 #pragma unroll
-        for (int j = 0; j < KS; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.0f;
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long v = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += v;
+            }
+            const unsigned here = __ballot_sync(0xffffffffu, before + sum > begin);
+            if (here) {
+                if (lane == __ffs(here) - 1) {
+                    const long long in = begin - (before + sum - (long long)n * a.c.Hkv);
+                    sh_seq = s0 + lane;
+                    sh_head = (int)(in / n);
+                    sh_page = (int)(in % n);
+                }
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
     }
+    __syncthreads();
+    int left = sh_pages, seq = sh_seq, hk = sh_head, page = sh_page;
+    if (left == 0) return;
+    int row0, n_new, ctx, page0;
+    int n_pages = few_pages(a, few_rows, seq, row0, n_new, ctx, page0);
+    // the next (sequence, kv head) of the run
+    auto next = [&] {
+        page = 0;
+        if (++hk < a.c.Hkv) return;
+        hk = 0;
+        do n_pages = few_pages(a, few_rows, ++seq, row0, n_new, ctx, page0);
+        while (n_pages == 0);
+    };
 
     if (warp == CF_WARPS) {
         if (lane == 0) {
             tma_prefetch_desc(&tmap);
             if (Q8) tma_prefetch_desc(&tmap_scales);
             int issued = 0;
-            for (int p = p_begin, s = 0, round = 0; p < p_end; ++p, s = s + 1 == n_stages ? (++round, 0) : s + 1) {
+            for (int s = 0, round = 0; issued < left; s = s + 1 == Z::STAGES ? (++round, 0) : s + 1) {
                 if (round > 0 && !mbar_wait(&empty_bar[s], (round - 1) & 1, &abort_flag, a.c.err, CF_ERR_EMPTY)) break;
-                const int page = cache_page(a.c, seq, (page0 + p) * JSM_PAGE_SIZE);
+                const int id = cache_page(a.c, seq, (page0 + page) * JSM_PAGE_SIZE);
                 uint8_t* dst = stages + s * Z::STAGE;
-                // Keys and values of a page come by one request (a slab of 64 columns each, for bf16), the scales of both by another: the rate of a thread's requests would
-                // bound the stream.  A page outside the pool: a place before the first page, which reads as zeros.
-                const int z = page < 0 ? -2 : 2 * page;
+                // Keys and values of a page come by one request (a slab of 64 columns each, for bf16), the scales of both by another.  A page outside the pool: a place
+                // before the first page, which reads as zeros.
+                const int z = id < 0 ? -2 : 2 * id;
                 mbar_expect_tx(&full_bar[s], 2 * Z::TILE + (Q8 ? 256 : 0));
                 if constexpr (Q8) {
                     tma_load_3d(dst, &tmap, 0, hk * (JSM_PAGE_SIZE * D / 128), z, &full_bar[s]);
@@ -104,16 +144,50 @@ __global__ void __launch_bounds__(CF_THREADS, NT == 1 ? 4 : 2) chunk_few_kernel(
 #pragma unroll
                     for (int c = 0; c < D / 64; ++c) tma_load_3d(dst + c * 16384, &tmap, c * 64, hk * JSM_PAGE_SIZE, z, &full_bar[s]);
                 }
-                issued = p - p_begin + 1;
+                if (++issued < left && ++page == n_pages) next();
             }
             if (abort_flag) {  // let the copies in flight land before the CTA exits (bounded)
                 const long long t0 = clock64();
-                for (int it = max(0, issued - n_stages); it < issued; ++it)
-                    while (!mbar_try_wait(&full_bar[it % n_stages], (it / n_stages) & 1) && clock64() - t0 < WAIT_LIMIT_CYCLES) {}
+                for (int it = max(0, issued - Z::STAGES); it < issued; ++it)
+                    while (!mbar_try_wait(&full_bar[it % Z::STAGES], (it / Z::STAGES) & 1) && clock64() - t0 < WAIT_LIMIT_CYCLES) {}
             }
         }
-    } else {
-        const int g = lane >> 2, t4 = lane & 3;
+        return;
+    }
+    const int g = lane >> 2, t4 = lane & 3;
+    const int mi = lane >> 3, mr = lane & 7;
+    const int krow = warp * 16 + (mi & 1) * 8 + mr, kchunk = mi >> 1;   // ldmatrix, keys
+    const int vrow = warp * 16 + (mi >> 1) * 8 + mr, vchunk = mi & 1;   // ldmatrix, values transposed
+    // 8-bit pages: places of this lane's pieces in a stage (the keys of a warp are whole swizzle groups apart)
+    uint32_t k_at[2], v_at[2][2];
+    if constexpr (Q8) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int byte = (warp * 16 + g + h * 8) * D + (D / 4) * t4, line = byte >> 7;
+            k_at[h] = line * 128 + ((((byte >> 4) & 7) ^ (line & 7)) << 4);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int vb = (warp * 16 + t4 * 2 + h * 8 + i) * D + (D / 8) * g, vl = vb >> 7;
+                v_at[h][i] = Z::TILE + vl * 128 + ((((vb >> 4) & 7) ^ (vl & 7)) << 4) + (D == 64 ? vb & 8 : 0);
+            }
+        }
+    }
+    float* sm_o = reinterpret_cast<float*>(stages + Z::STAGES * Z::STAGE);  // [warp][row][component]
+    bool ok = true;
+    int s = 0, round = 0;
+    for (bool first_piece = true;; first_piece = false) {  // a (sequence, kv head), or the run's piece of it
+        const int rows = n_new * a.G, lo = first_key(a.window, ctx - n_new);  // no row sees a key before it
+        const int here = min(left, n_pages - page);
+        const bool whole = here == n_pages;  // all of it: the result is final
+        float m[NT][2], l[NT][2];  // rows (lane % 4) * 2 and + 1 of each tile
+        float o[NT][KS][4];        // O^T
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            m[n][0] = m[n][1] = CF_NONE;
+            l[n][0] = l[n][1] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < KS; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.0f;
+        }
         // B operand of the scores: row n * 8 + g, components of thread t4 in each step
         uint32_t qb[NT][KS][2];
         int last[NT][2], first[NT][2];  // keys that the thread's two columns of each tile see
@@ -140,23 +214,6 @@ __global__ void __launch_bounds__(CF_THREADS, NT == 1 ? 4 : 2) chunk_few_kernel(
             }
         }
         const int all_from = first_key(a.window, ctx - 1), all_to = ctx - n_new;  // keys that every row sees
-        const int mi = lane >> 3, mr = lane & 7;
-        const int krow = warp * 16 + (mi & 1) * 8 + mr, kchunk = mi >> 1;   // ldmatrix, keys
-        const int vrow = warp * 16 + (mi >> 1) * 8 + mr, vchunk = mi & 1;   // ldmatrix, values transposed
-        // 8-bit pages: places of this lane's pieces in a stage (the keys of a warp are whole swizzle groups apart)
-        uint32_t k_at[2], v_at[2][2];
-        if constexpr (Q8) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int byte = (warp * 16 + g + h * 8) * D + (D / 4) * t4, line = byte >> 7;
-                k_at[h] = line * 128 + ((((byte >> 4) & 7) ^ (line & 7)) << 4);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int vb = (warp * 16 + t4 * 2 + h * 8 + i) * D + (D / 8) * g, vl = vb >> 7;
-                    v_at[h][i] = Z::TILE + vl * 128 + ((((vb >> 4) & 7) ^ (vl & 7)) << 4) + (D == 64 ? vb & 8 : 0);
-                }
-            }
-        }
         // 16 keys of a page; MASKED: some of them are hidden from some row (the pages at both ends of what the sequence sees)
         auto step = [&](auto masked_tag, const uint32_t at, const int key0) {
             constexpr bool MASKED = decltype(masked_tag)::value;
@@ -295,33 +352,30 @@ __global__ void __launch_bounds__(CF_THREADS, NT == 1 ? 4 : 2) chunk_few_kernel(
                 }
             }
         };
-        for (int p = p_begin, s = 0, round = 0; p < p_end; ++p, s = s + 1 == n_stages ? (++round, 0) : s + 1) {
-            if (!mbar_wait_warp(&full_bar[s], round & 1, &abort_flag, a.c.err, CF_ERR_FULL)) break;
+        for (int p = page; p < page + here; ++p) {
+            ok = ok && mbar_wait_warp(&full_bar[s], round & 1, &abort_flag, a.c.err, CF_ERR_FULL);
             const int key0 = (page0 + p) * JSM_PAGE_SIZE + warp * 16;
-            if (key0 >= all_from && key0 + 15 <= all_to) step(std::false_type{}, stages_u32 + s * Z::STAGE, key0);
-            else if (key0 < ctx && key0 + 16 > lo) step(std::true_type{}, stages_u32 + s * Z::STAGE, key0);
+            if (ok) {
+                if (key0 >= all_from && key0 + 15 <= all_to) step(std::false_type{}, stages_u32 + s * Z::STAGE, key0);
+                else if (key0 < ctx && key0 + 16 > lo) step(std::true_type{}, stages_u32 + s * Z::STAGE, key0);
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty_bar[s]);
+            if (++s == Z::STAGES) {
+                s = 0;
+                ++round;
+            }
         }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int sh = 4; sh < 32; sh <<= 1) l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], sh);
-    }
-    __syncthreads();
-    if (abort_flag) return;  // (the error is recorded)
-    // every stage has been consumed: the ring becomes [warp][row][component]
-    float* sm_o = reinterpret_cast<float*>(stages);
-    if (warp < CF_WARPS) {
-        const int g = lane >> 2, t4 = lane & 3;
+        // the four warps' sums meet (also after a wait that gave up: every warp comes by here as often)
+        if (!first_piece) cf_meet();  // the piece before has been read
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int sh = 4; sh < 32; sh <<= 1) l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], sh);
                 const int r = n * 8 + t4 * 2 + h;
-                float* dst = sm_o + (warp * NT * 8 + r) * D;
+                float* dst = sm_o + (warp * few_rows + r) * D;
 #pragma unroll
                 for (int j = 0; j < KS; ++j) {
                     dst[Q8 ? (D / 8) * g + 2 * j : j * 16 + g] = o[n][j][h];
@@ -332,60 +386,88 @@ __global__ void __launch_bounds__(CF_THREADS, NT == 1 ? 4 : 2) chunk_few_kernel(
                     sm_l[warp][r] = l[n][h];
                 }
             }
-    }
-    __syncthreads();
-    // a warp per row: the four warps' sums under their largest maximum
-    constexpr int N = D / 32;
-    for (int r = warp; r < rows; r += CF_WARPS + 1) {
-        float M = CF_NONE, L = 0.0f, acc[N];
+        cf_meet();
+        // a warp per row: the four warps' sums under their largest reference
+        constexpr int N = D / 32;
+        for (int r = warp; r < rows && !abort_flag; r += CF_WARPS) {
+            float M = CF_NONE, L = 0.0f, acc[N];
 #pragma unroll
-        for (int w = 0; w < CF_WARPS; ++w) M = fmaxf(M, sm_m[w][r]);
+            for (int w = 0; w < CF_WARPS; ++w) M = fmaxf(M, sm_m[w][r]);
 #pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+            for (int i = 0; i < N; ++i) acc[i] = 0.0f;
 #pragma unroll
-        for (int w = 0; w < CF_WARPS; ++w) {
-            const float f = fast_ex2(sm_m[w][r] - M);
-            L += f * sm_l[w][r];
+            for (int w = 0; w < CF_WARPS; ++w) {
+                const float f = fast_ex2(sm_m[w][r] - M);
+                L += f * sm_l[w][r];
 #pragma unroll
-            for (int i = 0; i < N; ++i) acc[i] += f * sm_o[(w * NT * 8 + r) * D + lane * N + i];
-        }
-        const int row = row0 + r / a.G, head = hk * a.G + r % a.G;
-        if (whole) {
-            bool fine = true;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                acc[i] /= L;
-                fine = fine && fabsf(acc[i]) <= 3.402823466e38f;
+                for (int i = 0; i < N; ++i) acc[i] += f * sm_o[(w * few_rows + r) * D + lane * N + i];
             }
-            if (__all_sync(0xffffffffu, fine)) {
-                __nv_bfloat16* dst = a.out + row * a.out_rs + (long long)head * D + lane * N;
+            const int row = row0 + r / a.G, head = hk * a.G + r % a.G;
+            if (whole) {
+                bool fine = true;
 #pragma unroll
-                for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16x2(acc[i], acc[i + 1]);
+                for (int i = 0; i < N; ++i) {
+                    acc[i] /= L;
+                    fine = fine && fabsf(acc[i]) <= 3.402823466e38f;
+                }
+                if (__all_sync(0xffffffffu, fine)) {
+                    __nv_bfloat16* dst = a.out + row * a.out_rs + (long long)head * D + lane * N;
+#pragma unroll
+                    for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16x2(acc[i], acc[i + 1]);
+                } else {
+                    attend_row<D, Q8>(a, seq, row, head, ctx - n_new + r / a.G);
+                }
             } else {
-                attend_row<D, Q8>(a, seq, row, head, ctx - n_new + r / a.G);
-            }
-        } else {
-            float* dst = part + (((long long)seq * a.c.Hkv + hk) * n_runs + run) * (few_rows * (D + 2)) + r * (D + 2);
+                // the run's first piece, or its last
+                float* dst = part + ((blockIdx.x * 2ll + (first_piece ? 0 : 1)) * few_rows + r) * (D + 2);
 #pragma unroll
-            for (int i = 0; i < N; i += 2) *reinterpret_cast<float2*>(dst + lane * N + i) = make_float2(acc[i], acc[i + 1]);
-            if (lane == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(M, L);
+                for (int i = 0; i < N; i += 2) *reinterpret_cast<float2*>(dst + lane * N + i) = make_float2(acc[i], acc[i + 1]);
+                if (lane == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(M, L);
+            }
         }
+        left -= here;
+        if (left == 0) return;
+        next();
     }
 }
 
-// The runs of a (row, head) under their largest reference, in the order of the runs.  A block per row (of the sequences of few rows) and head: each of four warps takes eight runs of every 32, all their
-// loads in flight, with a reference of its own; the warps meet in shared memory.  What depends on the lengths alone is worked out while the runs are still under way.
+// The pieces of a (row, head) under their largest reference, in the order of the runs.  A block per row (of the sequences of few rows) and head: each of four warps takes
+// eight pieces of every 32, all their loads in flight, with a reference of its own; the warps meet in shared memory.  What depends on the lengths alone is worked out
+// while the runs are still under way.
 constexpr int CM_RUNS = 8;
 template <int D, bool Q8>
-__global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant__ ChunkArgs a, int few_rows, int n_runs, int run_pages, const float* part) {
+__global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant__ ChunkArgs a, int few_rows, int n_runs, const float* part) {
     constexpr int N = D / 32;
     __shared__ float sm_m[4], sm_l[4], sm_o[4][D];
+    __shared__ long long sm_before[4], sm_all[4];
     const int tokens = gridDim.x / a.c.n_seqs, s = blockIdx.x / tokens, i = blockIdx.x % tokens, head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int row0 = 0, n_new = 0, ctx = 0;
-    const bool mine = chunk_lengths(a, s, row0, n_new, ctx) && n_new * a.G <= few_rows && i < n_new;
-    const int n_pages = (ctx - 1) / JSM_PAGE_SIZE + 1 - first_key(a.window, ctx - n_new) / JSM_PAGE_SIZE, n = mine ? (n_pages + run_pages - 1) / run_pages : 0;
-    const int t = row0 + i, hk = head / a.G, r = i * a.G + head % a.G, step = few_rows * (D + 2);
-    const float* src = part + ((long long)s * a.c.Hkv + hk) * n_runs * step + r * (D + 2);
+    int row0 = 0, n_new = 0, ctx = 0, page0 = 0;
+    long long before = 0, all = 0;
+    for (int k = threadIdx.x; k < a.c.n_seqs; k += 128) {
+        const int n = few_pages(a, few_rows, k, row0, n_new, ctx, page0);
+        all += n;
+        if (k < s) before += n;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        all += __shfl_xor_sync(0xffffffffu, all, o);
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+    }
+    if (lane == 0) {
+        sm_all[warp] = all;
+        sm_before[warp] = before;
+    }
+    __syncthreads();
+    const int n_pages = few_pages(a, few_rows, s, row0, n_new, ctx, page0);
+    const int t = row0 + i, hk = head / a.G, r = i * a.G + head % a.G;
+    const long long len = max(1ll, run_length((sm_all[0] + sm_all[1] + sm_all[2] + sm_all[3]) * a.c.Hkv, n_runs));
+    const long long from = (sm_before[0] + sm_before[1] + sm_before[2] + sm_before[3]) * a.c.Hkv + (long long)hk * n_pages;  // its first page in the row of work
+    const int c_first = (int)(from / len), n = n_pages > 0 && i < n_new ? (int)((from + n_pages - 1) / len) - c_first + 1 : 0;
+    // the first piece of a run of its own, but for the first run, whose last piece it is unless it begins there
+    const bool begins = from % len == 0;
+    const int step = 2 * few_rows * (D + 2);
+    const float* src = part + ((long long)c_first * 2 * few_rows + r) * (D + 2);
+    auto piece = [&](int c) { return src + (long long)c * step + (c == 0 && !begins ? few_rows * (D + 2) : 0); };
     chain_wait();
     chain_trigger();
     if (n <= 1) return;
@@ -395,10 +477,10 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant_
     for (int c0 = warp * CM_RUNS; c0 < n; c0 += 4 * CM_RUNS) {
         float v[CM_RUNS][N];
         float2 ml = make_float2(CF_NONE, 0.0f);
-        if (lane < CM_RUNS && c0 + lane < n) ml = *reinterpret_cast<const float2*>(src + (long long)(c0 + lane) * step + D);
+        if (lane < CM_RUNS && c0 + lane < n) ml = *reinterpret_cast<const float2*>(piece(c0 + lane) + D);
 #pragma unroll
         for (int c = 0; c < CM_RUNS; ++c) {
-            const float* x = src + (long long)min(c0 + c, n - 1) * step + lane * N;
+            const float* x = piece(min(c0 + c, n - 1)) + lane * N;
 #pragma unroll
             for (int i = 0; i < N; i += 2) *reinterpret_cast<float2*>(&v[c][i]) = *reinterpret_cast<const float2*>(x + i);
         }
@@ -451,21 +533,22 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant_
     for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16x2(acc[i], acc[i + 1]);
 }
 
-// Pages of a run: enough CTAs to fill the chip's slots (four per SM), runs of up to eight pages so that long contexts even out.
-FewPlan chunk_few_plan(int n_seqs, int max_new, int max_context, int Hkv, int window, int few_rows, int D) {
+// As many runs as the chip holds CTAs (8-bit pages, heads of 128: three per multiprocessor with three stages each 80.7 us for 64 contexts of 512 to 8192, four with two 87.0), of
+// two pages at least (one token over 4096 positions: 7.8 us, with runs of one page 8.1).
+FewPlan chunk_few_plan(int n_seqs, int max_new, int max_context, int Hkv, int window, int few_rows, int D, bool q8) {
     long long pages = (max_context + JSM_PAGE_SIZE - 1) / JSM_PAGE_SIZE;
     if (window > 0) pages = std::min(pages, ((long long)window + max_new + JSM_PAGE_SIZE - 3) / JSM_PAGE_SIZE + 1);
     FewPlan f;
-    const long long slots = 4ll * sm_count(), all = pages * n_seqs * Hkv;
-    f.run_pages = (int)std::min(8ll, std::max(1ll, (all + slots - 1) / slots));
-    f.n_runs = (int)((pages + f.run_pages - 1) / f.run_pages);
-    f.bytes = f.n_runs > 1 ? (size_t)n_seqs * Hkv * f.n_runs * few_rows * (D + 2) * sizeof(float) : 0;
+    const int per_sm = few_rows == 8 ? (q8 ? 3 : 2) : 2;
+    f.n_runs = (int)std::min((long long)per_sm * sm_count(), (pages * n_seqs * Hkv + 1) / 2);
+    f.merge = pages > 1;
+    f.bytes = f.merge ? (size_t)f.n_runs * 2 * few_rows * (D + 2) * sizeof(float) : 0;
     return f;
 }
 
 template <int D, int NT, bool Q8>
 static jsm_status few_go(const ChunkArgs& a, const FewPlan& f, float* part, cudaStream_t st) {
-    using Z = FewSizes<D, Q8>;
+    using Z = FewSizes<D, NT, Q8>;
     // pool and scales as [keys or values of a page][kv heads x positions][D]
     CUtensorMap map, scales;
     const uint64_t Hkv = a.c.Hkv, halves = (uint64_t)a.c.n_pages * 2, lines = JSM_PAGE_SIZE * D / 128;
@@ -474,13 +557,11 @@ static jsm_status few_go(const ChunkArgs& a, const FewPlan& f, float* part, cuda
     if (s == JSM_OK && Q8) s = make_tmap_u8_3d(&scales, a.c.scales, 128, Hkv, halves, 128, Hkv * 128, 128, 1, 2, false);
     if (s != JSM_OK) return s;
     static DeviceOnce once;
-    JSM_CUDA_CHECK(allow_shared(once, chunk_few_kernel<D, NT, Q8>, Z::smem(Z::STAGES, NT * 8)));
-    const int stages = std::min(f.run_pages, Z::STAGES);
-    JSM_CUDA_CHECK(launch_chained(chunk_few_kernel<D, NT, Q8>, dim3((unsigned)f.n_runs * a.c.n_seqs, a.c.Hkv), dim3(CF_THREADS), (size_t)Z::smem(stages, NT * 8), st, map, Q8 ? scales : map, a,
-                                  NT * 8, f.n_runs, f.run_pages, stages, part));
+    JSM_CUDA_CHECK(allow_shared(once, chunk_few_kernel<D, NT, Q8>, Z::SMEM));
+    JSM_CUDA_CHECK(launch_chained(chunk_few_kernel<D, NT, Q8>, dim3(f.n_runs), dim3(CF_THREADS), (size_t)Z::SMEM, st, map, Q8 ? scales : map, a, part));
     JSM_LAUNCH_CHECK();
-    if (f.n_runs > 1) {
-        JSM_CUDA_CHECK(launch_chained(chunk_merge_kernel<D, Q8>, dim3((unsigned)a.c.n_seqs * std::min(a.max_new, NT * 8 / a.G), a.Hq), dim3(128), 0, st, a, NT * 8, f.n_runs, f.run_pages, (const float*)part));
+    if (f.merge) {
+        JSM_CUDA_CHECK(launch_chained(chunk_merge_kernel<D, Q8>, dim3((unsigned)a.c.n_seqs * std::min(a.max_new, Z::ROWS / a.G), a.Hq), dim3(128), 0, st, a, Z::ROWS, f.n_runs, (const float*)part));
         JSM_LAUNCH_CHECK();
     }
     return JSM_OK;
