@@ -9,8 +9,8 @@
 //   warps 4-11    softmax, one thread per query row; register shares moved here from warps 0-3 (setmaxnreg)
 //   warps 12-15   8-bit caches: numbers of a raw page -> bf16(n * scale) in the swizzled tiles that the tensor cores read.  Every number is exact in bf16 and every product
 //                 rounded once, so scores and sums are those of a bf16 cache of these values; the conversion is spread over the whole group's rows
-// Few tiles and long contexts: the CTAs of a cluster share the key tiles of one pair of query tiles and meet in shared memory (each then joins its share of the rows, in
-// the order of the ranks), so that nothing goes through global memory and no second launch is needed.
+// Few tiles and long contexts: the CTAs of a cluster share the key tiles of one pair of query tiles; each sends the sums of the rows that another owns into that one's shared
+// memory and joins its own with what it was sent, so that nothing goes through global memory and no second launch is needed.
 // Values that no row of the CTA sees (behind the context, before the window) become zeros before they are multiplied; a row whose result is not a number is worked out
 // again over exactly its own keys (attend_row).  Every wait is bounded.
 #include "chunk_attn.cuh"
@@ -18,6 +18,7 @@
 #include "softmax_rows.cuh"
 #include "mma_utils.cuh"
 #include <math.h>
+#include <cmath>
 #include <algorithm>
 #include <mutex>
 
@@ -46,6 +47,7 @@ struct FlashArgs {
     int tile_tokens;   // tokens of a query tile
     int slots;         // pairs of query tiles, at most
     int share;         // CTAs (a cluster) of one pair of query tiles and kv head
+    uint32_t inv_G;    // row / G = row * inv_G >> 16 for the rows of a tile
 };
 
 __device__ __forceinline__ void ck_cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
@@ -55,45 +57,42 @@ __device__ __forceinline__ uint32_t ck_peer(uint32_t local, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
     return r;
 }
-__device__ __forceinline__ float2 ck_load2(uint32_t addr) {
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-    return v;
+__device__ __forceinline__ void ck_store2(uint32_t addr, float a, float b) {
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(a), "f"(b) : "memory");
 }
-__device__ __forceinline__ float4 ck_load4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
+__device__ __forceinline__ void ck_store4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 template <int N>
 __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// The slot-th pair of query tiles: its sequence and its number there; a whole warp.  False: there are fewer.
-__device__ __forceinline__ bool find_tile(const FlashArgs& f, int slot, int& seq, int& tile, int& n_tiles) {
+// The slot-th (sequence, pair of query tiles, kv head), for a whole warp; false: there are fewer.  The last tokens of a sequence, which see the most keys, come first
+// for all heads: long CTAs do not start last (one prompt of 4096 tokens 158 us, with the pairs of a head next to one another 188).
+__device__ __forceinline__ bool find_tile(const FlashArgs& f, long long slot, int& seq, int& hk, int& tile, int& row0, int& n_new, int& ctx) {
     const ChunkArgs& a = f.a;
     const int lane = threadIdx.x & 31, tokens = 2 * f.tile_tokens;
     for (int s0 = 0; s0 < a.c.n_seqs; s0 += 32) {
         const int s = s0 + lane;
         int n = 0;
-        if (s < a.c.n_seqs) {
-            const int from = a.c.starts[s], n_new = a.c.starts[s + 1] - from;
-            if (n_new > a.max_new || from < 0 || from + (long long)n_new > a.T) cache_error(a.c.err, CACHE_BAD_LENGTH);
-            else if (n_new > 0 && n_new * a.G > f.few_rows) n = (n_new + tokens - 1) / tokens;
-        }
-        int sum = n;
+        if (s < a.c.n_seqs && chunk_lengths(a, s, row0, n_new, ctx) && n_new * a.G > f.few_rows) n = (n_new + tokens - 1) / tokens;
+        long long sum = (long long)n * a.c.Hkv;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, sum, o);
+            const long long v = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += v;
         }
         const unsigned here = __ballot_sync(0xffffffffu, sum > slot);
         if (here) {
-            const int w = __ffs(here) - 1;
-            n_tiles = __shfl_sync(0xffffffffu, n, w);
-            tile = slot - (__shfl_sync(0xffffffffu, sum, w) - n_tiles);
+            const int w = __ffs(here) - 1, n_tiles = __shfl_sync(0xffffffffu, n, w);
+            const int in = (int)(slot - (__shfl_sync(0xffffffffu, sum, w) - (long long)n_tiles * a.c.Hkv));
+            hk = in % a.c.Hkv;
+            tile = n_tiles - 1 - in / a.c.Hkv;
             seq = s0 + w;
+            row0 = __shfl_sync(0xffffffffu, row0, w);
+            n_new = __shfl_sync(0xffffffffu, n_new, w);
+            ctx = __shfl_sync(0xffffffffu, ctx, w);
             return true;
         }
         slot -= __shfl_sync(0xffffffffu, sum, 31);
@@ -113,14 +112,17 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
     uint8_t* k_smem = tiles + 2 * Z::TILE;
     uint8_t* v_smem = k_smem + ST * Z::TILE;
     uint8_t* raw_smem = v_smem + ST * Z::TILE;
-    // a cluster's meeting, in place of tiles and rings: [256 rows][D] sums, then maximum and sum of the weights of each row
-    float2* sm_ml = reinterpret_cast<float2*>(tiles + 2 * CK_BM * D * 4);
+    // A cluster's meeting, in place of tiles and rings: the rows of eight softmax warps belong to the CTAs in equal shares; [sender][row of this CTA][D] sums and, behind them,
+    // [sender][row] references and sums of the weights.
+    const int own_rows = 2 * CK_BM / f.share;
+    uint8_t* recv = tiles;
+    uint8_t* recv_ml = tiles + (f.share - 1) * own_rows * (D * 4);
     __shared__ __align__(8) uint64_t q_full, o_done;
     __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], raw_full[4], raw_empty[4];
-    __shared__ __align__(8) uint64_t s_full[2], p_ready[2];
+    __shared__ __align__(8) uint64_t s_full[2], p_half[2], p_ready[2];
     __shared__ __align__(16) uint16_t raw_scales[4][JSM_PAGE_SIZE];
     __shared__ uint32_t tmem_base_smem;
-    __shared__ int abort_flag, sh_seq, sh_tile;
+    __shared__ int abort_flag, sh_seq, sh_head, sh_tile, sh_row0, sh_new, sh_ctx;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     chain_trigger();
@@ -135,7 +137,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
             mbar_init(&v_empty[s], 1);
         }
         for (int s = 0; s < 4; ++s) { mbar_init(&raw_full[s], 1); mbar_init(&raw_empty[s], 4); }
-        for (int t = 0; t < 2; ++t) { mbar_init(&s_full[t], 1); mbar_init(&p_ready[t], 4); }
+        for (int t = 0; t < 2; ++t) { mbar_init(&s_full[t], 1); mbar_init(&p_half[t], 4); mbar_init(&p_ready[t], 4); }
         mbar_fence_init();
     }
     if (warp == 1) {
@@ -143,13 +145,20 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
         tmem_relinquish();
     }
     chain_wait();
-    const int part = blockIdx.x % f.share, hk = blockIdx.x / f.share % a.c.Hkv;
+    const int part = blockIdx.x % f.share;
     if (warp == 0) {
-        int seq = -1, tile = 0, n = 0;
-        if (!find_tile(f, blockIdx.x / f.share / a.c.Hkv, seq, tile, n)) seq = -1;
+        int seq = -1, head = 0, tile = 0, row0 = 0, n_new = 0, ctx = 0;
+        if (!find_tile(f, blockIdx.x / f.share, seq, head, tile, row0, n_new, ctx)) {
+            seq = -1;
+            n_new = ctx = 0;
+        }
         if (lane == 0) {
+            sh_row0 = row0;
+            sh_new = n_new;
+            sh_ctx = ctx;
             sh_seq = seq;
-            sh_tile = n - 1 - tile;  // the last tokens see the most keys: first
+            sh_head = head;
+            sh_tile = tile;
         }
     }
     tc_fence_before();
@@ -157,9 +166,8 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
     tc_fence_after();
     const uint32_t tmem_base = tmem_base_smem;
     const uint32_t S_COL[2] = {0, 128}, O_COL[2] = {256, 256 + D};
-    const int seq = sh_seq;
-    int row0 = 0, n_new = 0, ctx = 0;
-    const bool work = seq >= 0 && chunk_lengths(a, seq, row0, n_new, ctx);
+    const int seq = sh_seq, hk = sh_head, row0 = sh_row0, n_new = sh_new, ctx = sh_ctx;
+    const bool work = seq >= 0;
 
     // query tile t: tokens tok[t] and up (none: tile empty); key tiles from the page that holds the first key of the first token
     const int tok[2] = {sh_tile * 2 * f.tile_tokens, (sh_tile * 2 + 1) * f.tile_tokens};
@@ -326,15 +334,20 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     if (active(t, j)) {
-                        if (!mbar_wait_warp(&p_ready[t], (j - jb[t]) & 1, &abort_flag, a.c.err, TC_TIMEOUT_MISC)) { ok = false; break; }
-                        tc_fence_after();
-                        if (elect_one()) {
+                        // The first half of the weights is taken while the second is being worked out: 2.24 -> 2.08 us per key tile.  (8-bit caches: 2.49 -> 2.55, so not there.)
 #pragma unroll
-                            for (int kk = 0; kk < CK_BN / 16; ++kk)
-                                mma_ts(tmem_base + O_COL[t], tmem_base + S_COL[t] + kk * 8, smem_desc_sw128_mn(v_addr + kk * 2048, Z::SLAB), idesc_pv,
-                                       (j > jb[t] || kk > 0) ? 1u : 0u);
+                        for (int half = 0; half < 2; ++half) {
+                            if ((half || !Q8) && !mbar_wait_warp(half ? &p_ready[t] : &p_half[t], (j - jb[t]) & 1, &abort_flag, a.c.err, TC_TIMEOUT_MISC)) { ok = false; break; }
+                            tc_fence_after();
+                            if ((half || !Q8) && elect_one()) {
+#pragma unroll
+                                for (int kk = Q8 ? 0 : half * 4; kk < half * 4 + 4; ++kk)
+                                    mma_ts(tmem_base + O_COL[t], tmem_base + S_COL[t] + kk * 8, smem_desc_sw128_mn(v_addr + kk * 2048, Z::SLAB), idesc_pv,
+                                           (j > jb[t] || kk > 0) ? 1u : 0u);
+                            }
+                            __syncwarp();
                         }
-                        __syncwarp();
+                        if (!ok) break;
                     }
                     if (t == 0 && more) {
                         if (!mbar_wait_warp(&k_full[s1], ((i + 1) / ST) & 1, &abort_flag, a.c.err, TC_TIMEOUT_FULL)) { ok = false; break; }
@@ -356,7 +369,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
         regs_inc<Q8 ? 200 : 224>();
         const int t = (warp - CK_SOFTMAX) / 4, quad = warp & 3, row = quad * 32 + lane;
         const int rows = f.tile_tokens * a.G;                       // rows of the tile that are queries
-        const int token = tok[t] + row / a.G, pos = past + token;   // (a row that is none has a position all the same)
+        const int token = tok[t] + (int)(row * f.inv_G >> 16), pos = past + token;   // (a row that is none has a position all the same)
         const bool query = work && row < rows && token < n_new;
         const uint32_t lane_addr = tmem_base + ((uint32_t)(quad * 32) << 16), s_addr = lane_addr + S_COL[t], o_addr = lane_addr + O_COL[t];
         const int pos_lo = past + tok[t], pos_hi = past + min(tok[t] + f.tile_tokens, n_new) - 1;  // first and last query of the tile
@@ -442,6 +455,12 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
                     w[i] = pack_bf16x2(p0, p1);
                 }
                 tmem_st16(s_addr + c, w);
+                if (!Q8 && c == 16) {
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_half[t]);
+                }
             }
             float la, lb;
             unpack2(fadd2(fadd2(ls2[0], ls2[1]), fadd2(ls2[2], ls2[3])), la, lb);
@@ -454,35 +473,84 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
         if (ok && n_max > j_lo) ok = mbar_wait_warp(&o_done, 0, &abort_flag, a.c.err, TC_TIMEOUT_ACC);
         tc_fence_after();
         const bool any = ok && je[t] > jb[t];  // (the whole query tile)
+        float own = 1.0f, L = l;  // factor of the sums in TMEM, sum of the weights
+        bool have = any;
+        int senders = 0;
+        float w_of[7];
         if (f.share > 1) {
-            // the row's sums into shared memory, 16-byte pieces swizzled by the row; every product has been taken, so tiles and rings are free
-            const int r = t * CK_BM + row;
-            sm_ml[r] = make_float2(any ? m_ref : CK_NONE, any ? l : 0.0f);
-            if (any) {
-                uint8_t* dst = tiles + (size_t)r * (D * 4);
+            ck_cluster_arrive();
+            ck_cluster_wait();  // every CTA has taken its products: tiles and rings may be overwritten
+            const int w = warp - CK_SOFTMAX, warps = 8 / f.share, owner = w / warps, r = w % warps * 32 + lane;
+            if (owner != part) {
+                const int from = part < owner ? part : part - 1;
+                const uint32_t to = ck_peer(smem_u32(recv) + (from * own_rows + r) * (D * 4), owner);
+                ck_store2(ck_peer(smem_u32(recv_ml) + (from * own_rows + r) * 8, owner), any ? m_ref : CK_NONE, any ? l : 0.0f);
+                if (any) {
 #pragma unroll
-                for (int c = 0; c < D; c += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(o_addr + c, o);
-                    tmem_ld_wait();
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(o_addr + c, o);
+                        tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(dst + ((((c + i) / 4) ^ (r & 7)) * 16)) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        for (int i = 0; i < 32; i += 4) ck_store4(to + ((((c + i) / 4) ^ (lane & 7)) * 16), o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    }
                 }
             }
-        } else if (any) {
-            const float inv = 1.0f / l;
+            ck_cluster_arrive();
+            ck_cluster_wait();  // the sums are here
+            have = false;
+            if (owner == part) {
+                const float2* ml = reinterpret_cast<const float2*>(recv_ml) + r;
+                senders = f.share - 1;
+                float M = any ? m_ref : CK_NONE;
+                for (int p = 0; p < senders; ++p) M = fmaxf(M, ml[p * own_rows].x);
+                own = any ? ex2_approx(m_ref - M) : 0.0f;
+                L = any ? l * own : 0.0f;
+#pragma unroll
+                for (int p = 0; p < 7; ++p)
+                    if (p < senders) {
+                        const float2 v = ml[p * own_rows];
+                        w_of[p] = v.x == CK_NONE && v.y == 0.0f ? -1.0f : ex2_approx(v.x - M);  // (-1: it had none of the row's keys)
+                        if (w_of[p] >= 0.0f || v.y != v.y) L = fmaf(w_of[p], v.y, L);
+                    }
+                have = tok[t] < n_new;
+            }
+        }
+        if (have) {
+            const float inv = 1.0f / L;
+            const int r_own = (warp - CK_SOFTMAX) % (8 / f.share) * 32 + lane;
             bool bad = false;
-            // a thread has a row: the warp's 32 rows pass through the queries' place and leave whole, 16 bytes per lane
-            uint8_t* staged = q_smem + t * Z::TILE + quad * (32 * D * 2);
+            // a thread has a row: the warp's 32 rows pass through shared memory (the queries' place) and leave whole, 16 bytes per lane
+            uint8_t* staged = (f.share > 1 ? recv_ml + (f.share - 1) * own_rows * 8 : tiles) + (warp - CK_SOFTMAX) * (32 * D * 2);
 #pragma unroll
             for (int c = 0; c < D; c += 32) {
-                uint32_t r[32];
-                tmem_ld32(o_addr + c, r);
-                tmem_ld_wait();
                 float x[32];
+                if (any) {
+                    uint32_t r[32];
+                    tmem_ld32(o_addr + c, r);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]) * own;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x[i] = 0.0f;
+                }
+#pragma unroll
+                for (int p = 0; p < 7; ++p)
+                    if (p < senders && w_of[p] >= 0.0f) {
+                        const uint8_t* src = recv + (p * own_rows + r_own) * (D * 4);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 v = *reinterpret_cast<const float4*>(src + ((((c + i) / 4) ^ (lane & 7)) * 16));
+                            x[i] = fmaf(w_of[p], v.x, x[i]);
+                            x[i + 1] = fmaf(w_of[p], v.y, x[i + 1]);
+                            x[i + 2] = fmaf(w_of[p], v.z, x[i + 2]);
+                            x[i + 3] = fmaf(w_of[p], v.w, x[i + 3]);
+                        }
+                    }
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
-                    x[i] = __uint_as_float(r[i]) * inv;
+                    x[i] *= inv;
                     bad = bad || !(fabsf(x[i]) <= 3.402823466e38f);
                 }
 #pragma unroll
@@ -495,9 +563,9 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
             const int piece = lane % PIECES;
 #pragma unroll 4
             for (int r = lane / PIECES; r < 32; r += STEP) {
-                const int at = quad * 32 + r, tk = tok[t] + at / a.G;
+                const int at = quad * 32 + r, in = (int)(at * f.inv_G >> 16), tk = tok[t] + in;
                 if (at < rows && tk < n_new)
-                    *reinterpret_cast<uint4*>(a.out + (row0 + tk) * a.out_rs + (long long)(hk * a.G + at % a.G) * D + piece * 8) =
+                    *reinterpret_cast<uint4*>(a.out + (row0 + tk) * a.out_rs + (long long)(hk * a.G + at - in * a.G) * D + piece * 8) =
                         *reinterpret_cast<const uint4*>(staged + r * (D * 2) + ((piece ^ (r & 7)) * 16));
             }
             __syncwarp();
@@ -571,95 +639,18 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
             }
         }
     }
+    if (f.share > 1 && (warp < CK_SOFTMAX || warp >= CK_CONVERT)) {  // (the meeting counts every thread)
+        ck_cluster_arrive();
+        ck_cluster_wait();
+        ck_cluster_arrive();
+        ck_cluster_wait();
+    }
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem_base, 512);
     }
-    if (f.share == 1) return;
-    ck_cluster_arrive();
-    ck_cluster_wait();  // every CTA's sums are in its shared memory
-    if (work && !abort_flag && warp >= CK_SOFTMAX && warp < CK_CONVERT) {
-        constexpr int N = D / 32, R = 4;
-        const int n_rows = f.tile_tokens * a.G;
-        const uint32_t sums = smem_u32(tiles), ml = smem_u32(sm_ml);
-        // Four rows at a time, every CTA's part of them requested before the first is used: lane 8 i + p has maximum and sum of row i in CTA p.
-        for (int k0 = (warp - CK_SOFTMAX) * R; part + f.share * k0 < 2 * CK_BM; k0 += 8 * R) {
-            int row[R], at[R], tk[R];
-            bool on[R];
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                row[i] = part + f.share * (k0 + i);
-                const int t = row[i] / CK_BM;
-                at[i] = row[i] % CK_BM;
-                tk[i] = (t ? tok[1] : tok[0]) + at[i] / a.G;
-                on[i] = row[i] < 2 * CK_BM && at[i] < n_rows && tk[i] < n_new;
-            }
-            if (!on[0] && !on[1] && !on[2] && !on[3]) continue;
-            const int li = lane >> 3, lp = lane & 7, lrow = part + f.share * (k0 + li);
-            float2 mine = make_float2(CK_NONE, 0.0f);
-            if (lp < f.share && lrow < 2 * CK_BM) mine = ck_load2(ck_peer(ml + lrow * 8, lp));
-            float M = mine.x;
-#pragma unroll
-            for (int o = 4; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-            const bool none = mine.x == CK_NONE && mine.y == 0.0f;  // that CTA had none of the row's keys
-            const float weight = none ? 0.0f : ex2_approx(mine.x - M);
-            float L = weight * mine.y;
-#pragma unroll
-            for (int o = 4; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-            float acc[R][N];
-#pragma unroll
-            for (int i = 0; i < R; ++i)
-#pragma unroll
-                for (int n = 0; n < N; ++n) acc[i][n] = 0.0f;
-            const unsigned nothing = __ballot_sync(0xffffffffu, none);
-#pragma unroll 2
-            for (int p = 0; p < f.share; ++p) {
-                float x[R][N];
-#pragma unroll
-                for (int i = 0; i < R; ++i) {
-                    const int r = min(row[i], 2 * CK_BM - 1);
-                    const uint32_t src = ck_peer(sums + r * (D * 4) + (((lane * N / 4) ^ (r & 7)) * 16) + (N == 2 ? (lane & 1) * 8 : 0), p);
-                    if constexpr (N == 4) {
-                        const float4 v = ck_load4(src);
-                        x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
-                    } else {
-                        const float2 v = ck_load2(src);
-                        x[i][0] = v.x; x[i][1] = v.y;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < R; ++i) {
-                    const float w = __shfl_sync(0xffffffffu, weight, i * 8 + p);
-                    if (!(nothing >> (i * 8 + p) & 1))
-#pragma unroll
-                        for (int n = 0; n < N; ++n) acc[i][n] = fmaf(w, x[i][n], acc[i][n]);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                if (!on[i]) continue;
-                const float inv = 1.0f / __shfl_sync(0xffffffffu, L, i * 8);
-                bool fine = true;
-#pragma unroll
-                for (int n = 0; n < N; ++n) {
-                    acc[i][n] *= inv;
-                    fine = fine && fabsf(acc[i][n]) <= 3.402823466e38f;
-                }
-                const int head = hk * a.G + at[i] % a.G;
-                if (__all_sync(0xffffffffu, fine)) {
-                    __nv_bfloat16* dst = a.out + (row0 + tk[i]) * a.out_rs + (long long)head * D + lane * N;
-#pragma unroll
-                    for (int n = 0; n < N; n += 2) *reinterpret_cast<uint32_t*>(dst + n) = pack_bf16x2(acc[i][n], acc[i][n + 1]);
-                } else {
-                    attend_row<D, Q8>(a, seq, row0 + tk[i], head, past + tk[i]);
-                }
-            }
-        }
-    }
-    ck_cluster_arrive();
-    ck_cluster_wait();  // no CTA leaves while a peer reads its shared memory
 }
 
 // clusters of S CTAs that the chip holds at once (15 of eight, 33 of four, although it has 148 multiprocessors)
@@ -695,20 +686,23 @@ static int flash_capacity(int S) {
 template <int D, bool Q8>
 static jsm_status flash_launch(const ChunkArgs& a, int few_rows, cudaStream_t st) {
     using Z = FlashSizes<D, Q8>;
-    FlashArgs f{a, few_rows, CK_BM / a.G, 0, 1};
+    FlashArgs f{a, few_rows, CK_BM / a.G, 0, 1, (65536u + a.G - 1) / a.G};
     const long long tokens = 2ll * f.tile_tokens, per_seq = (a.max_new + tokens - 1) / tokens;
     f.slots = (int)std::min(per_seq * a.c.n_seqs, a.T / tokens + a.c.n_seqs);
     static DeviceOnce once;
     JSM_CUDA_CHECK(allow_shared(once, chunk_flash_kernel<D, Q8>, (int)Z::SMEM));
-    // CTAs of a pair of query tiles: a key tile takes about 1.2 us, what is around the walk 5 us, the meeting of a cluster 3 us; those that do not fit at once wait
-    long long keys = a.max_context;
-    if (a.window > 0) keys = std::min(keys, (long long)a.window + tokens);
-    const long long key_tiles = (keys + CK_BN - 1) / CK_BN, pairs = (long long)f.slots * a.c.Hkv;
+    // CTAs of a pair of query tiles.  A key tile takes about 2 us, what is around the walk 6 us, the meeting of a cluster 3 us: the longest CTA, or the chip's share of all and
+    // half a CTA's time for the uneven end.  (Of a sequence that is all new tokens, a pair sees half of the keys on average.)
+    long long keys = a.max_context, mean = a.max_context - a.max_new / 2;
+    if (a.window > 0) { keys = std::min(keys, (long long)a.window + tokens); mean = std::min(mean, keys); }
+    const long long pairs = (long long)f.slots * a.c.Hkv;
+    const float key_tiles = (float)((keys + CK_BN - 1) / CK_BN), mean_tiles = (float)mean / CK_BN;
     float best = 0.0f;
     for (int S = 1; S <= 8; S *= 2) {
-        if (S > 1 && key_tiles < 4 * S) break;
+        if (S > 1 && key_tiles < 2 * S) break;
         const int cap = flash_capacity<D, Q8>(S);
-        const float cost = (float)((pairs + cap - 1) / cap) * (5.0f + (S > 1 ? 3.0f : 0.0f) + 1.2f * (float)((key_tiles + S - 1) / S));
+        const float around = 6.0f + (S > 1 ? 3.0f : 0.0f), longest = around + 2.0f * std::ceil(key_tiles / S), one = around + 2.0f * mean_tiles / S;
+        const float cost = pairs <= cap ? longest : std::max(longest, one * ((float)pairs / cap + 0.5f));
         if (S == 1 || cost < best) { best = cost; f.share = S; }
     }
     if (pairs * f.share > INT32_MAX) JSM_FAIL(JSM_UNSUPPORTED, "jsm_attn_chunk: %lld tiles of queries", pairs);
