@@ -21,6 +21,7 @@
 #include <cmath>
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 namespace jsm {
 
@@ -104,7 +105,7 @@ template <int D, bool Q8>
 __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
     chunk_flash_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_kv, const __grid_constant__ FlashArgs f) {
     using Z = FlashSizes<D, Q8>;
-    constexpr int ST = Z::ST, POLY = 1;
+    constexpr int ST = Z::ST;
     const ChunkArgs& a = f.a;
     extern __shared__ uint8_t ck_smem[];
     uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ck_smem) + 1023) & ~uintptr_t(1023));
@@ -427,41 +428,42 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
                     m_ref = mx;
                 }
             }
-            // p = 2^(s - m_ref) as bf16 pairs over the first 64 columns of S
+            // p = 2^(s - m_ref) as bf16 pairs over the first 64 columns of S.  Where keys are hidden the special-function unit takes all of them: the polynomial ends at 2^-126, and
+            // a hidden key's weight is nothing at all.
             uint64_t ls2[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) ls2[k] = pack2(0.0f, 0.0f);
             const uint64_t neg_m2 = pack2(-m_ref, -m_ref), sc2 = pack2(a.scale_log2, a.scale_log2);
+            auto weights = [&](auto poly) {
 #pragma unroll
-            for (int c = 0; c < CK_BN / 2; c += 16) {
-                uint32_t w[16];
+                for (int c = 0; c < CK_BN / 2; c += 16) {
+                    uint32_t w[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint64_t x2 = ffma2(pack2(sv[2 * (c + i)], sv[2 * (c + i) + 1]), sc2, neg_m2);
-                    float p0, p1;
-                    if ((i & 3) < POLY) {
-                        ex2_poly2(x2, p0, p1);
-                        if (masked) {  // (the polynomial ends at 2^-126: a hidden key's weight is nothing at all)
-                            if (sv[2 * (c + i)] == -INFINITY) p0 = 0.0f;
-                            if (sv[2 * (c + i) + 1] == -INFINITY) p1 = 0.0f;
+                    for (int i = 0; i < 16; ++i) {
+                        const uint64_t x2 = ffma2(pack2(sv[2 * (c + i)], sv[2 * (c + i) + 1]), sc2, neg_m2);
+                        float p0, p1;
+                        if ((i & 3) < decltype(poly)::value) {
+                            ex2_poly2(x2, p0, p1);
+                        } else {
+                            float x0, x1;
+                            unpack2(x2, x0, x1);
+                            p0 = ex2_approx(x0);
+                            p1 = ex2_approx(x1);
                         }
-                    } else {
-                        float x0, x1;
-                        unpack2(x2, x0, x1);
-                        p0 = ex2_approx(x0);
-                        p1 = ex2_approx(x1);
+                        ls2[i & 3] = fadd2(ls2[i & 3], pack2(p0, p1));
+                        w[i] = pack_bf16x2(p0, p1);
                     }
-                    ls2[i & 3] = fadd2(ls2[i & 3], pack2(p0, p1));
-                    w[i] = pack_bf16x2(p0, p1);
+                    tmem_st16(s_addr + c, w);
+                    if (!Q8 && c == 16) {
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&p_half[t]);
+                    }
                 }
-                tmem_st16(s_addr + c, w);
-                if (!Q8 && c == 16) {
-                    tmem_st_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_half[t]);
-                }
-            }
+            };
+            if (masked) weights(std::integral_constant<int, 0>{});
+            else weights(std::integral_constant<int, 1>{});
             float la, lb;
             unpack2(fadd2(fadd2(ls2[0], ls2[1]), fadd2(ls2[2], ls2[3])), la, lb);
             l += la + lb;
@@ -473,100 +475,114 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
         if (ok && n_max > j_lo) ok = mbar_wait_warp(&o_done, 0, &abort_flag, a.c.err, TC_TIMEOUT_ACC);
         tc_fence_after();
         const bool any = ok && je[t] > jb[t];  // (the whole query tile)
-        float own = 1.0f, L = l;  // factor of the sums in TMEM, sum of the weights
+        // What follows is executed once per CTA, mostly for the first time on its multiprocessor: rolled loops, because every line of code is fetched (unrolled, with the
+        // factors of up to seven senders in registers, the end of a CTA took 4.2 us instead of 1.6).
+        const int sw = warp - CK_SOFTMAX;
+        uint8_t* staged = (f.share > 1 ? recv_ml + (f.share - 1) * own_rows * 8 : tiles) + sw * (32 * D * 2);  // this warp's 32 rows pass through here
+        float own = 1.0f, L = l, M = m_ref;  // factor of the sums in TMEM, sum of the weights, reference of the row
         bool have = any;
         int senders = 0;
-        float w_of[7];
+        const int warps = 8 / f.share, owner = sw / warps, r_own = sw % warps * 32;  // of a cluster: who joins this warp's rows, and where they are there
+        auto sent_factor = [&](int p) {  // (0: that CTA had none of the row's keys)
+            const float2 v = reinterpret_cast<const float2*>(recv_ml)[p * own_rows + r_own + lane];
+            return make_float2(v.x == CK_NONE && v.y == 0.0f ? 0.0f : ex2_approx(v.x - M), v.y);
+        };
         if (f.share > 1) {
             ck_cluster_arrive();
             ck_cluster_wait();  // every CTA has taken its products: tiles and rings may be overwritten
-            const int w = warp - CK_SOFTMAX, warps = 8 / f.share, owner = w / warps, r = w % warps * 32 + lane;
             if (owner != part) {
-                const int from = part < owner ? part : part - 1;
-                const uint32_t to = ck_peer(smem_u32(recv) + (from * own_rows + r) * (D * 4), owner);
-                ck_store2(ck_peer(smem_u32(recv_ml) + (from * own_rows + r) * 8, owner), any ? m_ref : CK_NONE, any ? l : 0.0f);
+                const int at = (part < owner ? part : part - 1) * own_rows + r_own;
+                ck_store2(ck_peer(smem_u32(recv_ml) + (at + lane) * 8, owner), any ? m_ref : CK_NONE, any ? l : 0.0f);
                 if (any) {
-#pragma unroll
+                    // a row per thread would send 16 bytes to 32 places at a time: through shared memory, so that eight lanes send 128 bytes
+                    const uint32_t to = ck_peer(smem_u32(recv) + at * (D * 4), owner), here = smem_u32(staged);
+#pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         uint32_t o[32];
                         tmem_ld32(o_addr + c, o);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) ck_store4(to + ((((c + i) / 4) ^ (lane & 7)) * 16), o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        for (int i = 0; i < 8; ++i) sts128(here + lane * 128 + ((i ^ (lane & 7)) * 16), make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const int r = k * 4 + (lane >> 3), piece = lane & 7;
+                            const uint4 v = lds128(here + r * 128 + ((piece ^ (r & 7)) * 16));
+                            ck_store4(to + r * (D * 4) + (((c / 4 + piece) ^ (r & 7)) * 16), v.x, v.y, v.z, v.w);
+                        }
+                        __syncwarp();
                     }
                 }
             }
             ck_cluster_arrive();
             ck_cluster_wait();  // the sums are here
-            have = false;
-            if (owner == part) {
-                const float2* ml = reinterpret_cast<const float2*>(recv_ml) + r;
+            have = owner == part && tok[t] < n_new;
+            if (have) {
                 senders = f.share - 1;
-                float M = any ? m_ref : CK_NONE;
-                for (int p = 0; p < senders; ++p) M = fmaxf(M, ml[p * own_rows].x);
+                if (!any) M = CK_NONE;
+#pragma unroll 1
+                for (int p = 0; p < senders; ++p) M = fmaxf(M, reinterpret_cast<const float2*>(recv_ml)[p * own_rows + r_own + lane].x);
                 own = any ? ex2_approx(m_ref - M) : 0.0f;
                 L = any ? l * own : 0.0f;
-#pragma unroll
-                for (int p = 0; p < 7; ++p)
-                    if (p < senders) {
-                        const float2 v = ml[p * own_rows];
-                        w_of[p] = v.x == CK_NONE && v.y == 0.0f ? -1.0f : ex2_approx(v.x - M);  // (-1: it had none of the row's keys)
-                        if (w_of[p] >= 0.0f || v.y != v.y) L = fmaf(w_of[p], v.y, L);
-                    }
-                have = tok[t] < n_new;
+#pragma unroll 1
+                for (int p = 0; p < senders; ++p) {
+                    const float2 w = sent_factor(p);
+                    if (w.x != 0.0f || w.y != 0.0f) L = fmaf(w.x, w.y, L);
+                }
             }
         }
         if (have) {
             const float inv = 1.0f / L;
-            const int r_own = (warp - CK_SOFTMAX) % (8 / f.share) * 32 + lane;
             bool bad = false;
-            // a thread has a row: the warp's 32 rows pass through shared memory (the queries' place) and leave whole, 16 bytes per lane
-            uint8_t* staged = (f.share > 1 ? recv_ml + (f.share - 1) * own_rows * 8 : tiles) + (warp - CK_SOFTMAX) * (32 * D * 2);
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 float x[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) x[i] = 0.0f;
                 if (any) {
                     uint32_t r[32];
                     tmem_ld32(o_addr + c, r);
                     tmem_ld_wait();
 #pragma unroll
                     for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]) * own;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) x[i] = 0.0f;
                 }
-#pragma unroll
-                for (int p = 0; p < 7; ++p)
-                    if (p < senders && w_of[p] >= 0.0f) {
-                        const uint8_t* src = recv + (p * own_rows + r_own) * (D * 4);
+#pragma unroll 2
+                for (int p = 0; p < senders; ++p) {
+                    const float w = sent_factor(p).x;
+                    const uint8_t* src = recv + (p * own_rows + r_own + lane) * (D * 4);
+                    if (w != 0.0f)
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
                             const float4 v = *reinterpret_cast<const float4*>(src + ((((c + i) / 4) ^ (lane & 7)) * 16));
-                            x[i] = fmaf(w_of[p], v.x, x[i]);
-                            x[i + 1] = fmaf(w_of[p], v.y, x[i + 1]);
-                            x[i + 2] = fmaf(w_of[p], v.z, x[i + 2]);
-                            x[i + 3] = fmaf(w_of[p], v.w, x[i + 3]);
+                            x[i] = fmaf(w, v.x, x[i]);
+                            x[i + 1] = fmaf(w, v.y, x[i + 1]);
+                            x[i + 2] = fmaf(w, v.z, x[i + 2]);
+                            x[i + 3] = fmaf(w, v.w, x[i + 3]);
                         }
-                    }
+                }
+                float sum = 0.0f;  // (a component that is no number makes it one that is none either)
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
                     x[i] *= inv;
-                    bad = bad || !(fabsf(x[i]) <= 3.402823466e38f);
+                    sum = fmaf(x[i], 0.0f, sum);
                 }
+                bad = bad || sum != 0.0f;
 #pragma unroll
                 for (int i = 0; i < 32; i += 8)
                     *reinterpret_cast<uint4*>(staged + lane * (D * 2) + ((((c + i) / 8) ^ (lane & 7)) * 16)) =
                         make_uint4(pack_bf16x2(x[i], x[i + 1]), pack_bf16x2(x[i + 2], x[i + 3]), pack_bf16x2(x[i + 4], x[i + 5]), pack_bf16x2(x[i + 6], x[i + 7]));
             }
             __syncwarp();
+            // rows leave whole, 16 bytes per lane; lane r knows where row r goes
             constexpr int PIECES = D / 8, STEP = 32 / PIECES;
-            const int piece = lane % PIECES;
-#pragma unroll 4
-            for (int r = lane / PIECES; r < 32; r += STEP) {
-                const int at = quad * 32 + r, in = (int)(at * f.inv_G >> 16), tk = tok[t] + in;
-                if (at < rows && tk < n_new)
-                    *reinterpret_cast<uint4*>(a.out + (row0 + tk) * a.out_rs + (long long)(hk * a.G + at - in * a.G) * D + piece * 8) =
-                        *reinterpret_cast<const uint4*>(staged + r * (D * 2) + ((piece ^ (r & 7)) * 16));
+            const int piece = lane % PIECES, in = (int)(row * f.inv_G >> 16);
+            const long long goes = query ? (row0 + token) * a.out_rs + (long long)(hk * a.G + row - in * a.G) * D : -1;
+#pragma unroll 2
+            for (int r0 = 0; r0 < 32; r0 += STEP) {
+                const int r = r0 + lane / PIECES;
+                const long long at = __shfl_sync(0xffffffffu, goes, r);
+                const uint4 v = *reinterpret_cast<const uint4*>(staged + r * (D * 2) + ((piece ^ (r & 7)) * 16));
+                if (at >= 0) *reinterpret_cast<uint4*>(a.out + at + piece * 8) = v;
             }
             __syncwarp();
             unsigned again = __ballot_sync(0xffffffffu, bad && query);
