@@ -101,6 +101,42 @@ __device__ __forceinline__ bool find_tile(const FlashArgs& f, long long slot, in
     return false;
 }
 
+// What a CTA walks: query tile t has the tokens tok[t] and up (none: it is empty) and sees the key tiles jb[t] .. je[t]-1, counted from the page that holds the first key of the
+// CTA's first token; the CTA's own are j_lo .. n_max-1.  No row sees a key before lo or from end on.
+struct Walk {
+    int tok[2], jb[2], je[2], lo, base, end, j_lo, n_max;
+};
+__device__ __forceinline__ Walk walk_of(const FlashArgs& f, int tile, int n_new, int ctx, int part) {
+    Walk w;
+    const int past = ctx - n_new, window = f.a.window;
+    w.tok[0] = tile * 2 * f.tile_tokens;
+    w.tok[1] = w.tok[0] + f.tile_tokens;
+    w.lo = first_key(window, past + w.tok[0]);
+    w.base = w.lo / JSM_PAGE_SIZE * JSM_PAGE_SIZE;
+    w.end = past + min(w.tok[0] + 2 * f.tile_tokens, n_new);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        w.jb[t] = w.je[t] = 0;
+        if (w.tok[t] < n_new) {
+            w.jb[t] = (first_key(window, past + w.tok[t]) - w.base) / CK_BN;
+            w.je[t] = (past + min(w.tok[t] + f.tile_tokens, n_new) - 1 - w.base) / CK_BN + 1;
+        }
+    }
+    w.j_lo = w.jb[0];
+    w.n_max = max(w.je[0], w.je[1]);
+    if (f.share > 1) {  // this CTA's share of the key tiles
+        const int len = (w.n_max - w.j_lo + f.share - 1) / f.share, from = w.j_lo + part * len, to = min(w.n_max, from + len);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            w.jb[t] = max(w.jb[t], from);
+            w.je[t] = max(w.jb[t], min(w.je[t], to));
+        }
+        w.j_lo = min(from, to);
+        w.n_max = to;
+    }
+    return w;
+}
+
 template <int D, bool Q8>
 __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
     chunk_flash_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_kv, const __grid_constant__ FlashArgs f) {
@@ -127,7 +163,9 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     chain_trigger();
-    if (warp == 2 && elect_one()) {
+    if (warp == 0 && elect_one()) {
+        tma_prefetch_desc(&tmap_q);
+        tma_prefetch_desc(&tmap_kv);
         abort_flag = 0;
         mbar_init(&q_full, 1);
         mbar_init(&o_done, 1);
@@ -147,12 +185,15 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
     }
     chain_wait();
     const int part = blockIdx.x % f.share;
+    int pages = 0;  // warp 0: pages of 16 key tiles at a time, lane i has the i-th
+    auto load_pages = [&](int seq, const Walk& w, int j) {
+        const int p = w.base / JSM_PAGE_SIZE + 2 * j + lane;
+        return p * JSM_PAGE_SIZE < w.end ? cache_page(a.c, seq, p * JSM_PAGE_SIZE) : 0;
+    };
     if (warp == 0) {
+        __syncwarp();
         int seq = -1, head = 0, tile = 0, row0 = 0, n_new = 0, ctx = 0;
-        if (!find_tile(f, blockIdx.x / f.share, seq, head, tile, row0, n_new, ctx)) {
-            seq = -1;
-            n_new = ctx = 0;
-        }
+        if (!find_tile(f, blockIdx.x / f.share, seq, head, tile, row0, n_new, ctx)) seq = -1;
         if (lane == 0) {
             sh_row0 = row0;
             sh_new = n_new;
@@ -160,6 +201,20 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
             sh_seq = seq;
             sh_head = head;
             sh_tile = tile;
+        }
+        if (seq >= 0) {  // queries and the first pages are on their way before the block meets
+            const Walk w = walk_of(f, tile, n_new, ctx, part);
+            if (w.n_max > w.j_lo) {
+                pages = load_pages(seq, w, w.j_lo);
+                if (elect_one()) {
+                    const int n_q = w.tok[1] < n_new ? 2 : 1;
+                    mbar_expect_tx(&q_full, (uint32_t)(n_q * (D / 64) * f.tile_tokens * a.G) * 128);
+                    for (int t = 0; t < n_q; ++t)
+#pragma unroll
+                        for (int c = 0; c < D / 64; ++c) tma_load_3d(q_smem + t * Z::TILE + c * Z::SLAB, &tmap_q, c * 64, head * a.G, row0 + w.tok[t], &q_full);
+                }
+                __syncwarp();
+            }
         }
     }
     tc_fence_before();
@@ -170,58 +225,23 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
     const int seq = sh_seq, hk = sh_head, row0 = sh_row0, n_new = sh_new, ctx = sh_ctx;
     const bool work = seq >= 0;
 
-    // query tile t: tokens tok[t] and up (none: tile empty); key tiles from the page that holds the first key of the first token
-    const int tok[2] = {sh_tile * 2 * f.tile_tokens, (sh_tile * 2 + 1) * f.tile_tokens};
-    const int past = ctx - n_new;
-    const int lo = work ? first_key(a.window, past + tok[0]) : 0;   // no row of the CTA sees a key before it
-    const int base = lo / JSM_PAGE_SIZE * JSM_PAGE_SIZE;
-    int jb[2] = {0, 0}, je[2] = {0, 0};
-    if (work) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-            if (tok[t] < n_new) {
-                jb[t] = (first_key(a.window, past + tok[t]) - base) / CK_BN;
-                je[t] = (past + min(tok[t] + f.tile_tokens, n_new) - 1 - base) / CK_BN + 1;
-            }
-    }
-    int j_lo = jb[0], n_max = max(je[0], je[1]);
-    if (f.share > 1) {  // this CTA's share of the key tiles
-        const int len = (n_max - j_lo + f.share - 1) / f.share, from = j_lo + part * len, to = min(n_max, from + len);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            jb[t] = max(jb[t], from);
-            je[t] = max(jb[t], min(je[t], to));
-        }
-        j_lo = min(from, to);
-        n_max = to;
-    }
-    const int end = work ? past + min(tok[0] + 2 * f.tile_tokens, n_new) : 0;  // keys behind it: no row of the CTA sees them
+    Walk w = {};
+    if (work) w = walk_of(f, sh_tile, n_new, ctx, part);
+    const int past = ctx - n_new, lo = w.lo, base = w.base, end = w.end, j_lo = w.j_lo, n_max = w.n_max;
+    const int(&tok)[2] = w.tok, (&jb)[2] = w.jb, (&je)[2] = w.je;
 
     if (warp < CK_SOFTMAX) regs_dec<Q8 ? 40 : 56>();
     if (warp == 0) {
         if (work && n_max > j_lo) {
-            if (elect_one()) {
-                const uint32_t box = (uint32_t)(f.tile_tokens * a.G) * 128;
-                const int n_q = tok[1] < n_new ? 2 : 1;
-                mbar_expect_tx(&q_full, n_q * (D / 64) * box);
-                for (int t = 0; t < n_q; ++t)
-#pragma unroll
-                    for (int c = 0; c < D / 64; ++c) tma_load_3d(q_smem + t * Z::TILE + c * Z::SLAB, &tmap_q, c * 64, hk * a.G, row0 + tok[t], &q_full);
-            }
-            __syncwarp();
-            // pages of 16 key tiles at a time: lane i has the i-th; behind the context the last page again (hidden keys)
-            const int page0 = base / JSM_PAGE_SIZE, last_page = (end - 1) / JSM_PAGE_SIZE;
-            int pages = 0, k_issued = 0, v_issued = 0;
+            const int page0 = base / JSM_PAGE_SIZE, last_page = (end - 1) / JSM_PAGE_SIZE;  // (behind the context the last page again: hidden keys)
+            int k_issued = 0, v_issued = 0;
             auto page_row = [&](int i, int half, int value) {  // row of the pool where the page of a key tile's half starts
                 const int page = __shfl_sync(0xffffffffu, pages, (2 * i + half) & 31);
                 return page < 0 ? -JSM_PAGE_SIZE : (int)cache_row(a.c, page, value, hk, 0);  // (outside the pool: rows before the first one, zeros)
             };
             for (int j = j_lo; j < n_max; ++j) {
                 const int i = j - j_lo, s = i % ST;
-                if ((i & 15) == 0) {
-                    const int p = page0 + 2 * j + lane;
-                    pages = p <= last_page ? cache_page(a.c, seq, p * JSM_PAGE_SIZE) : 0;
-                }
+                if ((i & 15) == 0 && i > 0) pages = load_pages(seq, w, j);
                 int rows[2][2];
 #pragma unroll
                 for (int value = 0; value < 2; ++value)
