@@ -6,6 +6,7 @@
 // gives s = NaN: the whole row then reads back as NaN, which no reader can mistake for a number.
 // Bound by memory: 4 D bytes in and 2 D + 4 bytes out per token and kv head.
 #include "cache_view.cuh"
+#include <limits.h>
 #include <math.h>
 
 namespace jsm {
@@ -24,15 +25,22 @@ struct AppendArgs {
 constexpr float Q8_SMALLEST = 7.8886090522101180541e-31f;  // 2^-100
 constexpr float Q8_LARGEST = 1.7014118346046923173e38f;    // 2^127: 127 s stays a bf16 number
 
-// the scale of a row whose largest magnitude is `most`
+// The scale of a row whose largest magnitude is `most` (NaN: the row has one).  The quotient by 127 is correctly rounded: Markstein's theorem ("Computation of elementary
+// functions on the IBM RISC System/6000 processor", 1990) for the correctly rounded reciprocal of the divisor, one residual and one correction.
 __device__ __forceinline__ float q8_scale(float most) {
+    constexpr float INV = 1.0f / 127.0f;
+    const float q = __fmul_rn(most, INV), s = __fmaf_rn(__fmaf_rn(-127.0f, q, most), INV, q);
     if (most < Q8_SMALLEST) return 0.0f;
-    if (!(most <= Q8_LARGEST)) return __uint_as_float(0x7FC00000u);
-    return __uint_as_float((__float_as_uint(__fdiv_rn(most, 127.0f)) + 0xFFFFu) & 0xFFFF0000u);
+    return most <= Q8_LARGEST ? __uint_as_float((__float_as_uint(s) + 0xFFFFu) & 0xFFFF0000u) : __uint_as_float(0x7FC00000u);
 }
-__device__ __forceinline__ float q8_inverse(float scale) { return scale == 0.0f ? 0.0f : __fdiv_rn(1.0f, scale); }
+__device__ __forceinline__ float q8_inverse(float scale) { return scale == 0.0f ? 0.0f : __frcp_rn(scale); }
+__device__ __forceinline__ float max_nan(float a, float b) {  // a NaN stays one
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
 
-// any pitches, alignments and rotations: one warp per (token, keys or values, kv head)
+// any pitches and alignments: one warp per (token, keys or values, kv head)
 __global__ void __launch_bounds__(256) kv_append_q8_kernel(AppendArgs a) {
     __shared__ int found;
     chain_trigger();
@@ -53,7 +61,6 @@ __global__ void __launch_bounds__(256) kv_append_q8_kernel(AppendArgs a) {
         const int value = r / a.c.Hkv, h = r % a.c.Hkv;
         const __nv_bfloat16* src = (value ? a.v : a.k) + t * a.kv_rs + (long long)h * D;
         float x[8], most = 0.0f;
-        bool odd = false;  // (fmaxf passes over a NaN)
         for (int j = 0; j * 32 + lane < D; ++j) {
             const int i = j * 32 + lane;
             float y = __bfloat162float(src[i]);
@@ -68,11 +75,10 @@ __global__ void __launch_bounds__(256) kv_append_q8_kernel(AppendArgs a) {
                 y = second ? y2 : y1;
             }
             x[j] = y;
-            odd |= !(fabsf(y) <= 3.402823466e38f);
-            most = fmaxf(most, fabsf(y));
+            most = max_nan(most, fabsf(y));
         }
-        most = warp_max(most);
-        if (__any_sync(0xffffffffu, odd)) most = INFINITY;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
         const float scale = q8_scale(most), inv = q8_inverse(scale);
         const long long row = cache_row(a.c, page, value, h, pos);
         int8_t* dst = static_cast<int8_t*>(a.c.pool) + row * D;
@@ -81,104 +87,178 @@ __global__ void __launch_bounds__(256) kv_append_q8_kernel(AppendArgs a) {
     }
 }
 
-// Whole 16-byte pieces: LPR lanes have eight components each of a row (token, keys or values, kv head); a row's first loads do not wait for its page.  The partner of a
-// half is fetched a second time (from L1) rather than passed between lanes: the lanes of a half are four to sixteen apart in four registers.
-// Rounding to a whole number: adding 1.5 * 2^23 leaves it in the low bits of the sum.
-__device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
-    x[0] = bf16lo(w.x); x[1] = bf16hi(w.x); x[2] = bf16lo(w.y); x[3] = bf16hi(w.y);
-    x[4] = bf16lo(w.z); x[5] = bf16hi(w.z); x[6] = bf16lo(w.w); x[7] = bf16hi(w.w);
+// The places of up to PLACES consecutive rows of new tokens from t0 on, for a whole block: position, and row of the pool of kv head 0's key (-1: the row is left alone); row r of the
+// token's keys and values, keys of all heads first, lies JSM_PAGE_SIZE * r behind it
+constexpr int PLACES = 16;
+__device__ __forceinline__ void find_places(const CacheView& c, int T, int t0, int n, int table_len, int* seq, int* pos, int* base) {
+    if (threadIdx.x < PLACES) seq[threadIdx.x] = -1;
+    __syncthreads();
+    for (int s = threadIdx.x; s < c.n_seqs; s += blockDim.x) {
+        const int from = c.starts[s], to = c.starts[s + 1];
+        for (int k = max(0, from - t0); k < n && t0 + k < to; ++k) seq[k] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x < n) {
+        const int k = threadIdx.x, s = seq[k];
+        int first, n_new, ctx, p = -1;
+        if (s >= 0 && cache_lengths(c, s, T, first, n_new, ctx)) {
+            const int at = ctx - n_new + t0 + k - first;
+            pos[k] = at;
+            if (at < table_len) p = cache_page(c, s, at);
+            else cache_error(c.err, CACHE_BAD_POSITION);
+        }
+        base[k] = p < 0 ? -1 : (int)cache_row(c, p, 0, 0, pos[k]);
+    }
+    __syncthreads();
 }
-template <int LPR>
-__global__ void __launch_bounds__(256) kv_append_q8_vec_kernel(AppendArgs a) {
-    constexpr int ROWS = 256 / LPR, U = 4;
-    __shared__ int found;
+
+// Whole 16-byte pieces: LPR lanes have two pieces of eight components each of a row (token, keys or values, kv head), up to PLACES tokens per block; a thread's first loads do not
+// wait for the places.  A lane's pieces hold both components of its pairs (halves: a piece of each half), so that a rotation stays within the lane and its eight table
+// entries serve all heads of a token.  Products that are rounded on their own before a sum are not packed: a packed product and a packed sum behind it leave the
+// assembler as one operation with one rounding.  Rounding to a whole number: adding 1.5 * 2^23 leaves it in the low bits of the sum.
+// Prompts of 7887 tokens of 32 kv heads of 128, APPEND_US us (APPEND_RATE TB/s of 6.5); one lane per eight components with the partner of a half fetched a second time 74 us.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {  // of the magnitudes; a NaN stays one
+    float d;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// row r of token k, and the one `step` rows on
+__device__ __forceinline__ void advance(int& k, int& r, int step, int per_token) {
+    r += step;
+    if (r >= per_token) {
+        r -= per_token;
+        ++k;
+        if (r >= per_token) {
+            k += r / per_token;
+            r %= per_token;
+        }
+    }
+}
+enum { TURN_NONE = 0, TURN_ADJACENT = 1, TURN_HALF = 2, TURN_ANY = 3 };  // any: parts that are no multiple of 16, element by element
+template <int LPR, int TURN>
+__global__ void __launch_bounds__(256, 4) kv_append_q8_vec_kernel(AppendArgs a, int per_block) {
+    constexpr int ROWS = 256 / LPR, U = 2;  // rows of a block's turn, turns whose loads are in flight
+    __shared__ int sh_seq[PLACES], sh_pos[PLACES], sh_base[PLACES];
     chain_trigger();
     chain_wait();
-    const int t = blockIdx.x, D = a.c.D, Hkv = a.c.Hkv, n_rows = 2 * Hkv;
-    const int i0 = threadIdx.x % LPR * 8, group = threadIdx.x / LPR;
-    const bool on = i0 < D, turns = a.table && i0 < a.rot;
-    const int half = a.rot / 2;
-    const bool second = !a.adjacent && i0 >= half;
-    uint4 w[U], w2[U];
-    auto load = [&](int r0) {
+    const int D = a.c.D, Hkv = a.c.Hkv, per_token = 2 * Hkv, t0 = blockIdx.x * per_block, n_tokens = min(per_block, a.T - t0), n_rows = n_tokens * per_token;
+    const int l = threadIdx.x % LPR, group = threadIdx.x / LPR, half = a.rot / 2;
+    const bool on = l * 16 < D, turns = TURN != TURN_NONE && l * 16 < a.rot;
+    const int i0 = TURN == TURN_HALF && turns ? l * 8 : l * 16, i1 = TURN == TURN_HALF && turns ? i0 + half : i0 + 8;  // first components of the lane's pieces
+    const __nv_bfloat16* v_src = a.v - (long long)Hkv * D;
+    uint4 w[U][2];
+    // rows of the block, token after token, keys before values: row r of token k
+    auto load = [&](int k, int r) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * ROWS;
-            if (r >= n_rows || !on) break;
-            const __nv_bfloat16* src = (r < Hkv ? a.k + t * a.kv_rs + (long long)r * D : a.v + t * a.kv_rs + (long long)(r - Hkv) * D) + i0;
-            w[u] = *reinterpret_cast<const uint4*>(src);
-            if (r < Hkv && turns && !a.adjacent) w2[u] = *reinterpret_cast<const uint4*>(second ? src - half : src + half);
+            const __nv_bfloat16* src = (r < Hkv ? a.k : v_src) + (t0 + k) * a.kv_rs + r * D;
+            w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
+            if (on && k < n_tokens) {
+                w[u][0] = *reinterpret_cast<const uint4*>(src + i0);
+                w[u][1] = *reinterpret_cast<const uint4*>(src + i1);
+            }
+            advance(k, r, ROWS, per_token);
         }
     };
-    load(group);
-    const int s = find_sequence(a.c, t, &found);
-    if (s < 0) return;
-    int first, n_new, ctx;
-    if (!cache_lengths(a.c, s, a.T, first, n_new, ctx)) return;
-    const int pos = ctx - n_new + t - first;
-    if (a.table && pos >= a.table_len) {
-        if (threadIdx.x == 0) cache_error(a.c.err, CACHE_BAD_POSITION);
-        return;
-    }
-    const int page = cache_page(a.c, s, pos);
-    if (page < 0) return;
-    float c[8], sn[8];  // adjacent: four pairs; halves: eight
-    if (turns) {
-        const float4* e = reinterpret_cast<const float4*>(a.table + (long long)pos * half + (a.adjacent ? i0 / 2 : second ? i0 - half : i0));
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i < 2 || !a.adjacent) {
-                const float4 v = e[i];
-                c[2 * i] = v.x; sn[2 * i] = v.y; c[2 * i + 1] = v.z; sn[2 * i + 1] = v.w;
-            }
-    }
+    int k = 0, r = 0;
+    advance(k, r, group, per_token);
+    load(k, r);
+    find_places(a.c, a.T, t0, n_tokens, TURN != TURN_NONE ? a.table_len : INT_MAX, sh_seq, sh_pos, sh_base);
     const int ahead = threadIdx.x % 32 / LPR;  // (a warp's rows take their turns together: lanes meet in shuffles)
-    for (int r0 = group; r0 - ahead < n_rows; r0 += U * ROWS) {
-        if (r0 != group) load(r0);
+    int have = -1;                             // the token whose table entries are here; pairs that do not turn: 1 and 0
+    float c[8], sn[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        c[i] = 1.0f;
+        sn[i] = 0.0f;
+    }
+    for (int row = group; row - ahead < n_rows; row += U * ROWS) {
+        if (row != group) load(k, r);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * ROWS;
-            float x[8] = {0, 0, 0, 0, 0, 0, 0, 0}, most = 0.0f, sum = 0.0f;
-            if (r < n_rows && on) {
-                unpack8(w[u], x);
-                if (r < Hkv && turns) {
-                    if (a.adjacent) {
+            if (row + u * ROWS - ahead >= n_rows) break;
+            const int base = k < n_tokens ? sh_base[k] : -1;
+            float x[16];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) rotate_pair(x[2 * i], x[2 * i + 1], c[i], sn[i], x[2 * i], x[2 * i + 1]);
-                    } else {
-                        float y[8];
-                        unpack8(w2[u], y);
+            for (int p = 0; p < 2; ++p) {
+                const uint32_t in[4] = {w[u][p].x, w[u][p].y, w[u][p].z, w[u][p].w};
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            float y1, y2;
-                            rotate_pair(second ? y[i] : x[i], second ? x[i] : y[i], c[i], sn[i], y1, y2);
-                            x[i] = second ? y2 : y1;
-                        }
+                for (int i = 0; i < 4; ++i) {
+                    x[p * 8 + 2 * i] = bf16lo(in[i]);
+                    x[p * 8 + 2 * i + 1] = bf16hi(in[i]);
+                }
+            }
+            if (TURN == TURN_ANY && r < Hkv && turns && base >= 0) {
+                const __nv_bfloat16* src = a.k + (t0 + k) * a.kv_rs + r * D;
+                const float2* e = a.table + (long long)sh_pos[k] * half;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int d = l * 16 + i;
+                    if (d >= a.rot) break;
+                    const bool second = a.adjacent ? d & 1 : d >= half;
+                    const float2 v = e[a.adjacent ? d / 2 : second ? d - half : d];
+                    const float z = __bfloat162float(src[a.adjacent ? d ^ 1 : second ? d - half : d + half]);
+                    x[i] = __fadd_rn(__fmul_rn(x[i], v.x), __fmul_rn(z, second ? v.y : -v.y));
+                }
+            } else if (TURN != TURN_NONE && TURN != TURN_ANY && r < Hkv) {
+                if (have != k && turns && base >= 0) {
+                    have = k;
+                    const float4* e = reinterpret_cast<const float4*>(a.table + (long long)sh_pos[k] * half + l * 8);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 v = e[i];
+                        c[2 * i] = v.x; sn[2 * i] = v.y; c[2 * i + 1] = v.z; sn[2 * i + 1] = v.w;
                     }
                 }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    most = fmaxf(most, fabsf(x[i]));
-                    sum += x[i] * 0.0f;  // a NaN where a component is one, or infinite (fmaxf passes over a NaN)
+                    const int i1_ = TURN == TURN_ADJACENT ? 2 * i : i, i2_ = TURN == TURN_ADJACENT ? 2 * i + 1 : i + 8;
+                    rotate_pair(x[i1_], x[i2_], c[i], sn[i], x[i1_], x[i2_]);
                 }
-                if (!(sum == 0.0f)) most = INFINITY;
             }
+            float most = 0.0f;
 #pragma unroll
-            for (int o = LPR / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            if (r >= n_rows || !on) continue;
-            const float scale = q8_scale(most), inv = q8_inverse(scale);
-            uint32_t n[8];
+            for (int i = 0; i < 16; i += 2) most = max3_abs(most, x[i], x[i + 1]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) n[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], inv), 12582912.0f));
-            uint2 o;
-            o.x = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
-            o.y = __byte_perm(__byte_perm(n[4], n[5], 0x0040), __byte_perm(n[6], n[7], 0x0040), 0x5410);
-            if (!(scale == scale)) o = make_uint2(0, 0);
-            const long long row = r < Hkv ? cache_row(a.c, page, 0, r, pos) : cache_row(a.c, page, 1, r - Hkv, pos);
-            *reinterpret_cast<uint2*>(static_cast<int8_t*>(a.c.pool) + row * D + i0) = o;
-            if (i0 == 0) a.c.scales[row] = (uint16_t)(__float_as_uint(scale) >> 16);
+            for (int o = LPR / 2; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const float scale = q8_scale(most), inv = scale == scale ? q8_inverse(scale) : 0.0f;
+            uint32_t out[4];
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                uint32_t n[4];  // 1.5 * 2^23 + the number
+#pragma unroll
+                for (int j = 0; j < 4; ++j) n[j] = __float_as_uint(__fadd_rn(__fmul_rn(x[i + j], inv), 12582912.0f));
+                out[i / 4] = scale == scale ? __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410) : 0u;
+            }
+            if (on && base >= 0) {
+                const int to = base + r * JSM_PAGE_SIZE;
+                int8_t* dst = static_cast<int8_t*>(a.c.pool) + (long long)to * D;
+                if (TURN == TURN_HALF) {
+                    *reinterpret_cast<uint2*>(dst + i0) = make_uint2(out[0], out[1]);
+                    *reinterpret_cast<uint2*>(dst + i1) = make_uint2(out[2], out[3]);
+                } else {
+                    *reinterpret_cast<uint4*>(dst + i0) = make_uint4(out[0], out[1], out[2], out[3]);
+                }
+                if (l == 0) a.c.scales[to] = (uint16_t)(__float_as_uint(scale) >> 16);
+            }
+            advance(k, r, ROWS, per_token);
         }
     }
+}
+template <int LPR>
+static cudaError_t append_vec_launch(const AppendArgs& a, int per_block, cudaStream_t st) {
+    const dim3 grid((a.T + per_block - 1) / per_block);
+    if (!a.table) return launch_chained(kv_append_q8_vec_kernel<LPR, TURN_NONE>, grid, dim3(256), 0, st, a, per_block);
+    if (a.rot % 16 || (reinterpret_cast<uintptr_t>(a.table) & 15)) return launch_chained(kv_append_q8_vec_kernel<LPR, TURN_ANY>, grid, dim3(256), 0, st, a, per_block);
+    return a.adjacent ? launch_chained(kv_append_q8_vec_kernel<LPR, TURN_ADJACENT>, grid, dim3(256), 0, st, a, per_block)
+                      : launch_chained(kv_append_q8_vec_kernel<LPR, TURN_HALF>, grid, dim3(256), 0, st, a, per_block);
+}
+
+// Tokens of a block: what finding their places costs is worth eight rows of every thread (a block per token: 63 us instead of APPEND_US), but the chip has eight blocks per
+// multiprocessor first.
+static int tokens_per_block(int T, int Hkv, int lanes) {
+    const int rows = 8 * (256 / lanes) / (2 * Hkv), blocks = T / (8 * sm_count()), n = rows < blocks ? rows : blocks;
+    return n < 1 ? 1 : n < PLACES ? n : PLACES;
 }
 
 struct ReadArgs {
@@ -213,66 +293,69 @@ __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a) {
     }
 }
 
-// whole 16-byte pieces of the outputs: eight components per lane, four rows' loads in flight
+// whole 16-byte pieces of the outputs: eight components per lane, four rows' loads in flight, PLACES tokens or one per block
 template <int LPR, bool Q8, bool F32>
-__global__ void __launch_bounds__(256) kv_read_vec_kernel(ReadArgs a) {
+__global__ void __launch_bounds__(256) kv_read_vec_kernel(ReadArgs a, int per_block) {
     constexpr int ROWS = 256 / LPR, U = 4;
-    __shared__ int found;
+    __shared__ int sh_seq[PLACES], sh_pos[PLACES], sh_base[PLACES];
     chain_trigger();
     chain_wait();
-    const int t = blockIdx.x, D = a.c.D, Hkv = a.c.Hkv, n_rows = 2 * Hkv;
+    const int D = a.c.D, Hkv = a.c.Hkv, per_token = 2 * Hkv, t0 = blockIdx.x * per_block, n_tokens = min(per_block, a.T - t0);
     const int i0 = threadIdx.x % LPR * 8, group = threadIdx.x / LPR;
-    const int s = find_sequence(a.c, t, &found);
-    if (s < 0 || i0 >= D) return;
-    int first, n_new, ctx;
-    if (!cache_lengths(a.c, s, a.T, first, n_new, ctx)) return;
-    const int pos = ctx - n_new + t - first;
-    const int page = cache_page(a.c, s, pos);
-    if (page < 0) return;
-    for (int r0 = group; r0 < n_rows; r0 += U * ROWS) {
+    find_places(a.c, a.T, t0, n_tokens, INT_MAX, sh_seq, sh_pos, sh_base);
+    if (i0 >= D) return;
+    int k = 0, r = 0;
+    advance(k, r, group, per_token);
+    while (k < n_tokens) {
         uint4 w[U];
         uint32_t scale[U];
+        int k1 = k, r1 = r;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * ROWS;
-            if (r >= n_rows) break;
-            const long long row = r < Hkv ? cache_row(a.c, page, 0, r, pos) : cache_row(a.c, page, 1, r - Hkv, pos);
-            if constexpr (Q8) {
-                const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.c.pool) + row * D + i0);
-                w[u].x = v.x;
-                w[u].z = v.y;
-                scale[u] = a.c.scales[row] * 0x00010001u;
-            } else {
-                w[u] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.c.pool) + row * D + i0);
+            if (k1 >= n_tokens) break;
+            if (sh_base[k1] >= 0) {
+                const int at = sh_base[k1] + r1 * JSM_PAGE_SIZE;
+                if constexpr (Q8) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(a.c.pool) + (long long)at * D + i0);
+                    w[u].x = v.x;
+                    w[u].z = v.y;
+                    scale[u] = a.c.scales[at] * 0x00010001u;
+                } else {
+                    w[u] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.c.pool) + (long long)at * D + i0);
+                }
             }
+            advance(k1, r1, ROWS, per_token);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * ROWS;
-            if (r >= n_rows) break;
-            uint4 o = w[u];
-            if constexpr (Q8) {
-                o.x = q8_value2(__byte_perm(w[u].x, 0, 0x1100), scale[u]);
-                o.y = q8_value2(__byte_perm(w[u].x, 0, 0x3322), scale[u]);
-                o.z = q8_value2(__byte_perm(w[u].z, 0, 0x1100), scale[u]);
-                o.w = q8_value2(__byte_perm(w[u].z, 0, 0x3322), scale[u]);
+            if (k >= n_tokens) break;
+            if (sh_base[k] >= 0) {
+                uint4 o = w[u];
+                if constexpr (Q8) {
+                    o.x = q8_value2(__byte_perm(w[u].x, 0, 0x1100), scale[u]);
+                    o.y = q8_value2(__byte_perm(w[u].x, 0, 0x3322), scale[u]);
+                    o.z = q8_value2(__byte_perm(w[u].z, 0, 0x1100), scale[u]);
+                    o.w = q8_value2(__byte_perm(w[u].z, 0, 0x3322), scale[u]);
+                }
+                const long long to = (t0 + k) * a.out_rs + (r < Hkv ? r : r - Hkv) * D + i0;
+                void* out = r < Hkv ? a.k_out : a.v_out;
+                if constexpr (F32) {
+                    float* dst = static_cast<float*>(out) + to;
+                    reinterpret_cast<float4*>(dst)[0] = make_float4(bf16lo(o.x), bf16hi(o.x), bf16lo(o.y), bf16hi(o.y));
+                    reinterpret_cast<float4*>(dst)[1] = make_float4(bf16lo(o.z), bf16hi(o.z), bf16lo(o.w), bf16hi(o.w));
+                } else {
+                    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + to) = o;
+                }
             }
-            const long long to = t * a.out_rs + (long long)(r < Hkv ? r : r - Hkv) * D + i0;
-            void* out = r < Hkv ? a.k_out : a.v_out;
-            if constexpr (F32) {
-                float* dst = static_cast<float*>(out) + to;
-                reinterpret_cast<float4*>(dst)[0] = make_float4(bf16lo(o.x), bf16hi(o.x), bf16lo(o.y), bf16hi(o.y));
-                reinterpret_cast<float4*>(dst)[1] = make_float4(bf16lo(o.z), bf16hi(o.z), bf16lo(o.w), bf16hi(o.w));
-            } else {
-                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + to) = o;
-            }
+            advance(k, r, ROWS, per_token);
         }
     }
 }
 template <int LPR>
 static cudaError_t read_vec_launch(const ReadArgs& a, cudaStream_t st) {
-    if (a.c.scales) return a.f32 ? launch_chained(kv_read_vec_kernel<LPR, true, true>, dim3(a.T), dim3(256), 0, st, a) : launch_chained(kv_read_vec_kernel<LPR, true, false>, dim3(a.T), dim3(256), 0, st, a);
-    return a.f32 ? launch_chained(kv_read_vec_kernel<LPR, false, true>, dim3(a.T), dim3(256), 0, st, a) : launch_chained(kv_read_vec_kernel<LPR, false, false>, dim3(a.T), dim3(256), 0, st, a);
+    const int n = tokens_per_block(a.T, a.c.Hkv, LPR);
+    if (a.c.scales) return a.f32 ? launch_chained(kv_read_vec_kernel<LPR, true, true>, dim3((a.T + n - 1) / n), dim3(256), 0, st, a, n) : launch_chained(kv_read_vec_kernel<LPR, true, false>, dim3((a.T + n - 1) / n), dim3(256), 0, st, a, n);
+    return a.f32 ? launch_chained(kv_read_vec_kernel<LPR, false, true>, dim3((a.T + n - 1) / n), dim3(256), 0, st, a, n) : launch_chained(kv_read_vec_kernel<LPR, false, false>, dim3((a.T + n - 1) / n), dim3(256), 0, st, a, n);
 }
 
 // what the calls over a paged cache check alike
@@ -316,12 +399,14 @@ extern "C" jsm_status jsm_kv_append_q8(void* d_pool, void* d_scales, int n_pages
     a.T = T;
     a.table = reinterpret_cast<const float2*>(d_rope_table);
     a.table_len = table_len; a.rot = rot_dim; a.adjacent = layout == JSM_ROPE_ADJACENT;
-    const uintptr_t at = reinterpret_cast<uintptr_t>(d_k) | reinterpret_cast<uintptr_t>(d_v) | reinterpret_cast<uintptr_t>(d_rope_table);
-    const bool pieces = !(at & 15) && kv_row_stride % 8 == 0 && (!d_rope_table || (layout == JSM_ROPE_ADJACENT ? rot_dim : rot_dim / 2) % 8 == 0);
-    JSM_CUDA_CHECK(!pieces    ? launch_chained(kv_append_q8_kernel, dim3(T), dim3(256), 0, as_stream(stream), a)
-                   : D <= 64  ? launch_chained(kv_append_q8_vec_kernel<8>, dim3(T), dim3(256), 0, as_stream(stream), a)
-                   : D <= 128 ? launch_chained(kv_append_q8_vec_kernel<16>, dim3(T), dim3(256), 0, as_stream(stream), a)
-                              : launch_chained(kv_append_q8_vec_kernel<32>, dim3(T), dim3(256), 0, as_stream(stream), a));
+    const bool pieces = !((reinterpret_cast<uintptr_t>(d_k) | reinterpret_cast<uintptr_t>(d_v)) & 15) && kv_row_stride % 8 == 0;
+    const int lanes = D <= 64 ? 4 : D <= 128 ? 8 : 16, n = tokens_per_block(T, Hkv, lanes);
+    const cudaStream_t st = as_stream(stream);
+    const cudaError_t e = !pieces      ? launch_chained(kv_append_q8_kernel, dim3(T), dim3(256), 0, st, a)
+                          : lanes == 4 ? append_vec_launch<4>(a, n, st)
+                          : lanes == 8 ? append_vec_launch<8>(a, n, st)
+                                       : append_vec_launch<16>(a, n, st);
+    JSM_CUDA_CHECK(e);
     JSM_LAUNCH_CHECK();
     return JSM_OK;
 }

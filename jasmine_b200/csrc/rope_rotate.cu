@@ -31,32 +31,33 @@ __device__ __forceinline__ float rot_load<__nv_bfloat16>(const __nv_bfloat16* p)
 __device__ __forceinline__ void rot_store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void rot_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// any sizes, pitches and alignments: a thread per pair or unrotated component
+// any sizes, pitches and alignments: a thread has a pair or an unrotated component, and walks the heads with its table entry
 template <typename T>
 __global__ void __launch_bounds__(256) rope_rotate_scalar_kernel(RotateArgs a) {
     chain_trigger();
     chain_wait();
-    const int half = a.rot / 2, units = a.D - half, heads = a.Hq + a.Hk;
-    for (int t = blockIdx.x; t < a.T; t += gridDim.x) {
-        const int pos = a.positions ? a.positions[t] : t;
-        if (pos < 0 || pos >= a.table_len) {
-            if (threadIdx.x == 0) cache_error(a.err, CACHE_BAD_POSITION);
-            continue;
-        }
-        for (int i = threadIdx.x; i < heads * units; i += blockDim.x) {
-            const int h = i / units, u = i % units;
+    const int half = a.rot / 2, units = a.D - half, heads = a.Hq + a.Hk, head_lanes = max(1, 256 / units);
+    const int u0 = units < 256 ? threadIdx.x % units : threadIdx.x, hl = units < 256 ? threadIdx.x / units : 0;
+    if (hl >= head_lanes) return;
+    const int t = blockIdx.x, pos = a.positions ? a.positions[t] : t;
+    if (pos < 0 || pos >= a.table_len) {
+        if (threadIdx.x == 0) cache_error(a.err, CACHE_BAD_POSITION);
+        return;
+    }
+    for (int u = u0; u < units; u += 256) {
+        const float2 e = u < half ? a.table[(long long)pos * half + u] : make_float2(0.0f, 0.0f);
+        const int i1 = u < half ? (a.adjacent ? 2 * u : u) : u + half, i2 = a.adjacent ? 2 * u + 1 : u + half;
+        for (int h = hl; h < heads; h += head_lanes) {
             const bool is_q = h < a.Hq;
             const T* src = is_q ? static_cast<const T*>(a.q) + t * a.q_rs + (long long)h * a.D : static_cast<const T*>(a.k) + t * a.k_rs + (long long)(h - a.Hq) * a.D;
             T* dst = is_q ? static_cast<T*>(a.q_out) + t * a.qo_rs + (long long)h * a.D : static_cast<T*>(a.k_out) + t * a.ko_rs + (long long)(h - a.Hq) * a.D;
             if (u < half) {
-                const float2 e = a.table[(long long)pos * half + u];
-                const int i1 = a.adjacent ? 2 * u : u, i2 = a.adjacent ? 2 * u + 1 : u + half;
                 float y1, y2;
                 rotate_pair(rot_load(src + i1), rot_load(src + i2), e.x, a.sign * e.y, y1, y2);
                 rot_store(dst + i1, y1);
                 rot_store(dst + i2, y2);
             } else {
-                dst[u + half] = src[u + half];
+                dst[i1] = src[i1];
             }
         }
     }
@@ -101,25 +102,11 @@ __global__ void __launch_bounds__(RV_THREADS) rope_rotate_vec_kernel(RotateArgs 
     if (hl >= head_lanes) return;
     const int rotated = (ADJACENT ? a.rot : a.rot / 2) / V;      // units that are
     const int first = (ADJACENT || u < rotated ? u : u + rotated) * V;  // component of the unit's (first) piece
-    const int t = blockIdx.x, pos = a.positions ? a.positions[t] : t;
-    if (pos < 0 || pos >= a.table_len) {
-        if (threadIdx.x == 0) cache_error(a.err, CACHE_BAD_POSITION);
-        return;
-    }
-    float c[PAIRS], s[PAIRS];
-    if (u < rotated) {
-        const float4* e = reinterpret_cast<const float4*>(a.table + (long long)pos * (a.rot / 2) + u * PAIRS);
-#pragma unroll
-        for (int i = 0; i < PAIRS / 2; ++i) {
-            const float4 v = e[i];
-            c[2 * i] = v.x; s[2 * i] = a.sign * v.y; c[2 * i + 1] = v.z; s[2 * i + 1] = a.sign * v.w;
-        }
-    }
+    const int t = blockIdx.x, half = a.rot / 2;
     const T *q = static_cast<const T*>(a.q) + t * a.q_rs + first, *k = static_cast<const T*>(a.k) + t * a.k_rs + first;
     T *qo = static_cast<T*>(a.q_out) + t * a.qo_rs + first, *ko = static_cast<T*>(a.k_out) + t * a.ko_rs + first;
-    const int half = a.rot / 2;
-    for (int h0 = hl; h0 < heads; h0 += U * head_lanes) {
-        uint4 w[U], w2[U];
+    uint4 w[U], w2[U];
+    auto load = [&](int h0) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const int h = h0 + i * head_lanes;
@@ -128,6 +115,24 @@ __global__ void __launch_bounds__(RV_THREADS) rope_rotate_vec_kernel(RotateArgs 
             w[i] = *reinterpret_cast<const uint4*>(src);
             if (!ADJACENT && u < rotated) w2[i] = *reinterpret_cast<const uint4*>(src + half);
         }
+    };
+    load(hl);  // (before position and table: one latency of three in a row)
+    const int pos = a.positions ? a.positions[t] : t;
+    if (pos < 0 || pos >= a.table_len) {
+        if (threadIdx.x == 0) cache_error(a.err, CACHE_BAD_POSITION);
+        return;
+    }
+    float c[PAIRS], s[PAIRS];
+    if (u < rotated) {
+        const float4* e = reinterpret_cast<const float4*>(a.table + (long long)pos * half + u * PAIRS);
+#pragma unroll
+        for (int i = 0; i < PAIRS / 2; ++i) {
+            const float4 v = e[i];
+            c[2 * i] = v.x; s[2 * i] = a.sign * v.y; c[2 * i + 1] = v.z; s[2 * i + 1] = a.sign * v.w;
+        }
+    }
+    for (int h0 = hl; h0 < heads; h0 += U * head_lanes) {
+        if (h0 != hl) load(h0);
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const int h = h0 + i * head_lanes;
@@ -189,7 +194,7 @@ extern "C" jsm_status jsm_rope_rotate(const void* d_q, int64_t q_row_stride, voi
     const int64_t pitches = (Hq ? q_row_stride | q_out_row_stride : 0) | (Hkv ? k_row_stride | k_out_row_stride : 0);
     if (!((odd | reinterpret_cast<uintptr_t>(d_table)) & 15) && pitches % V == 0 && D % V == 0 && (layout == JSM_ROPE_ADJACENT ? rot_dim : rot_dim / 2) % V == 0 && D / V <= RV_THREADS)
         return dtype == JSM_F32 ? rotate_vec_launch<float>(a, as_stream(stream)) : rotate_vec_launch<__nv_bfloat16>(a, as_stream(stream));
-    const dim3 grid(T < sm_count() * 8 ? T : sm_count() * 8);
+    const dim3 grid(T);
     if (dtype == JSM_F32) JSM_CUDA_CHECK(launch_chained(rope_rotate_scalar_kernel<float>, grid, dim3(256), 0, as_stream(stream), a));
     else JSM_CUDA_CHECK(launch_chained(rope_rotate_scalar_kernel<__nv_bfloat16>, grid, dim3(256), 0, as_stream(stream), a));
     JSM_LAUNCH_CHECK();

@@ -33,6 +33,10 @@ CASES = [  # new, ctx, Hkv, D, rot, layout
     ([20, 20], [21, 90], 4, 256, 100, jb.ROPE_HALF),
     ([300], [300], 32, 128, 2, jb.ROPE_HALF),
     ([7], [7], 2, 240, 16, jb.ROPE_ADJACENT),
+    ([1300, 1250], [1300, 1400], 2, 128, 128, jb.ROPE_HALF),   # several tokens a block, across the border of two sequences
+    ([900, 0, 1700], [950, 4, 1700], 1, 64, 62, jb.ROPE_ADJACENT),
+    ([50], [50], 3, 256, 256, jb.ROPE_HALF),
+    ([50], [50], 2, 192, 90, jb.ROPE_HALF),
 ]
 
 
