@@ -64,7 +64,8 @@ __global__ void __launch_bounds__(256) rope_rotate_scalar_kernel(RotateArgs a) {
 }
 
 // Whole 16-byte pieces: a thread has one unit of a head - a piece of each half, a piece of adjacent pairs, or a piece that is not rotated - with its table entries in
-// registers, and takes that unit of every HL-th head, four heads' loads in flight.
+// registers, and takes that unit of every HL-th head, four heads' loads in flight.  8192 rows of 32 + 8 heads of 128 with 64 rotated (bf16, 170 MB): 33.5 us, 5.1 TB/s of the
+// measured 6.5; without streaming loads and stores 36.1, with position and table ahead of the rows 40.7.
 template <typename T>
 struct RotPiece {
     static constexpr int V = 16 / sizeof(T);
@@ -112,8 +113,8 @@ __global__ void __launch_bounds__(RV_THREADS) rope_rotate_vec_kernel(RotateArgs 
             const int h = h0 + i * head_lanes;
             if (h >= heads) break;
             const T* src = h < a.Hq ? q + (long long)h * a.D : k + (long long)(h - a.Hq) * a.D;
-            w[i] = *reinterpret_cast<const uint4*>(src);
-            if (!ADJACENT && u < rotated) w2[i] = *reinterpret_cast<const uint4*>(src + half);
+            w[i] = __ldcs(reinterpret_cast<const uint4*>(src));
+            if (!ADJACENT && u < rotated) w2[i] = __ldcs(reinterpret_cast<const uint4*>(src + half));
         }
     };
     load(hl);  // (before position and table: one latency of three in a row)
@@ -148,11 +149,11 @@ __global__ void __launch_bounds__(RV_THREADS) rope_rotate_vec_kernel(RotateArgs 
                     y.unpack(w2[i]);
 #pragma unroll
                     for (int n = 0; n < PAIRS; ++n) rotate_pair(x.x[n], y.x[n], c[n], s[n], x.x[n], y.x[n]);
-                    *reinterpret_cast<uint4*>(dst + half) = y.pack();
+                    __stcs(reinterpret_cast<uint4*>(dst + half), y.pack());
                 }
                 w[i] = x.pack();
             }
-            *reinterpret_cast<uint4*>(dst) = w[i];
+            __stcs(reinterpret_cast<uint4*>(dst), w[i]);
         }
     }
 }
