@@ -3,7 +3,7 @@
 // The query rows of a kv head's group are one matrix, token after token, head after head within a token (row = token * G + head): a short portion of grouped
 // queries fills the 128 rows of a tensor-core tile, and a key tile is fetched once for the whole group.  A CTA owns two such tiles of one (sequence, kv head)
 // and walks the keys of its pages in tiles of 128 (two pages), as flash_attn.cu does: scores one key tile ahead of the products with V, the softmax of one
-// query tile beside the tensor work of the other, the accumulator rescaled only where the maximum grew by 2^8, a quarter of the exponentials on the FMA pipe.
+// query tile beside the tensor work of the other.
 //   warp 0        copies: Q once (a box of tokens x heads x 64 components), key and value pages through rings
 //   warp 1        issues the products: S_t = Q_t K^T, O_t += P_t V (P_t in TMEM over the first half of S_t)
 //   warps 4-11    softmax, one thread per query row; register shares moved here from warps 0-3 (setmaxnreg)
@@ -19,6 +19,8 @@
 #include "mma_utils.cuh"
 #include <math.h>
 #include <cmath>
+#include <limits.h>
+#include <stdlib.h>
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -29,7 +31,8 @@ using namespace tc;
 
 constexpr int CK_BM = 128, CK_BN = 128;
 constexpr int CK_SOFTMAX = 4, CK_CONVERT = 12;  // first warp of a role
-constexpr float CK_RESCALE = 8.0f;
+constexpr float CK_RESCALE = 8.0f;             // the maximum is above the reference by so many powers of two: the reference follows
+constexpr float CK_RAISE = 16777216.0f;        // a key tile's sum of weights is above 2^24: the reference is raised
 constexpr float CK_NONE = -1.0e30f;             // the maximum of a row that has seen nothing
 
 template <int D, bool Q8>
@@ -46,8 +49,8 @@ struct FlashArgs {
     ChunkArgs a;
     int few_rows;      // sequences of so many rows are another kernel's
     int tile_tokens;   // tokens of a query tile
-    int slots;         // pairs of query tiles, at most
-    int share;         // CTAs (a cluster) of one pair of query tiles and kv head
+    int cluster;       // CTAs of a cluster
+    int walk_tiles;    // key tiles that a CTA should walk at most: a sequence of more gives a pair of query tiles to 2, 4 .. CTAs of a cluster
     uint32_t inv_G;    // row / G = row * inv_G >> 16 for the rows of a tile
 };
 
@@ -69,36 +72,49 @@ __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.a
 template <int N>
 __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// The slot-th (sequence, pair of query tiles, kv head), for a whole warp; false: there are fewer.  The last tokens of a sequence, which see the most keys, come first
-// for all heads: long CTAs do not start last (one prompt of 4096 tokens 158 us, with the pairs of a head next to one another 188).
-__device__ __forceinline__ bool find_tile(const FlashArgs& f, long long slot, int& seq, int& hk, int& tile, int& row0, int& n_new, int& ctx) {
+// What a CTA is for: the cluster'th group of CTAs, of which it is number `rank`, serves so many pairs of query tiles of a sequence as the `share` CTAs of each leave room for; -1: none.
+// For a whole warp.  The last tokens of a sequence, which see the most keys, come first for all heads: long CTAs do not start last (one prompt of 4096 tokens 158 us, with
+// the pairs of a head next to one another 188).
+struct Place {
+    int seq, hk, tile, share, row0, n_new, ctx;
+};
+__device__ __forceinline__ Place find_tile(const FlashArgs& f, long long cluster, int rank) {
     const ChunkArgs& a = f.a;
     const int lane = threadIdx.x & 31, tokens = 2 * f.tile_tokens;
+    Place p = {-1, 0, 0, 1, 0, 0, 0};
     for (int s0 = 0; s0 < a.c.n_seqs; s0 += 32) {
         const int s = s0 + lane;
-        int n = 0;
-        if (s < a.c.n_seqs && chunk_lengths(a, s, row0, n_new, ctx) && n_new * a.G > f.few_rows) n = (n_new + tokens - 1) / tokens;
-        long long sum = (long long)n * a.c.Hkv;
+        int n = 0, share = 1, row0 = 0, n_new = 0, ctx = 0;
+        if (s < a.c.n_seqs && chunk_lengths(a, s, row0, n_new, ctx) && n_new * a.G > f.few_rows) {
+            n = (n_new + tokens - 1) / tokens;
+            const int keys = a.window > 0 ? min(ctx, a.window + tokens) : ctx;
+            while (share < f.cluster && keys > f.walk_tiles * share * CK_BN) share *= 2;
+        }
+        const long long groups = ((long long)n * a.c.Hkv * share + f.cluster - 1) / f.cluster;
+        long long sum = groups;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const long long v = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += v;
         }
-        const unsigned here = __ballot_sync(0xffffffffu, sum > slot);
+        const unsigned here = __ballot_sync(0xffffffffu, sum > cluster);
         if (here) {
             const int w = __ffs(here) - 1, n_tiles = __shfl_sync(0xffffffffu, n, w);
-            const int in = (int)(slot - (__shfl_sync(0xffffffffu, sum, w) - (long long)n_tiles * a.c.Hkv));
-            hk = in % a.c.Hkv;
-            tile = n_tiles - 1 - in / a.c.Hkv;
-            seq = s0 + w;
-            row0 = __shfl_sync(0xffffffffu, row0, w);
-            n_new = __shfl_sync(0xffffffffu, n_new, w);
-            ctx = __shfl_sync(0xffffffffu, ctx, w);
-            return true;
+            p.share = __shfl_sync(0xffffffffu, share, w);
+            const long long in = (cluster - __shfl_sync(0xffffffffu, sum - groups, w)) * (f.cluster / p.share) + rank / p.share;
+            p.row0 = __shfl_sync(0xffffffffu, row0, w);
+            p.n_new = __shfl_sync(0xffffffffu, n_new, w);
+            p.ctx = __shfl_sync(0xffffffffu, ctx, w);
+            if (in < (long long)n_tiles * a.c.Hkv) {
+                p.seq = s0 + w;
+                p.hk = (int)(in % a.c.Hkv);
+                p.tile = n_tiles - 1 - (int)(in / a.c.Hkv);
+            }
+            return p;
         }
-        slot -= __shfl_sync(0xffffffffu, sum, 31);
+        cluster -= __shfl_sync(0xffffffffu, sum, 31);
     }
-    return false;
+    return p;
 }
 
 // What a CTA walks: query tile t has the tokens tok[t] and up (none: it is empty) and sees the key tiles jb[t] .. je[t]-1, counted from the page that holds the first key of the
@@ -106,10 +122,10 @@ __device__ __forceinline__ bool find_tile(const FlashArgs& f, long long slot, in
 struct Walk {
     int tok[2], jb[2], je[2], lo, base, end, j_lo, n_max;
 };
-__device__ __forceinline__ Walk walk_of(const FlashArgs& f, int tile, int n_new, int ctx, int part) {
+__device__ __forceinline__ Walk walk_of(const FlashArgs& f, const Place& p, int part) {
     Walk w;
-    const int past = ctx - n_new, window = f.a.window;
-    w.tok[0] = tile * 2 * f.tile_tokens;
+    const int n_new = p.n_new, past = p.ctx - p.n_new, window = f.a.window;
+    w.tok[0] = p.tile * 2 * f.tile_tokens;
     w.tok[1] = w.tok[0] + f.tile_tokens;
     w.lo = first_key(window, past + w.tok[0]);
     w.base = w.lo / JSM_PAGE_SIZE * JSM_PAGE_SIZE;
@@ -124,8 +140,8 @@ __device__ __forceinline__ Walk walk_of(const FlashArgs& f, int tile, int n_new,
     }
     w.j_lo = w.jb[0];
     w.n_max = max(w.je[0], w.je[1]);
-    if (f.share > 1) {  // this CTA's share of the key tiles
-        const int len = (w.n_max - w.j_lo + f.share - 1) / f.share, from = w.j_lo + part * len, to = min(w.n_max, from + len);
+    if (p.share > 1) {  // this CTA's share of the key tiles
+        const int len = (w.n_max - w.j_lo + p.share - 1) / p.share, from = w.j_lo + part * len, to = min(w.n_max, from + len);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             w.jb[t] = max(w.jb[t], from);
@@ -149,17 +165,13 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
     uint8_t* k_smem = tiles + 2 * Z::TILE;
     uint8_t* v_smem = k_smem + ST * Z::TILE;
     uint8_t* raw_smem = v_smem + ST * Z::TILE;
-    // A cluster's meeting, in place of tiles and rings: the rows of eight softmax warps belong to the CTAs in equal shares; [sender][row of this CTA][D] sums and, behind them,
-    // [sender][row] references and sums of the weights.
-    const int own_rows = 2 * CK_BM / f.share;
-    uint8_t* recv = tiles;
-    uint8_t* recv_ml = tiles + (f.share - 1) * own_rows * (D * 4);
     __shared__ __align__(8) uint64_t q_full, o_done;
     __shared__ __align__(8) uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], raw_full[4], raw_empty[4];
     __shared__ __align__(8) uint64_t s_full[2], p_half[2], p_ready[2];
     __shared__ __align__(16) uint16_t raw_scales[4][JSM_PAGE_SIZE];
     __shared__ uint32_t tmem_base_smem;
-    __shared__ int abort_flag, sh_seq, sh_head, sh_tile, sh_row0, sh_new, sh_ctx;
+    __shared__ int abort_flag;
+    __shared__ Place sh_place;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     chain_trigger();
@@ -184,7 +196,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
         tmem_relinquish();
     }
     chain_wait();
-    const int part = blockIdx.x % f.share;
+    const int rank = blockIdx.x % f.cluster;  // (clusters are consecutive blocks)
     int pages = 0;  // warp 0: pages of 16 key tiles at a time, lane i has the i-th
     auto load_pages = [&](int seq, const Walk& w, int j) {
         const int p = w.base / JSM_PAGE_SIZE + 2 * j + lane;
@@ -192,26 +204,18 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
     };
     if (warp == 0) {
         __syncwarp();
-        int seq = -1, head = 0, tile = 0, row0 = 0, n_new = 0, ctx = 0;
-        if (!find_tile(f, blockIdx.x / f.share, seq, head, tile, row0, n_new, ctx)) seq = -1;
-        if (lane == 0) {
-            sh_row0 = row0;
-            sh_new = n_new;
-            sh_ctx = ctx;
-            sh_seq = seq;
-            sh_head = head;
-            sh_tile = tile;
-        }
-        if (seq >= 0) {  // queries and the first pages are on their way before the block meets
-            const Walk w = walk_of(f, tile, n_new, ctx, part);
+        const Place p = find_tile(f, blockIdx.x / f.cluster, rank);
+        if (lane == 0) sh_place = p;
+        if (p.seq >= 0) {  // queries and the first pages are on their way before the block meets
+            const Walk w = walk_of(f, p, rank % p.share);
             if (w.n_max > w.j_lo) {
-                pages = load_pages(seq, w, w.j_lo);
+                pages = load_pages(p.seq, w, w.j_lo);
                 if (elect_one()) {
-                    const int n_q = w.tok[1] < n_new ? 2 : 1;
+                    const int n_q = w.tok[1] < p.n_new ? 2 : 1;
                     mbar_expect_tx(&q_full, (uint32_t)(n_q * (D / 64) * f.tile_tokens * a.G) * 128);
                     for (int t = 0; t < n_q; ++t)
 #pragma unroll
-                        for (int c = 0; c < D / 64; ++c) tma_load_3d(q_smem + t * Z::TILE + c * Z::SLAB, &tmap_q, c * 64, head * a.G, row0 + w.tok[t], &q_full);
+                        for (int c = 0; c < D / 64; ++c) tma_load_3d(q_smem + t * Z::TILE + c * Z::SLAB, &tmap_q, c * 64, p.hk * a.G, p.row0 + w.tok[t], &q_full);
                 }
                 __syncwarp();
             }
@@ -222,11 +226,11 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
     tc_fence_after();
     const uint32_t tmem_base = tmem_base_smem;
     const uint32_t S_COL[2] = {0, 128}, O_COL[2] = {256, 256 + D};
-    const int seq = sh_seq, hk = sh_head, row0 = sh_row0, n_new = sh_new, ctx = sh_ctx;
+    const int seq = sh_place.seq, hk = sh_place.hk, row0 = sh_place.row0, n_new = sh_place.n_new, ctx = sh_place.ctx, share = sh_place.share, part = rank % share;
     const bool work = seq >= 0;
 
     Walk w = {};
-    if (work) w = walk_of(f, sh_tile, n_new, ctx, part);
+    if (work) w = walk_of(f, sh_place, part);
     const int past = ctx - n_new, lo = w.lo, base = w.base, end = w.end, j_lo = w.j_lo, n_max = w.n_max;
     const int(&tok)[2] = w.tok, (&jb)[2] = w.jb, (&je)[2] = w.je;
 
@@ -394,11 +398,35 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
         const bool query = work && row < rows && token < n_new;
         const uint32_t lane_addr = tmem_base + ((uint32_t)(quad * 32) << 16), s_addr = lane_addr + S_COL[t], o_addr = lane_addr + O_COL[t];
         const int pos_lo = past + tok[t], pos_hi = past + min(tok[t] + f.tile_tokens, n_new) - 1;  // first and last query of the tile
-        float m_ref = CK_NONE, l = 0.0f;
+        // Weights are 2^(score - reference), whatever the reference: bf16, fp32 sums and fp32 accumulators keep their precision over 2^100 and more.  So the maximum is looked for
+        // only where a row has no reference yet, or where keys are hidden; elsewhere a sum of weights above 2^24 raises the reference before the next key tile (a jump of
+        // more than 2^100 within one tile gives infinities: such a row is worked out again at the end).
+        float m_ref = query ? CK_NONE : 0.0f, l = 0.0f;
+        int raise = 0;
         bool ok = true;
+        auto rescale = [&](float alpha) {  // (TMEM accesses are the warp's: lanes whose reference stands use the factor 1)
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                uint32_t r[32];
+                tmem_ld32(o_addr + c, r);
+                tmem_ld_wait();
+                uint32_t w[16];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(r[half * 16 + i]) * alpha);
+                    tmem_st16(o_addr + c + half * 16, w);
+                }
+            }
+            l *= alpha;
+        };
         for (int j = jb[t]; j < je[t] && ok; ++j) {
             if (!mbar_wait_warp(&s_full[t], (j - jb[t]) & 1, &abort_flag, a.c.err, TC_TIMEOUT_ACC)) { ok = false; break; }
             tc_fence_after();
+            if (__any_sync(0xffffffffu, raise > 0)) {
+                rescale(ex2_approx((float)-raise));
+                m_ref += (float)raise;
+            }
             uint32_t sr[CK_BN];
 #pragma unroll
             for (int c = 0; c < CK_BN; c += 32) tmem_ld32(s_addr + c, reinterpret_cast<uint32_t(&)[32]>(sr[c]));
@@ -408,85 +436,61 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
             for (int i = 0; i < CK_BN; ++i) sv[i] = __uint_as_float(sr[i]);
             const int key0 = base + j * CK_BN;
             const bool masked = key0 + CK_BN - 1 > pos_lo || key0 < first_key(a.window, pos_hi);
-            if (masked) {
-                const int from = first_key(a.window, pos) - key0, to = pos - key0;
+            if (__any_sync(0xffffffffu, masked || m_ref == CK_NONE)) {
+                if (masked) {
+                    const int from = first_key(a.window, pos) - key0, to = pos - key0;
 #pragma unroll
-                for (int i = 0; i < CK_BN; ++i)
-                    if (i < from || i > to) sv[i] = -INFINITY;
-            }
-            float mxs[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) mxs[k] = sv[k];
-#pragma unroll
-            for (int i = 8; i + 16 <= CK_BN; i += 16)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) mxs[k] = fmax3(mxs[k], sv[i + k], sv[i + 8 + k]);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) mxs[k] = fmaxf(mxs[k], sv[CK_BN - 8 + k]);
-            float mx = fmaxf(fmax3(mxs[0], mxs[1], mxs[2]), fmaxf(fmax3(mxs[3], mxs[4], mxs[5]), fmaxf(mxs[6], mxs[7])));
-            mx *= a.scale_log2;
-            const bool grow = mx > m_ref + CK_RESCALE;
-            if (__any_sync(0xffffffffu, grow)) {  // (TMEM accesses are the warp's: lanes whose maximum stands use the factor 1)
-                const float alpha = grow ? ex2_approx(m_ref - mx) : 1.0f;
-                if (j > jb[t]) {
-#pragma unroll
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t r[32];
-                        tmem_ld32(o_addr + c, r);
-                        tmem_ld_wait();
-                        uint32_t w[16];
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(r[half * 16 + i]) * alpha);
-                            tmem_st16(o_addr + c + half * 16, w);
-                        }
-                    }
+                    for (int i = 0; i < CK_BN; ++i)
+                        if (i < from || i > to) sv[i] = -INFINITY;
                 }
-                if (grow) {
-                    l *= alpha;
-                    m_ref = mx;
+                float mxs[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) mxs[k] = sv[k];
+#pragma unroll
+                for (int i = 8; i + 16 <= CK_BN; i += 16)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) mxs[k] = fmax3(mxs[k], sv[i + k], sv[i + 8 + k]);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) mxs[k] = fmaxf(mxs[k], sv[CK_BN - 8 + k]);
+                float mx = fmaxf(fmax3(mxs[0], mxs[1], mxs[2]), fmaxf(fmax3(mxs[3], mxs[4], mxs[5]), fmaxf(mxs[6], mxs[7])));
+                mx *= a.scale_log2;
+                const bool grow = mx > m_ref + CK_RESCALE;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float alpha = grow ? ex2_approx(m_ref - mx) : 1.0f;
+                    if (j > jb[t]) rescale(alpha);
+                    if (grow) m_ref = mx;
                 }
             }
-            // p = 2^(s - m_ref) as bf16 pairs over the first 64 columns of S.  Where keys are hidden the special-function unit takes all of them: the polynomial ends at 2^-126, and
-            // a hidden key's weight is nothing at all.
+            // p = 2^(s - m_ref) as bf16 pairs over the first 64 columns of S.  All of them by the special-function unit: the warps are bound by issue here, a quarter by polynomials
+            // on the FMA pipe costs 3 %.
             uint64_t ls2[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) ls2[k] = pack2(0.0f, 0.0f);
             const uint64_t neg_m2 = pack2(-m_ref, -m_ref), sc2 = pack2(a.scale_log2, a.scale_log2);
-            auto weights = [&](auto poly) {
 #pragma unroll
-                for (int c = 0; c < CK_BN / 2; c += 16) {
-                    uint32_t w[16];
+            for (int c = 0; c < CK_BN / 2; c += 16) {
+                uint32_t w[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const uint64_t x2 = ffma2(pack2(sv[2 * (c + i)], sv[2 * (c + i) + 1]), sc2, neg_m2);
-                        float p0, p1;
-                        if ((i & 3) < decltype(poly)::value) {
-                            ex2_poly2(x2, p0, p1);
-                        } else {
-                            float x0, x1;
-                            unpack2(x2, x0, x1);
-                            p0 = ex2_approx(x0);
-                            p1 = ex2_approx(x1);
-                        }
-                        ls2[i & 3] = fadd2(ls2[i & 3], pack2(p0, p1));
-                        w[i] = pack_bf16x2(p0, p1);
-                    }
-                    tmem_st16(s_addr + c, w);
-                    if (!Q8 && c == 16) {
-                        tmem_st_wait();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&p_half[t]);
-                    }
+                for (int i = 0; i < 16; ++i) {
+                    float x0, x1;
+                    unpack2(ffma2(pack2(sv[2 * (c + i)], sv[2 * (c + i) + 1]), sc2, neg_m2), x0, x1);
+                    const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+                    ls2[i & 3] = fadd2(ls2[i & 3], pack2(p0, p1));
+                    w[i] = pack_bf16x2(p0, p1);
                 }
-            };
-            if (masked) weights(std::integral_constant<int, 0>{});
-            else weights(std::integral_constant<int, 1>{});
+                tmem_st16(s_addr + c, w);
+                if (!Q8 && c == 16) {
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_half[t]);
+                }
+            }
             float la, lb;
             unpack2(fadd2(fadd2(ls2[0], ls2[1]), fadd2(ls2[2], ls2[3])), la, lb);
-            l += la + lb;
+            const float sum = la + lb;
+            l += sum;
+            raise = sum > CK_RAISE ? (int)(__float_as_uint(sum) >> 23) - 127 : 0;
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -498,24 +502,29 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
         // What follows is executed once per CTA, mostly for the first time on its multiprocessor: rolled loops, because every line of code is fetched (unrolled, with the
         // factors of up to seven senders in registers, the end of a CTA took 4.2 us instead of 1.6).
         const int sw = warp - CK_SOFTMAX;
-        uint8_t* staged = (f.share > 1 ? recv_ml + (f.share - 1) * own_rows * 8 : tiles) + sw * (32 * D * 2);  // this warp's 32 rows pass through here
+        // The meeting of a pair's CTAs, in place of tiles and rings: the rows of the eight softmax warps belong to the CTAs in equal shares; [sender][row of this CTA][D] sums and,
+        // behind them, [sender][row] references and sums of the weights.
+        const int own_rows = 2 * CK_BM / share;
+        uint8_t* recv = tiles;
+        uint8_t* recv_ml = tiles + (share - 1) * own_rows * (D * 4);
+        uint8_t* staged = (share > 1 ? recv_ml + (share - 1) * own_rows * 8 : tiles) + sw * (32 * D * 2);  // this warp's 32 rows pass through here
         float own = 1.0f, L = l, M = m_ref;  // factor of the sums in TMEM, sum of the weights, reference of the row
         bool have = any;
         int senders = 0;
-        const int warps = 8 / f.share, owner = sw / warps, r_own = sw % warps * 32;  // of a cluster: who joins this warp's rows, and where they are there
+        const int warps = 8 / share, owner = sw / warps, r_own = sw % warps * 32;  // of a cluster: who joins this warp's rows, and where they are there
         auto sent_factor = [&](int p) {  // (0: that CTA had none of the row's keys)
             const float2 v = reinterpret_cast<const float2*>(recv_ml)[p * own_rows + r_own + lane];
             return make_float2(v.x == CK_NONE && v.y == 0.0f ? 0.0f : ex2_approx(v.x - M), v.y);
         };
-        if (f.share > 1) {
+        if (share > 1) {
             ck_cluster_arrive();
             ck_cluster_wait();  // every CTA has taken its products: tiles and rings may be overwritten
             if (owner != part) {
-                const int at = (part < owner ? part : part - 1) * own_rows + r_own;
-                ck_store2(ck_peer(smem_u32(recv_ml) + (at + lane) * 8, owner), any ? m_ref : CK_NONE, any ? l : 0.0f);
+                const int at = (part < owner ? part : part - 1) * own_rows + r_own, peer = rank - part + owner;
+                ck_store2(ck_peer(smem_u32(recv_ml) + (at + lane) * 8, peer), any ? m_ref : CK_NONE, any ? l : 0.0f);
                 if (any) {
                     // a row per thread would send 16 bytes to 32 places at a time: through shared memory, so that eight lanes send 128 bytes
-                    const uint32_t to = ck_peer(smem_u32(recv) + at * (D * 4), owner), here = smem_u32(staged);
+                    const uint32_t to = ck_peer(smem_u32(recv) + at * (D * 4), peer), here = smem_u32(staged);
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         uint32_t o[32];
@@ -538,7 +547,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
             ck_cluster_wait();  // the sums are here
             have = owner == part && tok[t] < n_new;
             if (have) {
-                senders = f.share - 1;
+                senders = share - 1;
                 if (!any) M = CK_NONE;
 #pragma unroll 1
                 for (int p = 0; p < senders; ++p) M = fmaxf(M, reinterpret_cast<const float2*>(recv_ml)[p * own_rows + r_own + lane].x);
@@ -675,7 +684,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8>::THREADS, 1)
             }
         }
     }
-    if (f.share > 1 && (warp < CK_SOFTMAX || warp >= CK_CONVERT)) {  // (the meeting counts every thread)
+    if (share > 1 && (warp < CK_SOFTMAX || warp >= CK_CONVERT)) {  // (the meeting counts every thread)
         ck_cluster_arrive();
         ck_cluster_wait();
         ck_cluster_arrive();
@@ -722,26 +731,28 @@ static int flash_capacity(int S) {
 template <int D, bool Q8>
 static jsm_status flash_launch(const ChunkArgs& a, int few_rows, cudaStream_t st) {
     using Z = FlashSizes<D, Q8>;
-    FlashArgs f{a, few_rows, CK_BM / a.G, 0, 1, (65536u + a.G - 1) / a.G};
+    FlashArgs f{a, few_rows, CK_BM / a.G, 1, INT_MAX, (65536u + a.G - 1) / a.G};
     const long long tokens = 2ll * f.tile_tokens, per_seq = (a.max_new + tokens - 1) / tokens;
-    f.slots = (int)std::min(per_seq * a.c.n_seqs, a.T / tokens + a.c.n_seqs);
+    const long long pairs = std::min(per_seq * a.c.n_seqs, a.T / tokens + a.c.n_seqs) * a.c.Hkv;  // at most
     static DeviceOnce once;
     JSM_CUDA_CHECK(allow_shared(once, chunk_flash_kernel<D, Q8>, (int)Z::SMEM));
-    // CTAs of a pair of query tiles.  A key tile takes about 2 us, what is around the walk 6 us, the meeting of a cluster 3 us: the longest CTA, or the chip's share of all and
-    // half a CTA's time for the uneven end.  (Of a sequence that is all new tokens, a pair sees half of the keys on average.)
+    // CTAs of a pair of query tiles.  A key tile takes about 2 us, what is around the walk 6 us, a meeting 3 us: the longest CTA, or the chip's share of all and half a CTA's time
+    // for the uneven end.  On average a pair of one sequence sees what lies before the middle of its new tokens, one of many sequences perhaps half of that.
     long long keys = a.max_context, mean = a.max_context - a.max_new / 2;
+    if (a.c.n_seqs > 1) mean /= 2;
     if (a.window > 0) { keys = std::min(keys, (long long)a.window + tokens); mean = std::min(mean, keys); }
-    const long long pairs = (long long)f.slots * a.c.Hkv;
-    const float key_tiles = (float)((keys + CK_BN - 1) / CK_BN), mean_tiles = (float)mean / CK_BN;
+    const int key_tiles = (int)((keys + CK_BN - 1) / CK_BN);
+    const float mean_tiles = (float)mean / CK_BN, likely = a.c.n_seqs > 1 ? (float)(a.T / tokens + a.c.n_seqs / 2 + 1) * a.c.Hkv : (float)pairs;
     float best = 0.0f;
     for (int S = 1; S <= 8; S *= 2) {
         if (S > 1 && key_tiles < 2 * S) break;
-        const int cap = flash_capacity<D, Q8>(S);
-        const float around = 6.0f + (S > 1 ? 3.0f : 0.0f), longest = around + 2.0f * std::ceil(key_tiles / S), one = around + 2.0f * mean_tiles / S;
-        const float cost = pairs <= cap ? longest : std::max(longest, one * ((float)pairs / cap + 0.5f));
-        if (S == 1 || cost < best) { best = cost; f.share = S; }
+        const int cap = flash_capacity<D, Q8>(S) * S, walk = (key_tiles + S - 1) / S;
+        const float around = 6.0f + (S > 1 ? 3.0f : 0.0f), longest = around + 2.0f * walk;
+        const float ctas = likely * std::max(1.0f, mean_tiles / walk), one = around + 2.0f * std::min(mean_tiles, (float)walk);
+        const float cost = ctas <= cap ? longest : std::max(longest, one * (ctas / cap + 0.5f));
+        if (S == 1 || cost < best) { best = cost; f.cluster = S; f.walk_tiles = walk; }
     }
-    if (pairs * f.share > INT32_MAX) JSM_FAIL(JSM_UNSUPPORTED, "jsm_attn_chunk: %lld tiles of queries", pairs);
+    if (pairs * f.cluster > INT32_MAX) JSM_FAIL(JSM_UNSUPPORTED, "jsm_attn_chunk: %lld tiles of queries", pairs);
     CUtensorMap mq, mkv;
     jsm_status s = make_tmap_bf16_3d(&mq, a.q, D, a.Hq, a.T, D, a.q_rs, 64, a.G, f.tile_tokens);
     if (s != JSM_OK) return s;
@@ -749,7 +760,7 @@ static jsm_status flash_launch(const ChunkArgs& a, int few_rows, cudaStream_t st
     s = Q8 ? make_tmap_u8_lines(&mkv, a.c.pool, rows * D / 128, JSM_PAGE_SIZE * D / 128) : make_tmap_bf16_2d(&mkv, a.c.pool, rows, D, D, JSM_PAGE_SIZE, 64);
     if (s != JSM_OK) return s;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(pairs * f.share));
+    cfg.gridDim = dim3((unsigned)(pairs * f.cluster));
     cfg.blockDim = dim3(Z::THREADS);
     cfg.dynamicSmemBytes = Z::SMEM;
     cfg.stream = st;
@@ -757,10 +768,10 @@ static jsm_status flash_launch(const ChunkArgs& a, int few_rows, cudaStream_t st
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = f.share;
+    attr[1].val.clusterDim.x = f.cluster;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = chained_launch_enabled() ? attr : attr + 1;
-    cfg.numAttrs = (chained_launch_enabled() ? 1 : 0) + (f.share > 1 ? 1 : 0);
+    cfg.numAttrs = (chained_launch_enabled() ? 1 : 0) + (f.cluster > 1 ? 1 : 0);
     JSM_CUDA_CHECK(cudaLaunchKernelEx(&cfg, chunk_flash_kernel<D, Q8>, mq, mkv, f));
     JSM_LAUNCH_CHECK();
     return JSM_OK;
