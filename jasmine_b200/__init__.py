@@ -591,11 +591,15 @@ def kv_append_q8(pool, scales, block_table, k, v, starts, context_lens, Hkv, D, 
 def kv_read(pool, block_table, starts, context_lens, T, Hkv, D, scales=None, dtype=None, k_out=None, v_out=None):
     """Keys and values [T, Hkv * D] (bf16, or dtype) of the new tokens' positions as the cache holds them (jsm_kv_read); rows of no sequence are left as they are."""
     torch = _torch()
+    m = _calls_module or _calls()
+    if m and dtype in (None, torch.bfloat16, torch.float32):
+        done = m.kv_read(pool, scales, block_table, starts, context_lens, T, Hkv, D, k_out, v_out, dtype is torch.float32)
+        if type(done) is tuple:
+            return done
+        if _done(done):
+            return k_out, v_out
     k_out = torch.empty(T, Hkv * D, dtype=dtype or torch.bfloat16, device=pool.device) if k_out is None else k_out
     v_out = torch.empty_like(k_out) if v_out is None else v_out
-    m = _calls_module or _calls()
-    if m and _done(m.kv_read(pool, scales, block_table, starts, context_lens, T, Hkv, D, k_out, v_out)):
-        return k_out, v_out
     at, seqs = _cache("kv_read", pool, scales, block_table, starts, context_lens, Hkv, D)
     for t in (k_out, v_out):
         _rows(t, Hkv * D, "kv_read: out")

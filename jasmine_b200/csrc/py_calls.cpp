@@ -299,16 +299,37 @@ JSM_FAST(kv_append_q8) {  // pool, scales, block_table, k, v, starts, context_le
     });
 }
 
-JSM_FAST(kv_read) {  // pool, scales, block_table, starts, context_lens, T, Hkv, D, k_out, v_out
+JSM_FAST(kv_read) {  // pool, scales, block_table, starts, context_lens, T, Hkv, D, k_out, v_out (both or neither), f32; with neither the new outputs come back
     int T, hkv, d;
     Cache c;
     Rows k, v;
-    JSM_NEED(n_args == 10 && as_int(a[5], T) && as_int(a[6], hkv) && as_int(a[7], d) && hkv > 0 && d > 0 && as_cache(a[0], a[1], a[2], a[3], a[4], hkv, d, c) &&
-             as_rows(a[8], (int64_t)hkv * d, k) && as_rows(a[9], (int64_t)hkv * d, v));
-    JSM_NEED(k.type >= 0 && k.type == v.type && k.T == T && v.T == T && k.pitch == v.pitch);
-    return status_of([&](void* st) {
+    JSM_NEED(n_args == 11 && as_int(a[5], T) && as_int(a[6], hkv) && as_int(a[7], d) && T >= 0 && hkv > 0 && d > 0 && as_cache(a[0], a[1], a[2], a[3], a[4], hkv, d, c));
+    JSM_NEED((a[8] == Py_None) == (a[9] == Py_None) && (a[10] == Py_True || a[10] == Py_False));
+    const bool fresh = a[8] == Py_None;
+    PyObject* out = nullptr;
+    if (fresh) {
+        const auto options = THPVariable_Unpack(a[0]).options().dtype(a[10] == Py_True ? at::kFloat : at::kBFloat16);
+        PyObject *ko = THPVariable_Wrap(at::empty({T, (int64_t)hkv * d}, options)), *vo = THPVariable_Wrap(at::empty({T, (int64_t)hkv * d}, options));
+        out = PyTuple_Pack(2, ko, vo);
+        Py_XDECREF(ko);
+        Py_XDECREF(vo);
+        if (!out) return nullptr;
+    }
+    const bool fits = as_rows(fresh ? PyTuple_GET_ITEM(out, 0) : a[8], (int64_t)hkv * d, k) && as_rows(fresh ? PyTuple_GET_ITEM(out, 1) : a[9], (int64_t)hkv * d, v) &&
+                      k.type >= 0 && k.type == v.type && k.T == T && v.T == T && k.pitch == v.pitch;
+    if (!fits) {
+        Py_XDECREF(out);
+        Py_RETURN_NONE;
+    }
+    PyObject* status = status_of([&](void* st) {
         return L.kv_read(c.pool, c.scales, c.pages, c.table, c.max_pages, c.starts, c.lens, c.seqs, T, hkv, d, k.data, v.data, k.pitch, (jsm_dtype)k.type, st);
     });
+    if (!fresh || !status || PyLong_AsLong(status) != 0) {
+        Py_XDECREF(out);
+        return status;
+    }
+    Py_DECREF(status);
+    return out;
 }
 
 JSM_FAST(attn_chunk) {  // q, pool, scales, block_table, starts, context_lens, Hq, Hkv, D, max_new, max_context, window, scale, scratch, out

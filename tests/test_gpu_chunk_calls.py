@@ -1,0 +1,164 @@
+"""The operators over new tokens as a program uses them: through the extension module and through ctypes, from several streams and graphs, many sequences, large pools."""
+import pytest
+import torch
+
+import jasmine_b200 as jb
+from cache_util import PAGE, Cache, check_attention
+from test_native_calls import both
+
+pytestmark = pytest.mark.gpu
+
+
+def test_both_ways_into_the_library(monkeypatch):
+    c = Cache([3, 0, 40, 1], [70, 9, 300, 130], 2, 128, 8, rows=2).to_device()
+    q, x = c.queries(8).cuda(), torch.randn(c.T, 2 * 2 * 128, device="cuda").bfloat16()
+    k, v = x[:, :256], x[:, 256:]
+    t = torch.randn(400, 64, 2, device="cuda")
+    at = torch.arange(c.T, dtype=torch.int32, device="cuda")
+    seqs = (c.table, c.starts, c.lens)
+    short = c.lens[:2].contiguous()
+
+    def append(pool=None, **kw):
+        a = dict(pool=c.pool.clone() if pool is None else pool, scales=c.scales.clone(), block_table=c.table, k=k, v=v, starts=c.starts, context_lens=c.lens, Hkv=2, D=128, rope=t, rot_dim=128)
+        a.update(kw)
+        jb.kv_append_q8(**a)
+        return a["pool"], a["scales"].view(torch.int16)
+
+    def read(**kw):
+        return jb.kv_read(c.pool, *seqs, c.T, 2, 128, **{**dict(scales=c.scales), **kw})
+
+    for call in (
+        lambda: jb.rope_rotate(q, k, t, 8, 2, 128, 128, at),
+        lambda: jb.rope_rotate(q, None, t, 8, 0, 128, 128, None, layout=jb.ROPE_ADJACENT, inverse=True)[0],
+        lambda: jb.rope_rotate(q, k, t, 8, 2, 128, 64, at),                # a table of another rotation
+        lambda: jb.rope_rotate(q, k.float(), t, 8, 2, 128, 128, at),
+        lambda: jb.rope_rotate(q, k[:2], t, 8, 2, 128, 128, at),
+        lambda: jb.rope_rotate(q.half(), None, t, 8, 0, 128, 128),
+        append, lambda: append(rope=None), lambda: append(k=k.float()), lambda: append(starts=c.starts[:3].contiguous()), lambda: append(pool=c.pool.bfloat16()),
+        lambda: append(rot_dim=64), lambda: append(layout=5),
+        lambda: [x[:44] for x in read(k_out=torch.zeros(c.T, 256, device="cuda"), v_out=torch.zeros(c.T, 256, device="cuda"))],
+        lambda: [x[:44] for x in read(dtype=torch.float32)], lambda: [x[:44] for x in read()], lambda: read(dtype=torch.float16),
+        lambda: read(scales=None), lambda: read(k_out=torch.zeros(c.T, 256, device="cuda"), v_out=torch.zeros(c.T, 256, device="cuda").bfloat16()),
+        lambda: c.attend(q)[:44], lambda: c.attend(q, 50, 0.2)[:44], lambda: c.attend(q, scratch=torch.empty(1 << 24, dtype=torch.uint8, device="cuda"))[:44],
+        lambda: c.attend(q, scratch=torch.empty(16, dtype=torch.uint8, device="cuda")), lambda: c.attend(q, -1), lambda: c.attend(q, 0, 0.0),
+        lambda: c.attend(q.float()), lambda: c.attend(q, out=torch.empty_like(q)[:5]),
+        lambda: jb.attn_chunk(q, c.pool, c.table, c.starts, short, 8, 2, 128, 40, 300, scales=c.scales),
+    ):
+        fast, slow = both(monkeypatch, call)
+        if isinstance(slow, tuple) and isinstance(slow[0], type):
+            assert fast == slow, call
+            continue
+        for a, b in zip(fast, slow) if isinstance(slow, (tuple, list)) else ((fast, slow),):
+            assert a is None and b is None or torch.equal(a, b)
+    jb.check_device_errors()
+
+
+@pytest.mark.parametrize("bits", (16, 8))
+def test_many_sequences(bits):
+    g = torch.Generator().manual_seed(8)
+    new = torch.randint(0, 4, (300,), generator=g).tolist() + [70, 0, 20] + torch.randint(0, 3, (40,), generator=g).tolist() + [33]
+    ctx = [n + p for n, p in zip(new, torch.randint(0, 200, (len(new),), generator=g).tolist())]
+    c = Cache(new, ctx, 2, 64, bits, seed=2, rows=3).to_device()
+    q = c.queries(4)
+    out = torch.full((c.T, 256), 2.0, dtype=torch.bfloat16, device="cuda")
+    got = c.attend(q.cuda(), out=out)
+    jb.check_device_errors()
+    check_attention(got, *c.reference(q))
+    assert bool((out[sum(new):] == 2).all())
+
+
+def test_no_new_tokens_at_all():
+    c = Cache([0, 0], [70, 0], 2, 64, 8, rows=5).to_device()
+    c.new = [1]  # (bounds of the call)
+    out = torch.full((5, 256), 2.0, dtype=torch.bfloat16, device="cuda")
+    c.attend(torch.zeros(5, 256, dtype=torch.bfloat16, device="cuda"), out=out)
+    jb.check_device_errors()
+    assert bool((out == 2).all())
+
+
+@pytest.mark.parametrize("bits", (16, 8))
+@pytest.mark.parametrize("new,ctx", [([1], [640]), ([130], [900])])
+def test_scores_that_jump_by_thousands(new, ctx, bits):
+    """Key after key the largest score grows, in one tile by more than any weight can hold: what the last keys do not outweigh is nothing."""
+    c = Cache(new, ctx, 1, 128, bits, seed=6)
+    for p in range(0, ctx[0], 50):
+        c.values[0][0, 0, p:p + 50] *= 0.01
+        c.values[0][0, 0, p + 20] = 4.0 * (p + 1)
+    c.write(0)
+    c.to_device()
+    q = c.queries(4).abs()
+    got = c.attend(q.cuda(), 0, 1.0)
+    # scores up to 128 * 4 * 850 = 4e5 in fp32 are off by some hundredths: weights of one key by itself are 1, others 0
+    check_attention(got, *c.reference(q, 0, 1.0))
+
+
+@pytest.mark.parametrize("new", ([1, 1], [60, 1]))
+def test_two_streams_and_two_graphs_at_a_time(new):
+    cs = [Cache(new, [2000, 700], 2, 128, b, seed=b).to_device() for b in (8, 16)]
+    qs = [c.queries(8).cuda() for c in cs]
+    want = [c.attend(q) for c, q in zip(cs, qs)]
+    torch.cuda.synchronize()
+    streams, outs, graphs = [torch.cuda.Stream() for _ in cs], [torch.empty_like(w) for w in want], []
+    for s, c, q, o in zip(streams, cs, qs, outs):
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                c.attend(q, out=o)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, outs))
+    for c, q, o in zip(cs, qs, outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            for _ in range(5):
+                c.attend(q, out=o)
+        graphs.append(g)
+        o.zero_()
+    for _ in range(4):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, outs))
+    jb.check_device_errors()
+
+
+@pytest.mark.parametrize("bits", (16, 8))
+@pytest.mark.parametrize("new", (1, 40))
+def test_places_beyond_32_bits(new, bits):
+    """A pool of more than 2^32 numbers, and a sequence whose pages lie at its end."""
+    Hkv, D, ctx = 8, 128, 150
+    pages = (1 << 32) // (2 * Hkv * PAGE * D) + 40
+    pool = torch.empty(pages, 2, Hkv, PAGE, D, dtype=torch.bfloat16 if bits == 16 else torch.int8, device="cuda")
+    small = Cache([new], [ctx], Hkv, D, bits, seed=1).to_device()
+    scales = torch.empty(pages, 2, Hkv, PAGE, dtype=torch.bfloat16, device="cuda") if bits == 8 else None
+    blocks = torch.tensor([[pages - 1, pages - 7, pages - 3]], dtype=torch.int32, device="cuda")
+    for b, s in zip(blocks[0].tolist(), small.table[0].tolist()):
+        pool[b] = small.pool[s]
+        if bits == 8:
+            scales[b] = small.scales[s]
+    q = small.queries(16)
+    got = jb.attn_chunk(q.cuda(), pool, blocks, small.starts, small.lens, 16, Hkv, D, new, ctx, scales=scales)
+    check_attention(got, *small.reference(q))
+    if bits == 8:
+        x = torch.randn(new, 2 * Hkv * D, device="cuda").bfloat16()
+        for p, s, t in ((pool, scales, blocks), (small.pool, small.scales, small.table)):
+            jb.kv_append_q8(p, s, t, x[:, :Hkv * D], x[:, Hkv * D:], small.starts, small.lens, Hkv, D)
+        a, b = (jb.kv_read(p, t, small.starts, small.lens, new, Hkv, D, scales=s) for p, s, t in ((pool, scales, blocks), (small.pool, small.scales, small.table)))
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    jb.check_device_errors()
+
+
+def test_queries_and_outputs_beyond_32_bits():
+    """Rows so far apart that their places pass 2^31 elements."""
+    c = Cache([50], [80], 1, 64, 16, seed=1).to_device()
+    q = c.queries(2)
+    pitch = (1 << 31) // 49 // 8 * 8 + 8
+    wide = torch.empty(49 * pitch + 128, dtype=torch.bfloat16, device="cuda")
+    rows = wide.as_strided((50, 128), (pitch, 1))
+    rows.copy_(q)
+    c.attend(rows, out=rows)
+    check_attention(rows, *c.reference(q))
+    t = torch.randn(100, 32, 2, device="cuda")
+    rows.copy_(q)
+    jb.rope_rotate(rows, None, t, 2, 0, 64, 64, q_out=rows)
+    assert torch.equal(rows, jb.rope_rotate(q.cuda(), None, t, 2, 0, 64, 64)[0])
+    jb.check_device_errors()
