@@ -548,10 +548,17 @@ def rope_rotate(q, k, table, Hq, Hkv, D, rot_dim, positions=None, layout=ROPE_HA
             _rows(t, n * D, "rope_rotate: " + what)
     if positions is not None:
         _ints(positions, (T,), "rope_rotate: positions")
+    _here("rope_rotate", q, k, table, positions, q_out, k_out)
     p = lambda t, n: (t.data_ptr(), _pitch(t)) if n else (None, 0)  # noqa: E731
     check(lib().jsm_rope_rotate(*p(q, Hq), *p(q_out, Hq), Hq, *p(k, Hkv), *p(k_out, Hkv), Hkv, dtype_of(x), D, table.data_ptr(), table.shape[0], rot_dim, layout,
                                 int(inverse), positions.data_ptr() if positions is not None else None, T, stream_ptr()))
     return q_out, k_out
+
+
+def _here(what, *tensors):
+    """The kernels run on torch's current device and reach what lies there."""
+    at = _torch().cuda.current_device() if all(t is None or t.is_cuda for t in tensors) else None
+    _need(at is not None and all(t is None or t.get_device() == at for t in tensors), f"{what}: tensors on the current CUDA device are wanted")
 
 
 def _cache(what, pool, scales, block_table, starts, context_lens, Hkv, D):
@@ -584,6 +591,7 @@ def kv_append_q8(pool, scales, block_table, k, v, starts, context_lens, Hkv, D, 
     if rope is not None:
         _need(rope.dtype == torch.float32 and rope.is_contiguous() and rope.dim() == 3 and tuple(rope.shape[1:]) == (rot_dim // 2, 2),
               "kv_append_q8: a contiguous fp32 table [positions, rot_dim / 2, 2] is wanted")
+    _here("kv_append_q8", pool, scales, block_table, k, v, starts, context_lens, rope)
     check(lib().jsm_kv_append_q8(*at, k.data_ptr(), v.data_ptr(), _pitch(k), *seqs, k.shape[0], Hkv, D, rope.data_ptr() if rope is not None else None,
                                  rope.shape[0] if rope is not None else 0, rot_dim, layout, stream_ptr()))
 
@@ -604,6 +612,7 @@ def kv_read(pool, block_table, starts, context_lens, T, Hkv, D, scales=None, dty
     for t in (k_out, v_out):
         _rows(t, Hkv * D, "kv_read: out")
     _need(k_out.shape == v_out.shape and k_out.shape[0] == T and k_out.dtype == v_out.dtype and _pitch(k_out) == _pitch(v_out), "kv_read: outputs of one shape, type and pitch")
+    _here("kv_read", pool, scales, block_table, starts, context_lens, k_out, v_out)
     check(lib().jsm_kv_read(*at, *seqs, T, Hkv, D, k_out.data_ptr(), v_out.data_ptr(), _pitch(k_out), dtype_of(k_out), stream_ptr()))
     return k_out, v_out
 
@@ -624,6 +633,7 @@ def attn_chunk(q, pool, block_table, starts, context_lens, Hq, Hkv, D, max_new, 
     if scratch is None:
         scratch = torch.empty(lib().jsm_attn_chunk_scratch_bytes(seqs[2], T, max_new, max_context, Hq, Hkv, D, window), dtype=torch.uint8, device=q.device)
     _need(scratch.is_contiguous(), "attn_chunk: contiguous scratch is wanted")
+    _here("attn_chunk", q, pool, scales, block_table, starts, context_lens, scratch, out)
     check(lib().jsm_attn_chunk(q.data_ptr(), _pitch(q), *at, *seqs, T, max_new, max_context, Hq, Hkv, D, window, scale, scratch.data_ptr(),
                                scratch.numel() * scratch.element_size(), out.data_ptr(), _pitch(out), stream_ptr()))
     return out

@@ -7,6 +7,7 @@
 // library is the one that Python has loaded (bind).
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
 #include <algorithm>
@@ -211,6 +212,11 @@ JSM_FAST(attn_decode) {  // q, pool, block_table, context_lens, Hq, Hkv, D, max_
     });
 }
 
+// the same on the current device, where the call runs
+const at::Tensor* here(PyObject* o) {
+    const at::Tensor* t = plain(o);
+    return t && t->get_device() == c10::cuda::current_device() ? t : nullptr;
+}
 // Rows [T, columns] of adjacent elements; a single row's pitch means nothing.
 struct Rows {
     void* data = nullptr;
@@ -218,7 +224,7 @@ struct Rows {
     int type = -1;
 };
 bool as_rows(PyObject* o, int64_t columns, Rows& r) {
-    const at::Tensor* t = plain(o);
+    const at::Tensor* t = here(o);
     if (!t || t->dim() != 2 || t->size(1) != columns || (columns > 1 && t->stride(1) != 1) || t->size(0) > INT32_MAX) return false;
     r.data = t->mutable_data_ptr();
     r.T = t->size(0);
@@ -227,7 +233,7 @@ bool as_rows(PyObject* o, int64_t columns, Rows& r) {
     return true;
 }
 bool as_ints(PyObject* o, std::initializer_list<int64_t> shape, const int32_t*& p) {
-    const at::Tensor* t = plain(o);
+    const at::Tensor* t = here(o);
     if (!t || t->scalar_type() != at::kInt || !t->is_contiguous() || t->dim() != (int64_t)shape.size() || !std::equal(shape.begin(), shape.end(), t->sizes().begin())) return false;
     p = (const int32_t*)t->mutable_data_ptr();
     return true;
@@ -237,7 +243,7 @@ bool as_rotation(PyObject* o, int rot, const float*& p, int& n) {
     p = nullptr;
     n = 0;
     if (o == Py_None) return true;
-    const at::Tensor* t = plain(o);
+    const at::Tensor* t = here(o);
     if (!t || t->scalar_type() != at::kFloat || !t->is_contiguous() || t->dim() != 3 || t->size(1) != rot / 2 || t->size(2) != 2 || t->size(0) > INT32_MAX) return false;
     p = (const float*)t->mutable_data_ptr();
     n = (int)t->size(0);
@@ -250,12 +256,12 @@ struct Cache {
     const int32_t *table, *starts, *lens;
 };
 bool as_cache(PyObject* pool, PyObject* scales, PyObject* table, PyObject* starts, PyObject* lens, int hkv, int d, Cache& c) {
-    const at::Tensor *p = plain(pool), *b = plain(table), *l = plain(lens);
+    const at::Tensor *p = here(pool), *b = here(table), *l = here(lens);
     if (!p || !b || !l || p->dim() != 5 || !p->is_contiguous() || p->size(1) != 2 || p->size(2) != hkv || p->size(3) != JSM_PAGE_SIZE || p->size(4) != d || p->size(0) > INT32_MAX)
         return false;
     if (b->dim() != 2 || l->dim() != 1 || b->size(1) > INT32_MAX || l->size(0) > INT32_MAX) return false;
     if (scales != Py_None) {
-        const at::Tensor* s = plain(scales);
+        const at::Tensor* s = here(scales);
         if (!s || s->scalar_type() != at::kBFloat16 || !s->is_contiguous() || s->dim() != 4 || !std::equal(s->sizes().begin(), s->sizes().end(), p->sizes().begin())) return false;
         c.scales = s->mutable_data_ptr();
     }
@@ -345,7 +351,7 @@ JSM_FAST(attn_chunk) {  // q, pool, scales, block_table, starts, context_lens, H
     size_t bytes = 0;
     at::Tensor own;
     if (a[13] != Py_None) {
-        JSM_NEED(as_pointer(a[13], scratch) && THPVariable_Unpack(a[13]).is_contiguous());
+        JSM_NEED(here(a[13]) && as_pointer(a[13], scratch) && THPVariable_Unpack(a[13]).is_contiguous());
         bytes = THPVariable_Unpack(a[13]).nbytes();
     } else if ((bytes = L.attn_chunk_scratch_bytes(c.seqs, (int)q.T, most_new, most, hq, hkv, d, window)) > 0) {
         own = at::empty({(int64_t)bytes}, THPVariable_Unpack(a[0]).options().dtype(at::kByte));

@@ -121,6 +121,18 @@ def test_the_python_calls_check_their_tensors():
         jb.attn_chunk(q, Hq=4, max_new=1, max_context=64, out=q[:2], **good)
 
 
+def test_the_python_calls_take_tensors_of_the_current_device():
+    """Memory of the host, or of another device, is not what the kernels reach: refused before anything runs."""
+    b, i = torch.bfloat16, torch.int32
+    pool, scales = torch.zeros(4, 2, 2, 64, 64, dtype=torch.int8), torch.zeros(4, 2, 2, 64, dtype=b)
+    cache = dict(block_table=torch.zeros(2, 2, dtype=i), starts=torch.zeros(3, dtype=i), context_lens=torch.zeros(2, dtype=i), scales=scales, Hkv=2, D=64)
+    k, q, t = torch.zeros(3, 128, dtype=b), torch.zeros(3, 256, dtype=b), torch.zeros(10, 32, 2)
+    for call in (lambda: jb.rope_rotate(q, k, t, 4, 2, 64, 64), lambda: jb.kv_append_q8(pool, k=k, v=k, **cache), lambda: jb.kv_read(pool, T=3, **cache),
+                 lambda: jb.attn_chunk(q, pool, Hq=4, max_new=1, max_context=64, scratch=torch.zeros(1 << 20, dtype=torch.uint8), **cache)):
+        with pytest.raises(jb.JsmError, match="current CUDA device"):
+            call()
+
+
 def test_scratch_of_arguments_that_cannot_be_right():
     f = jb.lib().jsm_attn_chunk_scratch_bytes
     f.restype = C.c_size_t

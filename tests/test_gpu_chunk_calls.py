@@ -43,6 +43,9 @@ def test_both_ways_into_the_library(monkeypatch):
         lambda: c.attend(q, scratch=torch.empty(16, dtype=torch.uint8, device="cuda")), lambda: c.attend(q, -1), lambda: c.attend(q, 0, 0.0),
         lambda: c.attend(q.float()), lambda: c.attend(q, out=torch.empty_like(q)[:5]),
         lambda: jb.attn_chunk(q, c.pool, c.table, c.starts, short, 8, 2, 128, 40, 300, scales=c.scales),
+        # memory of the host is refused before anything runs
+        lambda: jb.rope_rotate(q, k, t.cpu(), 8, 2, 128, 128, at), lambda: append(k=k.cpu(), v=v.cpu()), lambda: read(scales=c.scales.cpu()),
+        lambda: c.attend(q.cpu()), lambda: c.attend(q, scratch=torch.empty(1 << 24, dtype=torch.uint8)),
     ):
         fast, slow = both(monkeypatch, call)
         if isinstance(slow, tuple) and isinstance(slow[0], type):
