@@ -114,14 +114,18 @@ __device__ __forceinline__ void find_places(const CacheView& c, int T, int t0, i
 
 // Whole 16-byte pieces: LPR lanes have two pieces of eight components each of a row (token, keys or values, kv head), up to PLACES tokens per block; a thread's first loads do not
 // wait for the places.  A lane's pieces hold both components of its pairs (halves: a piece of each half), so that a rotation stays within the lane and its eight table
-// entries serve all heads of a token.  Products that are rounded on their own before a sum are not packed: a packed product and a packed sum behind it leave the
-// assembler as one operation with one rounding.  Rounding to a whole number: adding 1.5 * 2^23 leaves it in the low bits of the sum.
-// Prompts of 7887 tokens of 32 kv heads of 128 (192 MB in and out) 53 us, 3.6 TB/s of the measured 6.5, 60 % of the issue slots; a lane per eight components with the partner of a half
-// fetched a second time 74 us.
+// entries serve all heads of a token.  Products that are rounded on their own before a sum: two by one instruction, the sums one by one (mul2).  Rounding to a whole number:
+// adding 1.5 * 2^23 leaves it in the low bits of the sum.
+// Prompts of 7887 tokens of 32 kv heads of 128 (192 MB in and out) 47 us, 4.1 TB/s of the measured 6.5: latency at four blocks per multiprocessor, 57 % of the issue slots.  The loads
+// of two turns at a time, none while they are worked out, addresses in 64 bits: 53 us; a lane per eight components with the partner of a half fetched a second time 74 us.
 __device__ __forceinline__ float max3_abs(float a, float b, float c) {  // of the magnitudes; a NaN stays one
     float d;
     asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
+}
+// two products, each rounded (sums of them one by one: a packed sum behind a packed product leaves the assembler as one operation with one rounding)
+__device__ __forceinline__ void mul2(float& x, float& y, float a, float b, float c, float d) {
+    asm("{ .reg .b64 p, q; mov.b64 p, {%2, %3}; mov.b64 q, {%4, %5}; mul.rn.f32x2 p, p, q; mov.b64 {%0, %1}, p; }" : "=f"(x), "=f"(y) : "f"(a), "f"(b), "f"(c), "f"(d));
 }
 // row r of token k, and the one `step` rows on
 __device__ __forceinline__ void advance(int& k, int& r, int step, int per_token) {
@@ -138,7 +142,7 @@ __device__ __forceinline__ void advance(int& k, int& r, int step, int per_token)
 enum { TURN_NONE = 0, TURN_ADJACENT = 1, TURN_HALF = 2, TURN_ANY = 3 };  // any: parts that are no multiple of 16, element by element
 template <int LPR, int TURN>
 __global__ void __launch_bounds__(256, 4) kv_append_q8_vec_kernel(AppendArgs a, int per_block) {
-    constexpr int ROWS = 256 / LPR, U = 2;  // rows of a block's turn, turns whose loads are in flight
+    constexpr int ROWS = 256 / LPR;  // rows of a block's turn
     __shared__ int sh_seq[PLACES], sh_pos[PLACES], sh_base[PLACES];
     chain_trigger();
     chain_wait();
@@ -146,20 +150,15 @@ __global__ void __launch_bounds__(256, 4) kv_append_q8_vec_kernel(AppendArgs a, 
     const int l = threadIdx.x % LPR, group = threadIdx.x / LPR, half = a.rot / 2;
     const bool on = l * 16 < D, turns = TURN != TURN_NONE && l * 16 < a.rot;
     const int i0 = TURN == TURN_HALF && turns ? l * 8 : l * 16, i1 = TURN == TURN_HALF && turns ? i0 + half : i0 + 8;  // first components of the lane's pieces
-    const __nv_bfloat16* v_src = a.v - (long long)Hkv * D;
-    uint4 w[U][2];
-    // rows of the block, token after token, keys before values: row r of token k
+    // rows of the block, token after token, keys before values: row r of token k (a block's rows lie within 2^31 elements)
+    const int pitch = (int)a.kv_rs, apart = i1 - i0;
+    const __nv_bfloat16 *k_src = a.k + t0 * a.kv_rs + i0, *v_src = a.v + t0 * a.kv_rs + i0 - (long long)Hkv * D;
+    uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
     auto load = [&](int k, int r) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const __nv_bfloat16* src = (r < Hkv ? a.k : v_src) + (t0 + k) * a.kv_rs + r * D;
-            w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
-            if (on && k < n_tokens) {
-                w[u][0] = *reinterpret_cast<const uint4*>(src + i0);
-                w[u][1] = *reinterpret_cast<const uint4*>(src + i1);
-            }
-            advance(k, r, ROWS, per_token);
-        }
+        if (!on || k >= n_tokens) return;
+        const __nv_bfloat16* src = (r < Hkv ? k_src : v_src) + (k * pitch + r * D);
+        w[0] = *reinterpret_cast<const uint4*>(src);
+        w[1] = *reinterpret_cast<const uint4*>(src + apart);
     };
     int k = 0, r = 0;
     advance(k, r, group, per_token);
@@ -173,76 +172,76 @@ __global__ void __launch_bounds__(256, 4) kv_append_q8_vec_kernel(AppendArgs a, 
         c[i] = 1.0f;
         sn[i] = 0.0f;
     }
-    for (int row = group; row - ahead < n_rows; row += U * ROWS) {
-        if (row != group) load(k, r);
+    for (int row = group; row - ahead < n_rows; row += ROWS) {
+        const int base = k < n_tokens ? sh_base[k] : -1;
+        float x[16];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (row + u * ROWS - ahead >= n_rows) break;
-            const int base = k < n_tokens ? sh_base[k] : -1;
-            float x[16];
+        for (int p = 0; p < 2; ++p) {
+            const uint32_t in[4] = {w[p].x, w[p].y, w[p].z, w[p].w};
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                const uint32_t in[4] = {w[u][p].x, w[u][p].y, w[u][p].z, w[u][p].w};
+            for (int i = 0; i < 4; ++i) {
+                x[p * 8 + 2 * i] = bf16lo(in[i]);
+                x[p * 8 + 2 * i + 1] = bf16hi(in[i]);
+            }
+        }
+        const int k_now = k, r_now = r;
+        advance(k, r, ROWS, per_token);
+        load(k, r);  // (the next turn's, while this one is worked out)
+        if (TURN == TURN_ANY && r_now < Hkv && turns && base >= 0) {
+            const __nv_bfloat16* src = a.k + (t0 + k_now) * a.kv_rs + r_now * D;
+            const float2* e = a.table + (long long)sh_pos[k_now] * half;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int d = l * 16 + i;
+                if (d >= a.rot) break;
+                const bool second = a.adjacent ? d & 1 : d >= half;
+                const float2 v = e[a.adjacent ? d / 2 : second ? d - half : d];
+                const float z = __bfloat162float(src[a.adjacent ? d ^ 1 : second ? d - half : d + half]);
+                x[i] = __fadd_rn(__fmul_rn(x[i], v.x), __fmul_rn(z, second ? v.y : -v.y));
+            }
+        } else if (TURN != TURN_NONE && TURN != TURN_ANY && r_now < Hkv) {
+            if (have != k_now && turns && base >= 0) {
+                have = k_now;
+                const float4* e = reinterpret_cast<const float4*>(a.table + (long long)sh_pos[k_now] * half + l * 8);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x[p * 8 + 2 * i] = bf16lo(in[i]);
-                    x[p * 8 + 2 * i + 1] = bf16hi(in[i]);
+                    const float4 v = e[i];
+                    c[2 * i] = v.x; sn[2 * i] = v.y; c[2 * i + 1] = v.z; sn[2 * i + 1] = v.w;
                 }
             }
-            if (TURN == TURN_ANY && r < Hkv && turns && base >= 0) {
-                const __nv_bfloat16* src = a.k + (t0 + k) * a.kv_rs + r * D;
-                const float2* e = a.table + (long long)sh_pos[k] * half;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int d = l * 16 + i;
-                    if (d >= a.rot) break;
-                    const bool second = a.adjacent ? d & 1 : d >= half;
-                    const float2 v = e[a.adjacent ? d / 2 : second ? d - half : d];
-                    const float z = __bfloat162float(src[a.adjacent ? d ^ 1 : second ? d - half : d + half]);
-                    x[i] = __fadd_rn(__fmul_rn(x[i], v.x), __fmul_rn(z, second ? v.y : -v.y));
-                }
-            } else if (TURN != TURN_NONE && TURN != TURN_ANY && r < Hkv) {
-                if (have != k && turns && base >= 0) {
-                    have = k;
-                    const float4* e = reinterpret_cast<const float4*>(a.table + (long long)sh_pos[k] * half + l * 8);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float4 v = e[i];
-                        c[2 * i] = v.x; sn[2 * i] = v.y; c[2 * i + 1] = v.z; sn[2 * i + 1] = v.w;
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int i1_ = TURN == TURN_ADJACENT ? 2 * i : i, i2_ = TURN == TURN_ADJACENT ? 2 * i + 1 : i + 8;
-                    rotate_pair(x[i1_], x[i2_], c[i], sn[i], x[i1_], x[i2_]);
-                }
+            for (int i = 0; i < 8; ++i) {  // (two products by one instruction: no faster here)
+                const int i1_ = TURN == TURN_ADJACENT ? 2 * i : i, i2_ = TURN == TURN_ADJACENT ? 2 * i + 1 : i + 8;
+                rotate_pair(x[i1_], x[i2_], c[i], sn[i], x[i1_], x[i2_]);
             }
-            float most = 0.0f;
+        }
+        float most = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) most = max3_abs(most, x[i], x[i + 1]);
+        for (int i = 0; i < 16; i += 2) most = max3_abs(most, x[i], x[i + 1]);
 #pragma unroll
-            for (int o = LPR / 2; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-            const float scale = q8_scale(most), inv = scale == scale ? q8_inverse(scale) : 0.0f;
-            uint32_t out[4];
+        for (int o = LPR / 2; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const float scale = q8_scale(most), inv = q8_inverse(scale);
+        uint32_t out[4];
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                uint32_t n[4];  // 1.5 * 2^23 + the number
+        for (int i = 0; i < 16; i += 4) {
+            uint32_t n[4];  // 1.5 * 2^23 + the number
+            float y[4];
+            mul2(y[0], y[1], x[i], x[i + 1], inv, inv);
+            mul2(y[2], y[3], x[i + 2], x[i + 3], inv, inv);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) n[j] = __float_as_uint(__fadd_rn(__fmul_rn(x[i + j], inv), 12582912.0f));
-                out[i / 4] = scale == scale ? __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410) : 0u;
+            for (int j = 0; j < 4; ++j) n[j] = __float_as_uint(__fadd_rn(y[j], 12582912.0f));
+            out[i / 4] = scale == scale ? __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410) : 0u;
+        }
+        if (on && base >= 0) {
+            const int to = base + r_now * JSM_PAGE_SIZE;
+            int8_t* dst = static_cast<int8_t*>(a.c.pool) + (long long)to * D;
+            if (TURN == TURN_HALF) {
+                *reinterpret_cast<uint2*>(dst + i0) = make_uint2(out[0], out[1]);
+                *reinterpret_cast<uint2*>(dst + i1) = make_uint2(out[2], out[3]);
+            } else {
+                *reinterpret_cast<uint4*>(dst + i0) = make_uint4(out[0], out[1], out[2], out[3]);
             }
-            if (on && base >= 0) {
-                const int to = base + r * JSM_PAGE_SIZE;
-                int8_t* dst = static_cast<int8_t*>(a.c.pool) + (long long)to * D;
-                if (TURN == TURN_HALF) {
-                    *reinterpret_cast<uint2*>(dst + i0) = make_uint2(out[0], out[1]);
-                    *reinterpret_cast<uint2*>(dst + i1) = make_uint2(out[2], out[3]);
-                } else {
-                    *reinterpret_cast<uint4*>(dst + i0) = make_uint4(out[0], out[1], out[2], out[3]);
-                }
-                if (l == 0) a.c.scales[to] = (uint16_t)(__float_as_uint(scale) >> 16);
-            }
-            advance(k, r, ROWS, per_token);
+            if (l == 0) a.c.scales[to] = (uint16_t)(__float_as_uint(scale) >> 16);
         }
     }
 }
@@ -400,7 +399,7 @@ extern "C" jsm_status jsm_kv_append_q8(void* d_pool, void* d_scales, int n_pages
     a.T = T;
     a.table = reinterpret_cast<const float2*>(d_rope_table);
     a.table_len = table_len; a.rot = rot_dim; a.adjacent = layout == JSM_ROPE_ADJACENT;
-    const bool pieces = !((reinterpret_cast<uintptr_t>(d_k) | reinterpret_cast<uintptr_t>(d_v)) & 15) && kv_row_stride % 8 == 0;
+    const bool pieces = !((reinterpret_cast<uintptr_t>(d_k) | reinterpret_cast<uintptr_t>(d_v)) & 15) && kv_row_stride % 8 == 0 && kv_row_stride <= INT32_MAX / (2 * PLACES);
     const int lanes = D <= 64 ? 4 : D <= 128 ? 8 : 16, n = tokens_per_block(T, Hkv, lanes);
     const cudaStream_t st = as_stream(stream);
     const cudaError_t e = !pieces      ? launch_chained(kv_append_q8_kernel, dim3(T), dim3(256), 0, st, a)

@@ -74,6 +74,21 @@ def test_numbers_and_scales_to_the_bit(new, ctx, Hkv, D, rot, layout, aligned):
     assert torch.equal(c.scales.view(torch.int16), scales_before.view(torch.int16))
 
 
+def test_rows_far_apart():
+    """Pitches whose products with a block's tokens pass 32 bits."""
+    c, pitch = Cache([3], [70], 2, 64, 8, rows=1).to_device(), (1 << 26) + 64
+    x = torch.randn(4, 256, device="cuda").bfloat16()
+    far = torch.empty(3 * pitch + 256, dtype=torch.bfloat16, device="cuda").as_strided((4, 256), (pitch, 1))
+    far.copy_(x)
+    got = []
+    for rows in (x, far):
+        pool, scales = c.pool.clone(), c.scales.clone()
+        jb.kv_append_q8(pool, scales, c.table, rows[:, :128], rows[:, 128:], c.starts, c.lens, 2, 64, rope=table(64, 80), rot_dim=64)
+        got.append((pool, scales.view(torch.int16)))
+    jb.check_device_errors()
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]) and not torch.equal(got[0][0], c.pool)
+
+
 def test_rows_that_are_not_numbers_and_the_smallest():
     D, Hkv = 128, 2
     c = Cache([8], [8], Hkv, D, 8).to_device()
