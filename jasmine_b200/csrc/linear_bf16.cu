@@ -86,6 +86,21 @@ jsm_status make_tmap_u8_lines(CUtensorMap* map, const void* base, uint64_t lines
     return JSM_OK;
 }
 
+// [lines, 128] bytes in boxes of 64 bytes of box_lines lines, the 16-byte pieces of a line's half exchanged by (line / 2) % 4
+jsm_status make_tmap_u8_halves(CUtensorMap* map, const void* base, uint64_t lines, uint32_t box_lines) {
+    encode_tiled_fn enc = get_encode();
+    if (!enc) JSM_FAIL(JSM_CUDA, "cuTensorMapEncodeTiled is not available (no CUDA driver)");
+    if (reinterpret_cast<uintptr_t>(base) & 15) JSM_FAIL(JSM_INVALID_ARG, "TMA operand must be 16-byte aligned");
+    cuuint64_t dims[2] = {128, lines};
+    cuuint64_t strides[1] = {128};
+    cuuint32_t box[2] = {64, box_lines};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) JSM_FAIL(JSM_CUDA, "cuTensorMapEncodeTiled failed with %d (%llu lines)", (int)r, (unsigned long long)lines);
+    return JSM_OK;
+}
+
 jsm_status make_tmap_u8_3d(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t s1, uint64_t s2, uint32_t b0, uint32_t b1, uint32_t b2,
                            bool swizzle) {
     encode_tiled_fn enc = get_encode();

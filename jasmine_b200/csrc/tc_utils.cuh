@@ -227,6 +227,7 @@ jsm_status make_tmap_bf16_3d(CUtensorMap* map, const void* base, uint64_t d0, ui
 // int8 memory as lines of 128 bytes, box = box_lines lines, 128-byte swizzle
 jsm_status make_tmap_u8_lines(CUtensorMap* map, const void* base, uint64_t lines, uint32_t box_lines);
 // bytes [d2][d1][d0] with pitches s1, s2 in bytes, 128-byte swizzle (boxes 128 bytes wide) or none
+jsm_status make_tmap_u8_halves(CUtensorMap* map, const void* base, uint64_t lines, uint32_t box_lines);
 jsm_status make_tmap_u8_3d(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t s1, uint64_t s2, uint32_t b0, uint32_t b1, uint32_t b2,
                            bool swizzle);
 // device error word shared by the tensor-core kernels (one per device)

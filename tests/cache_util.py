@@ -75,10 +75,10 @@ class Cache:
     def queries(self, Hq, scale=1.0):
         return (torch.randn(self.T, Hq * self.D, generator=self.g) * scale).bfloat16()
 
-    def attend(self, q, window=0, scale=None, **kw):
+    def attend(self, q, window=0, scale=None, bounds=None, **kw):
         Hq = q.shape[1] // self.D
-        return jb.attn_chunk(q, self.pool, self.table, self.starts, self.lens, Hq, self.Hkv, self.D, max(self.new), max(self.ctx), scales=self.scales, window=window,
-                             scale=scale, **kw)
+        return jb.attn_chunk(q, self.pool, self.table, self.starts, self.lens, Hq, self.Hkv, self.D, *(bounds or (max(self.new), max(self.ctx))), scales=self.scales,
+                             window=window, scale=scale, **kw)
 
     def reference(self, q, window=0, scale=None):
         """(outputs, sum of weight times magnitude of the values) [T, Hq * D] in 64 bits; rows of no sequence are NaN."""

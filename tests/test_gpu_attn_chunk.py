@@ -84,6 +84,49 @@ def test_unseen_keys_have_no_part(new, ctx, window, bits, bad):
     check_attention(torch.where(fine, got, 0.0), torch.where(fine, want, 0.0), torch.where(fine, mag, 0.0))
 
 
+# Many tiles of queries and long contexts (by the bounds of the call): 8-bit caches are walked by pairs of CTAs.
+PAIRS = [
+    ([100], [500], 256, 32, 0, 6000),
+    ([100], [100], 256, 32, 0, 6000),
+    ([70], [2300], 256, 32, 2000, 6000),
+    ([65], [10300], 128, 16, 0, 20000),          # two pairs share the keys
+    ([130], [300], 160, 32, 0, 6000),            # tiles of 125 rows
+    ([90, 0, 20, 1], [400, 5, 20, 300], 128, 16, 0, 6000),
+    ([600], [600], 32, 32, 0, 9000),
+    ([200], [201], 96, 32, 0, 6000),
+]
+
+
+@pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("new,ctx,Hq,Hkv,window,most", PAIRS)
+def test_many_tiles_of_long_contexts(new, ctx, Hq, Hkv, window, most, bits):
+    c = Cache(new, ctx, Hkv, 128, bits, seed=sum(ctx), rows=2).to_device()
+    q = c.queries(Hq)
+    out = torch.full((c.T, Hq * 128), 3.0, dtype=torch.bfloat16, device="cuda")
+    got = c.attend(q.cuda(), window, bounds=(max(new), most), out=out)
+    jb.check_device_errors()
+    check_attention(got, *c.reference(q, window))
+    assert bool((out[sum(new):] == 3).all())
+    again = c.attend(q.cuda(), window, bounds=(max(new), most))
+    assert torch.equal(again[:sum(new)], got[:sum(new)])
+
+
+@pytest.mark.parametrize("bits", BITS)
+def test_many_tiles_sharp_scores_and_bad_numbers(bits):
+    c = Cache([100], [400], 32, 128, bits, seed=11)
+    c.values[0][1, 0, 350] = float("nan")       # a value that later queries see
+    c.values[0][0, 1, 399, 5] = float("inf")    # a key that the last query sees alone
+    c.write(0)
+    c.to_device()
+    q = c.queries(256, 6.0)
+    got = c.attend(q.cuda(), 0, 0.3, bounds=(100, 6000)).double().cpu()
+    want, mag = c.reference(q, 0, 0.3)
+    assert torch.equal(got.isfinite(), want.isfinite())
+    fine = want.isfinite()
+    # (scores as in test_sharp_scores)
+    check_attention(torch.where(fine, got, 0.0), torch.where(fine, want, 0.0), torch.where(fine, mag, 0.0) * 1.1)
+
+
 def test_rows_of_no_sequence_and_pitches():
     c = Cache([3, 0, 40, 1], [70, 9, 300, 130], 2, 128, 8, rows=7).to_device()
     q = c.queries(6)
