@@ -9,21 +9,49 @@ jsm_status cache_view_check(const char* who, CacheView& c, void* pool, void* sca
                             const int32_t* context_lens, int n_seqs, int T, int Hkv, int D);
 
 namespace {
-// What runs for a call: sequences of up to few_rows rows of queries per kv head take chunk_few.cu, the others (if there can be any) the other kernel.
+// What runs for a call: chunk_few.cu for sequences of up to few_tokens tokens, the other kernel for the others, if there can be any.
 struct Plan {
-    int few_rows;
+    int few_tokens;
     bool many;
     FewPlan few;
     size_t bytes;
 };
+// Up to 64 rows: groups of 16 rows in the kernel of few read the cache once each, the other kernel once for all of them, with tiles of 128 rows that are mostly empty and a start of its own.
+// What both take (us), as if every sequence were as long as the bounds: a page takes a run 1.3 (8-bit 1.2, heads of 64 0.65) and a further piece 5; a key tile 2 to 2.4, what is around it 6.
+//                                                                              groups   tiles
+//   12 sequences of 2 to 9 tokens in a window of 1024, heads of 64, 8-bit         12.2    23.5
+//   8 tokens of 8192 positions, 32 / 8 heads of 128                               20.1    28.7
+//   the same of 8 sequences of 2000                                               29      51
+//   32 sequences of 16 tokens of 300                                              54      36
+//   64 sequences of 8 tokens of 4096, 8-bit (bf16)                               276 (338) 312 (260)
+//   64 tokens of 4096 positions, 32 / 32 heads                                    41      27.5
+bool groups_win(int n_seqs, int T, int max_new, int max_context, int Hkv, int G, int D, int window, bool q8) {
+    auto seen = [&](int tokens, int unit) {  // pages or key tiles that so many tokens see at most
+        const long long all = (max_context + unit - 1) / unit;
+        return (float)(window > 0 ? std::min(all, ((long long)window + tokens + unit - 3) / unit + 1) : all);
+    };
+    auto parts = [&](int tokens) { return (float)std::min((long long)n_seqs * ((max_new + tokens - 1) / tokens), T / tokens + (long long)n_seqs) * Hkv; };
+    const int per = 16 / G, tile = 2 * (128 / G), sms = sm_count();
+    const float pages = seen(per, JSM_PAGE_SIZE), run = std::max(2.0f, pages * parts(per) / (2 * sms));
+    const float groups = 8.0f + (D == 64 ? 0.65f : q8 ? 1.2f : 1.3f) * run + 5.0f * std::max(0.0f, run / pages - 1.0f);
+    return groups < 18.0f + parts(tile) * (6.0f + (q8 ? 2.4f : 2.0f) * seen(tile, 128)) / sms;
+}
 Plan plan_of(int n_seqs, int T, int max_new, int max_context, int Hkv, int G, int D, int window, bool q8) {
     Plan p;
     const long long most = (long long)max_new * G;
-    p.few_rows = most <= 8 ? 8 : most <= 16 ? 16 : G <= 8 ? 8 : 16;
+    const int rows = most <= 8 ? 8 : most <= 16 || G > 8 ? 16 : 8;
+    if (most > 16 && most <= 64 && G <= 16 && groups_win(n_seqs, T, max_new, max_context, Hkv, G, D, window, q8)) {
+        p.few_tokens = max_new;
+        p.many = false;
+        p.few = chunk_few_plan(n_seqs, T, max_new, max_context, Hkv, G, window, 16, max_new, D, q8);
+        p.bytes = p.few.bytes;
+        return p;
+    }
+    p.few_tokens = rows / G;
     p.many = most > 16;
     // (with one sequence of more rows there is nothing for the kernel of few)
-    if (p.many && ((n_seqs == 1 && T == max_new) || G > p.few_rows)) p.few_rows = 0;
-    p.few = p.few_rows ? chunk_few_plan(n_seqs, max_new, max_context, Hkv, window, p.few_rows, D, q8) : FewPlan{0, false, 0};
+    if (p.many && n_seqs == 1 && T == max_new) p.few_tokens = 0;
+    p.few = p.few_tokens ? chunk_few_plan(n_seqs, T, max_new, max_context, Hkv, G, window, rows, p.few_tokens, D, q8) : FewPlan{};
     p.bytes = p.few.bytes;
     return p;
 }
@@ -70,8 +98,8 @@ extern "C" jsm_status jsm_attn_chunk(const void* d_q, int64_t q_row_stride, cons
     if (p.bytes && (!d_scratch || scratch_bytes < p.bytes || (reinterpret_cast<uintptr_t>(d_scratch) & 15)))
         JSM_FAIL(JSM_INVALID_ARG, "jsm_attn_chunk: %zu bytes of scratch (16-byte aligned), %zu are needed", d_scratch ? scratch_bytes : 0, p.bytes);
     if (p.many) {
-        const jsm_status m = chunk_flash_launch(a, p.few_rows, st);
+        const jsm_status m = chunk_flash_launch(a, p.few_tokens, st);
         if (m != JSM_OK) return m;
     }
-    return p.few_rows ? chunk_few_launch(a, p.few, p.few_rows, d_scratch, st) : JSM_OK;
+    return p.few_tokens ? chunk_few_launch(a, p.few, d_scratch, st) : JSM_OK;
 }

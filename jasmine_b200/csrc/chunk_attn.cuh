@@ -15,18 +15,20 @@ struct ChunkArgs {
     float scale_log2;
 };
 
-// Sequences with a few new tokens only (chunk_few.cu): runs of pages, whether partial results can meet, their bytes.
+// Sequences with a few new tokens only (chunk_few.cu).
 struct FewPlan {
-    int n_runs;
-    bool merge;
+    int rows;    // of queries per kv head and group: 8 or 16
+    int per;     // tokens of a group
+    int tokens;  // of a sequence at most; the others are left to another kernel
+    int n_runs;  // runs of pages
+    bool merge;  // whether partial results can meet
     size_t bytes;
 };
-FewPlan chunk_few_plan(int n_seqs, int max_new, int max_context, int Hkv, int window, int few_rows, int D, bool q8);
-// sequences of up to few_rows (8 or 16) rows of queries per kv head; the others are left to another kernel
-jsm_status chunk_few_launch(const ChunkArgs& a, const FewPlan& f, int few_rows, void* scratch, cudaStream_t st);
+FewPlan chunk_few_plan(int n_seqs, int T, int max_new, int max_context, int Hkv, int G, int window, int rows, int tokens, int D, bool q8);
+jsm_status chunk_few_launch(const ChunkArgs& a, const FewPlan& f, void* scratch, cudaStream_t st);
 
-// sequences of more than few_rows rows
-jsm_status chunk_flash_launch(const ChunkArgs& a, int few_rows, cudaStream_t st);
+// sequences of more than few_tokens tokens
+jsm_status chunk_flash_launch(const ChunkArgs& a, int few_tokens, cudaStream_t st);
 
 #ifdef __CUDACC__
 // lengths of a sequence that the kernels may rely on; false: no new tokens, or lengths that do not fit (an error)

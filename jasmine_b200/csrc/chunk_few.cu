@@ -1,8 +1,8 @@
 // Attention of a few new tokens of each sequence over a paged cache (bf16 or 8-bit): single tokens, drafts being verified.  Up to 16 rows of queries
-// (tokens x query heads of a kv head) share every cached byte, so the kernel is bound by the bytes of the cache.
+// (tokens x query heads of a kv head) share every cached byte, so the kernel is bound by the bytes of the cache; more rows are groups of tokens that read the cache once each.
 //
-// All pages that any (sequence, kv head) sees are one row of work, cut into equal runs, one per CTA: as many CTAs as the chip holds, each with the same number of bytes
-// however ragged the contexts are.  A run holds the end of one (sequence, kv head), perhaps whole ones, and the beginning of another: at most two partial results per
+// All pages that any (sequence, kv head, group) sees are one row of work, cut into equal runs, one per CTA: as many CTAs as the chip holds, each with the same number of bytes
+// however ragged the contexts are.  A run holds the end of one (sequence, kv head, group), perhaps whole ones, and the beginning of another: at most two partial results per
 // CTA, so the scratch does not grow with contexts or sequences.  A producer thread keeps a ring of pages in flight across these borders (TMA boxes in the 128-byte
 // swizzle); four warps have 16 keys of each page:
 //   scores, transposed:   S^T[16 keys x 8 rows] = K[16 x D] . Q^T,  keys as the 16-row operand of mma.m16n8k16, so that no row of it is padding
@@ -47,18 +47,34 @@ struct FewSizes {
     static constexpr int PER_SM = NT == 1 ? (Q8 ? 3 : 2) : 2;         // CTAs that share a multiprocessor
 };
 
-// Pages that the queries of sequence s see, from page0 on; 0 where it has none, or too many rows for this kernel.
-__device__ __forceinline__ int few_pages(const ChunkArgs& a, int few_rows, int s, int& row0, int& n_new, int& ctx, int& page0) {
-    if (!chunk_lengths(a, s, row0, n_new, ctx) || n_new * a.G > few_rows) return 0;
-    page0 = first_key(a.window, ctx - n_new) / JSM_PAGE_SIZE;
-    return (ctx - 1) / JSM_PAGE_SIZE + 1 - page0;
+// The rows of a sequence are taken in groups of `per` tokens, each with the keys that it sees: for this kernel a group is a sequence of its own.
+struct FewSeq {
+    int row0, n_new, ctx;
+};
+// sequence s, if it has new tokens and no more rows than this kernel takes
+__device__ __forceinline__ bool few_sequence(const ChunkArgs& a, const FewPlan& f, int s, FewSeq& q) { return chunk_lengths(a, s, q.row0, q.n_new, q.ctx) && q.n_new <= f.tokens; }
+__device__ __forceinline__ FewSeq few_group(const FewPlan& f, const FewSeq& q, int group) {
+    const int first = group * f.per, n = min(f.per, q.n_new - first);
+    return FewSeq{q.row0 + first, n, q.ctx - q.n_new + first + n};
+}
+// pages that the queries of a group see, from page0 on
+__device__ __forceinline__ int group_pages(const ChunkArgs& a, const FewSeq& q, int& page0) {
+    page0 = first_key(a.window, q.ctx - q.n_new) / JSM_PAGE_SIZE;
+    return (q.ctx - 1) / JSM_PAGE_SIZE + 1 - page0;
+}
+// all groups' of sequence s, for one kv head; 0: not this kernel's
+__device__ __forceinline__ int head_pages(const ChunkArgs& a, const FewPlan& f, int s, FewSeq& q) {
+    int sum = 0, page0;
+    if (s < a.c.n_seqs && few_sequence(a, f, s, q))
+        for (int g = 0; g * f.per < q.n_new; ++g) sum += group_pages(a, few_group(f, q, g), page0);
+    return sum;
 }
 // Pages of a run, of the `all` pages of the call
 __device__ __forceinline__ long long run_length(long long all, int n_runs) { return (all + n_runs - 1) / n_runs; }
 
 template <int D, int NT, bool Q8>
 __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk_few_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ CUtensorMap tmap_scales,
-                                                                                            const __grid_constant__ ChunkArgs a, float* __restrict__ part) {
+                                                                                            const __grid_constant__ ChunkArgs a, const __grid_constant__ FewPlan f, float* __restrict__ part) {
     using Z = FewSizes<D, NT, Q8>;
     constexpr int KS = D / 16;  // steps of 16 components; tiles of 16 components of O^T
     constexpr int few_rows = Z::ROWS;
@@ -66,7 +82,8 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
     uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(cf_dyn) + 1023) & ~uintptr_t(1023));
     const uint32_t stages_u32 = smem_u32(stages);
     __shared__ uint64_t full_bar[Z::STAGES], empty_bar[Z::STAGES];
-    __shared__ int abort_flag, sh_seq, sh_head, sh_page, sh_pages;
+    __shared__ int abort_flag, sh_seq, sh_head, sh_group, sh_page, sh_pages;
+    __shared__ FewSeq sh_q;
     __shared__ float sm_m[CF_WARPS][few_rows], sm_l[CF_WARPS][few_rows];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == CF_WARPS * 32) {
@@ -80,9 +97,9 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
     chain_wait();
     chain_trigger();  // (now: what the merge reads before its own wait was there before this kernel)
     if (warp == 0) {  // where this CTA's run begins
-        int row0, n_new, ctx, page0;
         long long all = 0;
-        for (int s0 = 0; s0 < a.c.n_seqs; s0 += 32) all += s0 + lane < a.c.n_seqs ? few_pages(a, few_rows, s0 + lane, row0, n_new, ctx, page0) : 0;
+        FewSeq q;
+        for (int s0 = 0; s0 < a.c.n_seqs; s0 += 32) all += head_pages(a, f, s0 + lane, q);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
         all *= a.c.Hkv;
@@ -90,7 +107,7 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
         if (lane == 0) sh_pages = (int)max(0ll, min(len, all - begin));
         long long before = 0;
         for (int s0 = 0; s0 < a.c.n_seqs && begin < all; s0 += 32) {
-            const int n = s0 + lane < a.c.n_seqs ? few_pages(a, few_rows, s0 + lane, row0, n_new, ctx, page0) : 0;
+            const int n = head_pages(a, f, s0 + lane, q);
             long long sum = (long long)n * a.c.Hkv;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -103,7 +120,14 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
                     const long long in = begin - (before + sum - (long long)n * a.c.Hkv);
                     sh_seq = s0 + lane;
                     sh_head = (int)(in / n);
-                    sh_page = (int)(in % n);
+                    int at = (int)(in % n), group = 0, page0;
+                    for (int k = group_pages(a, few_group(f, q, 0), page0); at >= k; k = group_pages(a, few_group(f, q, group), page0)) {
+                        at -= k;
+                        ++group;
+                    }
+                    sh_group = group;
+                    sh_page = at;
+                    sh_q = q;
                 }
                 break;
             }
@@ -111,17 +135,23 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
         }
     }
     __syncthreads();
-    int left = sh_pages, seq = sh_seq, hk = sh_head, page = sh_page;
+    int left = sh_pages, seq = sh_seq, hk = sh_head, group = sh_group, page = sh_page;
     if (left == 0) return;
-    int row0, n_new, ctx, page0;
-    int n_pages = few_pages(a, few_rows, seq, row0, n_new, ctx, page0);
-    // the next (sequence, kv head) of the run
+    FewSeq whole_seq = sh_q, q = few_group(f, whole_seq, group);
+    int page0, n_pages = group_pages(a, q, page0);
+    // the next (sequence, kv head, group) of the run
     auto next = [&] {
         page = 0;
-        if (++hk < a.c.Hkv) return;
-        hk = 0;
-        do n_pages = few_pages(a, few_rows, ++seq, row0, n_new, ctx, page0);
-        while (n_pages == 0);
+        if (++group * f.per >= whole_seq.n_new) {
+            group = 0;
+            if (++hk == a.c.Hkv) {
+                hk = 0;
+                do ++seq;
+                while (!few_sequence(a, f, seq, whole_seq));
+            }
+        }
+        q = few_group(f, whole_seq, group);
+        n_pages = group_pages(a, q, page0);
     };
 
     if (warp == CF_WARPS) {
@@ -175,8 +205,8 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
     float* sm_o = reinterpret_cast<float*>(stages + Z::STAGES * Z::STAGE);  // [warp][row][component]
     bool ok = true;
     int s = 0, round = 0;
-    for (bool first_piece = true;; first_piece = false) {  // a (sequence, kv head), or the run's piece of it
-        const int rows = n_new * a.G, lo = first_key(a.window, ctx - n_new);  // no row sees a key before it
+    for (bool first_piece = true;; first_piece = false) {  // a (sequence, kv head, group), or the run's piece of it
+        const int row0 = q.row0, n_new = q.n_new, ctx = q.ctx, rows = n_new * a.G, lo = first_key(a.window, ctx - n_new);  // no row sees a key before it
         const int here = min(left, n_pages - page);
         const bool whole = here == n_pages;  // all of it: the result is final
         float m[NT][2], l[NT][2];  // rows (lane % 4) * 2 and + 1 of each tile
@@ -431,20 +461,21 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
     }
 }
 
-// The pieces of a (row, head) under their largest reference, in the order of the runs.  A block per row (of the sequences of few rows) and head: each of four warps takes
-// eight pieces of every 32, all their loads in flight, with a reference of its own; the warps meet in shared memory.  What depends on the lengths alone is worked out
-// while the runs are still under way.
+// The pieces of a row under their largest reference, in the order of the runs.  Few groups (JOIN): a block per (sequence, kv head, group) and row, each of four warps takes eight pieces
+// of every 32, all their loads in flight, and they meet in shared memory.  Many groups, of a few pieces each: a warp per row (32 sequences of 8 tokens of 300, 32 heads: 32 us with the
+// runs, a block per row 46).  What depends on the lengths alone is worked out while the runs are still under way.
 constexpr int CM_RUNS = 8;
-template <int D, bool Q8>
-__global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant__ ChunkArgs a, int few_rows, int n_runs, const float* part) {
-    constexpr int N = D / 32;
+template <int D, bool Q8, bool JOIN>
+__global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant__ ChunkArgs a, const __grid_constant__ FewPlan f, const float* part) {
+    constexpr int N = D / 32, WARPS = JOIN ? 4 : 1;  // warps of a row
     __shared__ float sm_m[4], sm_l[4], sm_o[4][D];
     __shared__ long long sm_before[4], sm_all[4];
-    const int tokens = gridDim.x / a.c.n_seqs, s = blockIdx.x / tokens, i = blockIdx.x % tokens, head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int row0 = 0, n_new = 0, ctx = 0, page0 = 0;
+    const int most = gridDim.x / (a.c.n_seqs * a.c.Hkv), group = blockIdx.x % most, hk = blockIdx.x / most % a.c.Hkv, s = blockIdx.x / most / a.c.Hkv;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = JOIN ? blockIdx.y : blockIdx.y * 4 + warp, few_rows = f.rows;
     long long before = 0, all = 0;
+    FewSeq q = {0, 0, 0};
     for (int k = threadIdx.x; k < a.c.n_seqs; k += 128) {
-        const int n = few_pages(a, few_rows, k, row0, n_new, ctx, page0);
+        const int n = head_pages(a, f, k, q);
         all += n;
         if (k < s) before += n;
     }
@@ -457,12 +488,19 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant_
         sm_all[warp] = all;
         sm_before[warp] = before;
     }
+    int n_pages = 0, head_all = 0, groups_before = 0;
+    if (few_sequence(a, f, s, q))
+        for (int g = 0, page0; g * f.per < q.n_new; ++g) {
+            const int k = group_pages(a, few_group(f, q, g), page0);
+            if (g < group) groups_before += k;
+            if (g == group) n_pages = k;
+            head_all += k;
+        }
     __syncthreads();
-    const int n_pages = few_pages(a, few_rows, s, row0, n_new, ctx, page0);
-    const int t = row0 + i, hk = head / a.G, r = i * a.G + head % a.G;
-    const long long len = max(1ll, run_length((sm_all[0] + sm_all[1] + sm_all[2] + sm_all[3]) * a.c.Hkv, n_runs));
-    const long long from = (sm_before[0] + sm_before[1] + sm_before[2] + sm_before[3]) * a.c.Hkv + (long long)hk * n_pages;  // its first page in the row of work
-    const int c_first = (int)(from / len), n = n_pages > 0 && i < n_new ? (int)((from + n_pages - 1) / len) - c_first + 1 : 0;
+    const long long len = max(1ll, run_length((sm_all[0] + sm_all[1] + sm_all[2] + sm_all[3]) * a.c.Hkv, f.n_runs));
+    // the group's first page in the row of work
+    const long long from = (sm_before[0] + sm_before[1] + sm_before[2] + sm_before[3]) * a.c.Hkv + (long long)hk * head_all + groups_before;
+    const int c_first = (int)(from / len), n = n_pages > 0 ? (int)((from + n_pages - 1) / len) - c_first + 1 : 0;
     // the first piece of a run of its own, but for the first run, whose last piece it is unless it begins there
     const bool begins = from % len == 0;
     const int step = 2 * few_rows * (D + 2);
@@ -471,10 +509,12 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant_
     chain_wait();
     chain_trigger();
     if (n <= 1) return;
+    q = few_group(f, q, group);
+    if (r >= q.n_new * a.G) return;
     float m = CF_NONE, l = 0.0f, acc[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.0f;
-    for (int c0 = warp * CM_RUNS; c0 < n; c0 += 4 * CM_RUNS) {
+    for (int c0 = JOIN ? warp * CM_RUNS : 0; c0 < n; c0 += WARPS * CM_RUNS) {
         float v[CM_RUNS][N];
         float2 ml = make_float2(CF_NONE, 0.0f);
         if (lane < CM_RUNS && c0 + lane < n) ml = *reinterpret_cast<const float2*>(piece(c0 + lane) + D);
@@ -485,47 +525,51 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant_
             for (int i = 0; i < N; i += 2) *reinterpret_cast<float2*>(&v[c][i]) = *reinterpret_cast<const float2*>(x + i);
         }
         const float mn = fmaxf(m, warp_max(ml.x)), corr = fast_ex2(m - mn);
-        const float f = lane < CM_RUNS && c0 + lane < n ? fast_ex2(ml.x - mn) : 0.0f;
+        const float w0 = lane < CM_RUNS && c0 + lane < n ? fast_ex2(ml.x - mn) : 0.0f;
         m = mn;
-        l = fmaf(l, corr, warp_sum(f * ml.y));
+        l = fmaf(l, corr, warp_sum(w0 * ml.y));
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] *= corr;
 #pragma unroll
         for (int c = 0; c < CM_RUNS; ++c) {
-            const float w = __shfl_sync(0xffffffffu, f, c);
+            const float w = __shfl_sync(0xffffffffu, w0, c);
             if (c0 + c < n)
 #pragma unroll
                 for (int i = 0; i < N; ++i) acc[i] = fmaf(w, v[c][i], acc[i]);
         }
     }
-    if (lane == 0) {
-        sm_m[warp] = m;
-        sm_l[warp] = l;
-    }
+    if constexpr (JOIN) {
+        if (lane == 0) {
+            sm_m[warp] = m;
+            sm_l[warp] = l;
+        }
 #pragma unroll
-    for (int i = 0; i < N; ++i) sm_o[warp][lane * N + i] = acc[i];
-    __syncthreads();
-    if (warp != 0) return;
-    float M = CF_NONE, L = 0.0f;
+        for (int i = 0; i < N; ++i) sm_o[warp][lane * N + i] = acc[i];
+        __syncthreads();
+        if (warp != 0) return;
+        m = CF_NONE;
+        l = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_m[w]);
+        for (int w = 0; w < 4; ++w) m = fmaxf(m, sm_m[w]);
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+        for (int i = 0; i < N; ++i) acc[i] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const float f = fast_ex2(sm_m[w] - M);
-        L += f * sm_l[w];
+        for (int w = 0; w < 4; ++w) {
+            const float x = fast_ex2(sm_m[w] - m);
+            l += x * sm_l[w];
 #pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] += f * sm_o[w][lane * N + i];
+            for (int i = 0; i < N; ++i) acc[i] += x * sm_o[w][lane * N + i];
+        }
     }
     bool fine = true;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        acc[i] /= L;
+        acc[i] /= l;
         fine = fine && fabsf(acc[i]) <= 3.402823466e38f;
     }
+    const int t = q.row0 + r / a.G, head = hk * a.G + r % a.G;
     if (!__all_sync(0xffffffffu, fine)) {
-        attend_row<D, Q8>(a, s, t, head, ctx - n_new + i);
+        attend_row<D, Q8>(a, s, t, head, q.ctx - q.n_new + r / a.G);
         return;
     }
     __nv_bfloat16* dst = a.out + t * a.out_rs + (long long)head * D + lane * N;
@@ -535,14 +579,18 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant_
 
 // As many runs as the chip holds CTAs (8-bit pages, heads of 128: three per multiprocessor with three stages each 80.7 us for 64 contexts of 512 to 8192, four with two 87.0), of
 // two pages at least (one token over 4096 positions: 7.8 us, with runs of one page 8.1).
-FewPlan chunk_few_plan(int n_seqs, int max_new, int max_context, int Hkv, int window, int few_rows, int D, bool q8) {
+FewPlan chunk_few_plan(int n_seqs, int T, int max_new, int max_context, int Hkv, int G, int window, int rows, int tokens, int D, bool q8) {
     long long pages = (max_context + JSM_PAGE_SIZE - 1) / JSM_PAGE_SIZE;
     if (window > 0) pages = std::min(pages, ((long long)window + max_new + JSM_PAGE_SIZE - 3) / JSM_PAGE_SIZE + 1);
     FewPlan f;
-    const int per_sm = few_rows == 8 ? (q8 ? 3 : 2) : 2;
-    f.n_runs = (int)std::min((long long)per_sm * sm_count(), (pages * n_seqs * Hkv + 1) / 2);
+    f.rows = rows;
+    f.per = rows / G;
+    f.tokens = std::min(tokens, max_new);
+    const int per_sm = rows == 8 ? (q8 ? 3 : 2) : 2;
+    const long long groups = std::min((long long)n_seqs * ((f.tokens + f.per - 1) / f.per), T / f.per + (long long)n_seqs);
+    f.n_runs = (int)std::min((long long)per_sm * sm_count(), (pages * groups * Hkv + 1) / 2);
     f.merge = pages > 1;
-    f.bytes = f.merge ? (size_t)f.n_runs * 2 * few_rows * (D + 2) * sizeof(float) : 0;
+    f.bytes = f.merge ? (size_t)f.n_runs * 2 * rows * (D + 2) * sizeof(float) : 0;
     return f;
 }
 
@@ -558,23 +606,27 @@ static jsm_status few_go(const ChunkArgs& a, const FewPlan& f, float* part, cuda
     if (s != JSM_OK) return s;
     static DeviceOnce once;
     JSM_CUDA_CHECK(allow_shared(once, chunk_few_kernel<D, NT, Q8>, Z::SMEM));
-    JSM_CUDA_CHECK(launch_chained(chunk_few_kernel<D, NT, Q8>, dim3(f.n_runs), dim3(CF_THREADS), (size_t)Z::SMEM, st, map, Q8 ? scales : map, a, part));
+    JSM_CUDA_CHECK(launch_chained(chunk_few_kernel<D, NT, Q8>, dim3(f.n_runs), dim3(CF_THREADS), (size_t)Z::SMEM, st, map, Q8 ? scales : map, a, f, part));
     JSM_LAUNCH_CHECK();
     if (f.merge) {
-        JSM_CUDA_CHECK(launch_chained(chunk_merge_kernel<D, Q8>, dim3((unsigned)a.c.n_seqs * std::min(a.max_new, Z::ROWS / a.G), a.Hq), dim3(128), 0, st, a, Z::ROWS, f.n_runs, (const float*)part));
+        const unsigned groups = (unsigned)a.c.n_seqs * a.c.Hkv * ((f.tokens + f.per - 1) / f.per), rows = (unsigned)std::min(f.per, f.tokens) * a.G;
+        const bool join = groups * rows <= 8u * sm_count();
+        const cudaError_t e = join ? launch_chained(chunk_merge_kernel<D, Q8, true>, dim3(groups, rows), dim3(128), 0, st, a, f, (const float*)part)
+                                   : launch_chained(chunk_merge_kernel<D, Q8, false>, dim3(groups, (rows + 3) / 4), dim3(128), 0, st, a, f, (const float*)part);
+        JSM_CUDA_CHECK(e);
         JSM_LAUNCH_CHECK();
     }
     return JSM_OK;
 }
 
-jsm_status chunk_few_launch(const ChunkArgs& a, const FewPlan& f, int few_rows, void* scratch, cudaStream_t st) {
+jsm_status chunk_few_launch(const ChunkArgs& a, const FewPlan& f, void* scratch, cudaStream_t st) {
     float* part = static_cast<float*>(scratch);
     if (a.c.D == 64) {
-        if (a.c.scales) return few_rows == 8 ? few_go<64, 1, true>(a, f, part, st) : few_go<64, 2, true>(a, f, part, st);
-        return few_rows == 8 ? few_go<64, 1, false>(a, f, part, st) : few_go<64, 2, false>(a, f, part, st);
+        if (a.c.scales) return f.rows == 8 ? few_go<64, 1, true>(a, f, part, st) : few_go<64, 2, true>(a, f, part, st);
+        return f.rows == 8 ? few_go<64, 1, false>(a, f, part, st) : few_go<64, 2, false>(a, f, part, st);
     }
-    if (a.c.scales) return few_rows == 8 ? few_go<128, 1, true>(a, f, part, st) : few_go<128, 2, true>(a, f, part, st);
-    return few_rows == 8 ? few_go<128, 1, false>(a, f, part, st) : few_go<128, 2, false>(a, f, part, st);
+    if (a.c.scales) return f.rows == 8 ? few_go<128, 1, true>(a, f, part, st) : few_go<128, 2, true>(a, f, part, st);
+    return f.rows == 8 ? few_go<128, 1, false>(a, f, part, st) : few_go<128, 2, false>(a, f, part, st);
 }
 
 }  // namespace jsm

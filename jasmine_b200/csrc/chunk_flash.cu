@@ -54,7 +54,7 @@ struct FlashSizes {
 
 struct FlashArgs {
     ChunkArgs a;
-    int few_rows;      // sequences of so many rows are another kernel's
+    int few_tokens;    // sequences of so many tokens are another kernel's
     int tile_tokens;   // tokens of a query tile
     int tiles;         // query tiles of a unit: a CTA's two, or a pair's four
     int cluster;       // units of a cluster
@@ -135,7 +135,7 @@ __device__ __forceinline__ Place find_tile(const FlashArgs& f, long long cluster
     for (int s0 = 0; s0 < a.c.n_seqs; s0 += 32) {
         const int s = s0 + lane;
         int n = 0, share = 1, row0 = 0, n_new = 0, ctx = 0;
-        if (s < a.c.n_seqs && chunk_lengths(a, s, row0, n_new, ctx) && n_new * a.G > f.few_rows) {
+        if (s < a.c.n_seqs && chunk_lengths(a, s, row0, n_new, ctx) && n_new > f.few_tokens) {
             n = (n_new + tokens - 1) / tokens;
             const int keys = a.window > 0 ? min(ctx, a.window + tokens) : ctx;
             while (share < f.cluster && keys > f.walk_tiles * share * CK_BN) share *= 2;
@@ -862,10 +862,10 @@ static FlashPlan flash_plan(const ChunkArgs& a) {
 }
 
 template <int D, bool Q8, bool PAIR>
-static jsm_status flash_launch(const ChunkArgs& a, const FlashPlan& p, int few_rows, cudaStream_t st) {
+static jsm_status flash_launch(const ChunkArgs& a, const FlashPlan& p, int few_tokens, cudaStream_t st) {
     using Z = FlashSizes<D, Q8, PAIR>;
     constexpr int CTAS = PAIR ? 2 : 1;
-    const FlashArgs f{a, few_rows, CK_BM / a.G, 2 * CTAS, p.cluster, p.walk_tiles, (65536u + a.G - 1) / a.G};
+    const FlashArgs f{a, few_tokens, CK_BM / a.G, 2 * CTAS, p.cluster, p.walk_tiles, (65536u + a.G - 1) / a.G};
     if (p.units * f.cluster * CTAS > INT32_MAX) JSM_FAIL(JSM_UNSUPPORTED, "jsm_attn_chunk: %lld tiles of queries", p.units);
     static DeviceOnce once;
     const cudaError_t allowed = allow_shared(once, chunk_flash_kernel<D, Q8, PAIR>, (int)Z::SMEM);
@@ -899,18 +899,18 @@ static jsm_status flash_launch(const ChunkArgs& a, const FlashPlan& p, int few_r
 }
 
 template <int D, bool Q8>
-static jsm_status flash_launch(const ChunkArgs& a, int few_rows, cudaStream_t st) {
+static jsm_status flash_launch(const ChunkArgs& a, int few_tokens, cudaStream_t st) {
     const FlashPlan one = flash_plan<D, Q8, false>(a);
     if constexpr (Q8 && D == 128) {
         const FlashPlan two = flash_plan<D, Q8, true>(a);
-        if (two.cost < one.cost) return flash_launch<D, Q8, true>(a, two, few_rows, st);
+        if (two.cost < one.cost) return flash_launch<D, Q8, true>(a, two, few_tokens, st);
     }
-    return flash_launch<D, Q8, false>(a, one, few_rows, st);
+    return flash_launch<D, Q8, false>(a, one, few_tokens, st);
 }
 
-jsm_status chunk_flash_launch(const ChunkArgs& a, int few_rows, cudaStream_t st) {
-    if (a.c.D == 64) return a.c.scales ? flash_launch<64, true>(a, few_rows, st) : flash_launch<64, false>(a, few_rows, st);
-    return a.c.scales ? flash_launch<128, true>(a, few_rows, st) : flash_launch<128, false>(a, few_rows, st);
+jsm_status chunk_flash_launch(const ChunkArgs& a, int few_tokens, cudaStream_t st) {
+    if (a.c.D == 64) return a.c.scales ? flash_launch<64, true>(a, few_tokens, st) : flash_launch<64, false>(a, few_tokens, st);
+    return a.c.scales ? flash_launch<128, true>(a, few_tokens, st) : flash_launch<128, false>(a, few_tokens, st);
 }
 
 }  // namespace jsm

@@ -38,6 +38,15 @@ CASES = [
     ([2], [3], 100, 1, 128, 0),
     ([6], [100], 128, 1, 64, 0),
     ([50], [80], 65, 1, 128, 0),
+    # up to 64 rows: groups of 16
+    ([9, 3, 0, 16, 1], [700, 3, 9, 300, 129], 8, 2, 128, 0),
+    ([9, 5, 12], [400, 260, 130], 8, 2, 128, 100),
+    ([20, 2], [500, 70], 6, 2, 64, 0),
+    ([64], [1000], 2, 2, 64, 33),
+    ([4], [260], 16, 1, 128, 0),
+    ([33, 1], [33, 2000], 1, 1, 128, 0),
+    ([6, 6, 2, 6], [6, 70, 200, 64], 40, 4, 64, 0),
+    ([7] * 45, list(range(7, 52)), 8, 2, 128, 0),
 ]
 
 
@@ -64,7 +73,7 @@ def test_sharp_scores(new, ctx, Hq, bits):
 
 
 @pytest.mark.parametrize("bits", BITS)
-@pytest.mark.parametrize("new,ctx,window", [([1, 3], [200, 260], 0), ([100], [300], 0), ([100, 1], [300, 200], 70), ([4], [150], 20)])
+@pytest.mark.parametrize("new,ctx,window", [([1, 3], [200, 260], 0), ([100], [300], 0), ([100, 1], [300, 200], 70), ([4], [150], 20), ([9, 5], [200, 260], 0), ([16], [150], 20)])
 @pytest.mark.parametrize("bad", (float("nan"), float("inf"), -float("inf")))
 def test_unseen_keys_have_no_part(new, ctx, window, bits, bad):
     """Keys and values that are not numbers, at places that some queries see and others do not."""
@@ -153,7 +162,7 @@ def test_pages_behind_the_window_are_not_read(bits):
 
 
 @pytest.mark.parametrize("bits", BITS)
-@pytest.mark.parametrize("new,ctx", [([1] * 5, [3000, 40, 900, 64, 1]), ([150, 20], [2000, 90])])
+@pytest.mark.parametrize("new,ctx", [([1] * 5, [3000, 40, 900, 64, 1]), ([150, 20], [2000, 90]), ([5, 16], [2000, 90])])
 def test_the_same_bits_again_from_a_graph_and_on_another_stream(new, ctx, bits):
     c = Cache(new, ctx, 2, 128, bits, seed=4).to_device()
     q = c.queries(8).cuda()
