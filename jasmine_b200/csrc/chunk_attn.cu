@@ -25,16 +25,23 @@ struct Plan {
 //   32 sequences of 16 tokens of 300                                              54      36
 //   64 sequences of 8 tokens of 4096, 8-bit (bf16)                               276 (338) 312 (260)
 //   64 tokens of 4096 positions, 32 / 32 heads                                    41      27.5
+float seen(int max_context, int window, int tokens, int unit) {  // pages or key tiles that so many tokens see at most
+    const long long all = (max_context + unit - 1) / unit;
+    return (float)(window > 0 ? std::min(all, ((long long)window + tokens + unit - 3) / unit + 1) : all);
+}
 bool groups_win(int n_seqs, int T, int max_new, int max_context, int Hkv, int G, int D, int window, bool q8) {
-    auto seen = [&](int tokens, int unit) {  // pages or key tiles that so many tokens see at most
-        const long long all = (max_context + unit - 1) / unit;
-        return (float)(window > 0 ? std::min(all, ((long long)window + tokens + unit - 3) / unit + 1) : all);
-    };
     auto parts = [&](int tokens) { return (float)std::min((long long)n_seqs * ((max_new + tokens - 1) / tokens), T / tokens + (long long)n_seqs) * Hkv; };
     const int per = 16 / G, tile = 2 * (128 / G), sms = sm_count();
-    const float pages = seen(per, JSM_PAGE_SIZE), run = std::max(2.0f, pages * parts(per) / (2 * sms));
+    const float pages = seen(max_context, window, per, JSM_PAGE_SIZE), run = std::max(2.0f, pages * parts(per) / (2 * sms));
     const float groups = 8.0f + (D == 64 ? 0.65f : q8 ? 1.2f : 1.3f) * run + 5.0f * std::max(0.0f, run / pages - 1.0f);
-    return groups < 18.0f + parts(tile) * (6.0f + (q8 ? 2.4f : 2.0f) * seen(tile, 128)) / sms;
+    return groups < 18.0f + parts(tile) * (6.0f + (q8 ? 2.4f : 2.0f) * seen(max_context, window, tile, 128)) / sms;
+}
+// Sequences of few rows among others: tiles too where all of them together, contexts half of the bound on average, take the chip no longer than the longest sequence does: they run beside it,
+// without two more launches behind it (16 sequences of 1 to 256 tokens: 58 us, with the kernel of few 68; 8 in a window of 512: 24, 34).
+bool few_beside(int n_seqs, int T, int max_context, int Hkv, int G, int window, bool q8) {
+    const int tile = 2 * (128 / G);
+    const float key = q8 ? 2.4f : 2.0f, tiles = seen(max_context, window, tile, 128);
+    return (T / tile + (float)n_seqs) * Hkv * (6.0f + key * 0.5f * tiles) <= sm_count() * (6.0f + key * tiles);
 }
 Plan plan_of(int n_seqs, int T, int max_new, int max_context, int Hkv, int G, int D, int window, bool q8) {
     Plan p;
@@ -49,8 +56,8 @@ Plan plan_of(int n_seqs, int T, int max_new, int max_context, int Hkv, int G, in
     }
     p.few_tokens = rows / G;
     p.many = most > 16;
-    // (with one sequence of more rows there is nothing for the kernel of few)
-    if (p.many && n_seqs == 1 && T == max_new) p.few_tokens = 0;
+    // (sequences that are all as long as they can be: none has few rows; one that has all the same has tiles)
+    if (p.many && ((long long)n_seqs * max_new == T || few_beside(n_seqs, T, max_context, Hkv, G, window, q8))) p.few_tokens = 0;
     p.few = p.few_tokens ? chunk_few_plan(n_seqs, T, max_new, max_context, Hkv, G, window, rows, p.few_tokens, D, q8) : FewPlan{};
     p.bytes = p.few.bytes;
     return p;

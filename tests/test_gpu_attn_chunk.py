@@ -47,6 +47,10 @@ CASES = [
     ([33, 1], [33, 2000], 1, 1, 128, 0),
     ([6, 6, 2, 6], [6, 70, 200, 64], 40, 4, 64, 0),
     ([7] * 45, list(range(7, 52)), 8, 2, 128, 0),
+    # many sequences, both kinds: two kernels
+    ([1, 2, 40, 0, 1, 3, 1, 30, 1, 1, 2, 1, 1, 4], [100, 70, 60, 9, 300, 3, 1, 30, 65, 64, 130, 200, 7, 90], 64, 32, 128, 0),
+    ([1, 20, 3, 0, 1, 1, 9, 1, 2, 1, 1, 17], [200, 70, 60, 9, 300, 3, 10, 130, 65, 64, 130, 200], 40, 40, 64, 50),
+    ([1, 18, 1, 2, 1, 5, 1, 1, 17, 1], [100, 18, 60, 9, 300, 7, 10, 130, 65, 64], 192, 16, 128, 0),
 ]
 
 

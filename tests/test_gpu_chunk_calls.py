@@ -40,7 +40,7 @@ def test_both_ways_into_the_library(monkeypatch):
         lambda: [x[:44] for x in read(dtype=torch.float32)], lambda: [x[:44] for x in read()], lambda: read(dtype=torch.float16),
         lambda: read(scales=None), lambda: read(k_out=torch.zeros(c.T, 256, device="cuda"), v_out=torch.zeros(c.T, 256, device="cuda").bfloat16()),
         lambda: c.attend(q)[:44], lambda: c.attend(q, 50, 0.2)[:44], lambda: c.attend(q, scratch=torch.empty(1 << 24, dtype=torch.uint8, device="cuda"))[:44],
-        lambda: c.attend(q, scratch=torch.empty(16, dtype=torch.uint8, device="cuda")), lambda: c.attend(q, -1), lambda: c.attend(q, 0, 0.0),
+        lambda: c.attend(q, bounds=(4, 300), scratch=torch.empty(16, dtype=torch.uint8, device="cuda")), lambda: c.attend(q, -1), lambda: c.attend(q, 0, 0.0),
         lambda: c.attend(q.float()), lambda: c.attend(q, out=torch.empty_like(q)[:5]),
         lambda: jb.attn_chunk(q, c.pool, c.table, c.starts, short, 8, 2, 128, 40, 300, scales=c.scales),
         # memory of the host is refused before anything runs
