@@ -29,18 +29,19 @@ __device__ __forceinline__ void cache_error(int* err, int code) {
     if (err) atomicCAS(err, 0, code);
 }
 
+// of a sequence with new tokens
+__device__ __forceinline__ bool lengths_fit(const CacheView& c, int T, int first_row, int end, int ctx) {
+    if (first_row >= 0 && end <= T && ctx >= end - first_row && (ctx - 1) / JSM_PAGE_SIZE < c.max_pages) return true;
+    cache_error(c.err, CACHE_BAD_LENGTH);
+    return false;
+}
 // new tokens and context of sequence s; false (and an error) where they do not fit the table or one another
 __device__ __forceinline__ bool cache_lengths(const CacheView& c, int s, int T, int& first_row, int& n_new, int& ctx) {
     first_row = c.starts[s];
     const int end = c.starts[s + 1];
     n_new = end - first_row;
     ctx = c.context_lens[s];
-    if (n_new <= 0) return false;
-    if (first_row < 0 || end > T || ctx < n_new || (ctx - 1) / JSM_PAGE_SIZE >= c.max_pages) {
-        cache_error(c.err, CACHE_BAD_LENGTH);
-        return false;
-    }
-    return true;
+    return n_new > 0 && lengths_fit(c, T, first_row, end, ctx);
 }
 
 // The sequence of row t, for a whole block: every thread looks at one sequence, one round of loads for as many sequences as the block has threads.  -1: none.

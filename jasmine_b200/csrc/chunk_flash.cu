@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
     const int past = ctx - n_new, lo = w.lo, base = w.base, end = w.end, j_lo = w.j_lo, n_max = w.n_max;
     const int(&tok)[2] = w.tok, (&jb)[2] = w.jb, (&je)[2] = w.je;
 
-    if (warp < CK_SOFTMAX) regs_dec<Q8 ? 40 : 56>();
+    if (warp < CK_SOFTMAX) regs_dec<Q8 ? 56 : 72>();
     if (warp == 0) {
         if (work && n_max > j_lo) {
             const int page0 = base / JSM_PAGE_SIZE, last_page = (end - 1) / JSM_PAGE_SIZE;  // (behind the context the last page again: hidden keys)
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
             __syncwarp();
         }
     } else if (warp >= CK_SOFTMAX && warp < CK_CONVERT) {
-        regs_inc<Q8 ? 200 : 224>();
+        regs_inc<Q8 ? 192 : 216>();  // (200 and 40 for the first four warps: those spill, 152 us instead of 148 for 1000 tokens of 9000 positions of an 8-bit cache)
         const int t = (warp - CK_SOFTMAX) / 4, quad = warp & 3, row = quad * 32 + lane;
         const int rows = f.tile_tokens * a.G;                       // rows of the tile that are queries
         const int token = tok[t] + (int)(row * f.inv_G >> 16), pos = past + token;   // (a row that is none has a position all the same)

@@ -94,17 +94,20 @@ __device__ __forceinline__ void find_places(const CacheView& c, int T, int t0, i
     if (threadIdx.x < PLACES) seq[threadIdx.x] = -1;
     __syncthreads();
     for (int s = threadIdx.x; s < c.n_seqs; s += blockDim.x) {
-        const int from = c.starts[s], to = c.starts[s + 1];
-        for (int k = max(0, from - t0); k < n && t0 + k < to; ++k) seq[k] = s;
+        const int from = c.starts[s], to = c.starts[s + 1], ctx = c.context_lens[s];  // (one round of loads; the table is the other)
+        const int k0 = max(0, from - t0), k1 = to > t0 ? min(n, to - t0) : 0;
+        if (k0 < k1 && lengths_fit(c, T, from, to, ctx))
+            for (int k = k0; k < k1; ++k) {
+                seq[k] = s;
+                pos[k] = ctx - to + t0 + k;
+            }
     }
     __syncthreads();
     if (threadIdx.x < n) {
         const int k = threadIdx.x, s = seq[k];
-        int first, n_new, ctx, p = -1;
-        if (s >= 0 && cache_lengths(c, s, T, first, n_new, ctx)) {
-            const int at = ctx - n_new + t0 + k - first;
-            pos[k] = at;
-            if (at < table_len) p = cache_page(c, s, at);
+        int p = -1;
+        if (s >= 0) {
+            if (pos[k] < table_len) p = cache_page(c, s, pos[k]);
             else cache_error(c.err, CACHE_BAD_POSITION);
         }
         base[k] = p < 0 ? -1 : (int)cache_row(c, p, 0, 0, pos[k]);
