@@ -229,8 +229,8 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
             for (int ks = 0; ks < KS; ++ks) {
                 if constexpr (Q8) {
                     const uint2 w = r < rows ? *reinterpret_cast<const uint2*>(qp + (D / 4) * t4 + 4 * ks) : make_uint2(0, 0);
-                    qb[n][ks][0] = w.x;
-                    qb[n][ks][1] = w.y;
+                    qb[n][ks][0] = __byte_perm(w.x, w.y, 0x5410);  // components 0 and 2 of four, 1 and 3: the low bytes of a word of numbers, and the high ones
+                    qb[n][ks][1] = __byte_perm(w.x, w.y, 0x7632);
                 } else {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) qb[n][ks][h] = r < rows ? *reinterpret_cast<const uint32_t*>(qp + ks * 16 + h * 8 + t4 * 2) : 0u;
@@ -276,8 +276,8 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
                     uint32_t f[4];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        f[h] = q8_value2(__byte_perm(kw[h][ks], 0, 0x1100), ks2[h]);
-                        f[h + 2] = q8_value2(__byte_perm(kw[h][ks], 0, 0x3322), ks2[h]);
+                        f[h] = q8_value2(kw[h][ks], ks2[h]);
+                        f[h + 2] = q8_value2(kw[h][ks] >> 8, ks2[h]);
                     }
 #pragma unroll
                     for (int n = 0; n < NT; ++n) mma_16816(sc[n], f, qb[n][ks][0], qb[n][ks][1]);
