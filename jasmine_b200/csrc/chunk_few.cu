@@ -202,9 +202,34 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
             }
         }
     }
-    float* sm_o = reinterpret_cast<float*>(stages + Z::STAGES * Z::STAGE);  // [warp][row][component]
+    float* sm_o = reinterpret_cast<float*>(stages + Z::STAGES * Z::STAGE);  // [warp][row][component], pairs of components where the lanes of a store meet different banks
+    auto pair_at = [&](int w, int r, int p) {
+        const int turn = (((r >> 1) & 3) << (Q8 && D == 64 ? 0 : 2)) ^ (Q8 && D == 128 ? (p >> 3) & 7 : 0);
+        return sm_o + (w * few_rows + r) * D + (p ^ turn) * 2;
+    };
     bool ok = true;
     int s = 0, round = 0;
+    // B operand of the scores: row n * 8 + g, components of thread t4 in each step.  Of the next piece it is on its way while the sums of the one before meet.
+    uint32_t qb[NT][KS][2];
+    auto load_queries = [&] {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = n * 8 + g;
+            const __nv_bfloat16* qp = a.q + (q.row0 + r / a.G) * a.q_rs + (long long)(hk * a.G + r % a.G) * D;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if constexpr (Q8) {
+                    const uint2 w = r < q.n_new * a.G ? *reinterpret_cast<const uint2*>(qp + (D / 4) * t4 + 4 * ks) : make_uint2(0, 0);
+                    qb[n][ks][0] = w.x;
+                    qb[n][ks][1] = w.y;
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) qb[n][ks][h] = r < q.n_new * a.G ? *reinterpret_cast<const uint32_t*>(qp + ks * 16 + h * 8 + t4 * 2) : 0u;
+                }
+            }
+        }
+    };
+    load_queries();
     for (bool first_piece = true;; first_piece = false) {  // a (sequence, kv head, group), or the run's piece of it
         const int row0 = q.row0, n_new = q.n_new, ctx = q.ctx, rows = n_new * a.G, lo = first_key(a.window, ctx - n_new);  // no row sees a key before it
         const int here = min(left, n_pages - page);
@@ -218,30 +243,25 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
 #pragma unroll
             for (int j = 0; j < KS; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.0f;
         }
-        // B operand of the scores: row n * 8 + g, components of thread t4 in each step
-        uint32_t qb[NT][KS][2];
         int last[NT][2], first[NT][2];  // keys that the thread's two columns of each tile see
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int r = n * 8 + g;
-            const __nv_bfloat16* qp = a.q + (row0 + r / a.G) * a.q_rs + (long long)(hk * a.G + r % a.G) * D;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                if constexpr (Q8) {
-                    const uint2 w = r < rows ? *reinterpret_cast<const uint2*>(qp + (D / 4) * t4 + 4 * ks) : make_uint2(0, 0);
-                    qb[n][ks][0] = __byte_perm(w.x, w.y, 0x5410);  // components 0 and 2 of four, 1 and 3: the low bytes of a word of numbers, and the high ones
-                    qb[n][ks][1] = __byte_perm(w.x, w.y, 0x7632);
-                } else {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) qb[n][ks][h] = r < rows ? *reinterpret_cast<const uint32_t*>(qp + ks * 16 + h * 8 + t4 * 2) : 0u;
-                }
-            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int pos = ctx - n_new + min(n * 8 + t4 * 2 + h, rows - 1) / a.G;
                 last[n][h] = pos;
                 first[n][h] = first_key(a.window, pos);
             }
+        }
+        if constexpr (Q8) {  // components 0 and 2 of four, 1 and 3: the low bytes of a word of numbers, and the high ones
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const uint32_t x = qb[n][ks][0], y = qb[n][ks][1];
+                    qb[n][ks][0] = __byte_perm(x, y, 0x5410);
+                    qb[n][ks][1] = __byte_perm(x, y, 0x7632);
+                }
         }
         const int all_from = first_key(a.window, ctx - 1), all_to = ctx - n_new;  // keys that every row sees
         // 16 keys of a page; MASKED: some of them are hidden from some row (the pages at both ends of what the sequence sees)
@@ -396,6 +416,12 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
                 ++round;
             }
         }
+        const int now_seq = seq, now_hk = hk;
+        left -= here;
+        if (left > 0) {
+            next();
+            load_queries();
+        }
         // the four warps' sums meet (also after a wait that gave up: every warp comes by here as often)
         if (!first_piece) cf_meet();  // the piece before has been read
 #pragma unroll
@@ -405,11 +431,14 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
 #pragma unroll
                 for (int sh = 4; sh < 32; sh <<= 1) l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], sh);
                 const int r = n * 8 + t4 * 2 + h;
-                float* dst = sm_o + (warp * few_rows + r) * D;
 #pragma unroll
                 for (int j = 0; j < KS; ++j) {
-                    dst[Q8 ? (D / 8) * g + 2 * j : j * 16 + g] = o[n][j][h];
-                    dst[Q8 ? (D / 8) * g + 2 * j + 1 : j * 16 + g + 8] = o[n][j][h + 2];
+                    if constexpr (Q8) {
+                        *reinterpret_cast<float2*>(pair_at(warp, r, (D / 16) * g + j)) = make_float2(o[n][j][h], o[n][j][h + 2]);
+                    } else {
+                        pair_at(warp, r, j * 8 + (g >> 1))[g & 1] = o[n][j][h];
+                        pair_at(warp, r, j * 8 + 4 + (g >> 1))[g & 1] = o[n][j][h + 2];
+                    }
                 }
                 if (g == 0) {
                     sm_m[warp][r] = m[n][h];
@@ -430,9 +459,13 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
                 const float f = fast_ex2(sm_m[w][r] - M);
                 L += f * sm_l[w][r];
 #pragma unroll
-                for (int i = 0; i < N; ++i) acc[i] += f * sm_o[(w * few_rows + r) * D + lane * N + i];
+                for (int i = 0; i < N; i += 2) {
+                    const float2 v = *reinterpret_cast<const float2*>(pair_at(w, r, lane * (N / 2) + i / 2));
+                    acc[i] += f * v.x;
+                    acc[i + 1] += f * v.y;
+                }
             }
-            const int row = row0 + r / a.G, head = hk * a.G + r % a.G;
+            const int row = row0 + r / a.G, head = now_hk * a.G + r % a.G;
             if (whole) {
                 bool fine = true;
 #pragma unroll
@@ -445,7 +478,7 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
 #pragma unroll
                     for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16x2(acc[i], acc[i + 1]);
                 } else {
-                    attend_row<D, Q8>(a, seq, row, head, ctx - n_new + r / a.G);
+                    attend_row<D, Q8>(a, now_seq, row, head, ctx - n_new + r / a.G);
                 }
             } else {
                 // the run's first piece, or its last
@@ -455,9 +488,7 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
                 if (lane == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(M, L);
             }
         }
-        left -= here;
         if (left == 0) return;
-        next();
     }
 }
 
@@ -577,7 +608,7 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant_
     for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16x2(acc[i], acc[i + 1]);
 }
 
-// As many runs as the chip holds CTAs (8-bit pages, heads of 128: three per multiprocessor with three stages each 80.7 us for 64 contexts of 512 to 8192, four with two 87.0), of
+// As many runs as the chip holds CTAs (8-bit pages, heads of 128: three per multiprocessor with three stages each 80.7 us for 64 contexts of 512 to 8192, four with two 87.0; 77 by now), of
 // two pages at least (one token over 4096 positions: 7.8 us, with runs of one page 8.1).
 FewPlan chunk_few_plan(int n_seqs, int T, int max_new, int max_context, int Hkv, int G, int window, int rows, int tokens, int D, bool q8) {
     long long pages = (max_context + JSM_PAGE_SIZE - 1) / JSM_PAGE_SIZE;
