@@ -90,7 +90,8 @@ __global__ void __launch_bounds__(256) kv_append_q8_kernel(AppendArgs a) {
 // The places of up to PLACES consecutive rows of new tokens from t0 on, for a whole block: position, and row of the pool of kv head 0's key (-1: the row is left alone); row r of the
 // token's keys and values, keys of all heads first, lies JSM_PAGE_SIZE * r behind it
 constexpr int PLACES = 16;
-__device__ __forceinline__ void find_places(const CacheView& c, int T, int t0, int n, int table_len, int* seq, int* pos, int* base) {
+template <typename F>
+__device__ __forceinline__ void find_places(const CacheView& c, int T, int t0, int n, int table_len, int* seq, int* pos, int* base, F beside) {
     if (threadIdx.x < PLACES) seq[threadIdx.x] = -1;
     __syncthreads();
     for (int s = threadIdx.x; s < c.n_seqs; s += blockDim.x) {
@@ -103,6 +104,7 @@ __device__ __forceinline__ void find_places(const CacheView& c, int T, int t0, i
             }
     }
     __syncthreads();
+    beside();  // (positions are known, pages not yet)
     if (threadIdx.x < n) {
         const int k = threadIdx.x, s = seq[k];
         int p = -1;
@@ -116,11 +118,12 @@ __device__ __forceinline__ void find_places(const CacheView& c, int T, int t0, i
 }
 
 // Whole 16-byte pieces: LPR lanes have two pieces of eight components each of a row (token, keys or values, kv head), up to PLACES tokens per block; a thread's first loads do not
-// wait for the places.  A lane's pieces hold both components of its pairs (halves: a piece of each half), so that a rotation stays within the lane and its eight table
-// entries serve all heads of a token.  Products that are rounded on their own before a sum: two by one instruction, the sums one by one (mul2).  Rounding to a whole number:
+// wait for the places.  A lane's pieces hold both components of its pairs (halves: a piece of each half), so that a rotation stays within the lane.
+// Products that are rounded on their own before a sum: two by one instruction, the sums one by one (mul2).  Rounding to a whole number:
 // adding 1.5 * 2^23 leaves it in the low bits of the sum.
-// Prompts of 7887 tokens of 32 kv heads of 128 (192 MB in and out) 47 us, 4.1 TB/s of the measured 6.5: latency at four blocks per multiprocessor, 57 % of the issue slots.  The loads
-// of two turns at a time, none while they are worked out, addresses in 64 bits: 53 us; a lane per eight components with the partner of a half fetched a second time 74 us.
+// Prompts of 7887 tokens of 32 kv heads of 128 (192 MB in and out) 44 us, 4.4 TB/s of the measured 6.5: latency at five blocks per multiprocessor.  A token's table entries are in shared
+// memory: in registers they cost a block per multiprocessor, and a fetch in the middle of the rows (47 us).  The loads of two turns at a time, none while they are worked out, addresses in 64
+// bits: 53 us; a lane per eight components with the partner of a half fetched a second time 74 us.
 __device__ __forceinline__ float max3_abs(float a, float b, float c) {  // of the magnitudes; a NaN stays one
     float d;
     asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -144,9 +147,10 @@ __device__ __forceinline__ void advance(int& k, int& r, int step, int per_token)
 }
 enum { TURN_NONE = 0, TURN_ADJACENT = 1, TURN_HALF = 2, TURN_ANY = 3 };  // any: parts that are no multiple of 16, element by element
 template <int LPR, int TURN>
-__global__ void __launch_bounds__(256, 4) kv_append_q8_vec_kernel(AppendArgs a, int per_block) {
+__global__ void __launch_bounds__(256, TURN == TURN_ANY ? 4 : 5) kv_append_q8_vec_kernel(AppendArgs a, int per_block) {
     constexpr int ROWS = 256 / LPR;  // rows of a block's turn
     __shared__ int sh_seq[PLACES], sh_pos[PLACES], sh_base[PLACES];
+    __shared__ float4 sh_turn[TURN == TURN_ADJACENT || TURN == TURN_HALF ? PLACES * LPR * 4 : 1];  // of each token: two entries in 16 bytes, four of them for a lane, exchanged by lane
     chain_trigger();
     chain_wait();
     const int D = a.c.D, Hkv = a.c.Hkv, per_token = 2 * Hkv, t0 = blockIdx.x * per_block, n_tokens = min(per_block, a.T - t0), n_rows = n_tokens * per_token;
@@ -166,15 +170,17 @@ __global__ void __launch_bounds__(256, 4) kv_append_q8_vec_kernel(AppendArgs a, 
     int k = 0, r = 0;
     advance(k, r, group, per_token);
     load(k, r);
-    find_places(a.c, a.T, t0, n_tokens, TURN != TURN_NONE ? a.table_len : INT_MAX, sh_seq, sh_pos, sh_base);
     const int ahead = threadIdx.x % 32 / LPR;  // (a warp's rows take their turns together: lanes meet in shuffles)
-    int have = -1;                             // the token whose table entries are here; pairs that do not turn: 1 and 0
-    float c[8], sn[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        c[i] = 1.0f;
-        sn[i] = 0.0f;
-    }
+    find_places(a.c, a.T, t0, n_tokens, TURN != TURN_NONE ? a.table_len : INT_MAX, sh_seq, sh_pos, sh_base, [&] {
+        if constexpr (TURN == TURN_ADJACENT || TURN == TURN_HALF) {
+            const int pieces = half / 2;  // of a token's entries
+            for (int i = threadIdx.x; i < n_tokens * pieces; i += 256) {
+                const int token = i / pieces, c = i - token * pieces;
+                if (sh_seq[token] >= 0 && sh_pos[token] < a.table_len)
+                    sh_turn[token * (LPR * 4) + (c ^ ((c >> 3) & 3))] = reinterpret_cast<const float4*>(a.table + (long long)sh_pos[token] * half)[c];
+            }
+        }
+    });
     for (int row = group; row - ahead < n_rows; row += ROWS) {
         const int base = k < n_tokens ? sh_base[k] : -1;
         float x[16];
@@ -203,19 +209,17 @@ __global__ void __launch_bounds__(256, 4) kv_append_q8_vec_kernel(AppendArgs a, 
                 x[i] = __fadd_rn(__fmul_rn(x[i], v.x), __fmul_rn(z, second ? v.y : -v.y));
             }
         } else if (TURN != TURN_NONE && TURN != TURN_ANY && r_now < Hkv) {
-            if (have != k_now && turns && base >= 0) {
-                have = k_now;
-                const float4* e = reinterpret_cast<const float4*>(a.table + (long long)sh_pos[k_now] * half + l * 8);
+            if (turns) {  // (of a token without a place anything: it is not stored)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float4 v = e[i];
-                    c[2 * i] = v.x; sn[2 * i] = v.y; c[2 * i + 1] = v.z; sn[2 * i + 1] = v.w;
+                for (int i = 0; i < 8; i += 2) {
+                    const int c = l * 4 + i / 2;
+                    const float4 e = sh_turn[min(k_now, PLACES - 1) * (LPR * 4) + (c ^ ((c >> 3) & 3))];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int i1_ = TURN == TURN_ADJACENT ? 2 * (i + h) : i + h, i2_ = TURN == TURN_ADJACENT ? 2 * (i + h) + 1 : i + h + 8;
+                        rotate_pair(x[i1_], x[i2_], h ? e.z : e.x, h ? e.w : e.y, x[i1_], x[i2_]);
+                    }
                 }
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {  // (two products by one instruction: no faster here)
-                const int i1_ = TURN == TURN_ADJACENT ? 2 * i : i, i2_ = TURN == TURN_ADJACENT ? 2 * i + 1 : i + 8;
-                rotate_pair(x[i1_], x[i2_], c[i], sn[i], x[i1_], x[i2_]);
             }
         }
         float most = 0.0f;
@@ -305,7 +309,7 @@ __global__ void __launch_bounds__(256) kv_read_vec_kernel(ReadArgs a, int per_bl
     chain_wait();
     const int D = a.c.D, Hkv = a.c.Hkv, per_token = 2 * Hkv, t0 = blockIdx.x * per_block, n_tokens = min(per_block, a.T - t0);
     const int i0 = threadIdx.x % LPR * 8, group = threadIdx.x / LPR;
-    find_places(a.c, a.T, t0, n_tokens, INT_MAX, sh_seq, sh_pos, sh_base);
+    find_places(a.c, a.T, t0, n_tokens, INT_MAX, sh_seq, sh_pos, sh_base, [] {});
     if (i0 >= D) return;
     int k = 0, r = 0;
     advance(k, r, group, per_token);
