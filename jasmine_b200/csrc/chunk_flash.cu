@@ -11,7 +11,7 @@
 //                 rounded once, so scores and sums are those of a bf16 cache of these values; the conversion is spread over the whole group's rows
 // 8-bit caches, long contexts (PAIR): two CTAs walk the keys of four query tiles together (cta_group::2).  A product has 256 rows, 128 in each CTA's tensor memory; each CTA brings and
 // converts half of K (one page of two) and of V (64 of the 128 columns), so that a key tile is converted once for four query tiles, and operands come from shared memory half as
-// often: 173 -> 151 us for 1000 tokens of 9000 positions.  The even CTA issues the products of both; who writes its operands arrives at its barriers.  (bf16: 71 against 72 us for 512 of 8192,
+// often: 173 -> 148 us for 1000 tokens of 9000 positions.  The even CTA issues the products of both; who writes its operands arrives at its barriers.  (bf16: 71 against 72 us for 512 of 8192,
 // slower for prompts: without a conversion the hand-over between the CTAs costs what it saves.)
 // Few tiles and long contexts: the units (CTAs or pairs) of a cluster share the key tiles of their query tiles; each sends the sums of the rows that another owns into that one's shared
 // memory and joins its own with what it was sent, so that nothing goes through global memory and no second launch is needed.
@@ -77,7 +77,7 @@ __device__ __forceinline__ void ck_store4(uint32_t addr, uint32_t a, uint32_t b,
 }
 // ---- pairs of CTAs (cta_group::2): the even CTA of a pair issues the products of both -------------------------------------
 // Arrives at a barrier of this or the other CTA.  What the arrival announces lies in this CTA's shared or tensor memory, for this multiprocessor's tensor core, and is there already
-// (fence.proxy.async, tcgen05.wait::st); a release at the scope of the cluster waits for everything else that the thread has written (200 instead of 151 us).
+// (fence.proxy.async, tcgen05.wait::st); a release at the scope of the cluster waits for everything else that the thread has written (200 instead of 151 us then).
 __device__ __forceinline__ void ck_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 // mbar_wait_warp for a barrier at which the other CTA arrives too
 __device__ __forceinline__ bool ck_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
