@@ -81,14 +81,16 @@ __device__ __forceinline__ void ck_store4(uint32_t addr, uint32_t a, uint32_t b,
 __device__ __forceinline__ void ck_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 // mbar_wait_warp for a barrier at which the other CTA arrives too
 __device__ __forceinline__ bool ck_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
-    bool ok = false;
-    const long long t0 = clock64();
-    while (true) {
-        uint32_t done;
+    auto done = [&] {
+        uint32_t d;
         asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
-                     : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-        if (done) { ok = true; break; }
-        if (*abort_flag) break;
+                     : "=r"(d) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+        return d != 0;
+    };
+    bool ok = done();
+    for (const long long t0 = ok ? 0 : clock64(); !ok;) {
+        ok = done();
+        if (ok || *abort_flag) break;
         if (clock64() - t0 > WAIT_LIMIT_CYCLES) {
             *abort_flag = 1;
             if (err) atomicCAS(err, 0, code);
@@ -383,13 +385,15 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
             };
             bool ok = wait(&q_full, 0, TC_TIMEOUT_FULL);
             // S_t(j) = Q_t . K(j)^T over P_t(j - 1): the tensor pipe runs the products of this thread in order, the product with V has read P by then
-            auto issue_s = [&](int t, uint32_t k_addr) {
-                const uint32_t q_addr = smem_u32(q_smem + t * Z::TILE);
+            uint64_t q_desc[2] = {smem_desc_sw128(smem_u32(q_smem)), smem_desc_sw128(smem_u32(q_smem + Z::TILE))};
+            auto ready = [](uint64_t& desc) { asm volatile("" : "+l"(desc)); };  // (worked out here, not behind a wait)
+            ready(q_desc[0]);
+            ready(q_desc[1]);
+            auto issue_s = [&](int t, uint64_t k_desc) {
                 if (elect_one()) {
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
-                                                ck_mma_ss<PAIR>(tmem_base + S_COL[t], smem_desc_sw128(q_addr + (kk / 4) * Z::SLAB) + (uint64_t)((kk % 4) * 2), smem_desc_sw128(k_addr + (kk / 4) * Z::K_SLAB) + (uint64_t)((kk % 4) * 2),
-                               idesc_qk, kk > 0 ? 1u : 0u);
+                        ck_mma_ss<PAIR>(tmem_base + S_COL[t], q_desc[t] + (uint64_t)((kk / 4) * (Z::SLAB >> 4) + (kk % 4) * 2), k_desc + (uint64_t)((kk / 4) * (Z::K_SLAB >> 4) + (kk % 4) * 2), idesc_qk, kk > 0 ? 1u : 0u);
                     }
                     ck_commit<PAIR>(&s_full[t], pair_mask);
                 }
@@ -402,7 +406,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
                 if (ok) {
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
-                        if (active(t, j_lo)) issue_s(t, smem_u32(k_smem));
+                        if (active(t, j_lo)) issue_s(t, smem_desc_sw128(smem_u32(k_smem)));
                     if (elect_one()) ck_commit<PAIR>(&k_empty[0], pair_mask);
                     __syncwarp();
                 }
@@ -410,7 +414,8 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
             for (int j = j_lo; j < n_max && ok; ++j) {
                 const int i = j - j_lo, vs = i % ST, s1 = (i + 1) % ST;
                 const bool more = j + 1 < n_max;
-                if (!wait(&v_full[vs], (i / ST) & 1, TC_TIMEOUT_FULL)) { ok = false; break; }
+                // (the next keys too: nothing but the products themselves is to come between the weights' arrival and the next scores)
+                if (!wait(&v_full[vs], (i / ST) & 1, TC_TIMEOUT_FULL) || (more && !wait(&k_full[s1], ((i + 1) / ST) & 1, TC_TIMEOUT_FULL))) { ok = false; break; }
                 if (!Q8) {  // values that no row sees: a weight of zero meets a number
                     const int key0 = base + j * CK_BN;
                     if (key0 < lo || key0 + CK_BN > end) {
@@ -425,7 +430,9 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
                     }
                 }
                 tc_fence_after();
-                const uint32_t v_addr = smem_u32(v_smem + vs * Z::KV), k_addr = smem_u32(k_smem + s1 * Z::KV);
+                uint64_t v_desc = smem_desc_sw128_mn(smem_u32(v_smem + vs * Z::KV), Z::SLAB), k_desc = smem_desc_sw128(smem_u32(k_smem + s1 * Z::KV));
+                ready(v_desc);
+                ready(k_desc);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     if (active(t, j)) {
@@ -439,18 +446,14 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
                             if (elect_one()) {
 #pragma unroll
                                 for (int kk = half * BLOCKS; kk < (half + 1) * BLOCKS; ++kk)
-                                    ck_mma_ts<PAIR>(tmem_base + O_COL[t], tmem_base + S_COL[t] + kk * 8, smem_desc_sw128_mn(v_addr + kk * 2048, Z::SLAB), idesc_pv,
+                                    ck_mma_ts<PAIR>(tmem_base + O_COL[t], tmem_base + S_COL[t] + kk * 8, v_desc + (uint64_t)(kk * (2048 >> 4)), idesc_pv,
                                                     (j > jb[t] || kk > 0) ? 1u : 0u);
                             }
                             __syncwarp();
                         }
                         if (!ok) break;
                     }
-                    if (t == 0 && more) {
-                        if (!wait(&k_full[s1], ((i + 1) / ST) & 1, TC_TIMEOUT_FULL)) { ok = false; break; }
-                        tc_fence_after();
-                    }
-                    if (active(t, j + 1)) issue_s(t, k_addr);
+                    if (active(t, j + 1)) issue_s(t, k_desc);
                 }
                 if (!ok) break;
                 if (elect_one()) {
@@ -565,11 +568,11 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
                     ls2[i & 3] = fadd2(ls2[i & 3], pack2(p0, p1));
                     w[i] = pack_bf16x2(p0, p1);
                 }
-                tmem_st16(s_addr + c, w);
-                if (Z::HALVES && c == 16) {
+                if (Z::HALVES && c == 32) {  // (the stores of the first half are done by now)
                     tmem_st_wait();
                     weights_are_there(&p_half[t], half_to);
                 }
+                tmem_st16(s_addr + c, w);
             }
             float la, lb;
             unpack2(fadd2(fadd2(ls2[0], ls2[1]), fadd2(ls2[2], ls2[3])), la, lb);
