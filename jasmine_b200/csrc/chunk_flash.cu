@@ -11,7 +11,7 @@
 //                 rounded once, so scores and sums are those of a bf16 cache of these values; the conversion is spread over the whole group's rows
 // 8-bit caches, long contexts (PAIR): two CTAs walk the keys of four query tiles together (cta_group::2).  A product has 256 rows, 128 in each CTA's tensor memory; each CTA brings and
 // converts half of K (one page of two) and of V (64 of the 128 columns), so that a key tile is converted once for four query tiles, and operands come from shared memory half as
-// often: 173 -> 148 us for 1000 tokens of 9000 positions.  The even CTA issues the products of both; who writes its operands arrives at its barriers.  (bf16: 71 against 72 us for 512 of 8192,
+// often: 173 -> 148 us for 1000 tokens of 9000 positions (138 by now).  The even CTA issues the products of both; who writes its operands arrives at its barriers.  (bf16: 71 against 72 us for 512 of 8192,
 // slower for prompts: without a conversion the hand-over between the CTAs costs what it saves.)
 // Few tiles and long contexts: the units (CTAs or pairs) of a cluster share the key tiles of their query tiles; each sends the sums of the rows that another owns into that one's shared
 // memory and joins its own with what it was sent, so that nothing goes through global memory and no second launch is needed.
@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
                     if (grow) m_ref = mx;
                 }
             }
-            // p = 2^(s - m_ref) as bf16 pairs over the first 64 columns of S.  All of them by the special-function unit: the warps are bound by issue here, a quarter by polynomials
+            // p = 2^(s - m_ref) as bf16 pairs over the first 64 columns of S.  All of them by the special-function unit: a quarter by polynomials
             // on the FMA pipe costs 3 %.
             uint64_t ls2[4];
 #pragma unroll
