@@ -64,8 +64,8 @@ __global__ void __launch_bounds__(256) rope_rotate_scalar_kernel(RotateArgs a) {
 }
 
 // Whole 16-byte pieces: a thread has one unit of a head - a piece of each half, a piece of adjacent pairs, or a piece that is not rotated - with its table entries in
-// registers, and takes that unit of every HL-th head, four heads' loads in flight.  8192 rows of 32 + 8 heads of 128 with 64 rotated (bf16, 170 MB): 33.5 us, 5.1 TB/s of the
-// measured 6.5; without streaming loads and stores 36.1, with position and table ahead of the rows 40.7.
+// registers, and takes that unit of every HL-th head, four heads' loads in flight.  8192 rows of 32 + 8 heads of 128 with 64 rotated (bf16, 170 MB): 32.3 us, 5.3 TB/s of the
+// measured 6.5, with seven blocks per multiprocessor (six 33.5, ten spill: 46); without streaming loads and stores 36.1, with position and table ahead of the rows 40.7.
 template <typename T>
 struct RotPiece {
     static constexpr int V = 16 / sizeof(T);
@@ -95,7 +95,7 @@ struct RotPiece {
 
 constexpr int RV_THREADS = 128;
 template <typename T, bool ADJACENT>
-__global__ void __launch_bounds__(RV_THREADS) rope_rotate_vec_kernel(RotateArgs a, int units, int head_lanes) {
+__global__ void __launch_bounds__(RV_THREADS, 7) rope_rotate_vec_kernel(RotateArgs a, int units, int head_lanes) {
     constexpr int V = RotPiece<T>::V, PAIRS = ADJACENT ? V / 2 : V, U = 4;
     chain_trigger();
     chain_wait();
