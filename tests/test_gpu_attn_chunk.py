@@ -107,6 +107,7 @@ PAIRS = [
     ([90, 0, 20, 1], [400, 5, 20, 300], 128, 16, 0, 6000),
     ([600], [600], 32, 32, 0, 9000),
     ([200], [201], 96, 32, 0, 6000),
+    ([9], [300], 1024, 16, 0, 6000),             # two tokens a tile
 ]
 
 
@@ -122,6 +123,34 @@ def test_many_tiles_of_long_contexts(new, ctx, Hq, Hkv, window, most, bits):
     assert bool((out[sum(new):] == 3).all())
     again = c.attend(q.cuda(), window, bounds=(max(new), most))
     assert torch.equal(again[:sum(new)], got[:sum(new)])
+
+
+def test_many_tiles_on_two_streams_and_in_a_graph():
+    """Calls of pairs of CTAs and of both kinds of cache side by side, and replayed."""
+    cs = [Cache([100], [700], 32, 128, b, seed=b).to_device() for b in (8, 16, 8)]
+    qs = [c.queries(256).cuda() for c in cs]
+    first = [c.attend(q, bounds=(100, 6000)) for c, q in zip(cs, qs)]
+    side, outs = torch.cuda.Stream(), [torch.zeros_like(x) for x in first]
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for i, (c, q) in enumerate(zip(cs, qs)):
+            with torch.cuda.stream(side if i == 1 else torch.cuda.current_stream()):
+                c.attend(q, bounds=(100, 6000), out=outs[i])
+    side.synchronize()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(first, outs))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for i, (c, q) in enumerate(zip(cs, qs)):
+            c.attend(q, bounds=(100, 6000), out=outs[i])
+    for x in outs:
+        x.zero_()
+    cs[0].lens.fill_(500)  # the same call with another context
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(first[1], outs[1]) and torch.equal(first[2], outs[2])
+    assert torch.equal(cs[0].attend(qs[0], bounds=(100, 6000)), outs[0]) and not torch.equal(first[0], outs[0])
+    jb.check_device_errors()
 
 
 @pytest.mark.parametrize("bits", BITS)
