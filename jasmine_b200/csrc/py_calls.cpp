@@ -212,10 +212,11 @@ JSM_FAST(attn_decode) {  // q, pool, block_table, context_lens, Hq, Hkv, D, max_
     });
 }
 
-// the same on the current device, where the call runs
+// the same on the current device, where the call runs; the device is asked for once per call, under the interpreter's lock
+int call_device = -1;
 const at::Tensor* here(PyObject* o) {
     const at::Tensor* t = plain(o);
-    return t && t->get_device() == c10::cuda::current_device() ? t : nullptr;
+    return t && t->get_device() == call_device ? t : nullptr;
 }
 // Rows [T, columns] of adjacent elements; a single row's pitch means nothing.
 struct Rows {
@@ -274,6 +275,7 @@ bool as_cache(PyObject* pool, PyObject* scales, PyObject* table, PyObject* start
 }
 
 JSM_FAST(rope_rotate) {  // q, k, table, Hq, Hkv, D, rot, positions, layout, inverse, q_out, k_out
+    call_device = c10::cuda::current_device();
     int hq, hkv, d, rot, layout, n;
     const float* table;
     JSM_NEED(n_args == 12 && as_int(a[3], hq) && as_int(a[4], hkv) && as_int(a[5], d) && as_int(a[6], rot) && as_int(a[8], layout) && a[2] != Py_None &&
@@ -293,6 +295,7 @@ JSM_FAST(rope_rotate) {  // q, k, table, Hq, Hkv, D, rot, positions, layout, inv
 }
 
 JSM_FAST(kv_append_q8) {  // pool, scales, block_table, k, v, starts, context_lens, Hkv, D, rope, rot, layout
+    call_device = c10::cuda::current_device();
     int hkv, d, rot, layout, n;
     const float* table;
     Cache c;
@@ -306,6 +309,7 @@ JSM_FAST(kv_append_q8) {  // pool, scales, block_table, k, v, starts, context_le
 }
 
 JSM_FAST(kv_read) {  // pool, scales, block_table, starts, context_lens, T, Hkv, D, k_out, v_out (both or neither), f32; with neither the new outputs come back
+    call_device = c10::cuda::current_device();
     int T, hkv, d;
     Cache c;
     Rows k, v;
@@ -339,6 +343,7 @@ JSM_FAST(kv_read) {  // pool, scales, block_table, starts, context_lens, T, Hkv,
 }
 
 JSM_FAST(attn_chunk) {  // q, pool, scales, block_table, starts, context_lens, Hq, Hkv, D, max_new, max_context, window, scale, scratch, out
+    call_device = c10::cuda::current_device();
     int hq, hkv, d, most_new, most, window;
     float scale;
     Cache c;
