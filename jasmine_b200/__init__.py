@@ -530,6 +530,9 @@ def _ints(t, shape, what):
 def rope_rotate(q, k, table, Hq, Hkv, D, rot_dim, positions=None, layout=ROPE_HALF, inverse=False, q_out=None, k_out=None):
     """Query and key rows [T, Hq * D] and [T, Hkv * D] of any pitch, rotated on the first rot_dim components of every head (jsm_rope_rotate); inverse: the transposed
     rotation (the gradient).  Either may be None with no heads.  table: F32 [positions, rot_dim / 2, 2]."""
+    m = _calls_module or _calls()
+    if m and (q is None or q_out is not None) and (k is None or k_out is not None) and _done(m.rope_rotate(q, k, table, Hq, Hkv, D, rot_dim, positions, layout, inverse, q_out, k_out)):
+        return q_out, k_out
     torch = _torch()
     x = q if q is not None else k
     _need(x is not None, "rope_rotate: no rows")
@@ -537,7 +540,6 @@ def rope_rotate(q, k, table, Hq, Hkv, D, rot_dim, positions=None, layout=ROPE_HA
     _need((q is None) == (Hq == 0) and (k is None) == (Hkv == 0), "rope_rotate: rows without heads, or heads without rows")
     q_out = torch.empty(T, Hq * D, dtype=q.dtype, device=q.device) if q is not None and q_out is None else q_out
     k_out = torch.empty(T, Hkv * D, dtype=k.dtype, device=k.device) if k is not None and k_out is None else k_out
-    m = _calls_module or _calls()
     if m and _done(m.rope_rotate(q, k, table, Hq, Hkv, D, rot_dim, positions, layout, inverse, q_out, k_out)):
         return q_out, k_out
     _need(table.dtype == torch.float32 and table.is_contiguous() and table.dim() == 3 and tuple(table.shape[1:]) == (rot_dim // 2, 2), "rope_rotate: a contiguous "
@@ -598,14 +600,14 @@ def kv_append_q8(pool, scales, block_table, k, v, starts, context_lens, Hkv, D, 
 
 def kv_read(pool, block_table, starts, context_lens, T, Hkv, D, scales=None, dtype=None, k_out=None, v_out=None):
     """Keys and values [T, Hkv * D] (bf16, or dtype) of the new tokens' positions as the cache holds them (jsm_kv_read); rows of no sequence are left as they are."""
-    torch = _torch()
     m = _calls_module or _calls()
-    if m and dtype in (None, torch.bfloat16, torch.float32):
-        done = m.kv_read(pool, scales, block_table, starts, context_lens, T, Hkv, D, k_out, v_out, dtype is torch.float32)
+    if m and (dtype is None or dtype in (_torch().bfloat16, _torch().float32)):
+        done = m.kv_read(pool, scales, block_table, starts, context_lens, T, Hkv, D, k_out, v_out, dtype is not None and dtype is _torch().float32)
         if type(done) is tuple:
             return done
         if _done(done):
             return k_out, v_out
+    torch = _torch()
     k_out = torch.empty(T, Hkv * D, dtype=dtype or torch.bfloat16, device=pool.device) if k_out is None else k_out
     v_out = torch.empty_like(k_out) if v_out is None else v_out
     at, seqs = _cache("kv_read", pool, scales, block_table, starts, context_lens, Hkv, D)
@@ -619,13 +621,13 @@ def kv_read(pool, block_table, starts, context_lens, T, Hkv, D, scales=None, dty
 
 def attn_chunk(q, pool, block_table, starts, context_lens, Hq, Hkv, D, max_new, max_context, scales=None, window=0, scale=None, scratch=None, out=None):
     """Attention of the new tokens q [T, Hq * D] of every sequence over its paged cache, bf16 or (with scales) 8-bit (jsm_attn_chunk)."""
-    torch = _torch()
-    T = q.shape[0]
-    out = torch.empty(T, Hq * D, dtype=q.dtype, device=q.device) if out is None else out
+    if out is None:
+        out = _torch().empty(q.shape[0], Hq * D, dtype=q.dtype, device=q.device)
     scale = float(D) ** -0.5 if scale is None else scale
     m = _calls_module or _calls()
     if m and _done(m.attn_chunk(q, pool, scales, block_table, starts, context_lens, Hq, Hkv, D, max_new, max_context, window, scale, scratch, out)):
         return out
+    torch, T = _torch(), q.shape[0]
     at, seqs = _cache("attn_chunk", pool, scales, block_table, starts, context_lens, Hkv, D)
     for t, what in ((q, "q"), (out, "out")):
         _rows(t, Hq * D, "attn_chunk: " + what)
