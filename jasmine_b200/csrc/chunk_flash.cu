@@ -34,6 +34,7 @@ constexpr int CK_BM = 128, CK_BN = 128;
 constexpr int CK_SOFTMAX = 4, CK_CONVERT = 12;  // first warp of a role
 constexpr float CK_RESCALE = 8.0f;             // the maximum is above the reference by so many powers of two: the reference follows
 constexpr float CK_RAISE = 16777216.0f;        // a key tile's sum of weights is above 2^24: the reference is raised
+constexpr float CK_JUMP = 1.3292279957849159e36f;  // ... above 2^120: the row is worked out again.  2^-120 is a factor that keeps its bits (below 2^-126 ex2_approx returns zero)
 constexpr float CK_NONE = -1.0e30f;             // the maximum of a row that has seen nothing
 
 template <int D, bool Q8, bool PAIR>
@@ -474,8 +475,8 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
         const uint32_t lane_addr = tmem_base + ((uint32_t)(quad * 32) << 16), s_addr = lane_addr + S_COL[t], o_addr = lane_addr + O_COL[t];
         const int pos_lo = past + tok[t], pos_hi = past + min(tok[t] + f.tile_tokens, n_new) - 1;  // first and last query of the tile
         // Weights are 2^(score - reference), whatever the reference: bf16, fp32 sums and fp32 accumulators keep their precision over 2^100 and more.  So the maximum is looked for
-        // only where a row has no reference yet, or where keys are hidden; elsewhere a sum of weights above 2^24 raises the reference before the next key tile (a jump of
-        // more than 2^100 within one tile gives infinities: such a row is worked out again at the end).
+        // only where a row has no reference yet, or where keys are hidden; elsewhere a sum of weights above 2^24 raises the reference before the next key tile, or behind the last.  A
+        // key tile's sum above 2^120, or one that is infinite, makes the row's sum of weights a NaN: such a row is worked out again at the end.
         float m_ref = query ? CK_NONE : 0.0f, l = 0.0f;
         int raise = 0;
         bool ok = true;
@@ -577,7 +578,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
             float la, lb;
             unpack2(fadd2(fadd2(ls2[0], ls2[1]), fadd2(ls2[2], ls2[3])), la, lb);
             const float sum = la + lb;
-            l += sum;
+            l = sum > CK_JUMP ? NAN : l + sum;
             raise = sum > CK_RAISE ? (int)(__float_as_uint(sum) >> 23) - 127 : 0;
             tmem_st_wait();
             weights_are_there(&p_ready[t], ready_to);
@@ -594,7 +595,11 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
         uint8_t* recv = tiles;
         uint8_t* recv_ml = tiles + (share - 1) * own_rows * (D * 4);
         uint8_t* staged = (share > 1 ? recv_ml + (share - 1) * own_rows * 8 : tiles) + sw * (32 * D * 2);  // this warp's 32 rows pass through here
-        float own = 1.0f, L = l, M = m_ref;  // factor of the sums in TMEM, sum of the weights, reference of the row
+        // What the last key tile asks for: rows meet under references that their sums of weights are near to, so that a factor below 2^-126 is one of nothing.
+        const float fold = ex2_approx((float)-raise);
+        l *= fold;
+        m_ref += (float)raise;
+        float own = fold, L = l, M = m_ref;  // factor of the sums in TMEM, sum of the weights, reference of the row
         bool have = any;
         int senders = 0;
         const int warps = 8 / share, owner = sw / warps, r_own = sw % warps * 32;  // of a cluster: who joins this warp's rows, and where they are there
@@ -617,6 +622,8 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
                         tmem_ld32(o_addr + c, o);
                         tmem_ld_wait();
 #pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fold);
+#pragma unroll
                         for (int i = 0; i < 8; ++i) sts128(here + lane * 128 + ((i ^ (lane & 7)) * 16), make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
                         __syncwarp();
 #pragma unroll
@@ -637,8 +644,9 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
                 if (!any) M = CK_NONE;
 #pragma unroll 1
                 for (int p = 0; p < senders; ++p) M = fmaxf(M, reinterpret_cast<const float2*>(recv_ml)[p * own_rows + r_own + lane].x);
-                own = any ? ex2_approx(m_ref - M) : 0.0f;
-                L = any ? l * own : 0.0f;
+                const float w_own = ex2_approx(m_ref - M);
+                own = any ? w_own * fold : 0.0f;
+                L = any ? l * w_own : 0.0f;
 #pragma unroll 1
                 for (int p = 0; p < senders; ++p) {
                     const float2 w = sent_factor(p);
