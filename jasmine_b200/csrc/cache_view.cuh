@@ -35,12 +35,14 @@ __device__ __forceinline__ bool lengths_fit(const CacheView& c, int T, int first
     cache_error(c.err, CACHE_BAD_LENGTH);
     return false;
 }
-// new tokens and context of sequence s; false (and an error) where they do not fit the table or one another
+// new tokens and context of sequence s; false (and an error) where they do not fit the table or one another.  EARLY: for a kernel that has not waited for its predecessor (past L1)
+template <bool EARLY = false>
 __device__ __forceinline__ bool cache_lengths(const CacheView& c, int s, int T, int& first_row, int& n_new, int& ctx) {
-    first_row = c.starts[s];
-    const int end = c.starts[s + 1];
+    auto load = [](const int32_t* p) { return EARLY ? load_early(p) : *p; };
+    first_row = load(c.starts + s);
+    const int end = load(c.starts + s + 1);
     n_new = end - first_row;
-    ctx = c.context_lens[s];
+    ctx = load(c.context_lens + s);
     return n_new > 0 && lengths_fit(c, T, first_row, end, ctx);
 }
 

@@ -32,8 +32,9 @@ jsm_status chunk_flash_launch(const ChunkArgs& a, int few_tokens, cudaStream_t s
 
 #ifdef __CUDACC__
 // lengths of a sequence that the kernels may rely on; false: no new tokens, or lengths that do not fit (an error)
+template <bool EARLY = false>
 __device__ __forceinline__ bool chunk_lengths(const ChunkArgs& a, int s, int& first_row, int& n_new, int& ctx) {
-    if (!cache_lengths(a.c, s, a.T, first_row, n_new, ctx)) return false;
+    if (!cache_lengths<EARLY>(a.c, s, a.T, first_row, n_new, ctx)) return false;
     if (n_new <= a.max_new && ctx <= a.max_context) return true;
     cache_error(a.c.err, CACHE_BAD_LENGTH);
     return false;

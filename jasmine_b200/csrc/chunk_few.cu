@@ -52,7 +52,8 @@ struct FewSeq {
     int row0, n_new, ctx;
 };
 // sequence s, if it has new tokens and no more rows than this kernel takes
-__device__ __forceinline__ bool few_sequence(const ChunkArgs& a, const FewPlan& f, int s, FewSeq& q) { return chunk_lengths(a, s, q.row0, q.n_new, q.ctx) && q.n_new <= f.tokens; }
+template <bool EARLY = false>
+__device__ __forceinline__ bool few_sequence(const ChunkArgs& a, const FewPlan& f, int s, FewSeq& q) { return chunk_lengths<EARLY>(a, s, q.row0, q.n_new, q.ctx) && q.n_new <= f.tokens; }
 __device__ __forceinline__ FewSeq few_group(const FewPlan& f, const FewSeq& q, int group) {
     const int first = group * f.per, n = min(f.per, q.n_new - first);
     return FewSeq{q.row0 + first, n, q.ctx - q.n_new + first + n};
@@ -63,9 +64,10 @@ __device__ __forceinline__ int group_pages(const ChunkArgs& a, const FewSeq& q, 
     return (q.ctx - 1) / JSM_PAGE_SIZE + 1 - page0;
 }
 // all groups' of sequence s, for one kv head; 0: not this kernel's
+template <bool EARLY = false>
 __device__ __forceinline__ int head_pages(const ChunkArgs& a, const FewPlan& f, int s, FewSeq& q) {
     int sum = 0, page0;
-    if (s < a.c.n_seqs && few_sequence(a, f, s, q))
+    if (s < a.c.n_seqs && few_sequence<EARLY>(a, f, s, q))
         for (int g = 0; g * f.per < q.n_new; ++g) sum += group_pages(a, few_group(f, q, g), page0);
     return sum;
 }
@@ -95,7 +97,7 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
         mbar_fence_init();
     }
     chain_wait();
-    chain_trigger();  // (now: what the merge reads before its own wait was there before this kernel)
+    chain_trigger();  // (now: the lengths that the merge reads before its own wait were written before this kernel's wait ended)
     if (warp == 0) {  // where this CTA's run begins
         long long all = 0;
         FewSeq q;
@@ -494,7 +496,8 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
 
 // The pieces of a row under their largest reference, in the order of the runs.  Few groups (JOIN): a block per (sequence, kv head, group) and row, each of four warps takes eight pieces
 // of every 32, all their loads in flight, and they meet in shared memory.  Many groups, of a few pieces each: a warp per row (32 sequences of 8 tokens of 300, 32 heads: 32 us with the
-// runs, a block per row 46).  What depends on the lengths alone is worked out while the runs are still under way.
+// runs, a block per row 46).  What depends on the lengths alone is worked out while the runs are still under way: a kernel in front of the runs may have written them, but it has ended
+// when the runs let this one start, so that they are in L2; L1 may still hold older ones (load_early).
 constexpr int CM_RUNS = 8;
 template <int D, bool Q8, bool JOIN>
 __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant__ ChunkArgs a, const __grid_constant__ FewPlan f, const float* part) {
@@ -506,7 +509,7 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant_
     long long before = 0, all = 0;
     FewSeq q = {0, 0, 0};
     for (int k = threadIdx.x; k < a.c.n_seqs; k += 128) {
-        const int n = head_pages(a, f, k, q);
+        const int n = head_pages<true>(a, f, k, q);
         all += n;
         if (k < s) before += n;
     }
@@ -520,7 +523,7 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant_
         sm_before[warp] = before;
     }
     int n_pages = 0, head_all = 0, groups_before = 0;
-    if (few_sequence(a, f, s, q))
+    if (few_sequence<true>(a, f, s, q))
         for (int g = 0, page0; g * f.per < q.n_new; ++g) {
             const int k = group_pages(a, few_group(f, q, g), page0);
             if (g < group) groups_before += k;

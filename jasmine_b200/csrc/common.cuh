@@ -71,7 +71,9 @@ int sm_count();
 //     produces or consumes; it returns once the predecessor grid has completed and its writes are visible;
 //   * the one exception is load_early (below): what no kernel of the running pass writes.  It rests on two things that the host sees to: every
 //     pass ends in a wait for its stream, so that nothing of an earlier pass still runs, and a pass has every sequence once, so that
-//     what lies before a segment's first position was written by earlier passes.
+//     what lies before a segment's first position was written by earlier passes;
+//   * a kernel whose predecessor triggers only behind its own chain_wait (chunk_few_kernel) may read early what kernels in front of that
+//     predecessor have written: they had ended when it was let go.  With load_early too, because of L1.
 // Both are no-ops for a kernel launched without the attribute.
 bool chained_launch_enabled();  // JSM_PDL=0 in the environment turns the attribute off (plain stream order)
 

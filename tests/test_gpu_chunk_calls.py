@@ -165,3 +165,47 @@ def test_queries_and_outputs_beyond_32_bits():
     jb.rope_rotate(rows, None, t, 2, 0, 64, 64, q_out=rows)
     assert torch.equal(rows, jb.rope_rotate(q.cuda(), None, t, 2, 0, 64, 64)[0])
     jb.check_device_errors()
+
+
+@pytest.mark.parametrize("bits", (16, 8))
+@pytest.mark.parametrize("most", (1, 5))
+def test_lengths_that_a_kernel_writes_before_each_call(most, bits):
+    """A captured loop in which contexts grow across page borders and sequences drop out, no wait of the host between the steps, replayed."""
+    n, steps = 24, 14
+    ctx = [90 + 61 * b for b in range(n)]
+    c = Cache([most] * n, ctx, 2, 128, bits, seed=3, max_pages=(max(ctx) + 40 * steps) // PAGE + 1)
+    used = c.table.clamp(min=0)
+    c.table = torch.where(c.table < 0, used.flatten()[torch.arange(c.table.numel()) % used.shape[1]].view_as(c.table), c.table)  # (pages of other sequences: numbers, whatever they are)
+    for p in range(c.pool.shape[0]):  # no place is left that is not a number
+        if bits == 16:
+            c.pool[p].nan_to_num_(0.5)
+        else:
+            c.scales[p].nan_to_num_(0.02)
+    c.to_device()
+    q = c.queries(8).cuda()
+    bounds, grow = (most, max(ctx) + 40 * steps), torch.randint(0, 40, (steps, n), generator=c.g).int().cuda()
+    counts = torch.randint(0, most + 1, (steps, n), generator=c.g).int().cuda()
+    first, outs = c.lens.clone(), torch.zeros(steps, *q.shape, dtype=torch.bfloat16, device="cuda")
+
+    def step(i):
+        c.lens.add_(grow[i])
+        torch.cumsum(counts[i], 0, dtype=torch.int32, out=c.starts[1:])
+        c.attend(q, bounds=bounds, out=outs[i])
+
+    for i in range(steps):
+        step(i)
+        torch.cuda.synchronize()
+    want = outs.clone()
+    assert not torch.equal(want[0], want[1])
+    g = torch.cuda.CUDAGraph()
+    c.lens.copy_(first)
+    with torch.cuda.graph(g):
+        c.lens.copy_(first)
+        outs.zero_()
+        for i in range(steps):
+            step(i)
+    for _ in range(20):
+        g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs, want)
+    jb.check_device_errors()
