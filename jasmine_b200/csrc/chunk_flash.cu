@@ -11,7 +11,7 @@
 //                 rounded once, so scores and sums are those of a bf16 cache of these values; the conversion is spread over the whole group's rows
 // 8-bit caches, long contexts (PAIR): two CTAs walk the keys of four query tiles together (cta_group::2).  A product has 256 rows, 128 in each CTA's tensor memory; each CTA brings and
 // converts half of K (one page of two) and of V (64 of the 128 columns), so that a key tile is converted once for four query tiles, and operands come from shared memory half as
-// often: 173 -> 148 us for 1000 tokens of 9000 positions (138 by now).  The even CTA issues the products of both; who writes its operands arrives at its barriers.  (bf16: 71 against 72 us for 512 of 8192,
+// often: 173 -> 148 us for 1000 tokens of 9000 positions (143 by now).  The even CTA issues the products of both; what the other has written is announced to it.  (bf16: 71 against 72 us for 512 of 8192,
 // slower for prompts: without a conversion the hand-over between the CTAs costs what it saves.)
 // Few tiles and long contexts: the units (CTAs or pairs) of a cluster share the key tiles of their query tiles; each sends the sums of the rows that another owns into that one's shared
 // memory and joins its own with what it was sent, so that nothing goes through global memory and no second launch is needed.
@@ -77,20 +77,28 @@ __device__ __forceinline__ void ck_store4(uint32_t addr, uint32_t a, uint32_t b,
     asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 // ---- pairs of CTAs (cta_group::2): the even CTA of a pair issues the products of both -------------------------------------
-// Arrives at a barrier of this or the other CTA.  What the arrival announces lies in this CTA's shared or tensor memory, for this multiprocessor's tensor core, and is there already
-// (fence.proxy.async, tcgen05.wait::st); a release at the scope of the cluster waits for everything else that the thread has written (200 instead of 151 us then).
-__device__ __forceinline__ void ck_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
-// mbar_wait_warp for a barrier at which the other CTA arrives too
+// Arrivals at a barrier of the other CTA (or this one), and waits for such.  What lies in tensor memory is ordered by tcgen05.wait and the tcgen05 fences on both sides; arrival and wait carry
+// no more than the order of execution (relaxed, at the scope of the cluster).  What lies in shared memory needs a release and an acquire at that scope.  A thread pays for its release until all that it
+// has written is there (by the converting warps 189 us for 1000 tokens of 9000 positions, by all arrivals 205), so the writers arrive in their own CTA, and one warp of the
+// second CTA, which writes nothing itself, acquires that and releases it to the first: 143 us (139 with arrivals that release to their own CTA only, an order that the memory model does not give).
+__device__ __forceinline__ void ck_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void ck_arrive_tmem(uint32_t bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+template <bool TMEM>
+__device__ __forceinline__ bool ck_try_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t d;
+    if constexpr (TMEM)
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(d) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    else
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(d) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return d != 0;
+}
+// mbar_wait_warp for a barrier at which the other CTA of a pair, or its products, arrive too
+template <bool PAIR, bool TMEM = false>
 __device__ __forceinline__ bool ck_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
-    auto done = [&] {
-        uint32_t d;
-        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
-                     : "=r"(d) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-        return d != 0;
-    };
-    bool ok = done();
+    if constexpr (!PAIR) return mbar_wait_warp(bar, parity, abort_flag, err, code);
+    bool ok = ck_try_wait<TMEM>(bar, parity);
     for (const long long t0 = ok ? 0 : clock64(); !ok;) {
-        ok = done();
+        ok = ck_try_wait<TMEM>(bar, parity);
         if (ok || *abort_flag) break;
         if (clock64() - t0 > WAIT_LIMIT_CYCLES) {
             *abort_flag = 1;
@@ -234,13 +242,13 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
         tma_prefetch_desc(&tmap_q);
         tma_prefetch_desc(&tmap_kv);
         abort_flag = 0;
-        // the leader of a pair hears of the other CTA's copies from that one's warp 1, of its 8-bit pages and weights from the warps that write them
+        // the leader of a pair hears of the other CTA's queries and converted pages from that one's warp 1, of its weights from the warps that write them
         const int both = PAIR && leads ? 2 : 1;
         mbar_init(&q_full, both);
         mbar_init(&o_done, 1);
         for (int s = 0; s < ST; ++s) {
-            mbar_init(&k_full[s], Q8 ? 4 * both : both);
-            mbar_init(&v_full[s], Q8 ? 4 * both : both);
+            mbar_init(&k_full[s], Q8 ? 3 + both : both);
+            mbar_init(&v_full[s], Q8 ? 3 + both : both);
             mbar_init(&k_empty[s], 1);
             mbar_init(&v_empty[s], 1);
         }
@@ -375,14 +383,23 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
             }
         }
     } else if (warp == 1) {
-        if (PAIR && work && n_max > j_lo && !leads) {  // the leader hears that the other CTA's queries are there
-            if (mbar_wait_warp(&q_full, 0, &abort_flag, a.c.err, TC_TIMEOUT_FULL) && lane == 0) ck_arrive(ck_peer(smem_u32(&q_full), rank - 1));
+        if (PAIR && work && n_max > j_lo && !leads) {  // the leader hears that the other CTA's queries, keys and values are there
+            const uint32_t q_to = ck_peer(smem_u32(&q_full), rank - 1), k_to = ck_peer(smem_u32(k_full), rank - 1), v_to = ck_peer(smem_u32(v_full), rank - 1);
+            bool ok = mbar_wait_warp(&q_full, 0, &abort_flag, a.c.err, TC_TIMEOUT_FULL);
+            if (ok && lane == 0) ck_arrive(q_to);
+            for (int j = j_lo; j < n_max && ok; ++j) {
+                const int i = j - j_lo, s = i % ST;
+                ok = mbar_wait_warp(&k_full[s], (i / ST) & 1, &abort_flag, a.c.err, TC_TIMEOUT_FULL);
+                if (ok && lane == 0) ck_arrive(k_to + s * 8);
+                ok = ok && mbar_wait_warp(&v_full[s], (i / ST) & 1, &abort_flag, a.c.err, TC_TIMEOUT_FULL);
+                if (ok && lane == 0) ck_arrive(v_to + s * 8);
+            }
         }
         if (work && n_max > j_lo && leads) {
             constexpr uint32_t idesc_qk = instr_desc_bf16(PAIR ? 2 * CK_BM : CK_BM, CK_BN, 0, 0), idesc_pv = instr_desc_bf16(PAIR ? 2 * CK_BM : CK_BM, D, 0, 1);
             const uint32_t pair_mask = 3u << rank;
             auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-                return PAIR ? ck_wait_warp(bar, parity, &abort_flag, a.c.err, code) : mbar_wait_warp(bar, parity, &abort_flag, a.c.err, code);
+                return ck_wait_warp<PAIR>(bar, parity, &abort_flag, a.c.err, code);
             };
             bool ok = wait(&q_full, 0, TC_TIMEOUT_FULL);
             // S_t(j) = Q_t . K(j)^T over P_t(j - 1): the tensor pipe runs the products of this thread in order, the product with V has read P by then
@@ -502,12 +519,12 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                if (PAIR) ck_arrive(to);
+                if (PAIR) ck_arrive_tmem(to);
                 else mbar_arrive(bar);
             }
         };
         for (int j = jb[t]; j < je[t] && ok; ++j) {
-            if (!mbar_wait_warp(&s_full[t], (j - jb[t]) & 1, &abort_flag, a.c.err, TC_TIMEOUT_ACC)) { ok = false; break; }
+            if (!ck_wait_warp<PAIR, true>(&s_full[t], (j - jb[t]) & 1, &abort_flag, a.c.err, TC_TIMEOUT_ACC)) { ok = false; break; }
             tc_fence_after();
             if (PAIR && !mine) {
                 weights_are_there(&p_half[t], half_to);
@@ -583,7 +600,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
             tmem_st_wait();
             weights_are_there(&p_ready[t], ready_to);
         }
-        if (ok && n_max > j_lo) ok = mbar_wait_warp(&o_done, 0, &abort_flag, a.c.err, TC_TIMEOUT_ACC);
+        if (ok && n_max > j_lo) ok = ck_wait_warp<PAIR, true>(&o_done, 0, &abort_flag, a.c.err, TC_TIMEOUT_ACC);
         tc_fence_after();
         const bool any = ok && mine && je[t] > jb[t];  // (the whole query tile)
         // What follows is executed once per CTA, mostly for the first time on its multiprocessor: rolled loops, because every line of code is fetched (unrolled, with the
@@ -757,7 +774,6 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
             };
             constexpr std::integral_constant<int, 4> four{};
             constexpr std::integral_constant<int, 2> two{};
-            const uint32_t k_to = PAIR ? ck_peer(smem_u32(k_full), rank & ~1) : 0, v_to = PAIR ? ck_peer(smem_u32(v_full), rank & ~1) : 0;
             bool ok = true;
             for (int j = j_lo; j < n_max && ok; ++j) {
                 const int i = j - j_lo, s = i % ST;
@@ -765,7 +781,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
                 for (int slot = 0; slot < Z::SLOTS; ++slot) {
                     const int value = PAIR ? slot > 0 : slot >> 1, half = PAIR ? (slot ? slot - 1 : 0) : slot & 1;
                     const bool first = half == 0, last = half == 1 || (PAIR && !value);
-                    if (first && i >= ST && !mbar_wait_warp(value ? &v_empty[s] : &k_empty[s], ((i / ST) & 1) ^ 1, &abort_flag, a.c.err, TC_TIMEOUT_EMPTY)) { ok = false; break; }
+                    if (first && i >= ST && !ck_wait_warp<PAIR>(value ? &v_empty[s] : &k_empty[s], ((i / ST) & 1) ^ 1, &abort_flag, a.c.err, TC_TIMEOUT_EMPTY)) { ok = false; break; }
                     if (!mbar_wait_warp(&raw_full[slot], i & 1, &abort_flag, a.c.err, TC_TIMEOUT_FULL)) { ok = false; break; }
                     const uint32_t raw = raw_u32 + Z::raw_at(slot), scales = raw_sc + slot * (JSM_PAGE_SIZE * 2);
                     const uint32_t to = (value ? v_u32 : k_u32) + s * Z::KV + half * (JSM_PAGE_SIZE * 128);
@@ -779,10 +795,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
                     __syncwarp();
                     if (lane == 0) {
                         mbar_arrive(&raw_empty[slot]);
-                        if (last) {
-                            if (PAIR) ck_arrive((value ? v_to : k_to) + s * 8);
-                            else mbar_arrive(value ? &v_full[s] : &k_full[s]);
-                        }
+                        if (last) mbar_arrive(value ? &v_full[s] : &k_full[s]);
                     }
                 }
             }

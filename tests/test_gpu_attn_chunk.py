@@ -252,3 +252,21 @@ def test_lengths_and_pages_that_do_not_fit_are_reported():
         want[2:] = float("nan")
         check_attention(out, want, mag)
     jb.check_device_errors()
+
+
+def test_pairs_beside_other_work():
+    """Pairs of CTAs, again and again beside kernels that write: what the second CTA converts has arrived when the first multiplies it."""
+    c = Cache([100], [3000], 32, 128, 8, seed=21).to_device()
+    q = c.queries(256).cuda()
+    first = c.attend(q, bounds=(100, 6000))
+    check_attention(first, *c.reference(q))
+    side, x = torch.cuda.Stream(), torch.zeros(1 << 24, device="cuda")
+    side.wait_stream(torch.cuda.current_stream())
+    outs = [torch.zeros_like(first) for _ in range(40)]
+    for i, o in enumerate(outs):
+        with torch.cuda.stream(side):
+            x.add_(i)
+        c.attend(q, bounds=(100, 6000), out=o)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, first) for o in outs)
+    jb.check_device_errors()
