@@ -69,7 +69,7 @@ Plan plan_of(int n_seqs, int T, int max_new, int max_context, int Hkv, int G, in
 using namespace jsm;
 
 extern "C" size_t jsm_attn_chunk_scratch_bytes(int n_seqs, int T, int max_new, int max_context, int Hq, int Hkv, int D, int window) {
-    if (n_seqs <= 0 || T <= 0 || max_new <= 0 || max_context < max_new || Hkv <= 0 || Hq <= 0 || Hq % Hkv || (D != 64 && D != 128) || window < 0) return 0;
+    if (n_seqs <= 0 || T <= 0 || max_new <= 0 || max_context < max_new || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > 128 || (D != 64 && D != 128) || window < 0) return 0;
     // (the larger of both kinds of cache)
     return std::max(plan_of(n_seqs, T, max_new, max_context, Hkv, Hq / Hkv, D, window, false).bytes, plan_of(n_seqs, T, max_new, max_context, Hkv, Hq / Hkv, D, window, true).bytes);
 }

@@ -140,3 +140,12 @@ def test_scratch_of_arguments_that_cannot_be_right():
               (2, 3, 1, 64, 4, 2, 96)):
         assert f(*a, 0) == 0
     assert f(2, 3, 1, 64, 4, 2, 128, -1) == 0
+
+
+def test_scratch_of_more_heads_than_a_tile_has_rows():
+    """More than 128 query heads per kv head are refused by the attention; the query for its scratch, which comes first, says 0 (it divided by the tokens of a tile)."""
+    f = jb.lib().jsm_attn_chunk_scratch_bytes
+    for Hq, Hkv in ((129, 1), (258, 2), (1 << 16, 1)):
+        for n, T, most in ((2, 3, 2), (1, 1, 1), (5, 300, 100), (1, 200, 200)):
+            assert f(n, T, most, 300, Hq, Hkv, 128, 0) == 0
+    assert attend(Hq=258, q_rs=1 << 20, rs=1 << 20, scratch=None, bytes=0) == jb.UNSUPPORTED
