@@ -26,11 +26,11 @@ struct Plan {
 //   64 sequences of 8 tokens of 4096, 8-bit (bf16)                               276 (338) 312 (260)
 //   64 tokens of 4096 positions, 32 / 32 heads                                    41      27.5
 float seen(int max_context, int window, int tokens, int unit) {  // pages or key tiles that so many tokens see at most
-    const long long all = (max_context + unit - 1) / unit;
+    const long long all = ((long long)max_context + unit - 1) / unit;  // (a bound may be INT_MAX: none)
     return (float)(window > 0 ? std::min(all, ((long long)window + tokens + unit - 3) / unit + 1) : all);
 }
 bool groups_win(int n_seqs, int T, int max_new, int max_context, int Hkv, int G, int D, int window, bool q8) {
-    auto parts = [&](int tokens) { return (float)std::min((long long)n_seqs * ((max_new + tokens - 1) / tokens), T / tokens + (long long)n_seqs) * Hkv; };
+    auto parts = [&](int tokens) { return (float)std::min((long long)n_seqs * (((long long)max_new + tokens - 1) / tokens), T / tokens + (long long)n_seqs) * Hkv; };
     const int per = 16 / G, tile = 2 * (128 / G), sms = sm_count();
     const float pages = seen(max_context, window, per, JSM_PAGE_SIZE), run = std::max(2.0f, pages * parts(per) / (2 * sms));
     const float groups = 8.0f + (D == 64 ? 0.65f : q8 ? 1.2f : 1.3f) * run + 5.0f * std::max(0.0f, run / pages - 1.0f);

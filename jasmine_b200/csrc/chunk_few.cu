@@ -614,7 +614,7 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant_
 // As many runs as the chip holds CTAs (8-bit pages, heads of 128: three per multiprocessor with three stages each 80.7 us for 64 contexts of 512 to 8192, four with two 87.0; 77 by now), of
 // two pages at least (one token over 4096 positions: 7.8 us, with runs of one page 8.1).
 FewPlan chunk_few_plan(int n_seqs, int T, int max_new, int max_context, int Hkv, int G, int window, int rows, int tokens, int D, bool q8) {
-    long long pages = (max_context + JSM_PAGE_SIZE - 1) / JSM_PAGE_SIZE;
+    long long pages = ((long long)max_context + JSM_PAGE_SIZE - 1) / JSM_PAGE_SIZE;
     if (window > 0) pages = std::min(pages, ((long long)window + max_new + JSM_PAGE_SIZE - 3) / JSM_PAGE_SIZE + 1);
     FewPlan f;
     f.rows = rows;

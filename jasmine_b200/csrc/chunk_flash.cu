@@ -148,7 +148,7 @@ __device__ __forceinline__ Place find_tile(const FlashArgs& f, long long cluster
         int n = 0, share = 1, row0 = 0, n_new = 0, ctx = 0;
         if (s < a.c.n_seqs && chunk_lengths(a, s, row0, n_new, ctx) && n_new > f.few_tokens) {
             n = (n_new + tokens - 1) / tokens;
-            const int keys = a.window > 0 ? min(ctx, a.window + tokens) : ctx;
+            const int keys = a.window > 0 ? (int)min((long long)ctx, (long long)a.window + tokens) : ctx;
             while (share < f.cluster && keys > f.walk_tiles * share * CK_BN) share *= 2;
         }
         const long long groups = ((long long)n * a.c.Hkv * share + f.cluster - 1) / f.cluster;

@@ -149,3 +149,14 @@ def test_scratch_of_more_heads_than_a_tile_has_rows():
         for n, T, most in ((2, 3, 2), (1, 1, 1), (5, 300, 100), (1, 200, 200)):
             assert f(n, T, most, 300, Hq, Hkv, 128, 0) == 0
     assert attend(Hq=258, q_rs=1 << 20, rs=1 << 20, scratch=None, bytes=0) == jb.UNSUPPORTED
+
+
+@pytest.mark.parametrize("window", (0, 100, 2 ** 31 - 1))
+def test_scratch_of_calls_without_bounds(window):
+    """The largest number as a bound, "none": as much scratch as for any context that is long enough for the chip to be full."""
+    f, none = jb.lib().jsm_attn_chunk_scratch_bytes, 2 ** 31 - 1
+    for n, T, most in ((1, 1, 1), (4, 9, 3), (3, 3, 1), (40, 40, 1), (4, 400, 100)):
+        long = f(n, T, most, 1 << 30, 8, 2, 128, window)
+        assert f(n, T, most, none, 8, 2, 128, window) == long and (long > 0 or T == 400)
+        # (0: the tiles take such a call alone)
+        assert f(n, T, none, none, 8, 2, 128, window) >= 0

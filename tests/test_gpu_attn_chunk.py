@@ -270,3 +270,15 @@ def test_pairs_beside_other_work():
     torch.cuda.synchronize()
     assert all(torch.equal(o, first) for o in outs)
     jb.check_device_errors()
+
+
+@pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("new,ctx", [([1, 1], [700, 90]), ([3, 1, 40], [300, 20, 200]), ([150], [900]), ([9, 5], [200, 260])])
+def test_the_largest_numbers_as_bounds(new, ctx, bits):
+    c = Cache(new, ctx, 2, 128, bits, seed=13).to_device()
+    q = c.queries(8)
+    want = c.reference(q)
+    for bounds, window in (((max(new), 2 ** 31 - 1), 0), ((2 ** 31 - 1, 2 ** 31 - 1), 0), ((max(new), max(ctx)), 2 ** 31 - 1), ((2 ** 31 - 1, 2 ** 31 - 1), 2 ** 31 - 1)):
+        got = c.attend(q.cuda(), window, bounds=bounds)
+        jb.check_device_errors()
+        check_attention(got, *want, f"{bounds}, {window}")
