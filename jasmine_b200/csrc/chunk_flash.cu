@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
     int pages = 0;  // warp 0: pages of 16 key tiles at a time, lane i has the i-th
     auto load_pages = [&](int seq, const Walk& w, int j) {
         const int p = w.base / JSM_PAGE_SIZE + 2 * j + lane;
-        return p * JSM_PAGE_SIZE < w.end ? cache_page(a.c, seq, p * JSM_PAGE_SIZE) : 0;
+        return p <= (w.end - 1) / JSM_PAGE_SIZE ? cache_page(a.c, seq, p * JSM_PAGE_SIZE) : 0;  // (pages: the place of a key behind the context may pass 32 bits)
     };
     if (warp == 0) {
         __syncwarp();
@@ -436,11 +436,11 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
                 if (!wait(&v_full[vs], (i / ST) & 1, TC_TIMEOUT_FULL) || (more && !wait(&k_full[s1], ((i + 1) / ST) & 1, TC_TIMEOUT_FULL))) { ok = false; break; }
                 if (!Q8) {  // values that no row sees: a weight of zero meets a number
                     const int key0 = base + j * CK_BN;
-                    if (key0 < lo || key0 + CK_BN > end) {
+                    if (key0 < lo || end - key0 < CK_BN) {
                         uint8_t* vb = v_smem + vs * Z::KV;
                         for (int n = lane; n < CK_BN * (D / 8); n += 32) {
                             const int row = n / (D / 8), c = n % (D / 8);
-                            if (key0 + row < lo || key0 + row >= end)
+                            if (key0 + row < lo || row >= end - key0)
                                 *reinterpret_cast<uint4*>(vb + (c >> 3) * Z::SLAB + row * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
                         }
                         fence_proxy_async_smem();
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
 #pragma unroll
             for (int i = 0; i < CK_BN; ++i) sv[i] = __uint_as_float(sr[i]);
             const int key0 = base + j * CK_BN;
-            const bool masked = key0 + CK_BN - 1 > pos_lo || key0 < first_key(a.window, pos_hi);
+            const bool masked = pos_lo - key0 < CK_BN - 1 || key0 < first_key(a.window, pos_hi);
             if (__any_sync(0xffffffffu, masked || m_ref == CK_NONE)) {
                 if (masked) {
                     const int from = first_key(a.window, pos) - key0, to = pos - key0;

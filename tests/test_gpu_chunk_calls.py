@@ -209,3 +209,29 @@ def test_lengths_that_a_kernel_writes_before_each_call(most, bits):
     torch.cuda.synchronize()
     assert torch.equal(outs, want)
     jb.check_device_errors()
+
+
+@pytest.mark.parametrize("bits", (16, 8))
+@pytest.mark.parametrize("new,back", [(1, 0), (3, 1), (40, 0), (40, 5), (130, 37)])
+def test_the_last_positions_that_a_context_can_have(new, back, bits):
+    """Contexts that end at 2^31: a block table of as many pages as 32 bits count positions for, of which a window sees the last."""
+    Hkv, D, pages = 2, 64, (2 ** 31 - 1) // PAGE
+    ctx = 6 * PAGE - back
+    small = Cache([new], [ctx], Hkv, D, bits, seed=new).to_device()
+    blocks = torch.full((1, pages), -1, dtype=torch.int32, device="cuda")
+    blocks[0, -6:] = small.table[0, :6]
+    lens = torch.tensor([pages * PAGE - back], dtype=torch.int32, device="cuda")
+    q = small.queries(8)
+    got = jb.attn_chunk(q.cuda(), small.pool, blocks, small.starts, lens, 8, Hkv, D, new, 2 ** 31 - 1, scales=small.scales, window=200)
+    jb.check_device_errors()
+    check_attention(got, *small.reference(q, 200))
+    k, v = jb.kv_read(small.pool, blocks, small.starts, lens, new, Hkv, D, scales=small.scales, dtype=torch.float32)
+    want = small.values[0][:, :, ctx - new:].transpose(1, 2).reshape(2, new, -1)
+    assert torch.equal(k.cpu(), want[0]) and torch.equal(v.cpu(), want[1])
+    if bits == 8:
+        x = torch.randn(new, 2 * Hkv * D, device="cuda").bfloat16()
+        jb.kv_append_q8(small.pool, small.scales, blocks, x[:, :Hkv * D], x[:, Hkv * D:], small.starts, lens, Hkv, D)
+        far = jb.kv_read(small.pool, blocks, small.starts, lens, new, Hkv, D, scales=small.scales)
+        near = jb.kv_read(small.pool, small.table, small.starts, small.lens, new, Hkv, D, scales=small.scales)
+        assert torch.equal(far[0], near[0]) and torch.equal(far[1], near[1]) and not torch.equal(far[0].float().cpu(), want[0])
+    jb.check_device_errors()
