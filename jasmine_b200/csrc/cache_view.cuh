@@ -29,9 +29,9 @@ __device__ __forceinline__ void cache_error(int* err, int code) {
     if (err) atomicCAS(err, 0, code);
 }
 
-// of a sequence with new tokens
+// of a sequence whose first row is not its end: ascending, rows of the call, a context that holds them and that the table's row holds
 __device__ __forceinline__ bool lengths_fit(const CacheView& c, int T, int first_row, int end, int ctx) {
-    if (first_row >= 0 && end <= T && ctx >= end - first_row && (ctx - 1) / JSM_PAGE_SIZE < c.max_pages) return true;
+    if (first_row >= 0 && end > first_row && end <= T && ctx >= end - first_row && (ctx - 1) / JSM_PAGE_SIZE < c.max_pages) return true;
     cache_error(c.err, CACHE_BAD_LENGTH);
     return false;
 }
@@ -43,15 +43,19 @@ __device__ __forceinline__ bool cache_lengths(const CacheView& c, int s, int T, 
     const int end = load(c.starts + s + 1);
     n_new = end - first_row;
     ctx = load(c.context_lens + s);
-    return n_new > 0 && lengths_fit(c, T, first_row, end, ctx);
+    return end != first_row && lengths_fit(c, T, first_row, end, ctx);
 }
 
-// The sequence of row t, for a whole block: every thread looks at one sequence, one round of loads for as many sequences as the block has threads.  -1: none.
-__device__ __forceinline__ int find_sequence(const CacheView& c, int t, int* found) {
+// The sequence of row t of the T rows, for a whole block: every thread looks at one sequence, one round of loads for as many sequences as the block has threads.  -1: none.
+// Sequences that no row leads to because their own rows do not fit are reported here.
+__device__ __forceinline__ int find_sequence(const CacheView& c, int t, int T, int* found) {
     if (threadIdx.x == 0) *found = -1;
     __syncthreads();
-    for (int s = threadIdx.x; s < c.n_seqs; s += blockDim.x)
-        if (c.starts[s] <= t && t < c.starts[s + 1]) *found = s;
+    for (int s = threadIdx.x; s < c.n_seqs; s += blockDim.x) {
+        const int from = c.starts[s], to = c.starts[s + 1];
+        if (from <= t && t < to) *found = s;
+        if (from != to && (from < 0 || to < from || to > T)) cache_error(c.err, CACHE_BAD_LENGTH);
+    }
     __syncthreads();
     return *found;
 }

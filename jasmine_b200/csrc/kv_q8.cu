@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(256) kv_append_q8_kernel(AppendArgs a) {
     chain_trigger();
     chain_wait();
     const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = a.c.D;
-    const int s = find_sequence(a.c, t, &found);
+    const int s = find_sequence(a.c, t, a.T, &found);
     if (s < 0) return;
     int first, n_new, ctx;
     if (!cache_lengths(a.c, s, a.T, first, n_new, ctx)) return;
@@ -97,7 +97,7 @@ __device__ __forceinline__ void find_places(const CacheView& c, int T, int t0, i
     for (int s = threadIdx.x; s < c.n_seqs; s += blockDim.x) {
         const int from = c.starts[s], to = c.starts[s + 1], ctx = c.context_lens[s];  // (one round of loads; the table is the other)
         const int k0 = max(0, from - t0), k1 = to > t0 ? min(n, to - t0) : 0;
-        if (k0 < k1 && lengths_fit(c, T, from, to, ctx))
+        if (from != to && lengths_fit(c, T, from, to, ctx))
             for (int k = k0; k < k1; ++k) {
                 seq[k] = s;
                 pos[k] = ctx - to + t0 + k;
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a) {
     chain_trigger();
     chain_wait();
     const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = a.c.D;
-    const int s = find_sequence(a.c, t, &found);
+    const int s = find_sequence(a.c, t, a.T, &found);
     if (s < 0) return;
     int first, n_new, ctx;
     if (!cache_lengths(a.c, s, a.T, first, n_new, ctx)) return;

@@ -235,3 +235,48 @@ def test_the_last_positions_that_a_context_can_have(new, back, bits):
         near = jb.kv_read(small.pool, small.table, small.starts, small.lens, new, Hkv, D, scales=small.scales)
         assert torch.equal(far[0], near[0]) and torch.equal(far[1], near[1]) and not torch.equal(far[0].float().cpu(), want[0])
     jb.check_device_errors()
+
+
+@pytest.mark.parametrize("starts", ([0, 2, 0, 0], [0, 2, -3, -3], [0, 2, 9, 9], [0, 2, 2 ** 31 - 1, 2 ** 31 - 1], [0, 2, -2 ** 31, -2 ** 31]))
+@pytest.mark.parametrize("aligned", (True, False))
+def test_starts_that_go_down_or_leave_the_rows_are_reported(starts, aligned):
+    c = Cache([2, 3, 0], [70, 90, 5], 2, 64, 8, rows=3, seed=2).to_device()
+    good = c.starts.clone()
+    c.starts.copy_(torch.tensor(starts))
+    pad = 8 if aligned else 3
+    x = torch.randn(c.T, 256 + pad, device="cuda").bfloat16()
+    k, v = x[:, pad:pad + 128], x[:, pad + 128 - 128 * (not aligned):][:, :128]
+
+    def reported():
+        with pytest.raises(jb.JsmError, match="lengths of a sequence") as e:
+            jb.check_device_errors()
+        assert e.value.status == jb.INVALID_ARG
+
+    pools = []
+    for s in (c.starts, good):
+        pool, scales = c.pool.clone(), c.scales.clone()
+        jb.kv_append_q8(pool, scales, c.table, k, v, s, c.lens, 2, 64)
+        if s is c.starts:
+            reported()
+        pools.append((pool, scales.view(torch.int16)))
+    pages = c.table[0, :2].long()  # of the sequence whose rows are right
+    assert all(torch.equal(a[pages], b[pages]) for a, b in zip(*pools))
+    rest = torch.ones(c.pool.shape[0], dtype=torch.bool, device="cuda")
+    rest[pages] = False
+    assert torch.equal(pools[0][0][rest], c.pool[rest])
+    wide = torch.full((2, c.T, 128 + pad), 5.0, dtype=torch.bfloat16, device="cuda")
+    ko, vo = wide[0, :, pad:], wide[1, :, pad:]
+    jb.kv_read(c.pool, c.table, c.starts, c.lens, c.T, 2, 64, scales=c.scales, k_out=ko, v_out=vo)
+    reported()
+    k1, v1 = jb.kv_read(c.pool, c.table, good, c.lens, c.T, 2, 64, scales=c.scales)
+    assert torch.equal(ko[:2], k1[:2]) and torch.equal(vo[:2], v1[:2]) and bool((wide[:, 2:] == 5).all())
+    for Hq in (4, 32):  # both kernels
+        q = c.queries(Hq)
+        want, mag = c.reference(q)
+        want[2:] = float("nan")
+        out = torch.full((c.T, Hq * 64), 9.0, dtype=torch.bfloat16, device="cuda")
+        c.attend(q.cuda(), out=out)
+        reported()
+        check_attention(out, want, mag)
+        assert bool((out[2:] == 9).all())
+    jb.check_device_errors()
