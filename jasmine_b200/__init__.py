@@ -520,7 +520,7 @@ def _rows(t, columns, what):
 
 
 def _pitch(t):
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])  # (a single row's pitch means nothing)
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]  # (a single row's pitch means nothing)
 
 
 def _ints(t, shape, what):

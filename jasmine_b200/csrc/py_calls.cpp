@@ -229,7 +229,7 @@ bool as_rows(PyObject* o, int64_t columns, Rows& r) {
     if (!t || t->dim() != 2 || t->size(1) != columns || (columns > 1 && t->stride(1) != 1) || t->size(0) > INT32_MAX) return false;
     r.data = t->mutable_data_ptr();
     r.T = t->size(0);
-    r.pitch = r.T > 1 ? t->stride(0) : std::max(t->stride(0), columns);
+    r.pitch = r.T > 1 ? t->stride(0) : columns;
     r.type = type_of(*t);
     return true;
 }

@@ -280,3 +280,36 @@ def test_starts_that_go_down_or_leave_the_rows_are_reported(starts, aligned):
         check_attention(out, want, mag)
         assert bool((out[2:] == 9).all())
     jb.check_device_errors()
+
+
+@pytest.mark.parametrize("fast", (True, False))
+def test_one_row_of_any_parent(fast, monkeypatch):
+    """A single row's pitch means nothing: keys, values, queries and outputs that are pieces of different rows are one token's all the same."""
+    if not fast:
+        monkeypatch.setattr(jb, "_calls_module", False)
+        monkeypatch.setattr(jb, "_calls", lambda: False)
+    c = Cache([1], [130], 2, 128, 8, seed=4).to_device()
+    wide, odd = torch.randn(1, 2048, device="cuda").bfloat16(), torch.randn(1, 1029, device="cuda").bfloat16()
+    t = torch.randn(140, 64, 2, device="cuda")
+    piece = lambda x, at, n: x[:, at:at + n]  # noqa: E731
+    k, v = torch.randn(1, 256, device="cuda").bfloat16(), piece(wide, 512, 256)
+    got = []
+    for a, b in ((k, v), (k.clone(), v.contiguous()), (piece(odd, 0, 256).copy_(k), v)):
+        pool, scales = c.pool.clone(), c.scales.clone()
+        jb.kv_append_q8(pool, scales, c.table, a, b, c.starts, c.lens, 2, 128, rope=t, rot_dim=128)
+        got.append((pool, scales))
+    assert all(torch.equal(x[0], got[0][0]) and torch.equal(x[1].view(torch.int16), got[0][1].view(torch.int16)) for x in got)
+    pool, scales = got[0]
+    ko, vo = piece(torch.zeros(1, 1029, dtype=torch.bfloat16, device="cuda"), 0, 256), torch.zeros(1, 256, dtype=torch.bfloat16, device="cuda")
+    jb.kv_read(pool, c.table, c.starts, c.lens, 1, 2, 128, scales=scales, k_out=ko, v_out=vo)
+    k1, v1 = jb.kv_read(pool, c.table, c.starts, c.lens, 1, 2, 128, scales=scales)
+    assert torch.equal(ko, k1) and torch.equal(vo, v1)
+    q = torch.randn(1, 1024, device="cuda").bfloat16()
+    args = (c.table, c.starts, c.lens, 8, 2, 128, 1, 130)
+    want = jb.attn_chunk(q, pool, *args, scales=scales)
+    out = piece(torch.zeros(1, 1029, dtype=torch.bfloat16, device="cuda"), 0, 1024)
+    assert torch.equal(jb.attn_chunk(piece(odd, 0, 1024).copy_(q), pool, *args, scales=scales, out=out), want)
+    a, b = jb.rope_rotate(q, k, t, 8, 2, 128, 128)
+    x, y = jb.rope_rotate(piece(odd, 0, 1024).copy_(q), piece(wide, 0, 256).copy_(k), t, 8, 2, 128, 128, q_out=out, k_out=ko)
+    assert torch.equal(a, x) and torch.equal(b, y)
+    jb.check_device_errors()
