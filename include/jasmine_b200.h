@@ -344,7 +344,7 @@ jsm_status jsm_attn_decode_static_scratch(const void* d_q, int64_t q_row_stride,
  * jsm_attn_chunk: attention of the new tokens over everything their sequence has in the cache, the tokens themselves included (append first).  The
  * query at position p sees the keys max(0, p - window + 1) .. p (window 0: all before it); query head h reads kv head h / (Hq / Hkv).  The sum
  * runs over the keys that are seen only: what the others hold, infinities and NaN too, has no influence, and pages that no query of the call
- * sees are not read.  q, out: BF16 rows (16-byte aligned, pitch a multiple of 8); D 64 or 128; scale > 0; Hq / Hkv up to 128.
+ * sees are not read.  q, out: BF16 rows (16-byte aligned, pitch a multiple of 8; out may be q itself, but not overlap it otherwise); D 64 or 128; scale > 0; Hq / Hkv up to 128.
  * max_new, max_context: bounds of the new tokens and of the context of one sequence.  d_scratch: jsm_attn_chunk_scratch_bytes(...) bytes for these arguments on the
  * current device, at most some MB however long the contexts are (contents do not matter, before or after; 0: none is needed); calls that may run at the same time
  * need scratch of their own.  The same arguments give the same bits. */

@@ -713,10 +713,10 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
                         make_uint4(pack_bf16x2(x[i], x[i + 1]), pack_bf16x2(x[i + 2], x[i + 3]), pack_bf16x2(x[i + 4], x[i + 5]), pack_bf16x2(x[i + 6], x[i + 7]));
             }
             __syncwarp();
-            // rows leave whole, 16 bytes per lane; lane r knows where row r goes
+            // rows leave whole, 16 bytes per lane; lane r knows where row r goes (a row that is worked out again does not: the outputs may lie where its query is)
             constexpr int PIECES = D / 8, STEP = 32 / PIECES;
             const int piece = lane % PIECES, in = (int)(row * f.inv_G >> 16);
-            const long long goes = query ? (row0 + token) * a.out_rs + (long long)(hk * a.G + row - in * a.G) * D : -1;
+            const long long goes = query && !bad ? (row0 + token) * a.out_rs + (long long)(hk * a.G + row - in * a.G) * D : -1;
 #pragma unroll 2
             for (int r0 = 0; r0 < 32; r0 += STEP) {
                 const int r = r0 + lane / PIECES;

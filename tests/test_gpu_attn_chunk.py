@@ -282,3 +282,25 @@ def test_the_largest_numbers_as_bounds(new, ctx, bits):
         got = c.attend(q.cuda(), window, bounds=bounds)
         jb.check_device_errors()
         check_attention(got, *want, f"{bounds}, {window}")
+
+
+@pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("new,ctx,Hq,Hkv,most", [([1, 3], [200, 260], 8, 2, 300), ([100, 1], [300, 200], 8, 2, 300), ([9, 5], [200, 260], 8, 2, 300), ([65], [2000], 4, 1, 2000),
+                                                 ([100], [500], 256, 32, 6000)])
+def test_outputs_in_place_of_the_queries(new, ctx, Hq, Hkv, most, bits):
+    """Rows that are worked out again too: a query is read before its place is written."""
+    c = Cache(new, ctx, Hkv, 128, bits, seed=17)
+    for b, (n, x) in enumerate(zip(new, ctx)):
+        c.values[b][1, 0, x - 1 - n // 2] = float("nan")  # a value among the new tokens that some of them do not see
+        c.write(b)
+    c.to_device()
+    q = c.queries(Hq)
+    want, mag = c.reference(q)
+    got = c.attend(q.cuda(), bounds=(max(new), most))
+    same = q.cuda()
+    c.attend(same, bounds=(max(new), most), out=same)
+    jb.check_device_errors()
+    assert torch.equal(same.view(torch.int16), got.view(torch.int16))
+    assert torch.equal(got.isfinite().cpu(), want.isfinite())
+    fine = want.isfinite()
+    check_attention(torch.where(fine, same.double().cpu(), 0.0), torch.where(fine, want, 0.0), torch.where(fine, mag, 0.0))
