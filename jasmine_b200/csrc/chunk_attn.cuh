@@ -42,7 +42,8 @@ __device__ __forceinline__ bool chunk_lengths(const ChunkArgs& a, int s, int& fi
 __device__ __forceinline__ int first_key(int window, int pos) { return window > 0 ? max(0, pos - window + 1) : 0; }
 
 // One query row of one head by one warp, key after key in fp32, over exactly the keys that it sees: lane l has the components l * (D / 32) and up.
-// sum of p v, sum of p, as p = 2^(score - largest so far); o is the quotient.
+// sum of p v, sum of p, as p = 2^(score - largest so far); o is the quotient.  Values count 2^-32 of themselves until the end: a context has fewer than 2^31 keys, so a
+// sum of the largest bf16 numbers stays one of fp32 (and what is below 2^-94 loses bits; a row that comes here for another reason has outputs exact to 2^-118).
 template <int D, bool Q8>
 __device__ __noinline__ void attend_row(const ChunkArgs& a, int s, int row, int head, int pos) {
     constexpr int N = D / 32;
@@ -85,11 +86,11 @@ __device__ __noinline__ void attend_row(const ChunkArgs& a, int s, int row, int 
         m = mn;
         l = fmaf(l, corr, p);
 #pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = fmaf(o[i], corr, p * v[i]);
+        for (int i = 0; i < N; ++i) o[i] = fmaf(o[i], corr, p * (v[i] * 0x1p-32f));
     }
     __nv_bfloat16* dst = a.out + row * a.out_rs + (long long)head * D + lane * N;
 #pragma unroll
-    for (int i = 0; i < N; ++i) dst[i] = __float2bfloat16_rn(o[i] / l);
+    for (int i = 0; i < N; ++i) dst[i] = __float2bfloat16_rn(o[i] / l * 0x1p32f);
 }
 #endif
 

@@ -304,3 +304,26 @@ def test_outputs_in_place_of_the_queries(new, ctx, Hq, Hkv, most, bits):
     assert torch.equal(got.isfinite().cpu(), want.isfinite())
     fine = want.isfinite()
     check_attention(torch.where(fine, same.double().cpu(), 0.0), torch.where(fine, want, 0.0), torch.where(fine, mag, 0.0))
+
+
+@pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("new,ctx,Hq,Hkv,D,most", [([1, 3], [200, 1000], 8, 2, 128, 1000), ([100, 1], [300, 200], 8, 2, 64, 300), ([9, 5], [200, 260], 8, 2, 128, 300),
+                                                   ([65], [2000], 4, 1, 128, 2000), ([100], [500], 256, 32, 128, 6000)])
+def test_values_near_the_largest_number(new, ctx, Hq, Hkv, D, most, bits):
+    """Sums of a few of these values are beyond fp32; their means are not."""
+    c = Cache(new, ctx, Hkv, D, bits, seed=19)
+    top = 3.0e38 if bits == 16 else 1.7e38  # (an 8-bit cache has numbers up to 2^127)
+    for b, x in enumerate(ctx):
+        v = c.values[b][1]
+        v.copy_(torch.rand(v.shape, generator=c.g) * 0.5 + 0.5)
+        v[:, :, D // 2:] *= -1.0
+        v[:, :, :3] *= torch.where(torch.rand(v[:, :, :3].shape, generator=c.g) < 0.5, -1.0, 1.0)
+        v *= top
+        v[:, :, 5] = 1.0e-3  # (beside them)
+        c.write(b)
+    c.to_device()
+    q = c.queries(Hq)
+    got = c.attend(q.cuda(), bounds=(max(new), most))
+    jb.check_device_errors()
+    assert bool(got.isfinite().all())
+    check_attention(got, *c.reference(q))
