@@ -12,7 +12,8 @@
 // component an element of an operand stands for is free as long as both operands agree, so the pieces of a thread are the components that its operand
 // registers need, and the transposition of V costs no instruction beyond the byte permutation that spreads the numbers anyway.
 // Partial results meet in chunk_merge_kernel, in the order of the runs.
-// A row whose result is not a number is worked out again over exactly its own keys (attend_row): a weight of zero times what a hidden key holds is no zero then.
+// A row whose result is not a number, although its sum of weights is one, is worked out again over exactly its own keys (attend_row): a weight of zero times what a hidden key holds is no
+// zero then.
 #include "chunk_attn.cuh"
 #include "tc_utils.cuh"
 #include "mma_utils.cuh"
@@ -475,7 +476,7 @@ __global__ void __launch_bounds__(CF_THREADS, FewSizes<D, NT, Q8>::PER_SM) chunk
                     acc[i] /= L;
                     fine = fine && fabsf(acc[i]) <= 3.402823466e38f;
                 }
-                if (__all_sync(0xffffffffu, fine)) {
+                if (__all_sync(0xffffffffu, fine || L != L)) {  // (a sum of weights that is a NaN: from a score of a key that the row sees)
                     __nv_bfloat16* dst = a.out + row * a.out_rs + (long long)head * D + lane * N;
 #pragma unroll
                     for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack_bf16x2(acc[i], acc[i + 1]);
@@ -602,7 +603,7 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const __grid_constant_
         fine = fine && fabsf(acc[i]) <= 3.402823466e38f;
     }
     const int t = q.row0 + r / a.G, head = hk * a.G + r % a.G;
-    if (!__all_sync(0xffffffffu, fine)) {
+    if (!__all_sync(0xffffffffu, fine || l != l)) {  // (as there)
         attend_row<D, Q8>(a, s, t, head, q.ctx - q.n_new + r / a.G);
         return;
     }

@@ -15,8 +15,8 @@
 // slower for prompts: without a conversion the hand-over between the CTAs costs what it saves.)
 // Few tiles and long contexts: the units (CTAs or pairs) of a cluster share the key tiles of their query tiles; each sends the sums of the rows that another owns into that one's shared
 // memory and joins its own with what it was sent, so that nothing goes through global memory and no second launch is needed.
-// Values that no row of the CTA sees (behind the context, before the window) become zeros before they are multiplied; a row whose result is not a number is worked out
-// again over exactly its own keys (attend_row).  Every wait is bounded.
+// Values that no row of the CTA sees (behind the context, before the window) become zeros before they are multiplied; a row whose result is not a number, although its sum of weights is
+// one, is worked out again over exactly its own keys (attend_row).  Every wait is bounded.
 #include "chunk_attn.cuh"
 #include "tc_utils.cuh"
 #include "softmax_rows.cuh"
@@ -36,6 +36,7 @@ constexpr float CK_RESCALE = 8.0f;             // the maximum is above the refer
 constexpr float CK_RAISE = 16777216.0f;        // a key tile's sum of weights is above 2^24: the reference is raised
 constexpr float CK_JUMP = 1.3292279957849159e36f;  // ... above 2^120: the row is worked out again.  2^-120 is a factor that keeps its bits (below 2^-126 ex2_approx returns zero)
 constexpr float CK_NONE = -1.0e30f;             // the maximum of a row that has seen nothing
+constexpr float CK_AGAIN = -INFINITY;           // a row's sum of weights after such a jump
 
 template <int D, bool Q8, bool PAIR>
 struct FlashSizes {
@@ -493,7 +494,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
         const int pos_lo = past + tok[t], pos_hi = past + min(tok[t] + f.tile_tokens, n_new) - 1;  // first and last query of the tile
         // Weights are 2^(score - reference), whatever the reference: bf16, fp32 sums and fp32 accumulators keep their precision over 2^100 and more.  So the maximum is looked for
         // only where a row has no reference yet, or where keys are hidden; elsewhere a sum of weights above 2^24 raises the reference before the next key tile, or behind the last.  A
-        // key tile's sum above 2^120, or one that is infinite, makes the row's sum of weights a NaN: such a row is worked out again at the end.
+        // key tile's sum above 2^120, or one that is infinite, marks the row's sum of weights for good: such a row is worked out again at the end.
         float m_ref = query ? CK_NONE : 0.0f, l = 0.0f;
         int raise = 0;
         bool ok = true;
@@ -511,7 +512,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
                     tmem_st16(o_addr + c + half * 16, w);
                 }
             }
-            l *= alpha;
+            if (l != CK_AGAIN) l *= alpha;
         };
         const bool mine = tok[t] < n_new;  // (of a pair the other CTA may have a tile alone)
         const uint32_t half_to = PAIR ? ck_peer(smem_u32(&p_half[t]), rank & ~1) : 0, ready_to = PAIR ? ck_peer(smem_u32(&p_ready[t]), rank & ~1) : 0;
@@ -595,8 +596,8 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
             float la, lb;
             unpack2(fadd2(fadd2(ls2[0], ls2[1]), fadd2(ls2[2], ls2[3])), la, lb);
             const float sum = la + lb;
-            l = sum > CK_JUMP ? NAN : l + sum;
-            raise = sum > CK_RAISE ? (int)(__float_as_uint(sum) >> 23) - 127 : 0;
+            l = sum > CK_JUMP ? CK_AGAIN : l + sum;
+            raise = sum > CK_RAISE && sum <= CK_JUMP ? (int)(__float_as_uint(sum) >> 23) - 127 : 0;
             tmem_st_wait();
             weights_are_there(&p_ready[t], ready_to);
         }
@@ -614,7 +615,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
         uint8_t* staged = (share > 1 ? recv_ml + (share - 1) * own_rows * 8 : tiles) + sw * (32 * D * 2);  // this warp's 32 rows pass through here
         // What the last key tile asks for: rows meet under references that their sums of weights are near to, so that a factor below 2^-126 is one of nothing.
         const float fold = ex2_approx((float)-raise);
-        l *= fold;
+        if (l != CK_AGAIN) l *= fold;
         m_ref += (float)raise;
         float own = fold, L = l, M = m_ref;  // factor of the sums in TMEM, sum of the weights, reference of the row
         bool have = any;
@@ -663,17 +664,18 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
                 for (int p = 0; p < senders; ++p) M = fmaxf(M, reinterpret_cast<const float2*>(recv_ml)[p * own_rows + r_own + lane].x);
                 const float w_own = ex2_approx(m_ref - M);
                 own = any ? w_own * fold : 0.0f;
-                L = any ? l * w_own : 0.0f;
+                L = !any ? 0.0f : l == CK_AGAIN ? l : l * w_own;
 #pragma unroll 1
                 for (int p = 0; p < senders; ++p) {
                     const float2 w = sent_factor(p);
-                    if (w.x != 0.0f || w.y != 0.0f) L = fmaf(w.x, w.y, L);
+                    if (w.y == CK_AGAIN) L = w.y;
+                    else if (w.x != 0.0f || w.y != 0.0f) L = fmaf(w.x, w.y, L);
                 }
             }
         }
         if (have) {
             const float inv = 1.0f / L;
-            bool bad = false;
+            bool bad = L == CK_AGAIN;
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 float x[32];
@@ -713,6 +715,8 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
                         make_uint4(pack_bf16x2(x[i], x[i + 1]), pack_bf16x2(x[i + 2], x[i + 3]), pack_bf16x2(x[i + 4], x[i + 5]), pack_bf16x2(x[i + 6], x[i + 7]));
             }
             __syncwarp();
+            // (a sum of weights that is a NaN comes from a score that is no number, of a key that the row sees: nothing else would come out of it a second time)
+            bad = bad && L == L;
             // rows leave whole, 16 bytes per lane; lane r knows where row r goes (a row that is worked out again does not: the outputs may lie where its query is)
             constexpr int PIECES = D / 8, STEP = 32 / PIECES;
             const int piece = lane % PIECES, in = (int)(row * f.inv_G >> 16);

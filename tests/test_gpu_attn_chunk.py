@@ -327,3 +327,36 @@ def test_values_near_the_largest_number(new, ctx, Hq, Hkv, D, most, bits):
     jb.check_device_errors()
     assert bool(got.isfinite().all())
     check_attention(got, *c.reference(q))
+
+
+@pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("new,ctx,Hq,Hkv,most", [([256], [4096], 8, 2, 4096), ([512], [512], 8, 2, 512), ([1] * 4, [4096] * 4, 8, 2, 4096), ([9], [4096], 8, 2, 4096), ([100], [1500], 256, 32, 6000)])
+def test_a_key_that_is_no_number_costs_no_second_walk(new, ctx, Hq, Hkv, most, bits):
+    """All rows see it: they are NaN, and as soon as other numbers would be (each of them key by key a second time took 700 times as long)."""
+    c = Cache(new, ctx, Hkv, 128, bits, seed=23)
+    clean = [x.clone() for x in c.values]
+    times = []
+    for bad in (False, True):
+        for b, x in enumerate(clean):
+            c.values[b].copy_(x)
+            if bad:
+                c.values[b][0, 0, ctx[b] // 8, 3] = float("nan")
+            c.write(b)
+        pool, scales = c.pool.cuda(), c.scales.cuda() if bits == 8 else None
+        q = c.queries(Hq)
+        args = (pool, c.table.cuda(), c.starts.cuda(), torch.tensor(ctx, dtype=torch.int32, device="cuda"), Hq, Hkv, 128, max(new), most)
+        qd, ms = q.cuda(), []
+        for _ in range(5):
+            a, e = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            got = jb.attn_chunk(qd, *args, scales=scales)
+            e.record()
+            torch.cuda.synchronize()
+            ms.append(a.elapsed_time(e))
+        times.append(min(ms))
+        want, mag = c.reference(q)
+        assert torch.equal(got.isnan().cpu(), want.isnan())
+        fine = ~want.isnan()
+        check_attention(torch.where(fine, got.double().cpu(), 0.0), torch.where(fine, want, 0.0), torch.where(fine, mag, 0.0))
+    jb.check_device_errors()
+    assert times[1] < 20 * times[0], times
