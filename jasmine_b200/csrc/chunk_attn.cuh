@@ -81,7 +81,11 @@ __device__ __noinline__ void attend_row(const ChunkArgs& a, int s, int row, int 
 #pragma unroll
         for (int i = 0; i < N; ++i) sum = fmaf(q[i], k[i], sum);
         const float score = warp_sum(sum) * a.scale_log2;
-        if (score == -INFINITY) continue;  // weight 0 beside any other key
+        if (score == -INFINITY) {  // of weight 0 beside any other key, and 0 times an infinite value is no number
+#pragma unroll
+            for (int i = 0; i < N; ++i) o[i] = fmaf(0.0f, v[i], o[i]);
+            continue;
+        }
         const float mn = fmaxf(m, score), corr = exp2f(m - mn), p = exp2f(score - mn);
         m = mn;
         l = fmaf(l, corr, p);

@@ -360,3 +360,28 @@ def test_a_key_that_is_no_number_costs_no_second_walk(new, ctx, Hq, Hkv, most, b
         check_attention(torch.where(fine, got.double().cpu(), 0.0), torch.where(fine, want, 0.0), torch.where(fine, mag, 0.0))
     jb.check_device_errors()
     assert times[1] < 20 * times[0], times
+
+
+@pytest.mark.parametrize("new,ctx,Hq,Hkv,most", [([1, 3], [200, 260], 8, 2, 300), ([100, 1], [300, 200], 8, 2, 300), ([9, 5], [200, 260], 8, 2, 300), ([65], [2000], 4, 1, 2000),
+                                                 ([65], [2000], 4, 2, 2000)])
+def test_an_infinite_value_of_weight_zero(new, ctx, Hq, Hkv, most):
+    """A seen key whose score is -inf has no weight, and zero times its infinite value is no number; beside it, and without it, numbers stay numbers."""
+    c = Cache(new, ctx, Hkv, 128, 16, seed=29)
+    for b, (n, x) in enumerate(zip(new, ctx)):
+        for at, key in ((x // 3, -float("inf")), (x // 2, float("inf"))):
+            c.values[b][0, 0, at, 7] = key
+            c.values[b][1, 0, at, 9] = float("inf")
+        c.values[b][0, Hkv - 1, x - n // 2 - 1, 7] = -float("inf")  # of the new ones: not all see it
+        c.values[b][1, Hkv - 1, x - n // 2 - 1, 11] = -float("inf")
+        c.write(b)
+    c.to_device()
+    q = c.queries(Hq)
+    q.view(-1, Hq, 128)[:, ::2, 7] = q.view(-1, Hq, 128)[:, ::2, 7].abs() + 0.1  # both signs among the scores
+    got = c.attend(q.cuda(), bounds=(max(new), most))
+    jb.check_device_errors()
+    want, mag = c.reference(q)
+    assert torch.equal(got.isfinite().cpu(), want.isfinite())
+    # (heads of the first kv head see a score of +inf or an infinite value: with one kv head there is no number at all)
+    assert bool(want.isfinite().any()) == (Hkv > 1) and not bool(want.isfinite().all())
+    fine = want.isfinite()
+    check_attention(torch.where(fine, got.double().cpu(), 0.0), torch.where(fine, want, 0.0), torch.where(fine, mag, 0.0))
