@@ -313,3 +313,42 @@ def test_one_row_of_any_parent(fast, monkeypatch):
     x, y = jb.rope_rotate(piece(odd, 0, 1024).copy_(q), piece(wide, 0, 256).copy_(k), t, 8, 2, 128, 128, q_out=out, k_out=ko)
     assert torch.equal(a, x) and torch.equal(b, y)
     jb.check_device_errors()
+
+
+def test_a_step_over_a_bf16_cache():
+    """Rotate queries and keys (halves of a part of the head), append by sequence and position, attend: prompts, then one token or a few of each sequence."""
+    Hq, Hkv, D, rot, n, most = 8, 2, 128, 64, 3, 4
+    g = torch.Generator().manual_seed(5)
+    steps = [[100, 1, 64], [0, 70, 3], [1, 1, 1], [4, 0, 2]]
+    total = [sum(s[b] for s in steps) for b in range(n)]
+    rows = [torch.randn(t, (Hq + 2 * Hkv) * D, generator=g).bfloat16().cuda() for t in total]
+    pool = torch.full((n * most, 2, Hkv, PAGE, D), float("nan"), dtype=torch.bfloat16, device="cuda")
+    blocks = torch.randperm(n * most, generator=g).int().view(n, most).cuda()
+    t = torch.empty(256, rot // 2, 2, device="cuda")
+    jb.check(jb.lib().jsm_rope_scaled_table(t.data_ptr(), rot, 10000.0, 4.0, 64.0, 32.0, 1.0, 256))
+    done, outs, rotated = [0] * n, [[] for _ in range(n)], [[] for _ in range(n)]
+    for new in steps:
+        x = torch.cat([r[d:d + m] for r, d, m in zip(rows, done, new)])
+        at = torch.cat([torch.arange(d, d + m) for d, m in zip(done, new)]).int().cuda()
+        seq = torch.repeat_interleave(torch.arange(n), torch.tensor(new)).int().cuda()
+        done = [d + m for d, m in zip(done, new)]
+        starts = torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+        q, k = jb.rope_rotate(x[:, :Hq * D], x[:, Hq * D:(Hq + Hkv) * D], t, Hq, Hkv, D, rot, at)
+        v = x[:, (Hq + Hkv) * D:].contiguous()  # (keys and values of one pitch)
+        jb.kv_append(pool, blocks, k, v, seq, at, Hkv, D)
+        lens = torch.tensor(done, dtype=torch.int32, device="cuda")
+        out = jb.attn_chunk(q, pool, blocks, starts, lens, Hq, Hkv, D, max(new), max(done))
+        kr, vr = jb.kv_read(pool, blocks, starts, lens, len(x), Hkv, D)
+        assert torch.equal(kr, k) and torch.equal(vr, v)
+        for b, part in enumerate(zip(out.split(new), q.split(new), k.split(new))):
+            outs[b].append(part[0])
+            rotated[b].append(part[1:])
+    jb.check_device_errors()
+    for b in range(n):
+        q, k = (torch.cat([p[i] for p in rotated[b]]).double().view(total[b], -1, D) for i in (0, 1))
+        k, v = (x.repeat_interleave(Hq // Hkv, 1) for x in (k, rows[b][:, (Hq + Hkv) * D:].double().view(total[b], Hkv, D)))
+        s = torch.einsum("ihd,jhd->hij", q, k) * D ** -0.5
+        s = s.masked_fill(torch.ones(total[b], total[b], device="cuda").triu(1).bool(), -float("inf"))
+        w = torch.softmax(s, -1)
+        want, mag = (torch.einsum("hij,jhd->ihd", w, x).flatten(1).cpu() for x in (v, v.abs()))
+        check_attention(torch.cat(outs[b]), want, mag)
