@@ -330,7 +330,7 @@ jsm_status jsm_attn_decode_static_scratch(const void* d_q, int64_t q_row_stride,
 /* ---- new tokens of many sequences over a paged cache, bf16 or 8-bit (not in the reference) -------------------------------
  * Sequence s brings the rows d_starts[s] <= t < d_starts[s + 1] (I32 [n_seqs + 1], ascending; none, one, or many) of the T rows of the call; its context
  * d_context_lens[s] counts them, so row t is position d_context_lens[s] - (d_starts[s + 1] - t).  Rows of no sequence (behind the last
- * one, say) are neither read nor written.  A sequence whose lengths do not fit (more rows than context, a context beyond its table's
+ * one, say) have no part and are not written.  A sequence whose lengths do not fit (starts that go down or leave the T rows, more rows than context, a context beyond its table's
  * max_pages * 64, beyond max_new / max_context where a call has them) is left out, a page outside 0 .. n_pages-1 is not accessed (what would come from it is
  * meaningless); both are reported by jsm_check_device_errors (JSM_INVALID_ARG).  No two positions of a call may share a place in the pool.
  * Make the first call on a device outside a stream capture.

@@ -11,7 +11,7 @@
 //                 rounded once, so scores and sums are those of a bf16 cache of these values; the conversion is spread over the whole group's rows
 // 8-bit caches, long contexts (PAIR): two CTAs walk the keys of four query tiles together (cta_group::2).  A product has 256 rows, 128 in each CTA's tensor memory; each CTA brings and
 // converts half of K (one page of two) and of V (64 of the 128 columns), so that a key tile is converted once for four query tiles, and operands come from shared memory half as
-// often: 173 -> 148 us for 1000 tokens of 9000 positions (143 by now).  The even CTA issues the products of both; what the other has written is announced to it.  (bf16: 71 against 72 us for 512 of 8192,
+// often: 173 -> 148 us for 1000 tokens of 9000 positions (140 by now).  The even CTA issues the products of both; what the other has written is announced to it.  (bf16: 71 against 72 us for 512 of 8192,
 // slower for prompts: without a conversion the hand-over between the CTAs costs what it saves.)
 // Few tiles and long contexts: the units (CTAs or pairs) of a cluster share the key tiles of their query tiles; each sends the sums of the rows that another owns into that one's shared
 // memory and joins its own with what it was sent, so that nothing goes through global memory and no second launch is needed.
@@ -81,7 +81,8 @@ __device__ __forceinline__ void ck_store4(uint32_t addr, uint32_t a, uint32_t b,
 // Arrivals at a barrier of the other CTA (or this one), and waits for such.  What lies in tensor memory is ordered by tcgen05.wait and the tcgen05 fences on both sides; arrival and wait carry
 // no more than the order of execution (relaxed, at the scope of the cluster).  What lies in shared memory needs a release and an acquire at that scope.  A thread pays for its release until all that it
 // has written is there (by the converting warps 189 us for 1000 tokens of 9000 positions, by all arrivals 205), so the writers arrive in their own CTA, and one warp of the
-// second CTA, which writes nothing itself, acquires that and releases it to the first: 143 us (139 with arrivals that release to their own CTA only, an order that the memory model does not give).
+// second CTA, which writes nothing itself, acquires that and releases it to the first: 143 us (140 by now; 139 with arrivals that release to their own CTA only, an order that the memory model does not
+// give).
 __device__ __forceinline__ void ck_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void ck_arrive_tmem(uint32_t bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 template <bool TMEM>
@@ -741,8 +742,8 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
         if constexpr (Q8) {
             const int cw = warp - CK_CONVERT;
             // Reads and writes of 16 bytes, eight lanes at a time over all banks: the lanes have four pieces of two rows whose numbers differ in bit 0 (the places of the
-            // bf16 pieces) and, where a row is a whole line, in bit 2 (the places of the raw pieces).  The loop over the raw pages stays rolled: unrolled, the four warps
-            // wait for instructions (27 KB of them; 335 us for 1000 of 9000 positions).
+            // bf16 pieces) and, where a row is a whole line, in bit 2 (the places of the raw pieces).  The loop over the raw pages stays rolled: unrolled, 335 instead of 231 us for
+            // 1000 of 9000 positions at that time (counters: two warps on average were waiting for instructions whenever one was issued).
             const int c4 = lane & 3, second = (lane >> 2) & 1;
             const uint32_t k_u32 = smem_u32(k_smem), v_u32 = smem_u32(v_smem), raw_sc = smem_u32(raw_scales), raw_u32 = smem_u32(raw_smem);
             struct Turn { int row; uint32_t src, dst; };

@@ -121,7 +121,7 @@ __device__ __forceinline__ void find_places(const CacheView& c, int T, int t0, i
 // wait for the places.  A lane's pieces hold both components of its pairs (halves: a piece of each half), so that a rotation stays within the lane.
 // Products that are rounded on their own before a sum: two by one instruction, the sums one by one (mul2).  Rounding to a whole number:
 // adding 1.5 * 2^23 leaves it in the low bits of the sum.
-// Prompts of 7887 tokens of 32 kv heads of 128 (192 MB in and out) 44 us, 4.4 TB/s of the measured 6.5: latency at five blocks per multiprocessor.  A token's table entries are in shared
+// Prompts of 7887 tokens of 32 kv heads of 128 (194 MB in and out) 38 us alone, 5.1 TB/s of the measured 6.5 (44 between read-backs): latency at five blocks per multiprocessor.  A token's table entries are in shared
 // memory: in registers they cost a block per multiprocessor, and a fetch in the middle of the rows (47 us).  The loads of two turns at a time, none while they are worked out, addresses in 64
 // bits: 53 us; a lane per eight components with the partner of a half fetched a second time 74 us.
 __device__ __forceinline__ float max3_abs(float a, float b, float c) {  // of the magnitudes; a NaN stays one
@@ -129,7 +129,7 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {  // of th
     asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// two products, each rounded (sums of them one by one: a packed sum behind a packed product leaves the assembler as one operation with one rounding)
+// two products, each rounded (sums of them one by one: with add.rn.f32x2 behind mul.rn.f32x2 the results of 1024 random triples had the bits of one rounding, with scalar sums those of two)
 __device__ __forceinline__ void mul2(float& x, float& y, float a, float b, float c, float d) {
     asm("{ .reg .b64 p, q; mov.b64 p, {%2, %3}; mov.b64 q, {%4, %5}; mul.rn.f32x2 p, p, q; mov.b64 {%0, %1}, p; }" : "=f"(x), "=f"(y) : "f"(a), "f"(b), "f"(c), "f"(d));
 }
@@ -300,7 +300,8 @@ __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a) {
     }
 }
 
-// whole 16-byte pieces of the outputs: eight components per lane, four rows' loads in flight, up to PLACES tokens per block.  The same prompts read back (192 MB) 37 us, 5.2 TB/s.
+// whole 16-byte pieces of the outputs: eight components per lane, four rows' loads in flight, up to PLACES tokens per block.  The same prompts read back: 42 us alone, 4.6 TB/s (37 behind
+// the append, from L2 in part); to fp32 85 us, 3.8 TB/s; a bf16 cache to bf16 43 us, 6.0 TB/s, to fp32 79 us, 4.9 TB/s.
 template <int LPR, bool Q8, bool F32>
 __global__ void __launch_bounds__(256) kv_read_vec_kernel(ReadArgs a, int per_block) {
     constexpr int ROWS = 256 / LPR, U = 4;
