@@ -11,7 +11,7 @@
 //                 rounded once, so scores and sums are those of a bf16 cache of these values; the conversion is spread over the whole group's rows
 // 8-bit caches, long contexts (PAIR): two CTAs walk the keys of four query tiles together (cta_group::2).  A product has 256 rows, 128 in each CTA's tensor memory; each CTA brings and
 // converts half of K (one page of two) and of V (64 of the 128 columns), so that a key tile is converted once for four query tiles, and operands come from shared memory half as
-// often: 173 -> 148 us for 1000 tokens of 9000 positions (140 by now).  The even CTA issues the products of both; what the other has written is announced to it.  (bf16: 71 against 72 us for 512 of 8192,
+// often: 173 -> 148 us for 1000 tokens of 9000 positions (140 - 143 by now).  The even CTA issues the products of both; what the other has written is announced to it.  (bf16: 71 against 72 us for 512 of 8192,
 // slower for prompts: without a conversion the hand-over between the CTAs costs what it saves.)
 // Few tiles and long contexts: the units (CTAs or pairs) of a cluster share the key tiles of their query tiles; each sends the sums of the rows that another owns into that one's shared
 // memory and joins its own with what it was sent, so that nothing goes through global memory and no second launch is needed.
@@ -79,10 +79,10 @@ __device__ __forceinline__ void ck_store4(uint32_t addr, uint32_t a, uint32_t b,
 }
 // ---- pairs of CTAs (cta_group::2): the even CTA of a pair issues the products of both -------------------------------------
 // Arrivals at a barrier of the other CTA (or this one), and waits for such.  What lies in tensor memory is ordered by tcgen05.wait and the tcgen05 fences on both sides; arrival and wait carry
-// no more than the order of execution (relaxed, at the scope of the cluster).  What lies in shared memory needs a release and an acquire at that scope.  A thread pays for its release until all that it
-// has written is there (by the converting warps 189 us for 1000 tokens of 9000 positions, by all arrivals 205), so the writers arrive in their own CTA, and one warp of the
-// second CTA, which writes nothing itself, acquires that and releases it to the first: 143 us (140 by now; 139 with arrivals that release to their own CTA only, an order that the memory model does not
-// give).
+// no more than the order of execution (relaxed, at the scope of the cluster).  What lies in shared memory, or is overwritten there behind the last products, needs a release and an acquire at
+// that scope.  A thread pays for its release until all that it has written is there (by the converting warps 189 us for 1000 tokens of 9000 positions, by all arrivals 205), so the writers arrive in
+// their own CTA, and one warp of the second CTA, which writes nothing itself, acquires that and releases it to the first: 143 us (139 with arrivals that release to their own CTA only, an order
+// that the memory model does not give).
 __device__ __forceinline__ void ck_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void ck_arrive_tmem(uint32_t bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 template <bool TMEM>
@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(FlashSizes<D, Q8, PAIR>::THREADS, 1)
             tmem_st_wait();
             weights_are_there(&p_ready[t], ready_to);
         }
-        if (ok && n_max > j_lo) ok = ck_wait_warp<PAIR, true>(&o_done, 0, &abort_flag, a.c.err, TC_TIMEOUT_ACC);
+        if (ok && n_max > j_lo) ok = ck_wait_warp<PAIR>(&o_done, 0, &abort_flag, a.c.err, TC_TIMEOUT_ACC);
         tc_fence_after();
         const bool any = ok && mine && je[t] > jb[t];  // (the whole query tile)
         // What follows is executed once per CTA, mostly for the first time on its multiprocessor: rolled loops, because every line of code is fetched (unrolled, with the
